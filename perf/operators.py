@@ -222,7 +222,7 @@ def _evict_own(s):
     from fna2_b200.paged import naylis_evict
     c = s["case"]
     kept, lens, w = naylis_evict(s["key_weights"], s["pool"], s["table"], s["lens"], c["budget"], s["table_out"],
-                                 recent=c["recent"], sink=c["sink"], max_seqlen_k=s["max_len"])
+                                 recent=c["recent"], sink=c["sink"], heads=s["H"], max_seqlen_k=s["max_len"])
     return _evict_out(s, kept, lens, w)
 
 
