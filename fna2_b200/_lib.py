@@ -12,7 +12,7 @@ from typing import Optional
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("FNA2_LIB", os.path.join(HERE, "libfna2_b200.so"))
 
-FNA2_ABI_VERSION = 5
+FNA2_ABI_VERSION = 6
 FNA2_OK = 0
 FNA2_ERR_INVALID = -1
 FNA2_ERR_CUDA = -2
@@ -20,7 +20,8 @@ FNA2_ERR_WORKSPACE = -3
 
 EXPORTED = ["fna2_fwd", "fna2_bwd", "fna2_bwd_workspace_size", "fna2_last_error", "fna2_device_status",
             "fna2_abi_version", "fna2_bwd_noalloc", "fna2_qk_prep_fwd", "fna2_qk_prep_bwd", "fna2_decode", "fna2_decode_workspace_size",
-            "fna2_debug_watchdog", "fna2_fwd_workspace_size", "fna2_gemm"]
+            "fna2_debug_watchdog", "fna2_fwd_workspace_size", "fna2_gemm", "fna2_paged_append", "fna2_paged_attn",
+            "fna2_paged_attn_workspace_size", "fna2_key_weights", "fna2_key_weights_workspace_size", "fna2_evict"]
 FNA2_DTYPE_F32 = 0
 FNA2_DTYPE_BF16 = 1
 NOALLOC_SCRATCH_BYTES = 32 * 1024 * 1024  # FNA2_NOALLOC_SCRATCH_BYTES
@@ -161,6 +162,59 @@ class Fna2GemmArgs(ctypes.Structure):
     ]
 
 
+class Fna2PagedKV(ctypes.Structure):
+    _fields_ = [
+        ("num_pages", ctypes.c_int32), ("page_size", ctypes.c_int32), ("kv_heads", ctypes.c_int32),
+        ("graph_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32), ("rank", ctypes.c_int32),
+        ("k", ctypes.c_void_p), ("k_page_stride", _I64), ("k_token_stride", _I64), ("k_head_stride", _I64),
+        ("v", ctypes.c_void_p), ("v_page_stride", _I64), ("v_token_stride", _I64), ("v_head_stride", _I64),
+        ("rk", ctypes.c_void_p), ("rk_page_stride", _I64), ("rk_token_stride", _I64), ("rk_head_stride", _I64),
+    ]
+
+
+class Fna2AppendArgs(ctypes.Structure):
+    _fields_ = [
+        ("batch", ctypes.c_int32), ("heads", ctypes.c_int32), ("max_pages", ctypes.c_int32),
+        ("in_dtype", ctypes.c_int32), ("weight_dtype", ctypes.c_int32), ("rope_dtype", ctypes.c_int32),
+        ("total_tokens", _I64),
+        ("q", Fna2Rows), ("k", Fna2Rows), ("v", Fna2Rows), ("r_k", Fna2Rows), ("q_out", Fna2Rows),
+        ("page_table", ctypes.c_void_p), ("table_stride", _I64),
+        ("cache_seqlens", ctypes.c_void_p), ("cu_seqlens", ctypes.c_void_p), ("positions", ctypes.c_void_p),
+        ("q_weight", ctypes.c_void_p), ("k_weight", ctypes.c_void_p),
+        ("eps", ctypes.c_float), ("inv_freq", ctypes.c_void_p),
+    ]
+
+
+class Fna2PagedAttnArgs(ctypes.Structure):
+    _fields_ = [
+        ("batch", ctypes.c_int32), ("heads", ctypes.c_int32), ("total_q", ctypes.c_int32),
+        ("max_seqlen_q", ctypes.c_int32), ("max_seqlen_k", ctypes.c_int32),
+        ("max_pages", ctypes.c_int32), ("causal", ctypes.c_int32), ("num_splits", ctypes.c_int32),
+        ("softmax_scale", ctypes.c_float),
+        ("page_table", ctypes.c_void_p), ("table_stride", _I64),
+        ("cache_seqlens", ctypes.c_void_p), ("cu_seqlens_q", ctypes.c_void_p),
+        ("q", ctypes.c_void_p), ("q_token_stride", _I64), ("q_head_stride", _I64),
+        ("r_q", ctypes.c_void_p), ("rq_token_stride", _I64), ("rq_head_stride", _I64),
+        ("graph_scale", ctypes.c_void_p),
+        ("out", ctypes.c_void_p), ("out_token_stride", _I64), ("out_head_stride", _I64),
+        ("lse", ctypes.c_void_p), ("lse_head_stride", _I64),
+        ("key_weights", ctypes.c_void_p), ("kw_batch_stride", _I64), ("kw_head_stride", _I64),
+    ]
+
+
+class Fna2EvictArgs(ctypes.Structure):
+    _fields_ = [
+        ("batch", ctypes.c_int32), ("heads", ctypes.c_int32), ("max_seqlen_k", ctypes.c_int32),
+        ("max_pages", ctypes.c_int32), ("max_pages_out", ctypes.c_int32),
+        ("budget", ctypes.c_int32), ("sink", ctypes.c_int32), ("recent", ctypes.c_int32),
+        ("page_table", ctypes.c_void_p), ("table_stride", _I64),
+        ("page_table_out", ctypes.c_void_p), ("table_out_stride", _I64),
+        ("cache_seqlens", ctypes.c_void_p),
+        ("key_weights", ctypes.c_void_p), ("kw_batch_stride", _I64), ("kw_head_stride", _I64),
+        ("kept", ctypes.c_void_p), ("seqlens_out", ctypes.c_void_p), ("weights_out", ctypes.c_void_p),
+    ]
+
+
 _lib: Optional[ctypes.CDLL] = None
 
 
@@ -200,6 +254,18 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
     lib.fna2_debug_watchdog.restype = ctypes.c_int
     lib.fna2_gemm.argtypes = [ctypes.POINTER(Fna2GemmArgs), ctypes.c_void_p]
     lib.fna2_gemm.restype = ctypes.c_int
+    kv = ctypes.POINTER(Fna2PagedKV)
+    lib.fna2_paged_append.argtypes = [kv, ctypes.POINTER(Fna2AppendArgs), ctypes.c_void_p]
+    lib.fna2_paged_append.restype = ctypes.c_int
+    for name in ("fna2_paged_attn", "fna2_key_weights"):
+        f = getattr(lib, name)
+        f.argtypes = [kv, ctypes.POINTER(Fna2PagedAttnArgs), ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]
+        f.restype = ctypes.c_int
+        f = getattr(lib, name + "_workspace_size")
+        f.argtypes = [kv, ctypes.POINTER(Fna2PagedAttnArgs)]
+        f.restype = ctypes.c_size_t
+    lib.fna2_evict.argtypes = [kv, ctypes.POINTER(Fna2EvictArgs), ctypes.c_void_p]
+    lib.fna2_evict.restype = ctypes.c_int
     lib.fna2_abi_version.argtypes = []
     lib.fna2_abi_version.restype = ctypes.c_int
     v = lib.fna2_abi_version()

@@ -21,6 +21,10 @@
 #include "fna2_gemm.cu"
 #include "fna2_qkprep.cu"
 #include "fna2_decode.cu"
+#include "fna2_append.cu"
+#include "fna2_paged.cu"
+#include "fna2_keyweights.cu"
+#include "fna2_evict.cu"
 
 namespace fna2 {
 namespace {
@@ -662,5 +666,276 @@ extern "C" int fna2_decode(const Fna2DecodeArgs* a, void* workspace, size_t work
     p.ws = static_cast<float*>(workspace);
   }
   FNA2_CUDA(launch_decode(p, D, smem, static_cast<cudaStream_t>(stream)));
+  return FNA2_OK;
+}
+
+// ---------------------------------------------------------------------------
+// paged cache
+// ---------------------------------------------------------------------------
+namespace {
+
+bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+bool strides_ok(std::initializer_list<int64_t> v, int64_t vec = 8) {
+  for (int64_t x : v)
+    if (x < 0 || x % vec) return false;
+  return true;
+}
+
+// Checks of the pool and the page table, shared by every paged entry point.
+int paged_pool(const Fna2PagedKV* kv, int heads, const int32_t* table, int64_t table_stride, int max_pages,
+               PagedPool* d) {
+  FNA2_CHECK(kv != nullptr, "null pool");
+  FNA2_CHECK(kv->head_dim == 64 || kv->head_dim == 128, "head_dim must be 64 or 128 (got %d)", kv->head_dim);
+  FNA2_CHECK(kv->page_size >= 16 && kv->page_size <= 1024 && (kv->page_size & (kv->page_size - 1)) == 0,
+             "page_size must be a power of two from 16 to 1024 (got %d)", kv->page_size);
+  FNA2_CHECK(kv->num_pages >= 0 && kv->kv_heads > 0, "bad pool sizes");
+  FNA2_CHECK(heads > 0 && heads % kv->kv_heads == 0, "heads (%d) must be a positive multiple of kv_heads (%d)", heads,
+             kv->kv_heads);
+  FNA2_CHECK(heads <= 65535, "heads must be <= 65535");
+  FNA2_CHECK(kv->graph_heads >= 0 && kv->graph_heads <= heads, "graph_heads must be in [0, heads]");
+  if (kv->graph_heads > 0)
+    FNA2_CHECK(kv->rank > 0 && kv->rank <= 32 && kv->rank % 8 == 0, "rank must be 8, 16, 24 or 32 (got %d)", kv->rank);
+  FNA2_CHECK(kv->k && kv->v && (kv->rk || kv->graph_heads == 0), "null pool tensor");
+  FNA2_CHECK(aligned16(kv->k) && aligned16(kv->v) && aligned16(kv->rk), "pool tensors must be 16-byte aligned");
+  FNA2_CHECK(strides_ok({kv->k_page_stride, kv->k_token_stride, kv->k_head_stride, kv->v_page_stride,
+                         kv->v_token_stride, kv->v_head_stride}) &&
+                 (kv->graph_heads == 0 || strides_ok({kv->rk_page_stride, kv->rk_token_stride, kv->rk_head_stride})),
+             "pool strides must be non-negative multiples of 8 elements");
+  FNA2_CHECK(table != nullptr && max_pages >= 0 && table_stride >= max_pages, "bad page table");
+  FNA2_CHECK(static_cast<int64_t>(max_pages) * kv->page_size < (1ll << 31), "a sequence's pages hold 2^31 keys or more");
+  using bf = __nv_bfloat16;
+  d->pages = kv->num_pages;
+  d->page_log2 = 0;
+  while ((1 << d->page_log2) < kv->page_size) ++d->page_log2;
+  d->hkv = kv->kv_heads;
+  d->hg = kv->graph_heads;
+  d->rank = kv->graph_heads > 0 ? kv->rank : 16;
+  d->k = {static_cast<bf*>(kv->k), kv->k_page_stride, kv->k_token_stride, kv->k_head_stride};
+  d->v = {static_cast<bf*>(kv->v), kv->v_page_stride, kv->v_token_stride, kv->v_head_stride};
+  d->rk = {static_cast<bf*>(kv->rk), kv->rk_page_stride, kv->rk_token_stride, kv->rk_head_stride};
+  d->table = table;
+  d->table_sb = table_stride;
+  d->max_pages = max_pages;
+  return FNA2_OK;
+}
+
+// Checks shared by the attention and the key weights; *p gets the common parameters.
+template <class P>
+int paged_queries(const Fna2PagedKV* kv, const Fna2PagedAttnArgs* a, P* p) {
+  FNA2_CHECK(a != nullptr, "null arguments");
+  if (int rc = paged_pool(kv, a->heads, a->page_table, a->table_stride, a->max_pages, &p->kv)) return rc;
+  FNA2_CHECK(a->batch >= 0 && a->batch <= 65535 && a->total_q >= 0, "bad sizes (batch 0 to 65535)");
+  FNA2_CHECK(a->max_seqlen_q >= 0 && a->max_seqlen_k >= 0, "negative length bound");
+  FNA2_CHECK(a->max_seqlen_k <= static_cast<int64_t>(a->max_pages) * kv->page_size,
+             "max_seqlen_k (%d) is above what a page table row holds", a->max_seqlen_k);
+  FNA2_CHECK(a->softmax_scale > 0.f, "softmax_scale must be positive");
+  FNA2_CHECK(a->cache_seqlens && a->cu_seqlens_q, "null sequence tensor");
+  FNA2_CHECK(a->q != nullptr || a->total_q == 0, "null tensor pointer: q");
+  FNA2_CHECK(aligned16(a->q) && strides_ok({a->q_token_stride, a->q_head_stride}),
+             "q must be 16-byte aligned with strides of multiples of 8 elements");
+  if (kv->graph_heads > 0 && a->total_q > 0) {
+    FNA2_CHECK(a->r_q && a->graph_scale, "graph heads need r_q and graph_scale");
+    FNA2_CHECK(aligned16(a->r_q) && strides_ok({a->rq_token_stride, a->rq_head_stride}),
+               "r_q must be 16-byte aligned with strides of multiples of 8 elements");
+  }
+  FNA2_CHECK(!a->lse || a->lse_head_stride >= 0, "negative lse stride");
+  FNA2_CHECK(!a->key_weights || (a->kw_batch_stride >= 0 && a->kw_head_stride >= 0), "negative key_weights stride");
+  using bf = __nv_bfloat16;
+  p->bd = {a->batch, a->total_q, std::min(a->max_seqlen_q, a->total_q), a->max_seqlen_k, a->cu_seqlens_q,
+           a->cache_seqlens};
+  p->H = a->heads;
+  p->G = a->heads / kv->kv_heads;
+  p->RP = p->kv.rank <= 16 ? 16 : 32;
+  p->causal = a->causal ? 1 : 0;
+  p->scale = a->softmax_scale;
+  p->scale_log2 = a->softmax_scale * kLog2e;
+  p->q = static_cast<const bf*>(a->q), p->q_st = a->q_token_stride, p->q_sh = a->q_head_stride;
+  p->rq = static_cast<const bf*>(a->r_q), p->rq_st = a->rq_token_stride, p->rq_sh = a->rq_head_stride;
+  p->gs = a->graph_scale;
+  p->kw = a->key_weights, p->kw_sb = a->kw_batch_stride, p->kw_sh = a->kw_head_stride;
+  return FNA2_OK;
+}
+
+// Split, tile and workspace choices of one attention call.
+struct PagedPlan {
+  int RW;
+  bool logits;  // key weights from kept logits (few rows); otherwise recomputed by the key weights kernel
+  size_t smem, acc_bytes, ml_bytes, logit_bytes, lse_bytes, total;
+};
+
+size_t up256(size_t x) { return (x + 255) / 256 * 256; }
+
+int paged_plan(const Fna2PagedKV* kv, const Fna2PagedAttnArgs* a, PagedAttnParams* p, PagedPlan* l) {
+  const int D = kv->head_dim, max_rows = std::max(1, p->bd.max_q * p->G);
+  l->RW = max_rows <= 16 ? 1 : max_rows <= 32 ? 2 : 4;
+  for (;; l->RW /= 2) {
+    p->ng_max = std::min({p->G, 16 * l->RW, p->kv.hg});
+    p->nh_max = std::min({p->G, 16, p->kv.hg});
+    const FewSmem L(D, p->ng_max, p->nh_max, p->RP);
+    p->stages = 4;
+    while (p->stages > 2 && L.total(l->RW, p->stages) > 100 * 1024) --p->stages;
+    l->smem = std::max<size_t>(L.total(l->RW, p->stages), 512 + 64 * D * 4);
+    if (l->smem <= kMaxDynamicSmem || l->RW == 1) break;
+  }
+  FNA2_CHECK(l->smem <= kMaxDynamicSmem, "heads per KV head and rank need too much shared memory");
+  const int64_t row_blocks = (static_cast<int64_t>(max_rows) + 16 * l->RW - 1) / (16 * l->RW);
+  const int64_t ctas = static_cast<int64_t>(p->bd.B) * p->kv.hkv * row_blocks;
+  FNA2_CHECK(ctas < (1ll << 31), "too many query rows");
+  p->row_blocks = static_cast<int>(row_blocks);
+  int64_t splits = a->num_splits;
+  if (splits <= 0) {  // about two waves of two CTAs per SM, at least 256 keys a split
+    splits = std::max<int64_t>(1, std::min<int64_t>((4 * 148 + ctas - 1) / std::max<int64_t>(ctas, 1),
+                                                    (p->bd.max_k + 255) / 256));
+  }
+  splits = std::min<int64_t>(splits, 4096);
+  const int64_t chunk = (std::max(1, p->bd.max_k) + splits - 1) / splits;
+  p->chunk = static_cast<int>((chunk + 63) / 64 * 64);
+  p->ns = std::max(1, (p->bd.max_k + p->chunk - 1) / p->chunk);
+  const size_t th = static_cast<size_t>(p->bd.T) * p->H;
+  p->logit_sr = (static_cast<int64_t>(p->bd.max_k) + 15) / 16 * 16;
+  l->acc_bytes = p->ns > 1 ? up256(th * p->ns * D * 4) : 0;
+  l->logits = p->kw && max_rows <= 64;
+  l->ml_bytes = p->ns > 1 || l->logits ? up256(th * p->ns * 8) : 0;
+  l->logit_bytes = l->logits ? up256(static_cast<size_t>(p->bd.B) * p->kv.hkv * max_rows * p->logit_sr * 4) : 0;
+  l->lse_bytes = p->kw && !l->logits && !a->lse ? up256(th * 4) : 0;
+  l->total = l->acc_bytes + l->ml_bytes + l->logit_bytes + l->lse_bytes;
+  return FNA2_OK;
+}
+
+}  // namespace
+
+extern "C" int fna2_paged_append(const Fna2PagedKV* kv, const Fna2AppendArgs* a, void* stream) {
+  g_last_error.clear();
+  FNA2_CHECK(a != nullptr, "null arguments");
+  AppendParams p{};
+  if (int rc = paged_pool(kv, a->heads, a->page_table, a->table_stride, a->max_pages, &p.kv)) return rc;
+  FNA2_CHECK(a->batch >= 0 && a->total_tokens >= 0 && a->total_tokens < (1ll << 31), "bad sizes");
+  FNA2_CHECK(a->in_dtype == FNA2_DTYPE_F32 || a->in_dtype == FNA2_DTYPE_BF16, "bad in_dtype %d", a->in_dtype);
+  FNA2_CHECK(a->weight_dtype == FNA2_DTYPE_F32 || a->weight_dtype == FNA2_DTYPE_BF16, "bad weight_dtype %d",
+             a->weight_dtype);
+  FNA2_CHECK(a->rope_dtype == FNA2_DTYPE_F32 || a->rope_dtype == FNA2_DTYPE_BF16, "bad rope_dtype %d", a->rope_dtype);
+  FNA2_CHECK((a->q_weight == nullptr) == (a->k_weight == nullptr), "set both RMSNorm weights or neither");
+  FNA2_CHECK(aligned16(a->q_weight) && aligned16(a->k_weight), "RMSNorm weights must be 16-byte aligned");
+  FNA2_CHECK(a->eps >= 0.f, "eps must be >= 0");
+  FNA2_CHECK(a->cache_seqlens && a->cu_seqlens, "null sequence tensor");
+  if (a->batch == 0 || a->total_tokens == 0) return FNA2_OK;
+  const int eb = a->in_dtype == FNA2_DTYPE_BF16 ? 2 : 4;
+  if (int rc = check_rows(a->q, a->heads, eb, kv->head_dim, "q")) return rc;
+  if (int rc = check_rows(a->k, kv->kv_heads, eb, kv->head_dim, "k")) return rc;
+  if (int rc = check_rows(a->v, kv->kv_heads, eb, kv->head_dim, "v")) return rc;
+  if (int rc = check_rows(a->r_k, kv->graph_heads, eb, kv->rank, "r_k")) return rc;
+  if (int rc = check_rows(a->q_out, a->heads, 2, kv->head_dim, "q_out")) return rc;
+  p.T = static_cast<int>(a->total_tokens);
+  p.B = a->batch;
+  p.H = a->heads;
+  p.w_bf16 = a->weight_dtype == FNA2_DTYPE_BF16;
+  p.rope_bf16 = a->rope_dtype == FNA2_DTYPE_BF16;
+  p.q = {a->q.ptr, a->q.token_stride, a->q.head_stride};
+  p.k = {a->k.ptr, a->k.token_stride, a->k.head_stride};
+  p.v = {a->v.ptr, a->v.token_stride, a->v.head_stride};
+  p.rk = {a->r_k.ptr, a->r_k.token_stride, a->r_k.head_stride};
+  p.qo = static_cast<__nv_bfloat16*>(a->q_out.ptr), p.qo_ts = a->q_out.token_stride, p.qo_hs = a->q_out.head_stride;
+  p.cu = a->cu_seqlens;
+  p.lens = a->cache_seqlens;
+  p.positions = a->positions;
+  p.qw = a->q_weight;
+  p.kw = a->k_weight;
+  p.eps = a->eps;
+  p.inv_freq = a->inv_freq;
+  FNA2_CUDA(launch_append(p, kv->head_dim, eb, static_cast<cudaStream_t>(stream)));
+  return FNA2_OK;
+}
+
+extern "C" size_t fna2_paged_attn_workspace_size(const Fna2PagedKV* kv, const Fna2PagedAttnArgs* a) {
+  g_last_error.clear();
+  PagedAttnParams p{};
+  PagedPlan l;
+  if (paged_queries(kv, a, &p) || paged_plan(kv, a, &p, &l)) return 0;
+  return l.total;
+}
+
+extern "C" int fna2_paged_attn(const Fna2PagedKV* kv, const Fna2PagedAttnArgs* a, void* workspace,
+                               size_t workspace_bytes, void* stream) {
+  g_last_error.clear();
+  PagedAttnParams p{};
+  PagedPlan l;
+  if (int rc = paged_queries(kv, a, &p)) return rc;
+  if (int rc = paged_plan(kv, a, &p, &l)) return rc;
+  if (p.bd.B == 0 || p.bd.T == 0) return FNA2_OK;
+  FNA2_CHECK(a->out != nullptr && aligned16(a->out) && strides_ok({a->out_token_stride, a->out_head_stride}),
+             "out must be 16-byte aligned with strides of multiples of 8 elements");
+  if (l.total > 0) {
+    if (workspace == nullptr || workspace_bytes < l.total)
+      return fail(FNA2_ERR_WORKSPACE, "paged attention workspace: need %zu bytes, got %zu", l.total, workspace_bytes);
+    FNA2_CHECK((reinterpret_cast<uintptr_t>(workspace) & 255u) == 0, "workspace must be 256-byte aligned");
+  }
+  p.out = static_cast<__nv_bfloat16*>(a->out), p.o_st = a->out_token_stride, p.o_sh = a->out_head_stride;
+  p.lse = a->lse, p.lse_sh = a->lse_head_stride;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  p.ws_acc = l.acc_bytes ? reinterpret_cast<float*>(ws) : nullptr;
+  p.ws_ml = l.ml_bytes ? reinterpret_cast<float2*>(ws + l.acc_bytes) : nullptr;
+  p.logits = l.logits ? reinterpret_cast<float*>(ws + l.acc_bytes + l.ml_bytes) : nullptr;
+  if (l.lse_bytes) p.lse = reinterpret_cast<float*>(ws + l.acc_bytes + l.ml_bytes + l.logit_bytes), p.lse_sh = p.bd.T;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  FNA2_CUDA(kv->head_dim == 128 ? launch_paged_t<128>(p, l.RW, l.smem, st) : launch_paged_t<64>(p, l.RW, l.smem, st));
+  if (p.kw && !l.logits && p.bd.max_k > 0) {
+    KeyWeightsParams w{};
+    if (int rc = paged_queries(kv, a, &w)) return rc;
+    w.lse = p.lse, w.lse_sh = p.lse_sh;
+    FNA2_CUDA(launch_key_weights(w, kv->head_dim, st));
+  }
+  return FNA2_OK;
+}
+
+extern "C" size_t fna2_key_weights_workspace_size(const Fna2PagedKV* kv, const Fna2PagedAttnArgs* a) {
+  g_last_error.clear();
+  KeyWeightsParams p{};
+  if (paged_queries(kv, a, &p)) return 0;
+  return 0;
+}
+
+extern "C" int fna2_key_weights(const Fna2PagedKV* kv, const Fna2PagedAttnArgs* a, void* workspace,
+                                size_t workspace_bytes, void* stream) {
+  g_last_error.clear();
+  (void)workspace, (void)workspace_bytes;
+  KeyWeightsParams p{};
+  if (int rc = paged_queries(kv, a, &p)) return rc;
+  FNA2_CHECK(a->key_weights != nullptr && (a->lse != nullptr || a->total_q == 0), "key weights need lse and key_weights");
+  FNA2_CHECK(key_weights_smem(kv->head_dim, std::min(p.G, p.kv.hg), p.RP) <= kMaxDynamicSmem,
+             "heads per KV head and rank need too much shared memory");
+  if (p.bd.B == 0 || p.bd.T == 0 || p.bd.max_k == 0) return FNA2_OK;
+  p.lse = a->lse, p.lse_sh = a->lse_head_stride;
+  FNA2_CUDA(launch_key_weights(p, kv->head_dim, static_cast<cudaStream_t>(stream)));
+  return FNA2_OK;
+}
+
+extern "C" int fna2_evict(const Fna2PagedKV* kv, const Fna2EvictArgs* a, void* stream) {
+  g_last_error.clear();
+  FNA2_CHECK(a != nullptr, "null arguments");
+  EvictParams p{};
+  if (int rc = paged_pool(kv, a->heads, a->page_table, a->table_stride, a->max_pages, &p.kv)) return rc;
+  FNA2_CHECK(a->batch >= 0 && a->batch <= 65535, "bad batch");
+  FNA2_CHECK(a->max_seqlen_k >= 0 && a->max_seqlen_k <= static_cast<int64_t>(a->max_pages) * kv->page_size,
+             "max_seqlen_k (%d) is above what a page table row holds", a->max_seqlen_k);
+  FNA2_CHECK(a->page_table_out != nullptr && a->max_pages_out >= 0 && a->table_out_stride >= a->max_pages_out,
+             "bad output page table");
+  FNA2_CHECK(a->budget >= 1 && a->sink >= 0 && a->recent >= 0 && static_cast<int64_t>(a->sink) + a->recent <= a->budget,
+             "budget (%d) must be >= 1 and hold sink (%d) + recent (%d)", a->budget, a->sink, a->recent);
+  FNA2_CHECK(a->budget <= static_cast<int64_t>(a->max_pages_out) * kv->page_size &&
+                 static_cast<int64_t>(a->max_pages_out) * kv->page_size < (1ll << 31),
+             "the output page table holds fewer than budget (%d) keys", a->budget);
+  FNA2_CHECK(a->cache_seqlens && a->key_weights && a->kept && a->seqlens_out && a->weights_out, "null tensor pointer");
+  FNA2_CHECK(a->kw_batch_stride >= 0 && a->kw_head_stride >= 0, "negative key_weights stride");
+  if (a->batch == 0) return FNA2_OK;
+  p.lens = a->cache_seqlens;
+  p.B = a->batch;
+  p.G = a->heads / kv->kv_heads;
+  p.max_k = a->max_seqlen_k;
+  p.budget = a->budget, p.sink = a->sink, p.recent = a->recent;
+  p.w = a->key_weights, p.w_sb = a->kw_batch_stride, p.w_sh = a->kw_head_stride;
+  p.table_out = a->page_table_out, p.table_out_sb = a->table_out_stride;
+  p.cap_out = a->max_pages_out * kv->page_size;
+  p.kept = a->kept, p.lens_out = a->seqlens_out, p.w_out = a->weights_out;
+  FNA2_CUDA(launch_evict(p, kv->head_dim, static_cast<cudaStream_t>(stream)));
   return FNA2_OK;
 }

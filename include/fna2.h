@@ -50,7 +50,7 @@
 extern "C" {
 #endif
 
-#define FNA2_ABI_VERSION 5
+#define FNA2_ABI_VERSION 6
 
 #define FNA2_OK 0
 #define FNA2_ERR_INVALID (-1)
@@ -245,6 +245,109 @@ size_t fna2_decode_workspace_size(const Fna2DecodeArgs* args);
 
 int fna2_decode(const Fna2DecodeArgs* args, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * Paged cache: K, V and R_k of many sequences in pages of one pool.  No
+ * counterpart in the reference, whose cache is a growing concatenation without
+ * R_k (attention_fna2.py:428-432).
+ *
+ * A pool is three tensors [num_pages, page_size, heads, columns] (k, v:
+ * kv_heads x head_dim; rk: graph_heads x rank), bf16, column stride 1, bases
+ * and the other strides 16-byte aligned; page_size is a power of two, 16 to
+ * 1024.  Key j of sequence b is slot j % page_size of page
+ * page_table[b * table_stride + j / page_size].  Entries past a sequence's
+ * length are not read, and what a page holds past it is never used.
+ * page_table, cache_seqlens and cu_seqlens are int32 on the device and are not
+ * read on the host.  A sequence whose device-side values break the bounds given
+ * in the arguments is skipped before any access and a status is recorded
+ * (fna2_device_status: 631 append, 641 attention and key weights, 651 eviction).
+ * --------------------------------------------------------------------------- */
+typedef struct Fna2PagedKV {
+  int32_t num_pages, page_size, kv_heads, graph_heads, head_dim, rank;
+  void* k;  int64_t k_page_stride, k_token_stride, k_head_stride;
+  void* v;  int64_t v_page_stride, v_token_stride, v_head_stride;
+  void* rk; int64_t rk_page_stride, rk_token_stride, rk_head_stride; /* NULL when graph_heads == 0 */
+} Fna2PagedKV;
+
+/* New tokens into the cache: the QK-RMSNorm + RoPE of fna2_qk_prep_fwd (same
+ * arithmetic and roundings) at each sequence's own position, q to q_out and k,
+ * v, r_k as bf16 into slots cache_seqlens[b] + i of their sequences' pages.
+ * q, k, v, r_k are rows [T, heads, columns] of one type (in_dtype).  Token i of
+ * sequence b = packed token cu_seqlens[b] + i; its position is positions[b] + i
+ * (positions NULL: cache_seqlens[b] + i).  The caller advances cache_seqlens.
+ * Tokens outside [cu[0], cu[batch]) are not written. */
+typedef struct Fna2AppendArgs {
+  int32_t batch, heads, max_pages;
+  int32_t in_dtype, weight_dtype, rope_dtype;  /* FNA2_DTYPE_*, as in Fna2QkPrepArgs */
+  int64_t total_tokens;
+  Fna2Rows q, k, v, r_k;
+  Fna2Rows q_out;               /* bf16 */
+  const int32_t* page_table;  int64_t table_stride;
+  const int32_t* cache_seqlens; /* [batch] slots in use before the call */
+  const int32_t* cu_seqlens;    /* [batch + 1] */
+  const int32_t* positions;     /* [batch] or NULL */
+  const void* q_weight;         /* [head_dim] RMSNorm weights, or both NULL: no norm */
+  const void* k_weight;
+  float eps;
+  const float* inv_freq;        /* [head_dim / 2] fp32, or NULL: no RoPE */
+} Fna2AppendArgs;
+int fna2_paged_append(const Fna2PagedKV* kv, const Fna2AppendArgs* args, void* stream);
+
+/* Attention of each sequence's new tokens over its cached keys (the new tokens'
+ * own keys, already appended, are the last of them): the last query rows of the
+ * prefill op.  New token i of n sees key j iff j < cache_seqlens[b] and, when
+ * causal, j <= cache_seqlens[b] - n + i.  A row that sees no key gets out 0 and
+ * lse -inf.  out is bf16, lse (optional) fp32 [H][lse_head_stride].  With
+ * key_weights, the attention weight that each key received,
+ * sum over the new tokens and the query heads of the KV head of
+ * exp(S - LSE), is added to key_weights[b][kv_head][key]. */
+typedef struct Fna2PagedAttnArgs {
+  int32_t batch, heads, total_q;     /* sequences, H, packed new tokens */
+  int32_t max_seqlen_q, max_seqlen_k; /* bounds on every sequence's new tokens and cached keys */
+  int32_t max_pages, causal;
+  int32_t num_splits;                /* splits of a sequence's keys; 0 = chosen by the library */
+  float softmax_scale;
+  const int32_t* page_table;  int64_t table_stride;
+  const int32_t* cache_seqlens;      /* [batch] cached keys, the new tokens' included */
+  const int32_t* cu_seqlens_q;       /* [batch + 1] */
+  const void* q;    int64_t q_token_stride, q_head_stride;    /* [T, H, D] */
+  const void* r_q;  int64_t rq_token_stride, rq_head_stride;  /* [T, H_G, R] */
+  const float* graph_scale;          /* [H_G] */
+  void* out;        int64_t out_token_stride, out_head_stride;
+  float* lse;       int64_t lse_head_stride;                  /* or NULL */
+  float* key_weights; int64_t kw_batch_stride, kw_head_stride; /* or NULL */
+} Fna2PagedAttnArgs;
+size_t fna2_paged_attn_workspace_size(const Fna2PagedKV* kv, const Fna2PagedAttnArgs* args);
+int fna2_paged_attn(const Fna2PagedKV* kv, const Fna2PagedAttnArgs* args, void* workspace, size_t workspace_bytes,
+                    void* stream);
+
+/* The key weights alone, from queries and their LSE (args->lse is an input;
+ * out and num_splits are unused): e.g. the last tokens of a prompt voting on its
+ * keys.  Adds to key_weights. */
+size_t fna2_key_weights_workspace_size(const Fna2PagedKV* kv, const Fna2PagedAttnArgs* args);
+int fna2_key_weights(const Fna2PagedKV* kv, const Fna2PagedAttnArgs* args, void* workspace, size_t workspace_bytes,
+                     void* stream);
+
+/* Eviction: per sequence and KV head keep min(len, budget) keys: the first
+ * `sink`, the last `recent`, and of the others those of the largest key weight
+ * (ties to the lowest index, NaN below every number).  Their rows of K, V and of
+ * the KV head's query heads' R_k are copied in order to slots [0, kept) of the
+ * pages in page_table_out, which must not be pages of page_table's sequences.
+ * kept [batch][kv_heads][budget] gets the indices (-1 past the count), seqlens_out
+ * [batch] the counts, weights_out [batch][kv_heads][max_pages_out * page_size]
+ * the kept keys' weights (0 past the count). */
+typedef struct Fna2EvictArgs {
+  int32_t batch, heads, max_seqlen_k, max_pages, max_pages_out;
+  int32_t budget, sink, recent;      /* sink + recent <= budget */
+  const int32_t* page_table;     int64_t table_stride;
+  const int32_t* page_table_out; int64_t table_out_stride;
+  const int32_t* cache_seqlens;      /* [batch] */
+  const float* key_weights;      int64_t kw_batch_stride, kw_head_stride;
+  int32_t* kept;
+  int32_t* seqlens_out;
+  float* weights_out;
+} Fna2EvictArgs;
+int fna2_evict(const Fna2PagedKV* kv, const Fna2EvictArgs* args, void* stream);
+
 /* Message of the last failed call on this host thread ("" if none). */
 const char* fna2_last_error(void);
 
@@ -261,6 +364,12 @@ const char* fna2_last_error(void);
  *             (negative length, rows outside [0, total_q/total_k), or longer
  *             than max_seqlen_q/_k); the sequence is skipped, its out/lse rows
  *             are not written;
+ *   631       append: a sequence with inconsistent cache_seqlens / cu_seqlens or
+ *             a page id outside the pool (its tokens are not written);
+ *   641       paged attention, key weights: a sequence whose cu_seqlens or
+ *             cache_seqlens break the call's bounds (its rows are not written);
+ *   651       eviction: a length outside [0, max_seqlen_k], or a page id outside
+ *             the pool (the row is not copied);
  *   622       backward pre-pass, packed batch: the same check; the sequence
  *             gets no tiles and its gradient rows are not written.
  * Neither the reference nor this library checks cu_seqlens on the host (that
