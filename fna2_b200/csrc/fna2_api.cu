@@ -23,6 +23,7 @@
 #include "fna2_decode.cu"
 #include "fna2_append.cu"
 #include "fna2_paged.cu"
+#include "fna2_paged_many.cu"
 #include "fna2_keyweights.cu"
 #include "fna2_evict.cu"
 
@@ -759,15 +760,41 @@ int paged_queries(const Fna2PagedKV* kv, const Fna2PagedAttnArgs* a, P* p) {
 // Split, tile and workspace choices of one attention call.
 struct PagedPlan {
   int RW;
-  bool logits;  // key weights from kept logits (few rows); otherwise recomputed by the key weights kernel
+  bool few, many;  // kernels to launch
+  bool logits;     // key weights from kept logits (few rows everywhere); otherwise recomputed by the key weights kernel
   size_t smem, acc_bytes, ml_bytes, logit_bytes, lse_bytes, total;
 };
 
 size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 
+constexpr int kSms = 148;
+// Query rows per KV head (new tokens x query heads of the group) up to which a sequence is streamed
+// by the mma.sync kernel; above it the tensor-core kernel's 128-row tiles are worth filling.
+constexpr int kFewRows = 64;
+
+// Splits of the tensor-core kernel's keys: `base` CTAs without splits, `tiles` key tiles each.  One
+// CTA runs per SM; a tile takes about 2 us, a CTA's start and end 6 us, and the join moves 8 D bytes
+// per row and split.  Takes the count with the least estimated time.
+int many_splits(int64_t base, int64_t tiles, double row_bytes) {
+  int best = 1;
+  double best_us = 1e30;
+  for (int s = 1; s <= 32 && s <= std::max<int64_t>(1, tiles / 2); ++s) {
+    const double waves = static_cast<double>((base * s + kSms - 1) / kSms);
+    const double us = waves * (static_cast<double>((tiles + s - 1) / s) * 2.0 + 6.0) + (s > 1 ? 4.0 + s * row_bytes / 5e6 : 0.0);
+    if (us < best_us * 0.98) best_us = us, best = s;
+  }
+  return best;
+}
+
 int paged_plan(const Fna2PagedKV* kv, const Fna2PagedAttnArgs* a, PagedAttnParams* p, PagedPlan* l) {
   const int D = kv->head_dim, max_rows = std::max(1, p->bd.max_q * p->G);
-  l->RW = max_rows <= 16 ? 1 : max_rows <= 32 ? 2 : 4;
+  const bool all_few = max_rows <= kFewRows;
+  l->few = all_few || p->bd.B > 1;
+  l->many = !all_few;
+  p->few_rows = all_few ? max_rows : l->few ? kFewRows : 0;
+  // few rows: the row blocks of a CTA; in a mixed call most of these sequences add one token
+  const int few_max = std::min(max_rows, kFewRows);
+  l->RW = !all_few || max_rows <= 16 ? 1 : max_rows <= 32 ? 2 : 4;
   for (;; l->RW /= 2) {
     p->ng_max = std::min({p->G, 16 * l->RW, p->kv.hg});
     p->nh_max = std::min({p->G, 16, p->kv.hg});
@@ -778,27 +805,60 @@ int paged_plan(const Fna2PagedKV* kv, const Fna2PagedAttnArgs* a, PagedAttnParam
     if (l->smem <= kMaxDynamicSmem || l->RW == 1) break;
   }
   FNA2_CHECK(l->smem <= kMaxDynamicSmem, "heads per KV head and rank need too much shared memory");
-  const int64_t row_blocks = (static_cast<int64_t>(max_rows) + 16 * l->RW - 1) / (16 * l->RW);
-  const int64_t ctas = static_cast<int64_t>(p->bd.B) * p->kv.hkv * row_blocks;
-  FNA2_CHECK(ctas < (1ll << 31), "too many query rows");
-  p->row_blocks = static_cast<int>(row_blocks);
+  p->row_blocks = (few_max + 16 * l->RW - 1) / (16 * l->RW);
+  const int64_t ctas = static_cast<int64_t>(p->bd.B) * p->kv.hkv * (all_few ? p->row_blocks : 1);
+  FNA2_CHECK(static_cast<int64_t>(p->bd.B) * p->kv.hkv * p->row_blocks < (1ll << 31), "too many query rows");
+  const int64_t max_k = std::max(1, p->bd.max_k);
   int64_t splits = a->num_splits;
-  if (splits <= 0) {  // about two waves of two CTAs per SM, at least 256 keys a split
-    splits = std::max<int64_t>(1, std::min<int64_t>((4 * 148 + ctas - 1) / std::max<int64_t>(ctas, 1),
-                                                    (p->bd.max_k + 255) / 256));
-  }
+  if (splits <= 0)  // about two waves of two CTAs per SM, at least 256 keys a split
+    splits = std::max<int64_t>(1, std::min<int64_t>((4 * kSms + ctas - 1) / std::max<int64_t>(ctas, 1), (max_k + 255) / 256));
   splits = std::min<int64_t>(splits, 4096);
-  const int64_t chunk = (std::max(1, p->bd.max_k) + splits - 1) / splits;
-  p->chunk = static_cast<int>((chunk + 63) / 64 * 64);
-  p->ns = std::max(1, (p->bd.max_k + p->chunk - 1) / p->chunk);
+  p->chunk = static_cast<int>(((max_k + splits - 1) / splits + 63) / 64 * 64);
+  p->ns = l->few ? static_cast<int>((max_k + p->chunk - 1) / p->chunk) : 1;
+  if (l->many) {
+    // pairs of query tiles: at least `pairs`, at most one more per sequence that has more than few_rows rows
+    const int64_t pairs = (static_cast<int64_t>(p->bd.T) + 2 * kBlockM - 1) / (2 * kBlockM);
+    const int64_t longer = std::min<int64_t>(p->bd.B, static_cast<int64_t>(p->bd.T) * p->G / (p->few_rows + 1));
+    const int64_t tiles = (max_k + kBlockN - 1) / kBlockN;
+    const int64_t s = a->num_splits > 0 ? std::min<int64_t>(a->num_splits, tiles)
+                                        : many_splits(pairs * p->H, tiles, static_cast<double>(p->bd.T) * p->H * D * 8);
+    p->chunk_many = static_cast<int>((tiles + s - 1) / s) * kBlockN;
+    const int64_t ns = (max_k + p->chunk_many - 1) / p->chunk_many;
+    FNA2_CHECK((pairs + longer) * ns <= 65535, "too many query tiles and splits (%lld)", (long long)((pairs + longer) * ns));
+    p->many_items = static_cast<int>((pairs + longer) * ns);
+    p->ns = std::max(p->ns, static_cast<int>(ns));
+  }
   const size_t th = static_cast<size_t>(p->bd.T) * p->H;
   p->logit_sr = (static_cast<int64_t>(p->bd.max_k) + 15) / 16 * 16;
+  l->logits = p->kw && all_few;
   l->acc_bytes = p->ns > 1 ? up256(th * p->ns * D * 4) : 0;
-  l->logits = p->kw && max_rows <= 64;
   l->ml_bytes = p->ns > 1 || l->logits ? up256(th * p->ns * 8) : 0;
   l->logit_bytes = l->logits ? up256(static_cast<size_t>(p->bd.B) * p->kv.hkv * max_rows * p->logit_sr * 4) : 0;
   l->lse_bytes = p->kw && !l->logits && !a->lse ? up256(th * 4) : 0;
   l->total = l->acc_bytes + l->ml_bytes + l->logit_bytes + l->lse_bytes;
+  return FNA2_OK;
+}
+
+// Tensor maps over (column, slot, head, page): boxes of at most one page.
+int map_pages(CUtensorMap* m, const PagedRows& r, int cols, int heads, const PagedPool& kv, uint32_t box_cols,
+              uint32_t max_rows, CUtensorMapSwizzle swz, const char* what) {
+  const int page = 1 << kv.page_log2;
+  return make_map(m, r.ptr, cols, page, heads, kv.pages, r.st, r.sh, r.sp, box_cols,
+                  std::min<uint32_t>(page, max_rows), swz, what);
+}
+
+int many_maps(const PagedAttnParams& p, int D, ManyMaps* m) {
+  const CUtensorMapSwizzle r_swz = p.RP == 16 ? CU_TENSOR_MAP_SWIZZLE_32B : CU_TENSOR_MAP_SWIZZLE_64B;
+  if (int rc = make_map(&m->q, p.q, D, p.bd.T, p.H, 1, p.q_st, p.q_sh, 0, 64, kBlockM, CU_TENSOR_MAP_SWIZZLE_128B, "q"))
+    return rc;
+  if (int rc = map_pages(&m->k, p.kv.k, D, p.kv.hkv, p.kv, 64, kBlockN, CU_TENSOR_MAP_SWIZZLE_128B, "k pages")) return rc;
+  if (int rc = map_pages(&m->v, p.kv.v, D, p.kv.hkv, p.kv, 64, 64, CU_TENSOR_MAP_SWIZZLE_128B, "v pages")) return rc;
+  m->rq = m->q, m->rk = m->k;  // never dereferenced without graph heads
+  if (p.kv.hg > 0) {
+    if (int rc = make_map(&m->rq, p.rq, p.kv.rank, p.bd.T, p.kv.hg, 1, p.rq_st, p.rq_sh, 0, p.RP, kBlockM, r_swz, "r_q"))
+      return rc;
+    if (int rc = map_pages(&m->rk, p.kv.rk, p.kv.rank, p.kv.hg, p.kv, p.RP, kBlockN, r_swz, "rk pages")) return rc;
+  }
   return FNA2_OK;
 }
 
@@ -877,7 +937,13 @@ extern "C" int fna2_paged_attn(const Fna2PagedKV* kv, const Fna2PagedAttnArgs* a
   p.logits = l.logits ? reinterpret_cast<float*>(ws + l.acc_bytes + l.ml_bytes) : nullptr;
   if (l.lse_bytes) p.lse = reinterpret_cast<float*>(ws + l.acc_bytes + l.ml_bytes + l.logit_bytes), p.lse_sh = p.bd.T;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  FNA2_CUDA(kv->head_dim == 128 ? launch_paged_t<128>(p, l.RW, l.smem, st) : launch_paged_t<64>(p, l.RW, l.smem, st));
+  if (l.many) {
+    ManyMaps m;
+    if (int rc = many_maps(p, kv->head_dim, &m)) return rc;
+    FNA2_CUDA(launch_paged_many(m, p, kv->head_dim, st));
+  }
+  if (l.few) FNA2_CUDA(launch_paged_few(p, kv->head_dim, l.RW, l.smem, st));
+  FNA2_CUDA(launch_paged_tail(p, kv->head_dim, st));
   if (p.kw && !l.logits && p.bd.max_k > 0) {
     KeyWeightsParams w{};
     if (int rc = paged_queries(kv, a, &w)) return rc;

@@ -49,7 +49,17 @@ struct PagedAttnParams {
   float* kw;          // key weights, added to: [b * kw_sb + kh * kw_sh + j]
   int64_t kw_sb, kw_sh;
   int row_blocks, ng_max, nh_max, stages;
+  // Sequences of more than few_rows query rows (new tokens x query heads of a KV head) go to
+  // fna2_paged_many_kernel, the others to fna2_paged_few_kernel; a call launches those it may need.
+  int few_rows;
+  int chunk_many, many_items;  // keys per split there, upper bound on its (query tile pair, split) items
 };
+
+// Splits of a sequence that hold keys.
+__device__ __forceinline__ int paged_splits(const PagedAttnParams& p, const PagedSeq& s) {
+  const int chunk = s.n * p.G > p.few_rows ? p.chunk_many : p.chunk;
+  return max(1, (s.len + chunk - 1) / chunk);
+}
 
 constexpr int kFewThreads = 128;
 constexpr int kFewKeys = 16;  // keys per tile
@@ -91,10 +101,10 @@ __global__ void __launch_bounds__(kFewThreads) fna2_paged_few_kernel(const Paged
   if (!sq.ok && tid == 0) atomicCAS(&g_device_error, 0, kStatusBadSeqPaged);
   const int rows = sq.n * p.G;                 // row r: head r / n of the group, new token r % n
   const int r0 = rb * 16 * RW;                 // first row of this block
-  if (r0 >= rows) return;
+  if (r0 >= rows || rows > p.few_rows) return;
   const int past = sq.len - sq.n;              // may be negative: the first rows then see no key
   // splits of this sequence that hold keys (split 0 always exists: it writes rows that see nothing)
-  const int ns = max(1, (sq.len + p.chunk - 1) / p.chunk);
+  const int ns = paged_splits(p, sq);
   if (split >= ns) return;
   const int r_last = min(rows, r0 + 16 * RW) - 1;
   // graph heads of the block's rows, local to the group
@@ -347,7 +357,7 @@ __global__ void __launch_bounds__(128) fna2_paged_join_kernel(const PagedAttnPar
   const int b = warp_seq_of(p.bd.cu, p.bd.B, tok, lane);
   if (b < 0) return;
   const PagedSeq sq = paged_seq(p.bd, b);
-  const int ns = (sq.len + p.chunk - 1) / p.chunk;
+  const int ns = paged_splits(p, sq);
   if (!sq.ok || ns <= 1) return;  // written by the attention kernel
   const float2* ml = p.ws_ml + th * p.ns;
   float M = -INFINITY;
@@ -381,7 +391,7 @@ __global__ void __launch_bounds__(kLogitThreads) fna2_paged_logit_weights_kernel
   const PagedSeq sq = paged_seq(p.bd, b);
   if (static_cast<int>(blockIdx.x) * kLogitThreads >= sq.len) return;
   const int j = blockIdx.x * kLogitThreads + threadIdx.x, rows = sq.n * p.G;
-  const int ns = max(1, (sq.len + p.chunk - 1) / p.chunk), past = sq.len - sq.n;
+  const int ns = paged_splits(p, sq), past = sq.len - sq.n;
   __shared__ float s_lse[kLogitThreads];
   float w = 0.f;
   const float* x = p.logits + (static_cast<int64_t>(b) * p.kv.hkv + kh) * p.bd.max_q * p.G * p.logit_sr + j;
@@ -414,20 +424,31 @@ cudaError_t launch_paged_few_t(const PagedAttnParams& p, size_t smem, cudaStream
   auto kern = fna2_paged_few_kernel<D, RW>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
   if (e != cudaSuccess) return e;
-  const dim3 grid(p.bd.B * p.kv.hkv * p.row_blocks, p.ns);
+  const dim3 grid(p.bd.B * p.kv.hkv * p.row_blocks, (std::max(1, p.bd.max_k) + p.chunk - 1) / p.chunk);
   kern<<<grid, kFewThreads, smem, stream>>>(p);
   return cudaGetLastError();
 }
 
 template <int D>
-cudaError_t launch_paged_t(const PagedAttnParams& p, int RW, size_t smem, cudaStream_t stream) {
-  cudaError_t e = RW == 1   ? launch_paged_few_t<D, 1>(p, smem, stream)
-                  : RW == 2 ? launch_paged_few_t<D, 2>(p, smem, stream)
-                            : launch_paged_few_t<D, 4>(p, smem, stream);
-  if (e != cudaSuccess) return e;
+cudaError_t launch_paged_few_d(const PagedAttnParams& p, int RW, size_t smem, cudaStream_t stream) {
+  return RW == 1   ? launch_paged_few_t<D, 1>(p, smem, stream)
+         : RW == 2 ? launch_paged_few_t<D, 2>(p, smem, stream)
+                   : launch_paged_few_t<D, 4>(p, smem, stream);
+}
+
+inline cudaError_t launch_paged_few(const PagedAttnParams& p, int D, int RW, size_t smem, cudaStream_t stream) {
+  return D == 128 ? launch_paged_few_d<128>(p, RW, smem, stream) : launch_paged_few_d<64>(p, RW, smem, stream);
+}
+
+// What follows the attention kernels: the join of the splits and the weights from kept logits.
+inline cudaError_t launch_paged_tail(const PagedAttnParams& p, int D, cudaStream_t stream) {
+  cudaError_t e = cudaSuccess;
   if (p.ns > 1) {
     const int64_t blocks = (static_cast<int64_t>(p.bd.T) * p.H + 3) / 4;
-    fna2_paged_join_kernel<D><<<static_cast<unsigned>(blocks), 128, 0, stream>>>(p);
+    if (D == 128)
+      fna2_paged_join_kernel<128><<<static_cast<unsigned>(blocks), 128, 0, stream>>>(p);
+    else
+      fna2_paged_join_kernel<64><<<static_cast<unsigned>(blocks), 128, 0, stream>>>(p);
     if ((e = cudaGetLastError()) != cudaSuccess) return e;
   }
   if (p.logits) {
