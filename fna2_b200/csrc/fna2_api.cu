@@ -762,7 +762,7 @@ struct PagedPlan {
   int RW;
   bool few, many;  // kernels to launch
   bool logits;     // key weights from kept logits (few rows everywhere); otherwise recomputed by the key weights kernel
-  size_t smem, acc_bytes, ml_bytes, logit_bytes, lse_bytes, total;
+  size_t smem, acc_bytes, ml_bytes, logit_bytes, lse_bytes, kw_bytes, total;
 };
 
 size_t up256(size_t x) { return (x + 255) / 256 * 256; }
@@ -835,7 +835,8 @@ int paged_plan(const Fna2PagedKV* kv, const Fna2PagedAttnArgs* a, PagedAttnParam
   l->ml_bytes = p->ns > 1 || l->logits ? up256(th * p->ns * 8) : 0;
   l->logit_bytes = l->logits ? up256(static_cast<size_t>(p->bd.B) * p->kv.hkv * max_rows * p->logit_sr * 4) : 0;
   l->lse_bytes = p->kw && !l->logits && !a->lse ? up256(th * 4) : 0;
-  l->total = l->acc_bytes + l->ml_bytes + l->logit_bytes + l->lse_bytes;
+  l->kw_bytes = p->kw && !l->logits ? up256(th * 4) + up256(static_cast<size_t>(p->bd.T) * p->kv.hg * 4 * p->RP) : 0;
+  l->total = l->acc_bytes + l->ml_bytes + l->logit_bytes + l->lse_bytes + l->kw_bytes;
   return FNA2_OK;
 }
 
@@ -859,6 +860,32 @@ int many_maps(const PagedAttnParams& p, int D, ManyMaps* m) {
       return rc;
     if (int rc = map_pages(&m->rk, p.kv.rk, p.kv.rank, p.kv.hg, p.kv, p.RP, kBlockN, r_swz, "rk pages")) return rc;
   }
+  return FNA2_OK;
+}
+
+// Workspace of the key weights: R~_q hi / lo rows and the log2-domain LSE.
+size_t kw_rq2_bytes(const KeyWeightsParams& p) { return up256(static_cast<size_t>(p.bd.T) * p.kv.hg * 2 * p.RP * 2); }
+size_t kw_workspace_bytes(const KeyWeightsParams& p) {
+  return kw_rq2_bytes(p) + up256(static_cast<size_t>(p.bd.T) * p.H * 4);
+}
+
+int run_key_weights(KeyWeightsParams& p, int D, uint8_t* ws, cudaStream_t st) {
+  p.rq2 = reinterpret_cast<__nv_bfloat16*>(ws);
+  p.lse2 = reinterpret_cast<float*>(ws + kw_rq2_bytes(p));
+  p.qt = p.bd.max_q <= 64 ? 64 : 128;
+  const CUtensorMapSwizzle r_swz = p.RP == 16 ? CU_TENSOR_MAP_SWIZZLE_32B : CU_TENSOR_MAP_SWIZZLE_64B;
+  KwMaps m;
+  if (int rc = make_map(&m.q, p.q, D, p.bd.T, p.H, 1, p.q_st, p.q_sh, 0, 64, p.qt, CU_TENSOR_MAP_SWIZZLE_128B, "q"))
+    return rc;
+  if (int rc = map_pages(&m.k, p.kv.k, D, p.kv.hkv, p.kv, 64, kBlockN, CU_TENSOR_MAP_SWIZZLE_128B, "k pages")) return rc;
+  m.rq = m.q, m.rk = m.k;  // never dereferenced without graph heads
+  if (p.kv.hg > 0) {
+    const int64_t w = 2 * p.RP;
+    if (int rc = make_map(&m.rq, p.rq2, w, p.bd.T, p.kv.hg, 1, p.kv.hg * w, w, 0, p.RP, p.qt, r_swz, "r_q hi, lo"))
+      return rc;
+    if (int rc = map_pages(&m.rk, p.kv.rk, p.kv.rank, p.kv.hg, p.kv, p.RP, kBlockN, r_swz, "rk pages")) return rc;
+  }
+  FNA2_CUDA(launch_key_weights(m, p, D, st));
   return FNA2_OK;
 }
 
@@ -948,7 +975,7 @@ extern "C" int fna2_paged_attn(const Fna2PagedKV* kv, const Fna2PagedAttnArgs* a
     KeyWeightsParams w{};
     if (int rc = paged_queries(kv, a, &w)) return rc;
     w.lse = p.lse, w.lse_sh = p.lse_sh;
-    FNA2_CUDA(launch_key_weights(w, kv->head_dim, st));
+    if (int rc = run_key_weights(w, kv->head_dim, ws + (l.total - l.kw_bytes), st)) return rc;
   }
   return FNA2_OK;
 }
@@ -957,22 +984,23 @@ extern "C" size_t fna2_key_weights_workspace_size(const Fna2PagedKV* kv, const F
   g_last_error.clear();
   KeyWeightsParams p{};
   if (paged_queries(kv, a, &p)) return 0;
-  return 0;
+  return kw_workspace_bytes(p);
 }
 
 extern "C" int fna2_key_weights(const Fna2PagedKV* kv, const Fna2PagedAttnArgs* a, void* workspace,
                                 size_t workspace_bytes, void* stream) {
   g_last_error.clear();
-  (void)workspace, (void)workspace_bytes;
   KeyWeightsParams p{};
   if (int rc = paged_queries(kv, a, &p)) return rc;
   FNA2_CHECK(a->key_weights != nullptr && (a->lse != nullptr || a->total_q == 0), "key weights need lse and key_weights");
-  FNA2_CHECK(key_weights_smem(kv->head_dim, std::min(p.G, p.kv.hg), p.RP) <= kMaxDynamicSmem,
-             "heads per KV head and rank need too much shared memory");
   if (p.bd.B == 0 || p.bd.T == 0 || p.bd.max_k == 0) return FNA2_OK;
+  const size_t need = kw_workspace_bytes(p);
+  if (workspace == nullptr || workspace_bytes < need)
+    return fail(FNA2_ERR_WORKSPACE, "key weights workspace: need %zu bytes, got %zu", need, workspace_bytes);
+  FNA2_CHECK((reinterpret_cast<uintptr_t>(workspace) & 255u) == 0, "workspace must be 256-byte aligned");
+  FNA2_CHECK((p.bd.max_k + 2 * kBlockN - 1) / (2 * kBlockN) <= 65535, "max_seqlen_k is too large for key weights");
   p.lse = a->lse, p.lse_sh = a->lse_head_stride;
-  FNA2_CUDA(launch_key_weights(p, kv->head_dim, static_cast<cudaStream_t>(stream)));
-  return FNA2_OK;
+  return run_key_weights(p, kv->head_dim, static_cast<uint8_t*>(workspace), static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int fna2_evict(const Fna2PagedKV* kv, const Fna2EvictArgs* a, void* stream) {
