@@ -215,6 +215,14 @@ class Fna2EvictArgs(ctypes.Structure):
     ]
 
 
+class _Block:
+    """A parameter that points to an argument block: a ctypes structure, or the bytes of one."""
+
+    @classmethod
+    def from_param(cls, a):
+        return ctypes.c_char_p(a) if isinstance(a, bytes) else ctypes.byref(a)
+
+
 _lib: Optional[ctypes.CDLL] = None
 
 
@@ -255,16 +263,16 @@ def load(path: str = LIB_PATH) -> ctypes.CDLL:
     lib.fna2_gemm.argtypes = [ctypes.POINTER(Fna2GemmArgs), ctypes.c_void_p]
     lib.fna2_gemm.restype = ctypes.c_int
     kv = ctypes.POINTER(Fna2PagedKV)
-    lib.fna2_paged_append.argtypes = [kv, ctypes.POINTER(Fna2AppendArgs), ctypes.c_void_p]
+    lib.fna2_paged_append.argtypes = [kv, _Block, ctypes.c_void_p]
     lib.fna2_paged_append.restype = ctypes.c_int
     for name in ("fna2_paged_attn", "fna2_key_weights"):
         f = getattr(lib, name)
-        f.argtypes = [kv, ctypes.POINTER(Fna2PagedAttnArgs), ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]
+        f.argtypes = [kv, _Block, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]
         f.restype = ctypes.c_int
         f = getattr(lib, name + "_workspace_size")
-        f.argtypes = [kv, ctypes.POINTER(Fna2PagedAttnArgs)]
+        f.argtypes = [kv, _Block]
         f.restype = ctypes.c_size_t
-    lib.fna2_evict.argtypes = [kv, ctypes.POINTER(Fna2EvictArgs), ctypes.c_void_p]
+    lib.fna2_evict.argtypes = [kv, _Block, ctypes.c_void_p]
     lib.fna2_evict.restype = ctypes.c_int
     lib.fna2_abi_version.argtypes = []
     lib.fna2_abi_version.restype = ctypes.c_int

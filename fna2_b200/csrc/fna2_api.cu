@@ -798,11 +798,11 @@ int paged_plan(const Fna2PagedKV* kv, const Fna2PagedAttnArgs* a, PagedAttnParam
   for (;; l->RW /= 2) {
     p->ng_max = std::min({p->G, 16 * l->RW, p->kv.hg});
     p->nh_max = std::min({p->G, 16, p->kv.hg});
-    const FewSmem L(D, p->ng_max, p->nh_max, p->RP);
-    p->stages = 4;
-    while (p->stages > 2 && L.total(l->RW, p->stages) > 100 * 1024) --p->stages;
-    l->smem = std::max<size_t>(L.total(l->RW, p->stages), 512 + 64 * D * 4);
-    if (l->smem <= kMaxDynamicSmem || l->RW == 1) break;
+    // ring depth: at most 4 tiles, fewer where two CTAs per SM then fit
+    for (p->stages = 4; p->stages > 2; --p->stages)
+      if (FewSmem(D, l->RW, p->ng_max, p->nh_max, p->RP, p->stages).total <= 113 * 1024) break;
+    l->smem = std::max<size_t>(FewSmem(D, l->RW, p->ng_max, p->nh_max, p->RP, p->stages).total, 512 + 64 * D * 4);
+    if ((l->smem <= kMaxDynamicSmem && 2 * D / 64 + p->ng_max <= 32) || l->RW == 1) break;  // a lane per box
   }
   FNA2_CHECK(l->smem <= kMaxDynamicSmem, "heads per KV head and rank need too much shared memory");
   p->row_blocks = (few_max + 16 * l->RW - 1) / (16 * l->RW);
@@ -846,6 +846,15 @@ int map_pages(CUtensorMap* m, const PagedRows& r, int cols, int heads, const Pag
   const int page = 1 << kv.page_log2;
   return make_map(m, r.ptr, cols, page, heads, kv.pages, r.st, r.sh, r.sp, box_cols,
                   std::min<uint32_t>(page, max_rows), swz, what);
+}
+
+int few_maps(const PagedAttnParams& p, int D, FewMaps* m) {
+  if (int rc = map_pages(&m->k, p.kv.k, D, p.kv.hkv, p.kv, 64, kFewKeys, CU_TENSOR_MAP_SWIZZLE_128B, "k pages")) return rc;
+  if (int rc = map_pages(&m->v, p.kv.v, D, p.kv.hkv, p.kv, 64, kFewKeys, CU_TENSOR_MAP_SWIZZLE_128B, "v pages")) return rc;
+  m->rk = m->k;  // never dereferenced without graph heads
+  if (p.kv.hg == 0) return FNA2_OK;
+  return map_pages(&m->rk, p.kv.rk, p.kv.rank, p.kv.hg, p.kv, p.RP, kFewKeys,
+                   p.RP == 16 ? CU_TENSOR_MAP_SWIZZLE_32B : CU_TENSOR_MAP_SWIZZLE_64B, "rk pages");
 }
 
 int many_maps(const PagedAttnParams& p, int D, ManyMaps* m) {
@@ -969,7 +978,11 @@ extern "C" int fna2_paged_attn(const Fna2PagedKV* kv, const Fna2PagedAttnArgs* a
     if (int rc = many_maps(p, kv->head_dim, &m)) return rc;
     FNA2_CUDA(launch_paged_many(m, p, kv->head_dim, st));
   }
-  if (l.few) FNA2_CUDA(launch_paged_few(p, kv->head_dim, l.RW, l.smem, st));
+  if (l.few) {
+    FewMaps m;
+    if (int rc = few_maps(p, kv->head_dim, &m)) return rc;
+    FNA2_CUDA(launch_paged_few(m, p, kv->head_dim, l.RW, l.smem, st));
+  }
   FNA2_CUDA(launch_paged_tail(p, kv->head_dim, st));
   if (p.kw && !l.logits && p.bd.max_k > 0) {
     KeyWeightsParams w{};

@@ -18,9 +18,14 @@
 // One CTA serves (sequence, KV head, block of 16 RW query rows, key split).  A
 // query row is (query head of the KV group, new token), head-major, so that the
 // 16 rows of a warp span few heads.  4 warps: RW row blocks x 4/RW key groups; a
-// key group streams its own 16-key tiles through a ring of asynchronous copies
-// that its RW warps fill and read together (mma.sync m16n8k16, fp32
-// accumulation, online softmax in registers).  16 keys never cross a page.
+// key group streams its own 16-key tiles through a ring in shared memory that its
+// RW warps read together (mma.sync m16n8k16, fp32 accumulation, online softmax
+// in registers).  16 keys never cross a page, so a tile is one TMA box per 64
+// columns of K and V and one per head of R_k, issued by as many lanes; 128-byte
+// (R_k: 32- or 64-byte) swizzled rows give conflict-free ldmatrix reads.  (With one
+// cp.async per 16 bytes the address arithmetic was 3/4 of the 820 instructions a
+// tile took, and the kernel was bound by their issue at 5.1 TB/s.)
+// Bound: HBM; each cached key is read once per row block.
 #include "fna2_paged.cuh"
 
 namespace fna2 {
@@ -64,39 +69,41 @@ __device__ __forceinline__ int paged_splits(const PagedAttnParams& p, const Page
 constexpr int kFewThreads = 128;
 constexpr int kFewKeys = 16;  // keys per tile
 
-// Shared-memory geometry (host and device agree on it).
+// Shared-memory geometry (host and device agree on it): [A of the RW row blocks | K and V ring of
+// the key groups | R_k ring | barriers]; ng: graph heads of a block's rows, nh: heads that the 16
+// rows of one warp span.
 struct FewSmem {
-  int a_stride, k_stride, v_stride, stage;
-  // ng: graph heads of a block's rows; nh: heads that the 16 rows of one warp span
-  __host__ __device__ FewSmem(int D, int ng, int nh, int RP) {
+  int a_stride, kv_stage, r_head, r_stage, o_kv, o_r, o_bar, total;
+  __host__ __device__ FewSmem(int D, int RW, int ng, int nh, int RP, int stages) {
     a_stride = (D + 2 * nh * RP) * 2 + 16;
-    k_stride = (D + ng * RP) * 2 + 16;
-    v_stride = D * 2 + 16;
-    stage = kFewKeys * (k_stride + v_stride);
+    kv_stage = 2 * kFewKeys * D * 2;
+    r_head = kFewKeys * RP * 2;
+    r_stage = ng * r_head;
+    const int rings = 4 / RW * stages;
+    o_kv = (16 * RW * a_stride + 1023) / 1024 * 1024;
+    o_r = o_kv + rings * kv_stage;
+    o_bar = o_r + (rings * r_stage + 1023) / 1024 * 1024;
+    total = o_bar + 2 * rings * 8 + 16;
   }
-  __host__ __device__ int a_bytes(int RW) const { return 16 * RW * a_stride; }
-  __host__ __device__ int total(int RW, int stages) const { return a_bytes(RW) + 4 / RW * stages * stage; }
 };
 
-// Rendezvous of the RW warps of a key group (named barrier 1 + group).
-template <int RW>
-__device__ __forceinline__ void group_sync(int kg) {
-  if (RW == 1)
-    __syncwarp();
-  else
-    asm volatile("bar.sync %0, %1;" ::"r"(kg + 1), "n"(32 * RW) : "memory");
-}
-
 template <int D, int RW>
-__global__ void __launch_bounds__(kFewThreads) fna2_paged_few_kernel(const PagedAttnParams p) {
-  constexpr int KW = 4 / RW, GT = 32 * RW;  // key groups per CTA, threads per group
-  extern __shared__ __align__(16) uint8_t dsm[];
+__global__ void __launch_bounds__(kFewThreads, 2)
+    fna2_paged_few_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                          const __grid_constant__ CUtensorMap tmRk, const PagedAttnParams p) {
+  constexpr int KW = 4 / RW;  // key groups per CTA
+  constexpr int DC = D / 64;  // 64-column chunks of a K or V row
+  extern __shared__ __align__(1024) uint8_t dsm[];
+  if (smem_u32(dsm) & 1023u) {  // the swizzled layouts need it
+    if (threadIdx.x == 0) atomicCAS(&g_device_error, 0, kStatusSmemBase);
+    return;
+  }
   const int split = blockIdx.y;
   const int rb = blockIdx.x % p.row_blocks;
   const int kh = (blockIdx.x / p.row_blocks) % p.kv.hkv;
   const int b = blockIdx.x / (p.row_blocks * p.kv.hkv);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int rw = warp % RW, kg = warp / RW, gtid = tid % GT;
+  const int rw = warp % RW, kg = warp / RW;
   const PagedSeq sq = paged_seq(p.bd, b);
   if (!sq.ok && tid == 0) atomicCAS(&g_device_error, 0, kStatusBadSeqPaged);
   const int rows = sq.n * p.G;                 // row r: head r / n of the group, new token r % n
@@ -110,7 +117,60 @@ __global__ void __launch_bounds__(kFewThreads) fna2_paged_few_kernel(const Paged
   // graph heads of the block's rows, local to the group
   const int g_lo = r0 / sq.n, g_hi = min(r_last / sq.n, p.kv.hg - kh * p.G - 1);
   const int ng = max(0, g_hi - g_lo + 1);
-  const FewSmem L(D, p.ng_max, p.nh_max, p.RP);
+  const FewSmem L(D, RW, p.ng_max, p.nh_max, p.RP, p.stages);
+  uint64_t* full = reinterpret_cast<uint64_t*>(dsm + L.o_bar) + kg * p.stages;
+  uint64_t* empty = full + KW * p.stages;
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(dsm + L.o_bar + 2 * KW * p.stages * 8);
+  if (tid == 0) {
+    for (int s = 0; s < KW * p.stages; ++s) {
+      mbar_init(full + s, 1);
+      mbar_init(empty + s, RW);
+    }
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  __syncthreads();
+
+  // keys [k_begin, k_end) of this split that some row of the block sees
+  int seen = sq.len;
+  if (p.causal) {
+    // the largest new-token index among the block's rows
+    const int i_max = r_last - r0 + 1 >= sq.n || r_last / sq.n != r0 / sq.n ? sq.n - 1 : r_last % sq.n;
+    seen = max(0, past + i_max + 1);
+  }
+  const int k_begin = min(split * p.chunk, seen), k_end = min(seen, k_begin + p.chunk);
+  const int n_all = (k_end - k_begin + kFewKeys - 1) / kFewKeys;
+  const int n_tiles = n_all > kg ? (n_all - kg + KW - 1) / KW : 0;
+
+  // Ring of the key group: lane l issues box l of a tile (K chunks, V chunks, R_k heads).
+  uint8_t* kv_ring = dsm + L.o_kv + kg * p.stages * L.kv_stage;
+  uint8_t* r_ring = dsm + L.o_r + kg * p.stages * L.r_stage;
+  const int* table = p.kv.table + b * p.kv.table_sb;
+  const int lg = p.kv.page_log2, mask = (1 << lg) - 1;
+  const bool box = lane < 2 * DC + ng;
+  const CUtensorMap* map = lane < DC ? &tmK : lane < 2 * DC ? &tmV : &tmRk;
+  const int box_col = lane < 2 * DC ? lane % DC * 64 : 0;
+  const int box_head = lane < 2 * DC ? kh : kh * p.G + g_lo + lane - 2 * DC;
+  uint8_t* box_dst = lane < 2 * DC ? kv_ring + lane * (kFewKeys * 128) : r_ring + (lane - 2 * DC) * L.r_head;
+  const int box_step = lane < 2 * DC ? L.kv_stage : L.r_stage;
+  const int tile_bytes = L.kv_stage + ng * L.r_head;
+  int issued = 0, i_stage = 0, i_phase = 1;  // empty barriers: the first round passes
+  int j_next = k_begin + kg * kFewKeys;
+  int page_next = n_tiles > 0 ? __ldg(table + (j_next >> lg)) : 0;
+  auto issue = [&]() {
+    if (issued >= n_tiles) return;
+    const int page = page_next, slot = j_next & mask;
+    j_next += KW * kFewKeys;
+    ++issued;
+    if (issued < n_tiles) page_next = __ldg(table + (j_next >> lg));
+    if (RW > 1) mbar_wait(empty + i_stage, i_phase, abort_flag, 131);
+    if (lane == 0) mbar_expect_tx(full + i_stage, tile_bytes);
+    __syncwarp();
+    if (box) tma_load_4d(box_dst + i_stage * box_step, map, full + i_stage, box_col, slot, box_head, page);
+    if (++i_stage == p.stages) i_stage = 0, i_phase ^= 1;
+  };
+  if (rw == 0)
+    for (int s = 0; s < p.stages - 1; ++s) issue();
 
   // A = [q | R~_q hi, lo of the warp's heads] of this warp's 16 rows (rows past the end are zero)
   const int wr0 = r0 + rw * 16;
@@ -139,74 +199,29 @@ __global__ void __launch_bounds__(kFewThreads) fna2_paged_few_kernel(const Paged
       *reinterpret_cast<uint4*>(dst + p.RP * 2) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
     }
   }
-
-  uint8_t* ring = dsm + L.a_bytes(RW) + static_cast<size_t>(kg) * p.stages * L.stage;
-  if (p.kv.rank != p.RP) {  // columns [rank, RP) of every head are zero, and stay so
-    const int pad8 = (p.RP - p.kv.rank) / 8;
-    for (int e = gtid; e < p.stages * kFewKeys * ng * pad8; e += GT) {
-      const int c = e % pad8, g = e / pad8 % ng, r = e / (pad8 * ng) % kFewKeys, s = e / (pad8 * ng * kFewKeys);
-      *reinterpret_cast<uint4*>(ring + s * L.stage + r * L.k_stride + (D + g * p.RP + p.kv.rank + c * 8) * 2) =
-          make_uint4(0, 0, 0, 0);
-    }
-  }
   __syncthreads();
-
-  // keys [k_begin, k_end) of this split that some row of the block sees
-  int seen = sq.len;
-  if (p.causal) {
-    // the largest new-token index among the block's rows
-    const int i_max = r_last - r0 + 1 >= sq.n || r_last / sq.n != r0 / sq.n ? sq.n - 1 : r_last % sq.n;
-    seen = max(0, past + i_max + 1);
-  }
-  const int k_begin = min(split * p.chunk, seen), k_end = min(seen, k_begin + p.chunk);
-  const int n_all = (k_end - k_begin + kFewKeys - 1) / kFewKeys;
-  const int n_tiles = n_all > kg ? (n_all - kg + KW - 1) / KW : 0;
-  const int* table = p.kv.table + b * p.kv.table_sb;
-  const int mask = (1 << p.kv.page_log2) - 1;
-  constexpr int PPR = D / 8;                      // 16-byte pieces of a K or V row
-  const int r8 = p.kv.rank / 8, rpieces = ng * r8;
-  const int h_lo = kh * p.G + g_lo;
-
-  int issued = 0;
-  auto issue = [&]() {
-    if (issued < n_tiles) {
-      uint8_t* st = ring + (issued % p.stages) * L.stage;
-      const int j0 = k_begin + (kg + issued * KW) * kFewKeys;
-      const int page = __ldg(table + (j0 >> p.kv.page_log2)), slot = j0 & mask;
-      const bool page_ok = page >= 0 && page < p.kv.pages;
-      const __nv_bfloat16* ks = p.kv.k.ptr + (page_ok ? paged_off(p.kv.k, page, slot, kh) : 0);
-      const __nv_bfloat16* vs = p.kv.v.ptr + (page_ok ? paged_off(p.kv.v, page, slot, kh) : 0);
-      const int nv = page_ok ? k_end - j0 : 0;  // rows past the end are zero-filled: what a page holds there is never used
-      uint8_t* vd = st + kFewKeys * L.k_stride;
-#pragma unroll
-      for (int e = gtid; e < kFewKeys * PPR; e += GT) {
-        const int r = e / PPR, c = e % PPR;
-        const bool valid = r < nv;
-        dec_cp16(st + r * L.k_stride + c * 16, valid ? ks + r * p.kv.k.st + c * 8 : p.kv.k.ptr, valid);
-        dec_cp16(vd + r * L.v_stride + c * 16, valid ? vs + r * p.kv.v.st + c * 8 : p.kv.v.ptr, valid);
-      }
-      for (int e = gtid; e < kFewKeys * rpieces; e += GT) {
-        const int r = e / rpieces, c = e % rpieces, g = c / r8, cc = c % r8 * 8;
-        const bool valid = r < nv;
-        const __nv_bfloat16* src =
-            p.kv.rk.ptr + (valid ? paged_off(p.kv.rk, page, slot + r, h_lo + g) + cc : 0);
-        dec_cp16(st + r * L.k_stride + (D + g * p.RP + cc) * 2, src, valid);
-      }
-    }
-    ++issued;
-    dec_commit();
-  };
-  for (int s = 0; s < p.stages - 1; ++s) issue();
 
   const int g = lane >> 2, t = lane & 3;
   const int ra = wr0 + g, rc = ra + 8;  // the two rows of this thread's fragments
-  auto row_limit = [&](int r) { return r < rows ? (p.causal ? max(0, past + r % sq.n + 1) : sq.len) : 0; };
-  const int lim0 = min(k_end, row_limit(ra)), lim1 = min(k_end, row_limit(rc));
+  // (rows past the end are zero rows that see every key: they are not written)
+  auto row_limit = [&](int r) { return min(k_end, p.causal && r < rows ? max(0, past + r % sq.n + 1) : sq.len); };
+  const int lim0 = row_limit(ra), lim1 = row_limit(rc);
+  // tiles that end at or before every row's limit need no mask
+  const int lim_all = __reduce_min_sync(0xffffffffu, min(lim0, lim1));
+  const uint32_t a_addr = smem_u32(sa) + ((lane & 7) + ((lane >> 3) & 1) * 8) * L.a_stride + (lane >> 4) * 16;
+  uint32_t aq[D / 16][4];  // q fragments stay in registers
+#pragma unroll
+  for (int ks = 0; ks < D / 16; ++ks) ldsm_x4(aq[ks], a_addr + ks * 32);
+  // ldmatrix addresses within a swizzled tile; rows differ by lane & 7 (+ 8), so the XOR is a lane constant
+  const uint32_t k_row = (lane & 7) + (lane >> 4) * 8, k_sel = ((lane >> 3) & 1) * 16;
+  const uint32_t v_row = (lane & 7) + ((lane >> 3) & 1) * 8, v_sel = (lane >> 4) * 16;
+  const uint32_t k_off = k_row * 128, v_off = kFewKeys * D * 2 + v_row * 128, sw = (lane & 7) * 16;
+  const uint32_t r_off = k_row * p.RP * 2, r_sw = p.RP == 16 ? ((k_row >> 2) & 1) * 16 : ((k_row >> 1) & 3) * 16;
   float acc[D / 8][4];
 #pragma unroll
   for (int i = 0; i < D / 8; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
-  float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;  // log2 domain
-  const uint32_t a_addr = smem_u32(sa) + ((lane & 7) + ((lane >> 3) & 1) * 8) * L.a_stride + (lane >> 4) * 16;
+  // log2 domain: m the maximum that P is relative to, mt this thread's largest logit so far
+  float m0 = -INFINITY, m1 = -INFINITY, mt0 = -INFINITY, mt1 = -INFINITY, l0 = 0.f, l1 = 0.f;
   const float sl2 = p.scale_log2;
   float* lg0 = nullptr;
   float* lg1 = nullptr;
@@ -216,28 +231,35 @@ __global__ void __launch_bounds__(kFewThreads) fna2_paged_few_kernel(const Paged
     if (rc < rows) lg1 = base + rc * p.logit_sr;
   }
 
+  int stage = 0, phase = 0;
   for (int tt = 0; tt < n_tiles; ++tt) {
-    // the oldest tile has landed for this thread; after the rendezvous for the whole group, and
-    // everyone is done with the stage that the next issue refills
-    dec_wait(p.stages - 2);
-    group_sync<RW>(kg);
-    issue();
-    const uint8_t* st = ring + (tt % p.stages) * L.stage;
+    __syncwarp();  // (RW == 1) every lane is done with the stage that this issue refills
+    if (rw == 0) issue();
+    if (!mbar_wait(full + stage, phase, abort_flag, 132)) break;
+    uint8_t* kv = kv_ring + stage * L.kv_stage;
+    const uint32_t kv_addr = smem_u32(kv);
+    const uint32_t rk_addr = smem_u32(r_ring + stage * L.r_stage) + (wg_lo - g_lo) * L.r_head + r_off;
     const int j0 = k_begin + (kg + tt * KW) * kFewKeys;
+    if (j0 + kFewKeys > sq.len) {
+      // past the sequence's end a page holds anything: V rows become zero (P is 0 there, but 0 * NaN
+      // is not); K rows only reach logits that are masked.  The RW warps write the same zeros.
+      for (int e = lane; e < (j0 + kFewKeys - sq.len) * 8 * DC; e += 32)
+        *reinterpret_cast<uint4*>(kv + kFewKeys * D * 2 + e % DC * (kFewKeys * 128) +
+                                  (sq.len - j0) * 128 + e / DC * 16) = make_uint4(0, 0, 0, 0);
+      __syncwarp();
+    }
     float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
-    const uint32_t k_addr = smem_u32(st) + ((lane & 7) + (lane >> 4) * 8) * L.k_stride + ((lane >> 3) & 1) * 16;
 #pragma unroll
     for (int ks = 0; ks < D / 16; ++ks) {
-      uint32_t a[4], kb[4];
-      ldsm_x4(a, a_addr + ks * 32);
-      ldsm_x4(kb, k_addr + ks * 32);
-      mma_bf16(s0, a, kb[0], kb[1]);
-      mma_bf16(s1, a, kb[2], kb[3]);
+      uint32_t kb[4];
+      ldsm_x4(kb, kv_addr + (ks >> 2) * (kFewKeys * 128) + k_off + ((k_sel + (ks & 3) * 32) ^ sw));
+      mma_bf16(s0, aq[ks], kb[0], kb[1]);
+      mma_bf16(s1, aq[ks], kb[2], kb[3]);
     }
     for (int c = 0; c < wn; ++c)
       for (int ks = 0; ks < p.RP / 16; ++ks) {
         uint32_t a[4], kb[4];
-        ldsm_x4(kb, k_addr + (D + (wg_lo - g_lo + c) * p.RP) * 2 + ks * 32);
+        ldsm_x4(kb, rk_addr + c * L.r_head + ((k_sel + ks * 32) ^ r_sw));
         const uint32_t aw = a_addr + (D + 2 * c * p.RP) * 2 + ks * 32;
         ldsm_x4(a, aw);
         mma_bf16(s0, a, kb[0], kb[1]);
@@ -248,54 +270,67 @@ __global__ void __launch_bounds__(kFewThreads) fna2_paged_few_kernel(const Paged
       }
     // online softmax: row ra holds x[0..3], row rc x[4..7]; keys j0 + {2t, 2t+1, 8+2t, 9+2t}
     float x[8] = {s0[0], s0[1], s1[0], s1[1], s0[2], s0[3], s1[2], s1[3]};
-    const int kk[4] = {j0 + 2 * t, j0 + 2 * t + 1, j0 + 8 + 2 * t, j0 + 9 + 2 * t};
+    if (j0 + kFewKeys > lim_all) {
+      const int kk[4] = {j0 + 2 * t, j0 + 2 * t + 1, j0 + 8 + 2 * t, j0 + 9 + 2 * t};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      x[i] = kk[i] < lim0 ? x[i] * sl2 : -INFINITY;
-      x[4 + i] = kk[i] < lim1 ? x[4 + i] * sl2 : -INFINITY;
+      for (int i = 0; i < 4; ++i) {
+        x[i] = kk[i] < lim0 ? x[i] : -INFINITY;
+        x[4 + i] = kk[i] < lim1 ? x[4 + i] : -INFINITY;
+      }
     }
     if (lg0) {
-      *reinterpret_cast<float2*>(lg0 + kk[0]) = make_float2(x[0], x[1]);
-      *reinterpret_cast<float2*>(lg0 + kk[2]) = make_float2(x[2], x[3]);
+      *reinterpret_cast<float2*>(lg0 + j0 + 2 * t) = make_float2(x[0] * sl2, x[1] * sl2);
+      *reinterpret_cast<float2*>(lg0 + j0 + 8 + 2 * t) = make_float2(x[2] * sl2, x[3] * sl2);
     }
     if (lg1) {
-      *reinterpret_cast<float2*>(lg1 + kk[0]) = make_float2(x[4], x[5]);
-      *reinterpret_cast<float2*>(lg1 + kk[2]) = make_float2(x[6], x[7]);
+      *reinterpret_cast<float2*>(lg1 + j0 + 2 * t) = make_float2(x[4] * sl2, x[5] * sl2);
+      *reinterpret_cast<float2*>(lg1 + j0 + 8 + 2 * t) = make_float2(x[6] * sl2, x[7] * sl2);
     }
-    float mx0 = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), mx1 = fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7]));
-    mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 1));
-    mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 2));
-    mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 1));
-    mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 2));
-    const float n0 = fmaxf(m0, mx0), n1 = fmaxf(m1, mx1);
-    const float c0 = n0 == -INFINITY ? 1.f : exp2f(m0 - n0), c1 = n1 == -INFINITY ? 1.f : exp2f(m1 - n1);
-    const float b0 = n0 == -INFINITY ? 0.f : n0, b1 = n1 == -INFINITY ? 0.f : n1;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = exp2f(x[i] - b0), x[4 + i] = exp2f(x[4 + i] - b1);
-    l0 = l0 * c0 + ((x[0] + x[1]) + (x[2] + x[3]));
-    l1 = l1 * c1 + ((x[4] + x[5]) + (x[6] + x[7]));
-    m0 = n0, m1 = n1;
-    if (__any_sync(0xffffffffu, c0 != 1.f || c1 != 1.f)) {  // some row max moved
+    float mx0 = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) * sl2;
+    float mx1 = fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])) * sl2;
+    mt0 = fmaxf(mt0, mx0), mt1 = fmaxf(mt1, mx1);
+    // the maximum in use moves only when some logit is above it by more than 2^8 (P stays in range)
+    if (__any_sync(0xffffffffu, mx0 > m0 + 8.f || mx1 > m1 + 8.f)) {
+      mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 1));
+      mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 2));
+      mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 1));
+      mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 2));
+      const float n0 = fmaxf(m0, mx0), n1 = fmaxf(m1, mx1);
+      const float c0 = n0 == -INFINITY ? 1.f : ex2(m0 - n0), c1 = n1 == -INFINITY ? 1.f : ex2(m1 - n1);
+      m0 = n0, m1 = n1;
+      l0 *= c0, l1 *= c1;
 #pragma unroll
       for (int i = 0; i < D / 8; ++i) acc[i][0] *= c0, acc[i][1] *= c0, acc[i][2] *= c1, acc[i][3] *= c1;
     }
+    const float b0 = m0 == -INFINITY ? 0.f : m0, b1 = m1 == -INFINITY ? 0.f : m1;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = ex2(fmaf(x[i], sl2, -b0)), x[4 + i] = ex2(fmaf(x[4 + i], sl2, -b1));
+    l0 += (x[0] + x[1]) + (x[2] + x[3]);
+    l1 += (x[4] + x[5]) + (x[6] + x[7]);
     const uint32_t pa[4] = {pack_bf16(x[0], x[1]), pack_bf16(x[4], x[5]), pack_bf16(x[2], x[3]),
                             pack_bf16(x[6], x[7])};
-    const uint32_t v_addr = smem_u32(st + kFewKeys * L.k_stride) +
-                            ((lane & 7) + ((lane >> 3) & 1) * 8) * L.v_stride + (lane >> 4) * 16;
 #pragma unroll
     for (int d16 = 0; d16 < D / 16; ++d16) {
       uint32_t vb[4];
-      ldsm_x4_t(vb, v_addr + d16 * 32);
+      ldsm_x4_t(vb, kv_addr + (d16 >> 2) * (kFewKeys * 128) + v_off + ((v_sel + (d16 & 3) * 32) ^ sw));
       mma_bf16(acc[2 * d16], pa, vb[0], vb[1]);
       mma_bf16(acc[2 * d16 + 1], pa, vb[2], vb[3]);
     }
+    if (RW > 1) {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(empty + stage);
+    }
+    if (++stage == p.stages) stage = 0, phase ^= 1;
   }
-  dec_wait(0);
-  l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
-  l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
-  l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
-  l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
+  // sums and the true maximum over the row's four lanes; everything relative to that maximum
+#pragma unroll
+  for (int o = 1; o <= 2; o <<= 1) {
+    l0 += __shfl_xor_sync(0xffffffffu, l0, o);
+    l1 += __shfl_xor_sync(0xffffffffu, l1, o);
+    mt0 = fmaxf(mt0, __shfl_xor_sync(0xffffffffu, mt0, o));
+    mt1 = fmaxf(mt1, __shfl_xor_sync(0xffffffffu, mt1, o));
+  }
+  const float f0 = mt0 == -INFINITY ? 0.f : ex2(m0 - mt0), f1 = mt1 == -INFINITY ? 0.f : ex2(m1 - mt1);
 
   // join the KW key groups through shared memory (all rings are idle)
   __syncthreads();
@@ -304,13 +339,13 @@ __global__ void __launch_bounds__(kFewThreads) fna2_paged_few_kernel(const Paged
   float* co = cl + 64;                        // [KW][16 RW][D] acc
   const int slot = kg * 16 * RW + rw * 16 + g;
   if (t == 0) {
-    cm[slot] = m0, cm[slot + 8] = m1;
-    cl[slot] = l0, cl[slot + 8] = l1;
+    cm[slot] = mt0, cm[slot + 8] = mt1;
+    cl[slot] = l0 * f0, cl[slot + 8] = l1 * f1;
   }
 #pragma unroll
   for (int i = 0; i < D / 8; ++i) {
-    *reinterpret_cast<float2*>(co + slot * D + i * 8 + 2 * t) = make_float2(acc[i][0], acc[i][1]);
-    *reinterpret_cast<float2*>(co + (slot + 8) * D + i * 8 + 2 * t) = make_float2(acc[i][2], acc[i][3]);
+    *reinterpret_cast<float2*>(co + slot * D + i * 8 + 2 * t) = make_float2(acc[i][0] * f0, acc[i][1] * f0);
+    *reinterpret_cast<float2*>(co + (slot + 8) * D + i * 8 + 2 * t) = make_float2(acc[i][2] * f1, acc[i][3] * f1);
   }
   __syncthreads();
   const int nr = r_last - r0 + 1;
@@ -324,7 +359,7 @@ __global__ void __launch_bounds__(kFewThreads) fna2_paged_few_kernel(const Paged
     if (M != -INFINITY) {
 #pragma unroll
       for (int w = 0; w < KW; ++w) {
-        const float f = exp2f(cm[w * 16 * RW + row] - M);
+        const float f = ex2(cm[w * 16 * RW + row] - M);
         const float4 a = *reinterpret_cast<const float4*>(co + (w * 16 * RW + row) * D + d);
         Ls += cl[w * 16 * RW + row] * f;
         O.x += a.x * f, O.y += a.y * f, O.z += a.z * f, O.w += a.w * f;
@@ -419,25 +454,30 @@ __global__ void __launch_bounds__(kLogitThreads) fna2_paged_logit_weights_kernel
 // ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
+struct FewMaps {
+  CUtensorMap k, v, rk;
+};
+
 template <int D, int RW>
-cudaError_t launch_paged_few_t(const PagedAttnParams& p, size_t smem, cudaStream_t stream) {
+cudaError_t launch_paged_few_t(const FewMaps& m, const PagedAttnParams& p, size_t smem, cudaStream_t stream) {
   auto kern = fna2_paged_few_kernel<D, RW>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
   if (e != cudaSuccess) return e;
   const dim3 grid(p.bd.B * p.kv.hkv * p.row_blocks, (std::max(1, p.bd.max_k) + p.chunk - 1) / p.chunk);
-  kern<<<grid, kFewThreads, smem, stream>>>(p);
+  kern<<<grid, kFewThreads, smem, stream>>>(m.k, m.v, m.rk, p);
   return cudaGetLastError();
 }
 
 template <int D>
-cudaError_t launch_paged_few_d(const PagedAttnParams& p, int RW, size_t smem, cudaStream_t stream) {
-  return RW == 1   ? launch_paged_few_t<D, 1>(p, smem, stream)
-         : RW == 2 ? launch_paged_few_t<D, 2>(p, smem, stream)
-                   : launch_paged_few_t<D, 4>(p, smem, stream);
+cudaError_t launch_paged_few_d(const FewMaps& m, const PagedAttnParams& p, int RW, size_t smem, cudaStream_t stream) {
+  return RW == 1   ? launch_paged_few_t<D, 1>(m, p, smem, stream)
+         : RW == 2 ? launch_paged_few_t<D, 2>(m, p, smem, stream)
+                   : launch_paged_few_t<D, 4>(m, p, smem, stream);
 }
 
-inline cudaError_t launch_paged_few(const PagedAttnParams& p, int D, int RW, size_t smem, cudaStream_t stream) {
-  return D == 128 ? launch_paged_few_d<128>(p, RW, smem, stream) : launch_paged_few_d<64>(p, RW, smem, stream);
+inline cudaError_t launch_paged_few(const FewMaps& m, const PagedAttnParams& p, int D, int RW, size_t smem,
+                                    cudaStream_t stream) {
+  return D == 128 ? launch_paged_few_d<128>(m, p, RW, smem, stream) : launch_paged_few_d<64>(m, p, RW, smem, stream);
 }
 
 // What follows the attention kernels: the join of the splits and the weights from kept logits.

@@ -420,7 +420,7 @@ def test_python_refusals():
         naylis_evict(w, pool, d["table"], d["lens"], 8, d["table"][:, :1], recent=9, heads=4)
     with pytest.raises(ValueError, match="page_table_out"):
         naylis_evict(w, pool, d["table"], d["lens"], 8, d["table"][:1], heads=4)
-    with pytest.raises(ValueError, match="same dtype"):
+    with pytest.raises(TypeError, match="k must be"):
         qk_norm_rope_append(d["q"], d["q"][:, :2].float(), d["q"][:, :2], pool, d["table"], d["lens"], d["cu"])
     with pytest.raises(ValueError, match="r_k"):
         qk_norm_rope_append(d["q"], d["q"][:, :2], d["q"][:, :2], pool, d["table"], d["lens"], d["cu"])

@@ -28,6 +28,10 @@ def test_struct_layout_matches_c(tmp_path):
         c = getattr(_lib, s)
         want += [ctypes.sizeof(c)] + [getattr(c, n).offset for n in f]
     assert got == want
+    from fna2_b200 import paged  # the packed blocks of the Python layer end where the structures do
+    for block, s in ((paged._ATTN_ARGS, _lib.Fna2PagedAttnArgs), (paged._APPEND_ARGS, _lib.Fna2AppendArgs),
+                     (paged._EVICT_ARGS, _lib.Fna2EvictArgs)):
+        assert block.size == ctypes.sizeof(s)
 
 
 @pytest.fixture
