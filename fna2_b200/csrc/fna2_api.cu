@@ -761,17 +761,16 @@ int paged_queries(const Fna2PagedKV* kv, const Fna2PagedAttnArgs* a, P* p) {
 struct PagedPlan {
   int RW;
   bool few, many;  // kernels to launch
+  bool few_join, many_join;  // and what joins their parts
   bool logits;     // key weights from kept logits (few rows everywhere); otherwise recomputed by the key weights kernel
-  size_t smem, acc_bytes, ml_bytes, logit_bytes, lse_bytes, kw_bytes, total;
+  size_t smem;
+  // workspace offsets
+  size_t acc, ml, part_acc, part_ml, prefix, logit, lse2, lse, kw, total;
 };
 
 size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 
 constexpr int kSms = 148;
-// Query rows per KV head (new tokens x query heads of the group) up to which a sequence is streamed
-// by the mma.sync kernel; above it the tensor-core kernel's 128-row tiles are worth filling.
-constexpr int kFewRows = 64;
-
 // Splits of the tensor-core kernel's keys: `base` CTAs without splits, `tiles` key tiles each.  One
 // CTA runs per SM; a tile takes about 2 us, a CTA's start and end 6 us, and the join moves 8 D bytes
 // per row and split.  Takes the count with the least estimated time.
@@ -791,30 +790,31 @@ int paged_plan(const Fna2PagedKV* kv, const Fna2PagedAttnArgs* a, PagedAttnParam
   const bool all_few = max_rows <= kFewRows;
   l->few = all_few || p->bd.B > 1;
   l->many = !all_few;
-  p->few_rows = all_few ? max_rows : l->few ? kFewRows : 0;
-  // few rows: the row blocks of a CTA; in a mixed call most of these sequences add one token
-  const int few_max = std::min(max_rows, kFewRows);
+  p->few_rows = all_few ? max_rows : l->few ? kFewRowsMixed : 0;
+  const int few_max = std::min(max_rows, p->few_rows);
   l->RW = !all_few || max_rows <= 16 ? 1 : max_rows <= 32 ? 2 : 4;
   for (;; l->RW /= 2) {
     p->ng_max = std::min({p->G, 16 * l->RW, p->kv.hg});
     p->nh_max = std::min({p->G, 16, p->kv.hg});
-    // ring depth: at most 4 tiles, fewer where two CTAs per SM then fit
-    for (p->stages = 4; p->stages > 2; --p->stages)
-      if (FewSmem(D, l->RW, p->ng_max, p->nh_max, p->RP, p->stages).total <= 113 * 1024) break;
-    l->smem = std::max<size_t>(FewSmem(D, l->RW, p->ng_max, p->nh_max, p->RP, p->stages).total, 512 + 64 * D * 4);
+    // ring depth: about 64 KB of tiles per CTA, at most 8 and at least 2 of them
+    const FewSmem one(D, l->RW, p->ng_max, p->nh_max, p->RP, 1, p->few_rows);
+    p->stages = std::max(2, std::min(8, 72 * 1024 / ((one.kv_stage + one.r_stage) * (4 / l->RW))));
+    l->smem = FewSmem(D, l->RW, p->ng_max, p->nh_max, p->RP, p->stages, p->few_rows).total;
     if ((l->smem <= kMaxDynamicSmem && 2 * D / 64 + p->ng_max <= 32) || l->RW == 1) break;  // a lane per box
   }
   FNA2_CHECK(l->smem <= kMaxDynamicSmem, "heads per KV head and rank need too much shared memory");
-  p->row_blocks = (few_max + 16 * l->RW - 1) / (16 * l->RW);
-  const int64_t ctas = static_cast<int64_t>(p->bd.B) * p->kv.hkv * (all_few ? p->row_blocks : 1);
-  FNA2_CHECK(static_cast<int64_t>(p->bd.B) * p->kv.hkv * p->row_blocks < (1ll << 31), "too many query rows");
-  const int64_t max_k = std::max(1, p->bd.max_k);
-  int64_t splits = a->num_splits;
-  if (splits <= 0)  // about two waves of two CTAs per SM, at least 256 keys a split
-    splits = std::max<int64_t>(1, std::min<int64_t>((4 * kSms + ctas - 1) / std::max<int64_t>(ctas, 1), (max_k + 255) / 256));
-  splits = std::min<int64_t>(splits, 4096);
-  p->chunk = static_cast<int>(((max_k + splits - 1) / splits + 63) / 64 * 64);
-  p->ns = l->few ? static_cast<int>((max_k + p->chunk - 1) / p->chunk) : 1;
+  p->block_rows = 16 * l->RW;
+  p->unit_keys = 64 / l->RW;
+  p->row_blocks = std::max(1, (few_max + p->block_rows - 1) / p->block_rows);
+  const int64_t max_k = std::max(1, p->bd.max_k), lanes = static_cast<int64_t>(p->kv.hkv) * p->row_blocks;
+  const int64_t seq_units = (max_k + p->unit_keys - 1) / p->unit_keys;
+  // Sequences of at most 8 units (512 keys of up to 16 rows) are not worth the second launch that joins parts.
+  p->whole = a->num_splits <= 0 ? seq_units <= 8 : a->num_splits == 1;
+  // As many runs as two CTAs per SM allow (num_splits: that many per sequence), and no more than units.
+  const int64_t runs = a->num_splits > 0 ? static_cast<int64_t>(a->num_splits) * p->bd.B : 2 * kSms / lanes;
+  p->runs = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(runs, p->bd.B * (p->whole ? 1 : seq_units))));
+  FNA2_CHECK(p->runs * lanes < (1ll << 30), "too many splits (%d)", a->num_splits);
+  p->ns = 1;
   if (l->many) {
     // pairs of query tiles: at least `pairs`, at most one more per sequence that has more than few_rows rows
     const int64_t pairs = (static_cast<int64_t>(p->bd.T) + 2 * kBlockM - 1) / (2 * kBlockM);
@@ -826,17 +826,30 @@ int paged_plan(const Fna2PagedKV* kv, const Fna2PagedAttnArgs* a, PagedAttnParam
     const int64_t ns = (max_k + p->chunk_many - 1) / p->chunk_many;
     FNA2_CHECK((pairs + longer) * ns <= 65535, "too many query tiles and splits (%lld)", (long long)((pairs + longer) * ns));
     p->many_items = static_cast<int>((pairs + longer) * ns);
-    p->ns = std::max(p->ns, static_cast<int>(ns));
+    p->ns = static_cast<int>(ns);
   }
-  const size_t th = static_cast<size_t>(p->bd.T) * p->H;
-  p->logit_sr = (static_cast<int64_t>(p->bd.max_k) + 15) / 16 * 16;
   l->logits = p->kw && all_few;
-  l->acc_bytes = p->ns > 1 ? up256(th * p->ns * D * 4) : 0;
-  l->ml_bytes = p->ns > 1 || l->logits ? up256(th * p->ns * 8) : 0;
-  l->logit_bytes = l->logits ? up256(static_cast<size_t>(p->bd.B) * p->kv.hkv * max_rows * p->logit_sr * 4) : 0;
-  l->lse_bytes = p->kw && !l->logits && !a->lse ? up256(th * 4) : 0;
-  l->kw_bytes = p->kw && !l->logits ? up256(th * 4) + up256(static_cast<size_t>(p->bd.T) * p->kv.hg * 4 * p->RP) : 0;
-  l->total = l->acc_bytes + l->ml_bytes + l->logit_bytes + l->lse_bytes + l->kw_bytes;
+  l->many_join = l->many && p->ns > 1;
+  l->few_join = l->few && !p->whole && p->runs > 1;
+  p->logit_sr = (static_cast<int64_t>(p->bd.max_k) + 15) / 16 * 16;
+  const size_t th = static_cast<size_t>(p->bd.T) * p->H;
+  size_t at = 0;
+  auto take = [&at](bool need, size_t bytes) {
+    const size_t o = at;
+    if (need) at += (bytes + 255) / 256 * 256;
+    return o;
+  };
+  const size_t parts = static_cast<size_t>(p->runs) * lanes * 2 * p->block_rows;
+  l->acc = take(l->many_join, th * p->ns * D * 4);
+  l->ml = take(l->many_join, th * p->ns * 8);
+  l->part_acc = take(l->few_join, parts * D * 4);
+  l->part_ml = take(l->few_join, parts * 8);
+  l->prefix = take(l->few_join, (static_cast<size_t>(p->bd.B) + 1) * 8);
+  l->logit = take(l->logits, static_cast<size_t>(p->bd.B) * p->kv.hkv * max_rows * p->logit_sr * 4);
+  l->lse2 = take(l->logits, th * 4);
+  l->lse = take(p->kw && !l->logits && !a->lse, th * 4);
+  l->kw = take(p->kw && !l->logits, up256(th * 4) + up256(static_cast<size_t>(p->bd.T) * p->kv.hg * 4 * p->RP));
+  l->total = at;
   return FNA2_OK;
 }
 
@@ -968,10 +981,14 @@ extern "C" int fna2_paged_attn(const Fna2PagedKV* kv, const Fna2PagedAttnArgs* a
   p.out = static_cast<__nv_bfloat16*>(a->out), p.o_st = a->out_token_stride, p.o_sh = a->out_head_stride;
   p.lse = a->lse, p.lse_sh = a->lse_head_stride;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
-  p.ws_acc = l.acc_bytes ? reinterpret_cast<float*>(ws) : nullptr;
-  p.ws_ml = l.ml_bytes ? reinterpret_cast<float2*>(ws + l.acc_bytes) : nullptr;
-  p.logits = l.logits ? reinterpret_cast<float*>(ws + l.acc_bytes + l.ml_bytes) : nullptr;
-  if (l.lse_bytes) p.lse = reinterpret_cast<float*>(ws + l.acc_bytes + l.ml_bytes + l.logit_bytes), p.lse_sh = p.bd.T;
+  p.ws_acc = reinterpret_cast<float*>(ws + l.acc);
+  p.ws_ml = reinterpret_cast<float2*>(ws + l.ml);
+  p.part_acc = reinterpret_cast<float*>(ws + l.part_acc);
+  p.part_ml = reinterpret_cast<float2*>(ws + l.part_ml);
+  p.prefix = l.few_join ? reinterpret_cast<int64_t*>(ws + l.prefix) : nullptr;
+  p.logits = l.logits ? reinterpret_cast<float*>(ws + l.logit) : nullptr;
+  p.lse2 = l.logits ? reinterpret_cast<float*>(ws + l.lse2) : nullptr;
+  if (p.kw && !l.logits && !p.lse) p.lse = reinterpret_cast<float*>(ws + l.lse), p.lse_sh = p.bd.T;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (l.many) {
     ManyMaps m;
@@ -983,12 +1000,14 @@ extern "C" int fna2_paged_attn(const Fna2PagedKV* kv, const Fna2PagedAttnArgs* a
     if (int rc = few_maps(p, kv->head_dim, &m)) return rc;
     FNA2_CUDA(launch_paged_few(m, p, kv->head_dim, l.RW, l.smem, st));
   }
-  FNA2_CUDA(launch_paged_tail(p, kv->head_dim, st));
+  if (l.many_join) FNA2_CUDA(launch_paged_many_join(p, kv->head_dim, st));
+  if (l.few_join) FNA2_CUDA(launch_paged_few_join(p, kv->head_dim, st));
+  if (l.logits && p.bd.max_k > 0) FNA2_CUDA(launch_logit_weights(p, st));
   if (p.kw && !l.logits && p.bd.max_k > 0) {
     KeyWeightsParams w{};
     if (int rc = paged_queries(kv, a, &w)) return rc;
     w.lse = p.lse, w.lse_sh = p.lse_sh;
-    if (int rc = run_key_weights(w, kv->head_dim, ws + (l.total - l.kw_bytes), st)) return rc;
+    if (int rc = run_key_weights(w, kv->head_dim, ws + l.kw, st)) return rc;
   }
   return FNA2_OK;
 }
@@ -1043,6 +1062,7 @@ extern "C" int fna2_evict(const Fna2PagedKV* kv, const Fna2EvictArgs* a, void* s
   p.table_out = a->page_table_out, p.table_out_sb = a->table_out_stride;
   p.cap_out = a->max_pages_out * kv->page_size;
   p.kept = a->kept, p.lens_out = a->seqlens_out, p.w_out = a->weights_out;
-  FNA2_CUDA(launch_evict(p, kv->head_dim, static_cast<cudaStream_t>(stream)));
+  p.D = kv->head_dim;
+  FNA2_CUDA(launch_evict(p, static_cast<cudaStream_t>(stream)));
   return FNA2_OK;
 }

@@ -18,7 +18,7 @@ namespace fna2 {
 struct EvictParams {
   PagedPool kv;  // source table
   const int* lens;
-  int B, G, max_k, budget, sink, recent;
+  int B, G, D, max_k, budget, sink, recent;
   const float* w;
   int64_t w_sb, w_sh;
   const int* table_out;
@@ -28,6 +28,74 @@ struct EvictParams {
   int* lens_out;     // [B]
   float* w_out;      // [B][HKV][cap_out], 0 past the kept count
 };
+
+struct RowPlace {
+  int sp, ss, dp, ds;  // source page (-1: none) and slot, destination page and slot
+};
+
+// Copies kept rows [r0, r0 + ROWS) of (sequence b, KV head kh) with a block of THREADS threads.
+template <int THREADS, int ROWS>
+__device__ __forceinline__ void move_rows(const EvictParams& p, int b, int kh, int r0, RowPlace* s_at) {
+  const int* kept = p.kept + (static_cast<int64_t>(b) * p.kv.hkv + kh) * p.budget;
+  const int mask = (1 << p.kv.page_log2) - 1, tid = threadIdx.x;
+  if (tid < ROWS) {
+    const int r = r0 + tid, j = r < p.budget ? kept[r] : -1;
+    RowPlace a{-1, j & mask, -1, r & mask};
+    if (j >= 0) {
+      a.sp = __ldg(p.kv.table + b * p.kv.table_sb + (j >> p.kv.page_log2));
+      a.dp = __ldg(p.table_out + b * p.table_out_sb + (r >> p.kv.page_log2));
+      if (a.sp < 0 || a.sp >= p.kv.pages || a.dp < 0 || a.dp >= p.kv.pages) {
+        atomicCAS(&g_device_error, 0, kStatusBadSeqEvict);
+        a.sp = -1;
+      }
+    }
+    s_at[tid] = a;
+  }
+  __syncthreads();
+  // K and V: 2 D / 8 lanes a row, four rows in flight per lane
+  constexpr int U = 4;
+  const int warp = tid >> 5, lane = tid & 31, lpr = p.D / 4, rpw = 32 / lpr;
+  const int sub = lane % lpr, is_v = sub >= lpr / 2, col = sub % (lpr / 2) * 8;
+  const PagedRows kv = {is_v ? p.kv.v.ptr : p.kv.k.ptr, is_v ? p.kv.v.sp : p.kv.k.sp, is_v ? p.kv.v.st : p.kv.k.st,
+                        is_v ? p.kv.v.sh : p.kv.k.sh};
+  for (int base = warp * rpw * U; base < ROWS; base += THREADS / 32 * rpw * U) {
+    uint4 v[U];
+    __nv_bfloat16* dst[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int r = base + i * rpw + lane / lpr;
+      dst[i] = nullptr;
+      if (r < ROWS && s_at[r].sp >= 0) {
+        const RowPlace a = s_at[r];
+        v[i] = *reinterpret_cast<const uint4*>(kv.ptr + paged_off(kv, a.sp, a.ss, kh) + col);
+        dst[i] = kv.ptr + paged_off(kv, a.dp, a.ds, kh) + col;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+      if (dst[i]) *reinterpret_cast<uint4*>(dst[i]) = v[i];
+  }
+  // R_k of the KV head's query heads
+  const int r8 = p.kv.rank / 8, pieces = max(0, min(p.G, p.kv.hg - kh * p.G)) * r8;
+  for (int base = tid; base < ROWS * pieces; base += THREADS * U) {
+    uint4 v[U];
+    __nv_bfloat16* dst[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int e = base + i * THREADS, r = e / pieces, c = e % pieces;
+      dst[i] = nullptr;
+      if (e < ROWS * pieces && s_at[r].sp >= 0) {
+        const RowPlace a = s_at[r];
+        const int64_t at = (kh * p.G + c / r8) * p.kv.rk.sh + c % r8 * 8;
+        v[i] = *reinterpret_cast<const uint4*>(p.kv.rk.ptr + paged_off(p.kv.rk, a.sp, a.ss, 0) + at);
+        dst[i] = p.kv.rk.ptr + paged_off(p.kv.rk, a.dp, a.ds, 0) + at;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+      if (dst[i]) *reinterpret_cast<uint4*>(dst[i]) = v[i];
+  }
+}
 
 constexpr int kSelThreads = 1024;
 constexpr int kSelBins = 2048;
@@ -39,8 +107,11 @@ __device__ __forceinline__ uint32_t ordered_bits(float x) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
+// MOVE: the block also copies its rows (short sequences: one launch instead of two).
+template <bool MOVE>
 __global__ void __launch_bounds__(kSelThreads) fna2_evict_select_kernel(const EvictParams p) {
   __shared__ int hist[kSelBins];
+  __shared__ RowPlace s_at[MOVE ? kSelThreads : 1];
   __shared__ int s_warp[2][32];
   __shared__ int s_digit, s_above;
   const int kh = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -129,55 +200,36 @@ __global__ void __launch_bounds__(kSelThreads) fna2_evict_select_kernel(const Ev
   for (int i = keep + tid; i < p.budget; i += kSelThreads) kept[i] = -1;
   for (int i = keep + tid; i < p.cap_out; i += kSelThreads) w_out[i] = 0.f;
   if (kh == 0 && tid == 0) p.lens_out[b] = keep;
+  if (MOVE) {
+    for (int r0 = 0; r0 < keep; r0 += kSelThreads) {
+      __syncthreads();  // kept is written; s_at has been read
+      move_rows<kSelThreads, kSelThreads>(p, b, kh, r0, s_at);
+    }
+  }
 }
 
 constexpr int kMoveThreads = 128;
 constexpr int kMoveRows = 32;
 
-__global__ void __launch_bounds__(kMoveThreads) fna2_evict_move_kernel(const EvictParams p, int D) {
-  __shared__ int s_src[kMoveRows][2], s_dst[kMoveRows][2];  // page, slot
-  const int kh = blockIdx.y, b = blockIdx.z, r0 = blockIdx.x * kMoveRows, tid = threadIdx.x;
-  const int* kept = p.kept + (static_cast<int64_t>(b) * p.kv.hkv + kh) * p.budget;
-  const int mask = (1 << p.kv.page_log2) - 1;
-  if (tid < kMoveRows) {
-    const int r = r0 + tid, j = r < p.budget ? kept[r] : -1;
-    int sp = -1, dp = -1;
-    if (j >= 0) {
-      sp = __ldg(p.kv.table + b * p.kv.table_sb + (j >> p.kv.page_log2));
-      dp = __ldg(p.table_out + b * p.table_out_sb + (r >> p.kv.page_log2));
-      if (sp < 0 || sp >= p.kv.pages || dp < 0 || dp >= p.kv.pages) {
-        atomicCAS(&g_device_error, 0, kStatusBadSeqEvict);
-        sp = -1;
-      }
-    }
-    s_src[tid][0] = sp, s_src[tid][1] = j & mask;
-    s_dst[tid][0] = dp, s_dst[tid][1] = r & mask;
-  }
-  __syncthreads();
-  const int ppr = D / 8, r8 = p.kv.rank / 8, ng = max(0, min(p.G, p.kv.hg - kh * p.G));
-  const int pieces = 2 * ppr + ng * r8;
-  for (int e = tid; e < kMoveRows * pieces; e += kMoveThreads) {
-    const int r = e / pieces, c = e % pieces;
-    const int sp = s_src[r][0], ss = s_src[r][1], dp = s_dst[r][0], ds = s_dst[r][1];
-    if (sp < 0) continue;
-    if (c < 2 * ppr) {
-      const PagedRows& t = c < ppr ? p.kv.k : p.kv.v;
-      const int col = c % ppr * 8;
-      *reinterpret_cast<uint4*>(t.ptr + paged_off(t, dp, ds, kh) + col) =
-          *reinterpret_cast<const uint4*>(t.ptr + paged_off(t, sp, ss, kh) + col);
-    } else {
-      const int h = kh * p.G + (c - 2 * ppr) / r8, col = (c - 2 * ppr) % r8 * 8;
-      *reinterpret_cast<uint4*>(p.kv.rk.ptr + paged_off(p.kv.rk, dp, ds, h) + col) =
-          *reinterpret_cast<const uint4*>(p.kv.rk.ptr + paged_off(p.kv.rk, sp, ss, h) + col);
-    }
-  }
+__global__ void __launch_bounds__(kMoveThreads) fna2_evict_move_kernel(const EvictParams p) {
+  __shared__ RowPlace s_at[kMoveRows];
+  move_rows<kMoveThreads, kMoveRows>(p, blockIdx.z, blockIdx.y, blockIdx.x * kMoveRows, s_at);
 }
 
-inline cudaError_t launch_evict(const EvictParams& p, int D, cudaStream_t stream) {
-  fna2_evict_select_kernel<<<dim3(p.kv.hkv, p.B), kSelThreads, 0, stream>>>(p);
+// A block of the select kernel moves about 60 GB/s; up to this many kept rows that costs less than a
+// second launch.
+constexpr int kFusedBudget = 512;
+
+inline cudaError_t launch_evict(const EvictParams& p, cudaStream_t stream) {
+  const dim3 heads(p.kv.hkv, p.B);
+  if (p.budget <= kFusedBudget) {
+    fna2_evict_select_kernel<true><<<heads, kSelThreads, 0, stream>>>(p);
+    return cudaGetLastError();
+  }
+  fna2_evict_select_kernel<false><<<heads, kSelThreads, 0, stream>>>(p);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return e;
-  fna2_evict_move_kernel<<<dim3((p.budget + kMoveRows - 1) / kMoveRows, p.kv.hkv, p.B), kMoveThreads, 0, stream>>>(p, D);
+  fna2_evict_move_kernel<<<dim3((p.budget + kMoveRows - 1) / kMoveRows, p.kv.hkv, p.B), kMoveThreads, 0, stream>>>(p);
   return cudaGetLastError();
 }
 

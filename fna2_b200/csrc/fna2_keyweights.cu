@@ -307,7 +307,8 @@ template <int D, int RP>
 cudaError_t launch_key_weights_t(const KwMaps& m, const KeyWeightsParams& p, cudaStream_t stream) {
   using L = KwSmem<D, RP>;
   auto kern = fna2_key_weights_kernel<D, RP>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kTotal);
+  static std::atomic<uint64_t> allowed{0};
+  cudaError_t e = allow_smem(reinterpret_cast<const void*>(kern), allowed);
   if (e != cudaSuccess) return e;
   const int64_t n = static_cast<int64_t>(p.bd.T) * std::max<int64_t>(p.H, static_cast<int64_t>(p.kv.hg) * p.RP / 8);
   fna2_key_weights_prep_kernel<<<static_cast<unsigned>((n + 255) / 256), 256, 0, stream>>>(p);

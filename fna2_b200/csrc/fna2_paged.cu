@@ -15,17 +15,24 @@
 // rounding of the bias would show in them (2^-9 of the bias).  P is rounded to
 // bf16 for P V (the output is bf16); the row sums use the unrounded P.
 //
-// One CTA serves (sequence, KV head, block of 16 RW query rows, key split).  A
-// query row is (query head of the KV group, new token), head-major, so that the
-// 16 rows of a warp span few heads.  4 warps: RW row blocks x 4/RW key groups; a
-// key group streams its own 16-key tiles through a ring in shared memory that its
-// RW warps read together (mma.sync m16n8k16, fp32 accumulation, online softmax
-// in registers).  16 keys never cross a page, so a tile is one TMA box per 64
-// columns of K and V and one per head of R_k, issued by as many lanes; 128-byte
-// (R_k: 32- or 64-byte) swizzled rows give conflict-free ldmatrix reads.  (With one
-// cp.async per 16 bytes the address arithmetic was 3/4 of the 820 instructions a
-// tile took, and the kernel was bound by their issue at 5.1 TB/s.)
-// Bound: HBM; each cached key is read once per row block.
+// A unit is 64/RW keys of a sequence.  The units of all sequences, in order, are
+// cut into equal runs, whatever the lengths, and each run is taken by one CTA for
+// every (KV head, block of 16 RW query rows): as many runs as fill the GPU once, and
+// all heads' rows of the same keys are read at the same time (in a pool laid out by
+// token they are neighbours in memory; with runs cut per head instead, DRAM gave
+// 5.8 instead of 6.8 TB/s).  A run covers the end of one sequence, whole ones and the
+// start of another, and fna2_paged_few_join_kernel joins the sequences that were
+// cut.  A query row is (query head of the KV group, new token), head-major,
+// so that the 16 rows of a warp span few heads.  4 warps: RW row blocks x 4/RW key
+// groups; a key group streams its own 16-key tiles through a ring in shared memory
+// that its RW warps read together (mma.sync m16n8k16, fp32 accumulation, online
+// softmax in registers).  16 keys never cross a page, so a tile is one TMA box per
+// 64 columns of K and V and one per head of R_k, issued by as many lanes; 128-byte
+// (R_k: 32- or 64-byte) swizzled rows give conflict-free ldmatrix reads.
+// Bound: HBM; each cached key is read once per row block.  A warp takes about 1600
+// clk per tile, latency rather than issue (313 instructions), so an SM needs its 8
+// warps; about 140 KB of loads in flight per SM suffice (deeper rings measured the
+// same or slower).
 #include "fna2_paged.cuh"
 
 namespace fna2 {
@@ -46,35 +53,60 @@ struct PagedAttnParams {
   int64_t o_st, o_sh;
   float* lse;  // [H][lse_sh], or NULL
   int64_t lse_sh;
-  int chunk, ns;      // keys per split, splits per sequence at most
+  // tensor-core kernel: its splits of a sequence, at most ns of them
+  int ns;
   float* ws_acc;      // [(t * H + h) * ns + split][D]: unnormalised output of a split
   float2* ws_ml;      // [(t * H + h) * ns + split]: its row max (log2 domain) and sum
+  // mma.sync kernel: a CTA's first and last sequence may be parts of one
+  float* part_acc;    // [(cta * 2 + first or last) * block_rows + row][D]
+  float2* part_ml;    // [(cta * 2 + first or last) * block_rows + row]
+  int64_t* prefix;    // [B + 1] units before each sequence, then their number
+  float* lse2;        // [t * H + h] log2-domain LSE of the rows of sequences not cut (kept with logits)
   float* logits;      // key weights: [((b * HKV + kh) * max_q * G + row)][logit_sr] log2-domain logits, or NULL
   int64_t logit_sr;
   float* kw;          // key weights, added to: [b * kw_sb + kh * kw_sh + j]
   int64_t kw_sb, kw_sh;
-  int row_blocks, ng_max, nh_max, stages;
+  int block_rows;     // 16 RW
+  int unit_keys;      // 64 / RW
+  int whole;          // sequences are not cut (they are short): a unit is a sequence
+  int runs;           // at most
+  int row_blocks;     // row blocks per KV head; CTA = (run * HKV + KV head) * row_blocks + row block
+  int ng_max, nh_max, stages;
   // Sequences of more than few_rows query rows (new tokens x query heads of a KV head) go to
   // fna2_paged_many_kernel, the others to fna2_paged_few_kernel; a call launches those it may need.
   int few_rows;
   int chunk_many, many_items;  // keys per split there, upper bound on its (query tile pair, split) items
 };
 
-// Splits of a sequence that hold keys.
-__device__ __forceinline__ int paged_splits(const PagedAttnParams& p, const PagedSeq& s) {
-  const int chunk = s.n * p.G > p.few_rows ? p.chunk_many : p.chunk;
-  return max(1, (s.len + chunk - 1) / chunk);
+// Units of one sequence in the mma.sync kernel: 0 when it is not this kernel's.
+__device__ __forceinline__ int few_units(const PagedAttnParams& p, const PagedSeq& s) {
+  const int rows = s.n * p.G;
+  if (rows == 0 || rows > p.few_rows) return 0;
+  return p.whole ? 1 : max(1, (s.len + p.unit_keys - 1) / p.unit_keys);
 }
+// Runs that share U units (each takes at least one); the first unit of run c; the run of unit u.
+__device__ __forceinline__ int few_runs(const PagedAttnParams& p, int64_t U) {
+  return static_cast<int>(min(static_cast<int64_t>(p.runs), max(U, static_cast<int64_t>(1))));
+}
+__device__ __forceinline__ int64_t few_first(int64_t U, int C, int c) { return U * c / C; }
+__device__ __forceinline__ int few_run_of(int64_t U, int C, int64_t u) { return static_cast<int>(((u + 1) * C - 1) / U); }
+
+// Query rows per KV head (new tokens x query heads of the group) up to which a sequence is streamed
+// by the mma.sync kernel; above it the tensor-core kernel's 128-row tiles are worth filling.
+constexpr int kFewRows = 64;
+// ... in a call that has longer ones: its few-row sequences mostly add one token, in one 16-row block.
+constexpr int kFewRowsMixed = 16;
 
 constexpr int kFewThreads = 128;
 constexpr int kFewKeys = 16;  // keys per tile
 
 // Shared-memory geometry (host and device agree on it): [A of the RW row blocks | K and V ring of
-// the key groups | R_k ring | barriers]; ng: graph heads of a block's rows, nh: heads that the 16
+// the key groups | R_k ring | m, l and accumulators of the key groups | barriers]; ng: graph heads of a block's rows, nh: heads that the 16
 // rows of one warp span.
 struct FewSmem {
-  int a_stride, kv_stage, r_head, r_stage, o_kv, o_r, o_bar, total;
-  __host__ __device__ FewSmem(int D, int RW, int ng, int nh, int RP, int stages) {
+  int a_stride, kv_stage, r_head, r_stage, o_kv, o_r, o_join, o_bar, total;
+  // (of the row block's rows only `rows`, its bound, are joined)
+  __host__ __device__ FewSmem(int D, int RW, int ng, int nh, int RP, int stages, int rows) {
     a_stride = (D + 2 * nh * RP) * 2 + 16;
     kv_stage = 2 * kFewKeys * D * 2;
     r_head = kFewKeys * RP * 2;
@@ -82,10 +114,25 @@ struct FewSmem {
     const int rings = 4 / RW * stages;
     o_kv = (16 * RW * a_stride + 1023) / 1024 * 1024;
     o_r = o_kv + rings * kv_stage;
-    o_bar = o_r + (rings * r_stage + 1023) / 1024 * 1024;
-    total = o_bar + 2 * rings * 8 + 16;
+    o_join = o_r + (rings * r_stage + 1023) / 1024 * 1024;
+    o_bar = o_join + 512 + 4 / RW * (rows < 16 * RW ? rows : 16 * RW) * D * 4;
+    total = o_bar + 2 * rings * 8 + 64;
   }
 };
+
+// Four columns of a finished row: O = acc / (l + 1e-6), LSE = m + log(l + 1e-6).
+template <int D>
+__device__ __forceinline__ void few_store(const PagedAttnParams& p, int64_t tok, int h, int d, float M, float Ls,
+                                          const float4& O) {
+  const float inv = 1.f / (Ls + kEps);
+  *reinterpret_cast<uint2*>(p.out + tok * p.o_st + h * p.o_sh + d) =
+      make_uint2(pack_bf16(O.x * inv, O.y * inv), pack_bf16(O.z * inv, O.w * inv));
+  if (d == 0) {
+    const float lse2 = M == -INFINITY ? M : M + log2f(Ls + kEps);
+    if (p.lse) p.lse[h * p.lse_sh + tok] = lse2 * kLn2;
+    if (p.lse2) p.lse2[tok * p.H + h] = lse2;
+  }
+}
 
 template <int D, int RW>
 __global__ void __launch_bounds__(kFewThreads, 2)
@@ -98,65 +145,103 @@ __global__ void __launch_bounds__(kFewThreads, 2)
     if (threadIdx.x == 0) atomicCAS(&g_device_error, 0, kStatusSmemBase);
     return;
   }
-  const int split = blockIdx.y;
-  const int rb = blockIdx.x % p.row_blocks;
-  const int kh = (blockIdx.x / p.row_blocks) % p.kv.hkv;
-  const int b = blockIdx.x / (p.row_blocks * p.kv.hkv);
+  const int cta = blockIdx.x, lanes = p.kv.hkv * p.row_blocks, run = cta / lanes;
+  const int kh = cta % lanes / p.row_blocks, r0 = cta % p.row_blocks * (16 * RW);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int rw = warp % RW, kg = warp / RW;
-  const PagedSeq sq = paged_seq(p.bd, b);
-  if (!sq.ok && tid == 0) atomicCAS(&g_device_error, 0, kStatusBadSeqPaged);
-  const int rows = sq.n * p.G;                 // row r: head r / n of the group, new token r % n
-  const int r0 = rb * 16 * RW;                 // first row of this block
-  if (r0 >= rows || rows > p.few_rows) return;
-  const int past = sq.len - sq.n;              // may be negative: the first rows then see no key
-  // splits of this sequence that hold keys (split 0 always exists: it writes rows that see nothing)
-  const int ns = paged_splits(p, sq);
-  if (split >= ns) return;
-  const int r_last = min(rows, r0 + 16 * RW) - 1;
-  // graph heads of the block's rows, local to the group
-  const int g_lo = r0 / sq.n, g_hi = min(r_last / sq.n, p.kv.hg - kh * p.G - 1);
-  const int ng = max(0, g_hi - g_lo + 1);
-  const FewSmem L(D, RW, p.ng_max, p.nh_max, p.RP, p.stages);
+  const FewSmem L(D, RW, p.ng_max, p.nh_max, p.RP, p.stages, p.few_rows);
   uint64_t* full = reinterpret_cast<uint64_t*>(dsm + L.o_bar) + kg * p.stages;
   uint64_t* empty = full + KW * p.stages;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(dsm + L.o_bar + 2 * KW * p.stages * 8);
+  int64_t* s_scan = reinterpret_cast<int64_t*>(dsm + L.o_bar + 2 * KW * p.stages * 8 + 16);  // [4], prefix
+  int* s_first = const_cast<int*>(abort_flag) + 1;
   if (tid == 0) {
     for (int s = 0; s < KW * p.stages; ++s) {
-      mbar_init(full + s, 1);
-      mbar_init(empty + s, RW);
+      mbar_init(reinterpret_cast<uint64_t*>(dsm + L.o_bar) + s, 1);
+      mbar_init(reinterpret_cast<uint64_t*>(dsm + L.o_bar) + KW * p.stages + s, RW);
     }
     *abort_flag = 0;
     fence_mbar_init();
   }
+
+  // Number of units, this CTA's run [u, u_end) of them, and the sequence that unit u is in.
+  int64_t U = 0;
+  for (int b = tid; b < p.bd.B; b += kFewThreads) U += few_units(p, paged_seq(p.bd, b));
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) U += __shfl_xor_sync(0xffffffffu, U, o);
+  if (lane == 0) s_scan[warp] = U;
+  __syncthreads();
+  U = s_scan[0] + s_scan[1] + s_scan[2] + s_scan[3];
+  const int C = few_runs(p, U);
+  const int64_t u_beg = few_first(U, C, min(run, C)), u_end = few_first(U, C, min(run + 1, C));
+  int64_t carry = 0;
+  for (int base = 0; base < p.bd.B; base += kFewThreads) {
+    const int b = base + tid;
+    int units = 0;
+    if (b < p.bd.B) {
+      const PagedSeq s = paged_seq(p.bd, b);
+      if (!s.ok && cta == 0) atomicCAS(&g_device_error, 0, kStatusBadSeqPaged);
+      units = few_units(p, s);
+    }
+    int64_t incl = units;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += v;
+    }
+    __syncthreads();  // s_scan has been read
+    if (lane == 31) s_scan[warp] = incl;
+    __syncthreads();
+    int64_t pre = carry + incl - units;
+    for (int w = 0; w < warp; ++w) pre += s_scan[w];
+    carry += s_scan[0] + s_scan[1] + s_scan[2] + s_scan[3];
+    if (cta == 0 && b < p.bd.B && p.prefix) p.prefix[b] = pre;
+    if (units > 0 && pre <= u_beg && u_beg < pre + units) *s_first = b, s_scan[4] = pre;
+  }
+  if (cta == 0 && tid == 0 && p.prefix) p.prefix[p.bd.B] = U;
+  if (u_beg == u_end) return;
   __syncthreads();
 
-  // keys [k_begin, k_end) of this split that some row of the block sees
-  int seen = sq.len;
-  if (p.causal) {
-    // the largest new-token index among the block's rows
-    const int i_max = r_last - r0 + 1 >= sq.n || r_last / sq.n != r0 / sq.n ? sq.n - 1 : r_last % sq.n;
-    seen = max(0, past + i_max + 1);
-  }
-  const int k_begin = min(split * p.chunk, seen), k_end = min(seen, k_begin + p.chunk);
-  const int n_all = (k_end - k_begin + kFewKeys - 1) / kFewKeys;
-  const int n_tiles = n_all > kg ? (n_all - kg + KW - 1) / KW : 0;
+  // Current sequence: units [o_beg, o_end) of it.
+  int64_t u = u_beg, pre = s_scan[4];
+  int b = *s_first;
+  PagedSeq sq = paged_seq(p.bd, b);
+  int units = few_units(p, sq), rows, r_last, o_beg, o_end, past, g_lo, ng, k_begin, k_end, n_tiles;
+  const int* table;
+  auto segment = [&]() {
+    o_beg = static_cast<int>(u - pre);
+    o_end = static_cast<int>(min(static_cast<int64_t>(units), o_beg + (u_end - u)));
+    rows = sq.n * p.G;                          // row r: head r / n of the group, new token r % n
+    r_last = min(rows, r0 + 16 * RW) - 1;       // below r0: this block has no row of the sequence
+    past = sq.len - sq.n;                       // may be negative: the first rows then see no key
+    // graph heads of the block's rows, local to the group
+    g_lo = r0 / sq.n;
+    ng = max(0, min(r_last / sq.n, p.kv.hg - kh * p.G - 1) - g_lo + 1);
+    // keys that some row of the block sees
+    int seen = sq.len;
+    if (p.causal) {
+      const int i_max = r_last - r0 + 1 >= sq.n || r_last / sq.n != r0 / sq.n ? sq.n - 1 : r_last % sq.n;
+      seen = max(0, past + i_max + 1);
+    }
+    if (r0 >= rows) seen = 0;
+    k_begin = p.whole ? 0 : min(o_beg * p.unit_keys, seen);
+    k_end = p.whole ? seen : min(o_end * p.unit_keys, seen);
+    const int n_all = (k_end - k_begin + kFewKeys - 1) / kFewKeys;
+    n_tiles = n_all > kg ? (n_all - kg + KW - 1) / KW : 0;
+    table = p.kv.table + b * p.kv.table_sb;
+  };
+  segment();
 
   // Ring of the key group: lane l issues box l of a tile (K chunks, V chunks, R_k heads).
   uint8_t* kv_ring = dsm + L.o_kv + kg * p.stages * L.kv_stage;
   uint8_t* r_ring = dsm + L.o_r + kg * p.stages * L.r_stage;
-  const int* table = p.kv.table + b * p.kv.table_sb;
   const int lg = p.kv.page_log2, mask = (1 << lg) - 1;
-  const bool box = lane < 2 * DC + ng;
   const CUtensorMap* map = lane < DC ? &tmK : lane < 2 * DC ? &tmV : &tmRk;
   const int box_col = lane < 2 * DC ? lane % DC * 64 : 0;
-  const int box_head = lane < 2 * DC ? kh : kh * p.G + g_lo + lane - 2 * DC;
   uint8_t* box_dst = lane < 2 * DC ? kv_ring + lane * (kFewKeys * 128) : r_ring + (lane - 2 * DC) * L.r_head;
   const int box_step = lane < 2 * DC ? L.kv_stage : L.r_stage;
-  const int tile_bytes = L.kv_stage + ng * L.r_head;
   int issued = 0, i_stage = 0, i_phase = 1;  // empty barriers: the first round passes
-  int j_next = k_begin + kg * kFewKeys;
-  int page_next = n_tiles > 0 ? __ldg(table + (j_next >> lg)) : 0;
+  int j_next = 0, page_next = 0;
   auto issue = [&]() {
     if (issued >= n_tiles) return;
     const int page = page_next, slot = j_next & mask;
@@ -164,21 +249,33 @@ __global__ void __launch_bounds__(kFewThreads, 2)
     ++issued;
     if (issued < n_tiles) page_next = __ldg(table + (j_next >> lg));
     if (RW > 1) mbar_wait(empty + i_stage, i_phase, abort_flag, 131);
-    if (lane == 0) mbar_expect_tx(full + i_stage, tile_bytes);
+    if (lane == 0) mbar_expect_tx(full + i_stage, L.kv_stage + ng * L.r_head);
     __syncwarp();
-    if (box) tma_load_4d(box_dst + i_stage * box_step, map, full + i_stage, box_col, slot, box_head, page);
+    if (lane < 2 * DC + ng)
+      tma_load_4d(box_dst + i_stage * box_step, map, full + i_stage, box_col, slot,
+                  lane < 2 * DC ? kh : kh * p.G + g_lo + lane - 2 * DC, page);
     if (++i_stage == p.stages) i_stage = 0, i_phase ^= 1;
   };
-  if (rw == 0)
+  // The first tiles of a sequence; the ring is empty here.
+  auto start = [&]() {
+    if (rw != 0 || n_tiles == 0) return;
+    issued = 0;
+    j_next = k_begin + kg * kFewKeys;
+    page_next = __ldg(table + (j_next >> lg));
     for (int s = 0; s < p.stages - 1; ++s) issue();
+  };
+  start();
 
-  // A = [q | R~_q hi, lo of the warp's heads] of this warp's 16 rows (rows past the end are zero)
+  int stage = 0, phase = 0;
+  while (true) {
+  // A = [q | R~_q hi, lo of the warp's heads] of the row blocks' 16 rows each (rows past the end are zero)
   const int wr0 = r0 + rw * 16;
   const int wg_lo = wr0 / sq.n, wg_hi = min(min(rows - 1, wr0 + 15) / sq.n, p.kv.hg - kh * p.G - 1);
   const int wn = wr0 < rows ? max(0, wg_hi - wg_lo + 1) : 0;
   uint8_t* sa = dsm + rw * 16 * L.a_stride;
-  if (kg == 0) {
-    for (int e = lane; e < 16 * (D / 8); e += 32) {
+  {
+    const int part = kg * 32 + lane;  // of 32 KW threads
+    for (int e = part; e < 16 * (D / 8); e += 32 * KW) {
       const int row = e / (D / 8), c = e % (D / 8) * 8, r = wr0 + row;
       uint4 v = make_uint4(0, 0, 0, 0);
       if (r < rows)
@@ -186,7 +283,7 @@ __global__ void __launch_bounds__(kFewThreads, 2)
       *reinterpret_cast<uint4*>(sa + row * L.a_stride + c * 2) = v;
     }
     const int rp8 = p.RP / 8;
-    for (int e = lane; e < 16 * wn * rp8; e += 32) {
+    for (int e = part; e < 16 * wn * rp8; e += 32 * KW) {
       const int row = e / (wn * rp8), g = e / rp8 % wn, c = e % rp8 * 8, r = wr0 + row;
       uint32_t hi[4] = {0, 0, 0, 0}, lo[4] = {0, 0, 0, 0};
       if (r < rows && r / sq.n == wg_lo + g && c < p.kv.rank) {  // block-diagonal: a row holds its own head's R~_q
@@ -231,7 +328,6 @@ __global__ void __launch_bounds__(kFewThreads, 2)
     if (rc < rows) lg1 = base + rc * p.logit_sr;
   }
 
-  int stage = 0, phase = 0;
   for (int tt = 0; tt < n_tiles; ++tt) {
     __syncwarp();  // (RW == 1) every lane is done with the stage that this issue refills
     if (rw == 0) issue();
@@ -246,6 +342,7 @@ __global__ void __launch_bounds__(kFewThreads, 2)
       for (int e = lane; e < (j0 + kFewKeys - sq.len) * 8 * DC; e += 32)
         *reinterpret_cast<uint4*>(kv + kFewKeys * D * 2 + e % DC * (kFewKeys * 128) +
                                   (sq.len - j0) * 128 + e / DC * 16) = make_uint4(0, 0, 0, 0);
+      fence_proxy_async_smem();  // a later segment's tile is loaded into this stage
       __syncwarp();
     }
     float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
@@ -332,23 +429,40 @@ __global__ void __launch_bounds__(kFewThreads, 2)
   }
   const float f0 = mt0 == -INFINITY ? 0.f : ex2(m0 - mt0), f1 = mt1 == -INFINITY ? 0.f : ex2(m1 - mt1);
 
-  // join the KW key groups through shared memory (all rings are idle)
-  __syncthreads();
-  float* cm = reinterpret_cast<float*>(dsm);  // [KW][16 RW] m
-  float* cl = cm + 64;                        // [KW][16 RW] l
-  float* co = cl + 64;                        // [KW][16 RW][D] acc
-  const int slot = kg * 16 * RW + rw * 16 + g;
+  // join the KW key groups through shared memory
+  float* cm = reinterpret_cast<float*>(dsm + L.o_join);  // [KW][16 RW] m
+  float* cl = cm + 64;                                   // [KW][16 RW] l
+  float* co = cl + 64;                                   // [KW][rows kept][D] acc
+  const int kept = min(16 * RW, p.few_rows), la = rw * 16 + g;
   if (t == 0) {
-    cm[slot] = mt0, cm[slot + 8] = mt1;
-    cl[slot] = l0 * f0, cl[slot + 8] = l1 * f1;
+    cm[kg * 16 * RW + la] = mt0, cm[kg * 16 * RW + la + 8] = mt1;
+    cl[kg * 16 * RW + la] = l0 * f0, cl[kg * 16 * RW + la + 8] = l1 * f1;
   }
 #pragma unroll
   for (int i = 0; i < D / 8; ++i) {
-    *reinterpret_cast<float2*>(co + slot * D + i * 8 + 2 * t) = make_float2(acc[i][0] * f0, acc[i][1] * f0);
-    *reinterpret_cast<float2*>(co + (slot + 8) * D + i * 8 + 2 * t) = make_float2(acc[i][2] * f1, acc[i][3] * f1);
+    if (la < kept)
+      *reinterpret_cast<float2*>(co + (kg * kept + la) * D + i * 8 + 2 * t) = make_float2(acc[i][0] * f0, acc[i][1] * f0);
+    if (la + 8 < kept)
+      *reinterpret_cast<float2*>(co + (kg * kept + la + 8) * D + i * 8 + 2 * t) =
+          make_float2(acc[i][2] * f1, acc[i][3] * f1);
+  }
+  // the next sequence's loads start before this one's results are written
+  const bool cut = o_end - o_beg != units;
+  const int nr = r_last - r0 + 1, part = (cta * 2 + (u == u_beg ? 0 : 1)) * (16 * RW);
+  const int out_n = sq.n;
+  const int64_t out_q0 = sq.q0;
+  u += o_end - o_beg;
+  const bool more = u < u_end;
+  if (more) {
+    while (u - pre >= units) {
+      pre += units;
+      sq = paged_seq(p.bd, ++b);
+      units = few_units(p, sq);
+    }
+    segment();
+    start();
   }
   __syncthreads();
-  const int nr = r_last - r0 + 1;
   for (int e = tid; e < nr * (D / 4); e += kFewThreads) {
     const int row = e / (D / 4), d = e % (D / 4) * 4, r = r0 + row;
     float M = -INFINITY;
@@ -360,30 +474,133 @@ __global__ void __launch_bounds__(kFewThreads, 2)
 #pragma unroll
       for (int w = 0; w < KW; ++w) {
         const float f = ex2(cm[w * 16 * RW + row] - M);
-        const float4 a = *reinterpret_cast<const float4*>(co + (w * 16 * RW + row) * D + d);
+        const float4 a = *reinterpret_cast<const float4*>(co + (w * kept + row) * D + d);
         Ls += cl[w * 16 * RW + row] * f;
         O.x += a.x * f, O.y += a.y * f, O.z += a.z * f, O.w += a.w * f;
       }
     }
-    const int64_t tok = sq.q0 + r % sq.n;
-    const int h = kh * p.G + r / sq.n;
-    const int64_t w = (tok * p.H + h) * p.ns + split;
-    if (d == 0 && p.ws_ml) p.ws_ml[w] = make_float2(M, Ls);
-    if (ns == 1) {
-      const float inv = 1.f / (Ls + kEps);
-      *reinterpret_cast<uint2*>(p.out + tok * p.o_st + h * p.o_sh + d) =
-          make_uint2(pack_bf16(O.x * inv, O.y * inv), pack_bf16(O.z * inv, O.w * inv));
-      if (d == 0 && p.lse) p.lse[h * p.lse_sh + tok] = M == -INFINITY ? M : (M + log2f(Ls + kEps)) * kLn2;
+    if (cut) {
+      *reinterpret_cast<float4*>(p.part_acc + static_cast<int64_t>(part + row) * D + d) = O;
+      if (d == 0) p.part_ml[part + row] = make_float2(M, Ls);
     } else {
-      *reinterpret_cast<float4*>(p.ws_acc + w * D + d) = O;
+      few_store<D>(p, out_q0 + r % out_n, kh * p.G + r / out_n, d, M, Ls, O);
     }
+  }
+  if (!more) break;
   }
 }
 
-// Joins the splits of one (token, query head), a warp each: rescale to the
+// Joins the sequences that were cut: a warp per (KV head, query row) rescales the
+// row's parts to their common maximum.
+constexpr int kTailThreads = 256;
+constexpr int kTailRows = kTailThreads / 32;
+
+// Maximum and sum of a row over its parts [c0, c1] (lane i takes part c0 + i, + 32, ...).  part_f:
+// this lane's last part, its index in part_ml and its factor 2^(m - M) (whole row when <= 32 parts).
+struct RowParts {
+  float M, Ls, f;
+  int64_t w;
+};
+__device__ __forceinline__ RowParts row_parts(const PagedAttnParams& p, int64_t U, int C, int64_t s0, int c0, int c1,
+                                              int kh, int r, int lane) {
+  RowParts o{-INFINITY, 0.f, 0.f, 0};
+  const int lanes = p.kv.hkv * p.row_blocks, ln = kh * p.row_blocks + r / p.block_rows;
+  auto index = [&](int c) {
+    return ((static_cast<int64_t>(c) * lanes + ln) * 2 + (few_first(U, C, c) >= s0 ? 0 : 1)) * p.block_rows +
+           r % p.block_rows;
+  };
+  float2 v = make_float2(-INFINITY, 0.f);
+  for (int c = c0 + lane; c <= c1; c += 32) {
+    o.w = index(c);
+    v = p.part_ml[o.w];
+    o.M = fmaxf(o.M, v.x);
+  }
+#pragma unroll
+  for (int s = 16; s > 0; s >>= 1) o.M = fmaxf(o.M, __shfl_xor_sync(0xffffffffu, o.M, s));
+  if (o.M == -INFINITY) return o;
+  if (c1 - c0 < 32) {
+    o.f = ex2(v.x - o.M);
+    o.Ls = v.y * o.f;
+  } else {
+    for (int c = c0 + lane; c <= c1; c += 32) {
+      v = p.part_ml[index(c)];
+      o.Ls += v.y * ex2(v.x - o.M);
+    }
+  }
+#pragma unroll
+  for (int s = 16; s > 0; s >>= 1) o.Ls += __shfl_xor_sync(0xffffffffu, o.Ls, s);
+  return o;
+}
+
+template <int D>
+__global__ void __launch_bounds__(kTailThreads) fna2_paged_few_join_kernel(const PagedAttnParams p) {
+  const int kh = blockIdx.y, b = blockIdx.z, lane = threadIdx.x & 31;
+  const int r = blockIdx.x * kTailRows + (threadIdx.x >> 5);
+  const PagedSeq sq = paged_seq(p.bd, b);
+  const int units = few_units(p, sq);
+  if (units == 0 || r >= sq.n * p.G) return;
+  const int64_t U = p.prefix[p.bd.B], s0 = p.prefix[b];
+  const int C = few_runs(p, U);
+  const int c0 = few_run_of(U, C, s0), c1 = few_run_of(U, C, s0 + units - 1);
+  if (c0 == c1) return;  // written by the attention kernel
+  const RowParts o = row_parts(p, U, C, s0, c0, c1, kh, r, lane);
+  float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
+  constexpr int LD = D / 4;  // lanes that hold columns
+  const int d = lane % LD * 4;
+  if (o.M != -INFINITY)
+    for (int c = c0; c <= c1; c += 32) {
+      // lane i holds part c + i (for more than 32 parts: found again)
+      const RowParts q = c1 - c0 < 32 ? o : row_parts(p, U, C, s0, c, min(c1, c + 31), kh, r, lane);
+      const float scale = c1 - c0 < 32 ? 1.f : ex2(q.M - o.M);
+      for (int i = 0; i <= min(31, c1 - c); ++i) {
+        const int64_t w = __shfl_sync(0xffffffffu, q.w, i);
+        const float f = __shfl_sync(0xffffffffu, q.f, i) * scale;
+        const float4 a = *reinterpret_cast<const float4*>(p.part_acc + w * D + d);
+        O.x += a.x * f, O.y += a.y * f, O.z += a.z * f, O.w += a.w * f;
+      }
+    }
+  if (lane < LD) few_store<D>(p, sq.q0 + r % sq.n, kh * p.G + r / sq.n, d, o.M, o.Ls, O);
+}
+
+// Key weights of a call whose logits were kept: w[b, kh, j] += sum over the rows of
+// 2^(x - LSE), 4 keys a thread.
+constexpr int kLogitKeys = 4 * kTailThreads;
+
+__global__ void __launch_bounds__(kTailThreads) fna2_paged_logit_weights_kernel(const PagedAttnParams p) {
+  __shared__ float s_x[kFewRows];
+  const int kh = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
+  const PagedSeq sq = paged_seq(p.bd, b);
+  const int rows = sq.n * p.G, past = sq.len - sq.n, j = blockIdx.x * kLogitKeys + 4 * tid;
+  if (static_cast<int>(blockIdx.x) * kLogitKeys >= sq.len || rows == 0) return;
+  if (tid < rows) {
+    const float v = p.lse2[static_cast<int64_t>(sq.q0 + tid % sq.n) * p.H + kh * p.G + tid / sq.n];
+    s_x[tid] = v == -INFINITY ? INFINITY : v;  // a row without weight adds 0
+  }
+  __syncthreads();
+  if (j >= sq.len) return;
+  const float* x = p.logits + (static_cast<int64_t>(b) * p.kv.hkv + kh) * p.bd.max_q * p.G * p.logit_sr + j;
+  float w[4] = {0.f, 0.f, 0.f, 0.f};
+  int i = 0;  // new token of row r
+#pragma unroll 4
+  for (int r = 0; r < rows; ++r) {
+    // logits past what the row sees were not all written
+    const int lim = p.causal ? min(sq.len, past + i + 1) : sq.len;
+    i = i + 1 == sq.n ? 0 : i + 1;
+    const float4 v = j < lim ? *reinterpret_cast<const float4*>(x + r * p.logit_sr) : make_float4(0.f, 0.f, 0.f, 0.f);
+    const float vv[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) w[k] += j + k < lim ? ex2(vv[k] - s_x[r]) : 0.f;
+  }
+  float* kw = p.kw + b * p.kw_sb + kh * p.kw_sh + j;
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    if (j + k < sq.len) kw[k] += w[k];
+}
+
+// Joins the tensor-core kernel's splits of one (token, query head), a warp each: rescale to the
 // common max, O = acc / (l + 1e-6), LSE = m + log(l + 1e-6).
 template <int D>
-__global__ void __launch_bounds__(128) fna2_paged_join_kernel(const PagedAttnParams p) {
+__global__ void __launch_bounds__(128) fna2_paged_many_join_kernel(const PagedAttnParams p) {
   const int lane = threadIdx.x & 31;
   const int64_t th = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
   const int64_t tok = th / p.H;
@@ -392,8 +609,8 @@ __global__ void __launch_bounds__(128) fna2_paged_join_kernel(const PagedAttnPar
   const int b = warp_seq_of(p.bd.cu, p.bd.B, tok, lane);
   if (b < 0) return;
   const PagedSeq sq = paged_seq(p.bd, b);
-  const int ns = paged_splits(p, sq);
-  if (!sq.ok || ns <= 1) return;  // written by the attention kernel
+  const int ns = (sq.len + p.chunk_many - 1) / p.chunk_many;
+  if (sq.n * p.G <= p.few_rows || ns <= 1) return;  // written by the attention kernels
   const float2* ml = p.ws_ml + th * p.ns;
   float M = -INFINITY;
   for (int s = 0; s < ns; ++s) M = fmaxf(M, ml[s].x);
@@ -418,39 +635,6 @@ __global__ void __launch_bounds__(128) fna2_paged_join_kernel(const PagedAttnPar
   if (lane == 0 && p.lse) p.lse[h * p.lse_sh + tok] = M == -INFINITY ? M : (M + log2f(Ls + kEps)) * kLn2;
 }
 
-// Key weights of a call whose logits were kept: w[b, kh, j] += sum over the rows
-// of 2^(x - LSE).  One thread per key.
-constexpr int kLogitThreads = 256;
-__global__ void __launch_bounds__(kLogitThreads) fna2_paged_logit_weights_kernel(const PagedAttnParams p) {
-  const int kh = blockIdx.y, b = blockIdx.z;
-  const PagedSeq sq = paged_seq(p.bd, b);
-  if (static_cast<int>(blockIdx.x) * kLogitThreads >= sq.len) return;
-  const int j = blockIdx.x * kLogitThreads + threadIdx.x, rows = sq.n * p.G;
-  const int ns = paged_splits(p, sq), past = sq.len - sq.n;
-  __shared__ float s_lse[kLogitThreads];
-  float w = 0.f;
-  const float* x = p.logits + (static_cast<int64_t>(b) * p.kv.hkv + kh) * p.bd.max_q * p.G * p.logit_sr + j;
-  for (int base = 0; base < rows; base += kLogitThreads) {
-    __syncthreads();
-    if (base + static_cast<int>(threadIdx.x) < rows) {
-      const int r = base + threadIdx.x;
-      const int64_t th = static_cast<int64_t>(sq.q0 + r % sq.n) * p.H + kh * p.G + r / sq.n;
-      float M = -INFINITY, Ls = 0.f;
-      for (int s = 0; s < ns; ++s) M = fmaxf(M, p.ws_ml[th * p.ns + s].x);
-      if (M != -INFINITY)
-        for (int s = 0; s < ns; ++s) Ls += p.ws_ml[th * p.ns + s].y * exp2f(p.ws_ml[th * p.ns + s].x - M);
-      s_lse[threadIdx.x] = M == -INFINITY ? INFINITY : M + log2f(Ls + kEps);  // a row without weight adds 0
-    }
-    __syncthreads();
-    if (j < sq.len) {
-      const int n = min(kLogitThreads, rows - base);
-      for (int r = 0; r < n; ++r)
-        if (!p.causal || j <= past + (base + r) % sq.n) w += exp2f(x[(base + r) * p.logit_sr] - s_lse[r]);
-    }
-  }
-  if (j < sq.len) p.kw[b * p.kw_sb + kh * p.kw_sh + j] += w;
-}
-
 // ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
@@ -461,10 +645,10 @@ struct FewMaps {
 template <int D, int RW>
 cudaError_t launch_paged_few_t(const FewMaps& m, const PagedAttnParams& p, size_t smem, cudaStream_t stream) {
   auto kern = fna2_paged_few_kernel<D, RW>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  static std::atomic<uint64_t> allowed{0};
+  cudaError_t e = allow_smem(reinterpret_cast<const void*>(kern), allowed);
   if (e != cudaSuccess) return e;
-  const dim3 grid(p.bd.B * p.kv.hkv * p.row_blocks, (std::max(1, p.bd.max_k) + p.chunk - 1) / p.chunk);
-  kern<<<grid, kFewThreads, smem, stream>>>(m.k, m.v, m.rk, p);
+  kern<<<p.runs * p.kv.hkv * p.row_blocks, kFewThreads, smem, stream>>>(m.k, m.v, m.rk, p);
   return cudaGetLastError();
 }
 
@@ -480,23 +664,29 @@ inline cudaError_t launch_paged_few(const FewMaps& m, const PagedAttnParams& p, 
   return D == 128 ? launch_paged_few_d<128>(m, p, RW, smem, stream) : launch_paged_few_d<64>(m, p, RW, smem, stream);
 }
 
-// What follows the attention kernels: the join of the splits and the weights from kept logits.
-inline cudaError_t launch_paged_tail(const PagedAttnParams& p, int D, cudaStream_t stream) {
-  cudaError_t e = cudaSuccess;
-  if (p.ns > 1) {
-    const int64_t blocks = (static_cast<int64_t>(p.bd.T) * p.H + 3) / 4;
-    if (D == 128)
-      fna2_paged_join_kernel<128><<<static_cast<unsigned>(blocks), 128, 0, stream>>>(p);
-    else
-      fna2_paged_join_kernel<64><<<static_cast<unsigned>(blocks), 128, 0, stream>>>(p);
-    if ((e = cudaGetLastError()) != cudaSuccess) return e;
-  }
-  if (p.logits) {
-    const dim3 grid((p.bd.max_k + kLogitThreads - 1) / kLogitThreads, p.kv.hkv, p.bd.B);
-    fna2_paged_logit_weights_kernel<<<grid, kLogitThreads, 0, stream>>>(p);
-    e = cudaGetLastError();
-  }
-  return e;
+inline cudaError_t launch_paged_few_join(const PagedAttnParams& p, int D, cudaStream_t stream) {
+  const int rows = std::min(p.bd.max_q * p.G, p.few_rows);
+  const dim3 grid((rows + kTailRows - 1) / kTailRows, p.kv.hkv, p.bd.B);
+  if (D == 128)
+    fna2_paged_few_join_kernel<128><<<grid, kTailThreads, 0, stream>>>(p);
+  else
+    fna2_paged_few_join_kernel<64><<<grid, kTailThreads, 0, stream>>>(p);
+  return cudaGetLastError();
+}
+
+inline cudaError_t launch_logit_weights(const PagedAttnParams& p, cudaStream_t stream) {
+  const dim3 grid((p.bd.max_k + kLogitKeys - 1) / kLogitKeys, p.kv.hkv, p.bd.B);
+  fna2_paged_logit_weights_kernel<<<grid, kTailThreads, 0, stream>>>(p);
+  return cudaGetLastError();
+}
+
+inline cudaError_t launch_paged_many_join(const PagedAttnParams& p, int D, cudaStream_t stream) {
+  const int64_t blocks = (static_cast<int64_t>(p.bd.T) * p.H + 3) / 4;
+  if (D == 128)
+    fna2_paged_many_join_kernel<128><<<static_cast<unsigned>(blocks), 128, 0, stream>>>(p);
+  else
+    fna2_paged_many_join_kernel<64><<<static_cast<unsigned>(blocks), 128, 0, stream>>>(p);
+  return cudaGetLastError();
 }
 
 }  // namespace fna2

@@ -2,6 +2,8 @@
 // bounds of a call, and the split of one sequence's keys over CTAs.
 #pragma once
 
+#include <atomic>
+
 #include "fna2_kernels.cuh"
 #include "ptx.cuh"
 
@@ -83,6 +85,19 @@ __device__ __forceinline__ int warp_seq_of(const int* cu, int B, int64_t t, int 
     hi = min(lo + step, hi);
   }
   return lo;
+}
+
+// Lets a kernel use all of the dynamic shared memory, once per device (`done`: a
+// bit per device; the call costs about a microsecond, a small kernel takes five).
+inline cudaError_t allow_smem(const void* kern, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+  if (bit && (done.load(std::memory_order_relaxed) & bit)) return cudaSuccess;
+  e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxDynamicSmem);
+  if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+  return e;
 }
 
 }  // namespace fna2

@@ -61,8 +61,8 @@ struct ManyItem {
   int b, pair, split, ns;
 };
 
-// Work item `idx` of the call: the sequences' (pair of query tiles, split), in
-// packing order, heaviest pair first.  Every warp finds it by itself (a scan over
+// Work item `idx` of the call: the sequences' (split, pair of query tiles), in
+// packing order, the pairs of a split together (they read the same keys), heaviest first.  Every warp finds it by itself (a scan over
 // the sequences, 32 a round); false when idx is past the last item.
 __device__ __forceinline__ bool many_item(const PagedAttnParams& p, int idx, int lane, ManyItem* it) {
   int carry = 0;
@@ -90,8 +90,9 @@ __device__ __forceinline__ bool many_item(const PagedAttnParams& p, int idx, int
       it->b = base + src;
       it->ns = __shfl_sync(0xffffffffu, ns, src);
       it->sq = paged_seq(p.bd, it->b);
-      it->pair = (it->sq.n + 2 * kBlockM - 1) / (2 * kBlockM) - 1 - local / it->ns;
-      it->split = local % it->ns;
+      const int pairs = (it->sq.n + 2 * kBlockM - 1) / (2 * kBlockM);
+      it->split = local / pairs;
+      it->pair = pairs - 1 - local % pairs;
       return true;
     }
     carry += __shfl_sync(0xffffffffu, incl, 31);
@@ -502,7 +503,8 @@ template <int D, int RP>
 cudaError_t launch_paged_many_t(const ManyMaps& m, const PagedAttnParams& p, cudaStream_t stream) {
   using L = ManySmem<D, RP>;
   auto kern = fna2_paged_many_kernel<D, RP>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kTotal);
+  static std::atomic<uint64_t> allowed{0};
+  cudaError_t e = allow_smem(reinterpret_cast<const void*>(kern), allowed);
   if (e != cudaSuccess) return e;
   kern<<<dim3(p.H, p.many_items), kFwdThreads, L::kTotal, stream>>>(m.q, m.k, m.v, m.rq, m.rk, p);
   return cudaGetLastError();

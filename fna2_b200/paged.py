@@ -76,6 +76,11 @@ def _table(t: torch.Tensor, name: str = "page_table") -> torch.Tensor:
     return t if t.stride(1) == 1 and t.stride(0) >= t.shape[1] else t.contiguous()
 
 
+def _empty(like: torch.Tensor) -> torch.Tensor:
+    return torch.empty_like(like) if like.is_contiguous() else torch.empty(like.shape, dtype=like.dtype,
+                                                                           device=like.device)
+
+
 def _stream(device: torch.device) -> int:
     return torch._C._cuda_getCurrentRawStream(device.index)  # current_stream(device).cuda_stream, without the object
 
@@ -159,7 +164,7 @@ def qk_norm_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, pool:
             f = f.detach().to(device=q.device, dtype=torch.float32).contiguous()
         _want(f.numel() == D // 2, "rope.inv_freq must have head_dim / 2 entries")
         f_p = f.data_ptr()
-    out = torch.empty((T, H, D), dtype=torch.bfloat16, device=q.device)
+    out = _empty(q) if dt is torch.bfloat16 else torch.empty((T, H, D), dtype=torch.bfloat16, device=q.device)
     a = _APPEND_ARGS.pack(B, H, max_pages, _DT[dt], w_dt, rope_dt, T, q_p, q_0, q_1, k_p, k_0, k_1, v_p, v_0, v_1, r_p,
                           r_0, r_1, out.data_ptr(), H * D, D, table.data_ptr(), table.stride(0), lens.data_ptr(),
                           cu.data_ptr(), 0 if positions is None else positions.data_ptr(), wq_p, wk_p, eps, f_p)
@@ -235,7 +240,7 @@ def flash_naylis_paged(q: torch.Tensor, pool: PagedKV, page_table: torch.Tensor,
     Returns out [T, H, D] bf16 (and lse fp32 [H, T] if return_lse)."""
     _want(q.dim() == 3, f"q must be [T, H, D] (got {tuple(q.shape)})")
     T, H, D = q.shape
-    out = torch.empty((T, H, D), dtype=torch.bfloat16, device=q.device)
+    out = _empty(q)
     lse = torch.empty((H, T), dtype=torch.float32, device=q.device) if return_lse else None
     _attention("fna2_paged_attn", q, pool, page_table, cache_seqlens, cu_seqlens_q, max_seqlen_q, r_q, graph_scale,
                softmax_scale, is_causal, key_weights, max_seqlen_k, num_splits, out, lse)
@@ -288,7 +293,7 @@ def naylis_evict(key_weights: torch.Tensor, pool: PagedKV, page_table: torch.Ten
     w_0, w_1, _ = key_weights.stride()
     dev = pool.device
     kept = torch.empty((B, pool.kv_heads, max(budget, 0)), dtype=torch.int32, device=dev)
-    lens_out = torch.empty(B, dtype=torch.int32, device=dev)
+    lens_out = torch.empty_like(lens)
     w_out = torch.empty((B, pool.kv_heads, pages_out * pool.page_size), dtype=torch.float32, device=dev)
     a = _EVICT_ARGS.pack(B, heads, max_k, max_pages, pages_out, budget, sink, recent, table.data_ptr(), table.stride(0),
                          table_out.data_ptr(), table_out.stride(0), lens.data_ptr(), key_weights.data_ptr(), w_0, w_1,
