@@ -770,7 +770,6 @@ struct PagedPlan {
 
 size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 
-constexpr int kSms = 148;
 // Splits of the tensor-core kernel's keys: `base` CTAs without splits, `tiles` key tiles each.  One
 // CTA runs per SM; a tile takes about 2 us, a CTA's start and end 6 us, and the join moves 8 D bytes
 // per row and split.  Takes the count with the least estimated time.
@@ -848,7 +847,7 @@ int paged_plan(const Fna2PagedKV* kv, const Fna2PagedAttnArgs* a, PagedAttnParam
   l->logit = take(l->logits, static_cast<size_t>(p->bd.B) * p->kv.hkv * max_rows * p->logit_sr * 4);
   l->lse2 = take(l->logits, th * 4);
   l->lse = take(p->kw && !l->logits && !a->lse, th * 4);
-  l->kw = take(p->kw && !l->logits, up256(th * 4) + up256(static_cast<size_t>(p->bd.T) * p->kv.hg * 4 * p->RP));
+  l->kw = take(p->kw && !l->logits, up256(th * 4) + up256(static_cast<size_t>(p->bd.T) * p->kv.hg * 4 * p->RP) + 256);
   l->total = at;
   return FNA2_OK;
 }
@@ -888,22 +887,24 @@ int many_maps(const PagedAttnParams& p, int D, ManyMaps* m) {
 // Workspace of the key weights: R~_q hi / lo rows and the log2-domain LSE.
 size_t kw_rq2_bytes(const KeyWeightsParams& p) { return up256(static_cast<size_t>(p.bd.T) * p.kv.hg * 2 * p.RP * 2); }
 size_t kw_workspace_bytes(const KeyWeightsParams& p) {
-  return kw_rq2_bytes(p) + up256(static_cast<size_t>(p.bd.T) * p.H * 4);
+  return kw_rq2_bytes(p) + up256(static_cast<size_t>(p.bd.T) * p.H * 4) + 256;
 }
 
 int run_key_weights(KeyWeightsParams& p, int D, uint8_t* ws, cudaStream_t st) {
   p.rq2 = reinterpret_cast<__nv_bfloat16*>(ws);
   p.lse2 = reinterpret_cast<float*>(ws + kw_rq2_bytes(p));
-  p.qt = p.bd.max_q <= 64 ? 64 : 128;
+  p.next = reinterpret_cast<int*>(ws + kw_workspace_bytes(p) - 256);
+  const int qt = kw_query_tile(p);
+  FNA2_CHECK(static_cast<int64_t>(p.bd.B) * p.kv.hkv * ((p.bd.max_k + 255) / 256) < (1ll << 30), "too many key tiles");
   const CUtensorMapSwizzle r_swz = p.RP == 16 ? CU_TENSOR_MAP_SWIZZLE_32B : CU_TENSOR_MAP_SWIZZLE_64B;
   KwMaps m;
-  if (int rc = make_map(&m.q, p.q, D, p.bd.T, p.H, 1, p.q_st, p.q_sh, 0, 64, p.qt, CU_TENSOR_MAP_SWIZZLE_128B, "q"))
+  if (int rc = make_map(&m.q, p.q, D, p.bd.T, p.H, 1, p.q_st, p.q_sh, 0, 64, qt, CU_TENSOR_MAP_SWIZZLE_128B, "q"))
     return rc;
   if (int rc = map_pages(&m.k, p.kv.k, D, p.kv.hkv, p.kv, 64, kBlockN, CU_TENSOR_MAP_SWIZZLE_128B, "k pages")) return rc;
   m.rq = m.q, m.rk = m.k;  // never dereferenced without graph heads
   if (p.kv.hg > 0) {
     const int64_t w = 2 * p.RP;
-    if (int rc = make_map(&m.rq, p.rq2, w, p.bd.T, p.kv.hg, 1, p.kv.hg * w, w, 0, p.RP, p.qt, r_swz, "r_q hi, lo"))
+    if (int rc = make_map(&m.rq, p.rq2, w, p.bd.T, p.kv.hg, 1, p.kv.hg * w, w, 0, p.RP, qt, r_swz, "r_q hi, lo"))
       return rc;
     if (int rc = map_pages(&m.rk, p.kv.rk, p.kv.rank, p.kv.hg, p.kv, p.RP, kBlockN, r_swz, "rk pages")) return rc;
   }
@@ -1030,7 +1031,6 @@ extern "C" int fna2_key_weights(const Fna2PagedKV* kv, const Fna2PagedAttnArgs* 
   if (workspace == nullptr || workspace_bytes < need)
     return fail(FNA2_ERR_WORKSPACE, "key weights workspace: need %zu bytes, got %zu", need, workspace_bytes);
   FNA2_CHECK((reinterpret_cast<uintptr_t>(workspace) & 255u) == 0, "workspace must be 256-byte aligned");
-  FNA2_CHECK((p.bd.max_k + 2 * kBlockN - 1) / (2 * kBlockN) <= 65535, "max_seqlen_k is too large for key weights");
   p.lse = a->lse, p.lse_sh = a->lse_head_stride;
   return run_key_weights(p, kv->head_dim, static_cast<uint8_t*>(workspace), static_cast<cudaStream_t>(stream));
 }

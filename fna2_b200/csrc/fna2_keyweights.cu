@@ -6,15 +6,19 @@
 // Key-stationary on the tensor cores: the transposed scores S^T = [K | R_k | R_k]
 // [Q | R~_q hi | R~_q lo]^T put a key on every TMEM lane, so the thread that owns
 // a key sums its weights over the columns in a register: no reduction between
-// threads, no atomics, a result that does not depend on timing.  A CTA owns a
-// pair of 128-key tiles of one (sequence, KV head) and streams (query head, tile of
-// QT queries) units through a two-stage ring: Q, R~_q hi and lo, and the R_k rows
-// of that head for its keys.  QT is 64 when no sequence has more queries, else 128.
+// threads, no atomics on the result, which does not depend on timing.  An item is a
+// pair of 128-key tiles of one (sequence, KV head); its units are the (query head,
+// tile of QT queries) that see it.  One persistent CTA per SM draws items from a
+// counter and streams their units through a two-stage ring: Q, R~_q hi and lo, and
+// the R_k rows of that head for its keys.  QT is 64 when no sequence has more
+// queries (K is then double-buffered: an item is only as many units as there are
+// heads), else 128.
 //   warps 0-3 / 4-7  sum key tile 0 / 1 (thread t = key t = TMEM lane t)
-//   warp 8           TMA producer (K and R_k page by page, as in fna2_paged_many.cu)
-//   warp 9           TMEM allocation, MMA issue; S^T of key tile i, unit u in the
-//                    TMEM buffer 2 i + (u & 1), so a tile's MMAs run while the
-//                    previous unit is summed
+//   warp 8           draws items, TMA producer (K and R_k page by page, as in
+//                    fna2_paged_many.cu)
+//   warp 9           TMEM allocation, MMA issue; S^T of key tile i alternates between
+//                    two TMEM buffers, so a tile's MMAs run while the previous one
+//                    is summed
 // A small kernel first writes R~_q hi / lo rows and the log2-domain LSE.
 // Bound: one exp2 per (key, query, head), 16 per clock and SM: 2 x 128 x 128 of them
 // take 2048 clk per unit, the 2 x (D + 2 r_pad)/16 MMAs about 1300.
@@ -37,13 +41,14 @@ struct KeyWeightsParams {
   float* kw;
   int64_t kw_sb, kw_sh;
   __nv_bfloat16* rq2;  // workspace: [T][H_G][2 RP] R~_q hi, lo
-  float* lse2;         // workspace: [H][T] LSE * log2(e), +inf for a row without weight
-  int qt;              // queries per unit
+  float* lse2;         // workspace: [H][T] -LSE * log2(e), -inf for a row without weight
+  int* next;           // workspace: item counter, zeroed by the prep kernel
 };
 
-// R~_q = gs/scale * R_q as hi + lo, columns [rank, RP) zero; LSE in the log2 domain.
+// R~_q = gs/scale * R_q as hi + lo, columns [rank, RP) zero; -LSE in the log2 domain.
 __global__ void __launch_bounds__(256) fna2_key_weights_prep_kernel(const KeyWeightsParams p) {
   const int64_t e = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (e == 0) *p.next = 0;
   const int r8 = p.RP / 8;
   const int64_t n_r = static_cast<int64_t>(p.bd.T) * p.kv.hg * r8, n_l = static_cast<int64_t>(p.bd.T) * p.H;
   if (e < n_r) {
@@ -59,64 +64,109 @@ __global__ void __launch_bounds__(256) fna2_key_weights_prep_kernel(const KeyWei
   if (e < n_l) {
     const int64_t h = e / p.bd.T, t = e % p.bd.T;
     const float v = p.lse[h * p.lse_sh + t];
-    p.lse2[e] = v == -INFINITY ? INFINITY : v * kLog2e;
+    p.lse2[e] = v == -INFINITY ? v : -v * kLog2e;
   }
 }
 
 constexpr int kKwThreads = 320;
 
-template <int D, int RP>
+template <int D, int RP, int QT>
 struct KwSmem {
-  static constexpr int kTile = 128 * D * 2;   // K tile, Q tile
-  static constexpr int kRTile = 128 * RP * 2;  // R_k of a key tile; R~_q hi or lo
+  static constexpr int kTile = 128 * D * 2;    // K tile
+  static constexpr int kRTile = 128 * RP * 2;  // R_k of a key tile
+  static constexpr int kQTile = QT * D * 2;
+  static constexpr int kRqTile = QT * RP * 2;  // R~_q hi or lo
   static constexpr int kChunk = 128 * 128;     // 64 columns of a 128-row tile
-  static constexpr int oK = 0;                               // key tiles 0, 1
-  static constexpr int oStage = oK + 2 * kTile;              // 2 x [Q | R_k 0, 1 | R~_q hi, lo | LSE]
-  static constexpr int sQ = 0, sRk = kTile, sRq = sRk + 2 * kRTile, sLse = sRq + 2 * kRTile;
+  static constexpr int kQChunk = QT * 128;
+  static constexpr int kKStages = QT == 64 ? 2 : 1;
+  static constexpr int oK = 0;                                // kKStages x key tiles 0, 1
+  static constexpr int oStage = oK + kKStages * 2 * kTile;    // 2 x [Q | R_k 0, 1 | R~_q hi, lo | -LSE]
+  static constexpr int sQ = 0, sRk = kQTile, sRq = sRk + 2 * kRTile, sLse = sRq + 2 * kRqTile;
   static constexpr int kStage = sLse + 1024;
   static constexpr int oBar = oStage + 2 * kStage;
-  static constexpr int oMisc = oBar + 16 * 8;
-  static constexpr int kUsed = oMisc + 16;
+  static constexpr int oMisc = oBar + 20 * 8;
+  static constexpr int oItem = oMisc + 16;                    // kKStages x KwItem
+  static constexpr int kUsed = oItem + kKStages * 32;
   static constexpr int kTotal = kUsed + 1024;
   static_assert(kTotal <= kMaxDynamicSmem, "shared memory budget");
+  static_assert(kStage % 1024 == 0, "swizzle atoms stay aligned");
 };
 
 enum KwBar {
-  kWbKFull = 0,
-  kWbFull = 1,    // +stage: the unit's operands
-  kWbEmpty = 3,   // +stage: MMAs that read it are done, and its LSE has been read (1 + 8 arrivals)
-  kWbSFull = 5,   // +2 tile + buffer
-  kWbSEmpty = 9,  // +2 tile + buffer (one arrival per warp)
+  kWbKFull = 0,    // +K stage: K and the item's description
+  kWbKEmpty = 2,   // +K stage: its MMAs are done, every sum warp has left the item (1 + 8 arrivals)
+  kWbFull = 4,     // +stage: the unit's operands
+  kWbEmpty = 6,    // +stage: MMAs that read it are done, and its LSE has been read (1 + 8 arrivals)
+  kWbSFull = 8,    // +2 tile + buffer
+  kWbSEmpty = 12,  // +2 tile + buffer (one arrival per warp)
 };
 
-template <int D, int RP>
+struct KwItem {
+  int b, kh, k0, len, n, u0, per_head, n_units;  // n_units < 0: no more items; u0: first query tile
+};
+
+// Item `idx`: (pair of key tiles, KV head) of the sequences in packing order, KV heads of a pair
+// together, early keys (which the most queries see) first.  Called by a whole warp.
+__device__ __forceinline__ KwItem kw_item(const KeyWeightsParams& p, int idx, int lane, int QT) {
+  KwItem it;
+  it.n_units = -1;
+  int carry = 0;
+  for (int base = 0; base < p.bd.B; base += 32) {
+    const int b = base + lane;
+    PagedSeq s{0, 0, 0, false};
+    int cnt = 0;
+    if (b < p.bd.B) {
+      s = paged_seq(p.bd, b);
+      if (!s.ok) atomicCAS(&g_device_error, 0, kStatusBadSeqPaged);
+      if (s.n > 0) cnt = (s.len + 2 * kBlockN - 1) / (2 * kBlockN) * p.kv.hkv;
+    }
+    int incl = cnt;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += u;
+    }
+    const unsigned hit = __ballot_sync(0xffffffffu, idx < carry + incl);
+    if (hit) {
+      const int src = __ffs(hit) - 1;
+      const int local = idx - carry - (__shfl_sync(0xffffffffu, incl, src) - __shfl_sync(0xffffffffu, cnt, src));
+      it.b = base + src;
+      it.kh = local % p.kv.hkv;
+      it.k0 = local / p.kv.hkv * 2 * kBlockN;
+      it.len = __shfl_sync(0xffffffffu, s.len, src);
+      it.n = __shfl_sync(0xffffffffu, s.n, src);
+      const int n_qt = (it.n + QT - 1) / QT;
+      it.u0 = p.causal ? min(n_qt, max(0, it.k0 - (it.len - it.n)) / QT) : 0;  // earlier tokens see none of these keys
+      it.per_head = n_qt - it.u0;
+      it.n_units = it.per_head * p.G;
+      return it;
+    }
+    carry += __shfl_sync(0xffffffffu, incl, 31);
+  }
+  return it;
+}
+
+template <int D, int RP, int QT>
 __global__ void __launch_bounds__(kKwThreads, 1)
     fna2_key_weights_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                             const __grid_constant__ CUtensorMap tmRq, const __grid_constant__ CUtensorMap tmRk,
                             const KeyWeightsParams p) {
-  using L = KwSmem<D, RP>;
+  using L = KwSmem<D, RP, QT>;
+  constexpr int KS = L::kKStages;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::oBar);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::oMisc);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::oMisc + 4);
+  volatile KwItem* items = reinterpret_cast<volatile KwItem*>(smem + L::oItem);
   const int warp = warp_id(), lane = lane_id(), tid = threadIdx.x;
-  const int kh = blockIdx.x, b = blockIdx.z, k0 = blockIdx.y * 2 * kBlockN;
-  const PagedSeq sq = paged_seq(p.bd, b);
-  if (!sq.ok && tid == 0) atomicCAS(&g_device_error, 0, kStatusBadSeqPaged);
-  if (k0 >= sq.len || sq.n == 0) return;
-  const int past = sq.len - sq.n, QT = p.qt;
-  const bool two = k0 + kBlockN < sq.len;  // the second key tile has keys
-  // query tiles [u0, n_qt): earlier tokens see none of these keys
-  const int n_qt = (sq.n + QT - 1) / QT, u0 = p.causal ? min(n_qt, max(0, k0 - past) / QT) : 0;
-  const int per_head = n_qt - u0, n_units = per_head * p.G;
-  if (n_units == 0) return;
 
   if (tid == 0) {
-    mbar_init(&bars[kWbKFull], 1);
     for (int s = 0; s < 2; ++s) {
+      mbar_init(&bars[kWbKFull + s], 1);
+      mbar_init(&bars[kWbKEmpty + s], 9);
       mbar_init(&bars[kWbFull + s], 1);
-      mbar_init(&bars[kWbEmpty + s], two ? 9 : 5);
+      mbar_init(&bars[kWbEmpty + s], 9);
     }
     for (int s = 0; s < 4; ++s) {
       mbar_init(&bars[kWbSFull + s], 1);
@@ -133,162 +183,207 @@ __global__ void __launch_bounds__(kKwThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  const int hg_local = p.kv.hg - kh * p.G;  // heads of the group below this carry the bias
 
   if (warp == 8) {
     // ------------------------------------------------------------ producer
-    const int* table = p.kv.table + b * p.kv.table_sb;
-    const int lg = p.kv.page_log2, mask = (1 << lg) - 1;
-    const int bk = min(1 << lg, kBlockN);  // rows of a box; lane l owns box l of the two key tiles (at most 16)
-    const int key = k0 + lane * bk;
-    const bool mine = lane * bk < 2 * kBlockN && key < sq.len;
-    const int page = mine ? __ldg(table + (key >> lg)) : 0;
-    const int boxes = __popc(__ballot_sync(0xffffffffu, mine));
-    const int tile = lane * bk / kBlockN, row = lane * bk % kBlockN;
     if (lane == 0) {
       tma_prefetch_desc(&tmQ);
-      mbar_expect_tx(&bars[kWbKFull], boxes * bk * D * 2);
+      tma_prefetch_desc(&tmK);
     }
-    __syncwarp();
-    if (mine) {
-#pragma unroll
-      for (int c = 0; c < D / 64; ++c)
-        tma_load_4d(smem + L::oK + tile * L::kTile + c * L::kChunk + row * 128, &tmK, &bars[kWbKFull], c * 64,
-                    key & mask, kh, page);
-    }
-    for (int u = 0; u < n_units; ++u) {
-      const int s = u & 1, g = u / per_head, h = kh * p.G + g;
-      const int i0 = (u0 + u % per_head) * QT, tok = sq.q0 + i0;
-      const bool graph = g < hg_local;
-      uint8_t* st = smem + L::oStage + s * L::kStage;
-      // this unit's LSE (columns past the end: +inf, which adds 0)
-      float lse[4];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int i = lane + 32 * k;
-        lse[k] = i < QT && i0 + i < sq.n ? p.lse2[static_cast<int64_t>(h) * p.bd.T + tok + i] : INFINITY;
-      }
-      const bool free = u < 2 || mbar_wait(&bars[kWbEmpty + s], ((u >> 1) - 1) & 1, abort_flag, 121);
+    const int lg = p.kv.page_log2, mask = (1 << lg) - 1;
+    const int bk = min(1 << lg, kBlockN);  // rows of a box; lane l owns box l of the two key tiles (at most 16)
+    const int tile = lane * bk / kBlockN, row = lane * bk % kBlockN;
+    int gu = 0;  // units so far
+    for (int n = 0;; ++n) {
+      const int ks = n % KS;
+      int idx = 0;
+      if (lane == 0) idx = atomicAdd(p.next, 1);
+      idx = __shfl_sync(0xffffffffu, idx, 0);
+      const KwItem it = kw_item(p, idx, lane, QT);
+      const bool free = n < KS || mbar_wait(&bars[kWbKEmpty + ks], (n / KS - 1) & 1, abort_flag, 120);
       if (!__all_sync(0xffffffffu, free)) break;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) reinterpret_cast<float*>(st + L::sLse)[lane + 32 * k] = lse[k];
+      const int key = it.k0 + lane * bk;
+      const bool mine = it.n_units >= 0 && lane * bk < 2 * kBlockN && key < it.len;
+      const int page = mine ? __ldg(p.kv.table + it.b * p.kv.table_sb + (key >> lg)) : 0;
+      const int boxes = __popc(__ballot_sync(0xffffffffu, mine));
+      if (lane == 0) {  // (the arrival also publishes the description)
+        volatile KwItem* d = items + ks;
+        d->b = it.b, d->kh = it.kh, d->k0 = it.k0, d->len = it.len, d->n = it.n, d->u0 = it.u0;
+        d->per_head = it.per_head, d->n_units = it.n_units;
+        mbar_expect_tx(&bars[kWbKFull + ks], boxes * bk * D * 2);
+      }
       __syncwarp();
-      if (lane == 0) {  // (the arrival also publishes the LSE)
-        mbar_expect_tx(&bars[kWbFull + s], QT * (D + (graph ? 2 * RP : 0)) * 2 + (graph ? boxes * bk * RP * 2 : 0));
+      if (it.n_units < 0) break;
+      if (mine) {
 #pragma unroll
         for (int c = 0; c < D / 64; ++c)
-          tma_load_4d(st + L::sQ + c * L::kChunk, &tmQ, &bars[kWbFull + s], c * 64, tok, h, 0);
-        if (graph) {
-          tma_load_4d(st + L::sRq, &tmRq, &bars[kWbFull + s], 0, tok, h, 0);
-          tma_load_4d(st + L::sRq + L::kRTile, &tmRq, &bars[kWbFull + s], RP, tok, h, 0);
-        }
+          tma_load_4d(smem + L::oK + (2 * ks + tile) * L::kTile + c * L::kChunk + row * 128, &tmK,
+                      &bars[kWbKFull + ks], c * 64, key & mask, it.kh, page);
       }
       __syncwarp();
-      if (mine && graph)
-        tma_load_4d(st + L::sRk + tile * L::kRTile + row * RP * 2, &tmRk, &bars[kWbFull + s], 0, key & mask, h, page);
-      __syncwarp();
+      const int q0 = __ldg(p.bd.cu + it.b);
+      bool ok = true;
+      for (int u = 0; u < it.n_units; ++u, ++gu) {
+        const int s = gu & 1, h = it.kh * p.G + u / it.per_head;
+        const int i0 = (it.u0 + u % it.per_head) * QT, tok = q0 + i0;
+        const bool graph = h < p.kv.hg;
+        uint8_t* st = smem + L::oStage + s * L::kStage;
+        // this unit's -LSE (columns past the end: -inf, which adds 0)
+        float lse[QT / 32];
+#pragma unroll
+        for (int k = 0; k < QT / 32; ++k) {
+          const int i = lane + 32 * k;
+          lse[k] = i0 + i < it.n ? p.lse2[static_cast<int64_t>(h) * p.bd.T + tok + i] : -INFINITY;
+        }
+        const bool room = gu < 2 || mbar_wait(&bars[kWbEmpty + s], ((gu >> 1) - 1) & 1, abort_flag, 121);
+        ok = __all_sync(0xffffffffu, room);
+        if (!ok) break;
+#pragma unroll
+        for (int k = 0; k < QT / 32; ++k) reinterpret_cast<float*>(st + L::sLse)[lane + 32 * k] = lse[k];
+        __syncwarp();
+        if (lane == 0) {  // (the arrival also publishes the LSE)
+          mbar_expect_tx(&bars[kWbFull + s], QT * (D + (graph ? 2 * RP : 0)) * 2 + (graph ? boxes * bk * RP * 2 : 0));
+#pragma unroll
+          for (int c = 0; c < D / 64; ++c)
+            tma_load_4d(st + L::sQ + c * L::kQChunk, &tmQ, &bars[kWbFull + s], c * 64, tok, h, 0);
+          if (graph) {
+            tma_load_4d(st + L::sRq, &tmRq, &bars[kWbFull + s], 0, tok, h, 0);
+            tma_load_4d(st + L::sRq + L::kRqTile, &tmRq, &bars[kWbFull + s], RP, tok, h, 0);
+          }
+        }
+        __syncwarp();
+        if (mine && graph)
+          tma_load_4d(st + L::sRk + tile * L::kRTile + row * RP * 2, &tmRk, &bars[kWbFull + s], 0, key & mask, h, page);
+        __syncwarp();
+      }
+      if (!ok) break;
     }
   } else if (warp == 9) {
     // ------------------------------------------------------------ MMA issuer
-    const uint32_t idesc = QT == 64 ? make_idesc_bf16(kBlockN, 64, 0, 0) : make_idesc_bf16(kBlockN, 128, 0, 0);
+    constexpr uint32_t idesc = make_idesc_bf16(kBlockN, QT, 0, 0);
     constexpr uint32_t r_layout = RP == 16 ? kSwizzle32B : kSwizzle64B;
     constexpr uint32_t r_sbo = 8 * RP * 2;
-    bool ok = mbar_wait(&bars[kWbKFull], 0, abort_flag, 221);
-    for (int u = 0; ok && u < n_units; ++u) {
-      const int s = u & 1;
-      const bool graph = u / per_head < hg_local;
-      if (!mbar_wait_spin(&bars[kWbFull + s], (u >> 1) & 1, abort_flag, 222)) break;
-      const uint32_t st = smem_u32(smem + L::oStage + s * L::kStage);
-      for (int i = 0; i < (two ? 2 : 1); ++i) {
-        const int buf = 2 * i + s;
-        if (u >= 2 && !mbar_wait_spin(&bars[kWbSEmpty + buf], ((u >> 1) - 1) & 1, abort_flag, 223)) {
+    int gu = 0, used[2] = {0, 0};
+    bool ok = true;
+    for (int n = 0; ok; ++n) {
+      const int ks = n % KS;
+      if (!mbar_wait(&bars[kWbKFull + ks], (n / KS) & 1, abort_flag, 221)) break;
+      const int n_units = items[ks].n_units, per_head = items[ks].per_head, h0 = items[ks].kh * p.G;
+      const int tiles = items[ks].k0 + kBlockN < items[ks].len ? 2 : 1;
+      if (n_units < 0) break;
+      for (int u = 0; ok && u < n_units; ++u, ++gu) {
+        const int s = gu & 1;
+        const bool graph = h0 + u / per_head < p.kv.hg;
+        if (!mbar_wait_spin(&bars[kWbFull + s], (gu >> 1) & 1, abort_flag, 222)) {
           ok = false;
           break;
         }
-        tc_fence_after();
-        if (elect_one()) {
-          const uint32_t tS = tmem + 128 * buf;
-          const uint32_t sK = smem_u32(smem + L::oK + i * L::kTile);
+        const uint32_t st = smem_u32(smem + L::oStage + s * L::kStage);
 #pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk) {
-            const uint32_t off = (kk >> 2) * L::kChunk + (kk & 3) * 32;
-            mma_ss(tS, make_sdesc(sK + off, 16, 1024, kSwizzle128B),
-                   make_sdesc(st + L::sQ + off, 16, 1024, kSwizzle128B), idesc, kk > 0);
+        for (int i = 0; i < 2; ++i) {
+          if (i >= tiles) continue;
+          const int buf = 2 * i + (used[i] & 1);
+          if (used[i] >= 2 && !mbar_wait_spin(&bars[kWbSEmpty + buf], ((used[i] >> 1) - 1) & 1, abort_flag, 223)) {
+            ok = false;
+            break;
           }
-          if (graph) {
+          ++used[i];
+          tc_fence_after();
+          if (elect_one()) {
+            const uint32_t tS = tmem + 128 * buf;
+            const uint32_t sK = smem_u32(smem + L::oK + (2 * ks + i) * L::kTile);
 #pragma unroll
-            for (int kk = 0; kk < RP / 16; ++kk) {
-              const uint64_t rk = make_sdesc(st + L::sRk + i * L::kRTile + kk * 32, 16, r_sbo, r_layout);
-              mma_ss(tS, rk, make_sdesc(st + L::sRq + kk * 32, 16, r_sbo, r_layout), idesc, 1);
-              mma_ss(tS, rk, make_sdesc(st + L::sRq + L::kRTile + kk * 32, 16, r_sbo, r_layout), idesc, 1);
+            for (int kk = 0; kk < D / 16; ++kk)
+              mma_ss(tS, make_sdesc(sK + (kk >> 2) * L::kChunk + (kk & 3) * 32, 16, 1024, kSwizzle128B),
+                     make_sdesc(st + L::sQ + (kk >> 2) * L::kQChunk + (kk & 3) * 32, 16, 1024, kSwizzle128B), idesc,
+                     kk > 0);
+            if (graph) {
+#pragma unroll
+              for (int kk = 0; kk < RP / 16; ++kk) {
+                const uint64_t rk = make_sdesc(st + L::sRk + i * L::kRTile + kk * 32, 16, r_sbo, r_layout);
+                mma_ss(tS, rk, make_sdesc(st + L::sRq + kk * 32, 16, r_sbo, r_layout), idesc, 1);
+                mma_ss(tS, rk, make_sdesc(st + L::sRq + L::kRqTile + kk * 32, 16, r_sbo, r_layout), idesc, 1);
+              }
+            }
+            mma_commit(&bars[kWbSFull + buf]);
+            if (i == tiles - 1) mma_commit(&bars[kWbEmpty + s]);
+          }
+          __syncwarp();
+        }
+      }
+      if (ok && elect_one()) mma_commit(&bars[kWbKEmpty + ks]);
+      __syncwarp();
+    }
+  } else {
+    // ------------------------------------------------------------ sums (warpgroup i = key tile i)
+    const int wi = warp >> 2;
+    const uint32_t t_lane = tmem + 256 * wi + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+    const float2 sl2 = make_float2(p.scale_log2, p.scale_log2);
+    int gu = 0, used = 0;
+    bool ok = true;
+    for (int n = 0; ok; ++n) {
+      const int ks = n % KS;
+      if (!mbar_wait(&bars[kWbKFull + ks], (n / KS) & 1, abort_flag, 320)) break;
+      const int n_units = items[ks].n_units, per_head = items[ks].per_head, u0 = items[ks].u0, nq = items[ks].n;
+      const int len = items[ks].len, tile0 = items[ks].k0 + wi * kBlockN, j = tile0 + (tid & 127), past = len - nq;
+      if (n_units < 0) break;
+      const bool mine = tile0 < len;
+      float* dst = p.kw + items[ks].b * p.kw_sb + items[ks].kh * p.kw_sh + j;
+      float w = mine && j < len ? *dst : 0.f;
+      for (int u = 0; u < n_units; ++u, ++gu) {
+        const int s = gu & 1, buf = used & 1;
+        if (!mbar_wait(&bars[kWbFull + s], (gu >> 1) & 1, abort_flag, 321) ||
+            (mine && !mbar_wait(&bars[kWbSFull + 2 * wi + buf], (used >> 1) & 1, abort_flag, 322))) {
+          ok = false;
+          break;
+        }
+        if (mine) {
+          ++used;
+          tc_fence_after();
+          const int i0 = (u0 + u % per_head) * QT;
+          const float4* lse4 = reinterpret_cast<const float4*>(smem + L::oStage + s * L::kStage + L::sLse);
+          // columns [first, nq - i0) belong to queries that see the key; a NaN score of another sequence's
+          // query is never read into a sum
+          const int first = p.causal ? j - past - i0 : 0;
+          const bool whole = (!p.causal || tile0 + kBlockN - 1 <= past + i0) && i0 + QT <= nq;
+          float2 a[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+          uint32_t r[2][32];
+          tmem_ld32(t_lane + 128 * buf, r[0]);
+#pragma unroll
+          for (int c = 0; c < QT / 32; ++c) {
+            uint32_t* x = r[c & 1];
+            tmem_ld_wait32(x);
+            if (c + 1 < QT / 32) tmem_ld32(t_lane + 128 * buf + 32 * (c + 1), r[(c + 1) & 1]);
+            const int lo = first - 32 * c, hi = nq - i0 - 32 * c;
+#pragma unroll
+            for (int k = 0; k < 32; k += 4) {
+              const float4 l = lse4[8 * c + k / 4];
+              const float2 y0 = __ffma2_rn(f32x2(x[k], x[k + 1]), sl2, make_float2(l.x, l.y));
+              const float2 y1 = __ffma2_rn(f32x2(x[k + 2], x[k + 3]), sl2, make_float2(l.z, l.w));
+              float2 e0 = make_float2(ex2(y0.x), ex2(y0.y)), e1 = make_float2(ex2(y1.x), ex2(y1.y));
+              if (!whole) {
+                e0.x = k >= lo && k < hi ? e0.x : 0.f;
+                e0.y = k + 1 >= lo && k + 1 < hi ? e0.y : 0.f;
+                e1.x = k + 2 >= lo && k + 2 < hi ? e1.x : 0.f;
+                e1.y = k + 3 >= lo && k + 3 < hi ? e1.y : 0.f;
+              }
+              a[0] = __fadd2_rn(a[0], e0);
+              a[1] = __fadd2_rn(a[1], e1);
             }
           }
-          mma_commit(&bars[kWbSFull + buf]);
-          if (i == (two ? 1 : 0)) mma_commit(&bars[kWbEmpty + s]);
+          w += (a[0].x + a[0].y) + (a[1].x + a[1].y);
+          tc_fence_before();
         }
         __syncwarp();
-      }
-    }
-  } else if (two || warp < 4) {
-    // ------------------------------------------------------------ sums (warpgroup i = key tile i)
-    const int wi = warp >> 2, j = k0 + wi * kBlockN + (tid & 127);
-    const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const float sl2 = p.scale_log2;
-    const int tile_last = k0 + wi * kBlockN + kBlockN - 1;
-    float w = 0.f;
-    bool ok = true;
-    for (int u = 0; u < n_units; ++u) {
-      const int s = u & 1, buf = 2 * wi + s;
-      const int i0 = (u0 + u % per_head) * QT;
-      if (!mbar_wait(&bars[kWbFull + s], (u >> 1) & 1, abort_flag, 321) ||
-          !mbar_wait(&bars[kWbSFull + buf], (u >> 1) & 1, abort_flag, 322)) {
-        ok = false;
-        break;
-      }
-      tc_fence_after();
-      const float4* lse4 = reinterpret_cast<const float4*>(smem + L::oStage + s * L::kStage + L::sLse);
-      // columns of queries that see the key start here (0: all); a NaN score of another sequence's
-      // query or of a page's unused slot is never read into a sum
-      const int first = p.causal ? j - past - i0 : 0;
-      const bool whole = (!p.causal || tile_last <= past + i0) && i0 + QT <= sq.n;
-      float a4[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 1
-      for (int c = 0; c < QT / 32; ++c) {
-        uint32_t r[32];
-        tmem_ld32(tmem + 128 * buf + 32 * c + lane_base, r);
-        tmem_ld_wait32(r);
-        if (whole) {
-#pragma unroll
-          for (int k = 0; k < 32; k += 4) {
-            const float4 l = lse4[8 * c + k / 4];
-            a4[0] += ex2(fmaf(__uint_as_float(r[k]), sl2, -l.x));
-            a4[1] += ex2(fmaf(__uint_as_float(r[k + 1]), sl2, -l.y));
-            a4[2] += ex2(fmaf(__uint_as_float(r[k + 2]), sl2, -l.z));
-            a4[3] += ex2(fmaf(__uint_as_float(r[k + 3]), sl2, -l.w));
-          }
-        } else {
-          const int lo = first - 32 * c, hi = sq.n - i0 - 32 * c;
-#pragma unroll
-          for (int k = 0; k < 32; k += 4) {
-            const float4 l = lse4[8 * c + k / 4];
-            const float ll[4] = {l.x, l.y, l.z, l.w};
-#pragma unroll
-            for (int m = 0; m < 4; ++m) {
-              const float x = ex2(fmaf(__uint_as_float(r[k + m]), sl2, -ll[m]));
-              a4[m] += k + m >= lo && k + m < hi ? x : 0.f;
-            }
-          }
+        if (lane == 0) {
+          if (mine) mbar_arrive(&bars[kWbSEmpty + 2 * wi + buf]);
+          mbar_arrive(&bars[kWbEmpty + s]);
         }
       }
-      w += (a4[0] + a4[1]) + (a4[2] + a4[3]);
-      tc_fence_before();
+      if (ok && mine && j < len) *dst = w;
       __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(&bars[kWbSEmpty + buf]);
-        mbar_arrive(&bars[kWbEmpty + s]);
-      }
+      if (lane == 0) mbar_arrive(&bars[kWbKEmpty + ks]);
     }
-    if (ok && j < sq.len) p.kw[b * p.kw_sb + kh * p.kw_sh + j] += w;
   }
 
   tc_fence_before();
@@ -303,24 +398,33 @@ struct KwMaps {
   CUtensorMap q, k, rq, rk;
 };
 
-template <int D, int RP>
+// Queries per unit.
+inline int kw_query_tile(const KeyWeightsParams& p) { return p.bd.max_q <= 64 ? 64 : 128; }
+
+template <int D, int RP, int QT>
 cudaError_t launch_key_weights_t(const KwMaps& m, const KeyWeightsParams& p, cudaStream_t stream) {
-  using L = KwSmem<D, RP>;
-  auto kern = fna2_key_weights_kernel<D, RP>;
+  using L = KwSmem<D, RP, QT>;
+  auto kern = fna2_key_weights_kernel<D, RP, QT>;
   static std::atomic<uint64_t> allowed{0};
   cudaError_t e = allow_smem(reinterpret_cast<const void*>(kern), allowed);
   if (e != cudaSuccess) return e;
   const int64_t n = static_cast<int64_t>(p.bd.T) * std::max<int64_t>(p.H, static_cast<int64_t>(p.kv.hg) * p.RP / 8);
   fna2_key_weights_prep_kernel<<<static_cast<unsigned>((n + 255) / 256), 256, 0, stream>>>(p);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
-  const dim3 grid(p.kv.hkv, (p.bd.max_k + 2 * kBlockN - 1) / (2 * kBlockN), p.bd.B);
-  kern<<<grid, kKwThreads, L::kTotal, stream>>>(m.q, m.k, m.rq, m.rk, p);
+  const int64_t items = static_cast<int64_t>(p.bd.B) * p.kv.hkv * ((p.bd.max_k + 2 * kBlockN - 1) / (2 * kBlockN));
+  kern<<<static_cast<unsigned>(std::min<int64_t>(items, kSms)), kKwThreads, L::kTotal, stream>>>(m.q, m.k, m.rq, m.rk, p);
   return cudaGetLastError();
 }
 
+template <int D, int RP>
+cudaError_t launch_key_weights_r(const KwMaps& m, const KeyWeightsParams& p, cudaStream_t stream) {
+  return kw_query_tile(p) == 64 ? launch_key_weights_t<D, RP, 64>(m, p, stream)
+                                : launch_key_weights_t<D, RP, 128>(m, p, stream);
+}
+
 inline cudaError_t launch_key_weights(const KwMaps& m, const KeyWeightsParams& p, int D, cudaStream_t stream) {
-  if (D == 64) return p.RP == 16 ? launch_key_weights_t<64, 16>(m, p, stream) : launch_key_weights_t<64, 32>(m, p, stream);
-  return p.RP == 16 ? launch_key_weights_t<128, 16>(m, p, stream) : launch_key_weights_t<128, 32>(m, p, stream);
+  if (D == 64) return p.RP == 16 ? launch_key_weights_r<64, 16>(m, p, stream) : launch_key_weights_r<64, 32>(m, p, stream);
+  return p.RP == 16 ? launch_key_weights_r<128, 16>(m, p, stream) : launch_key_weights_r<128, 32>(m, p, stream);
 }
 
 }  // namespace fna2

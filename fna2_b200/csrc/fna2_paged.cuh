@@ -9,6 +9,8 @@
 
 namespace fna2 {
 
+constexpr int kSms = 148;  // of a B200
+
 // Site codes recorded in g_device_error (read by fna2_device_status).
 constexpr int kStatusSmemBase = 199;      // the dynamic shared memory base was not 1024-byte aligned
 constexpr int kStatusBadSeqAppend = 631;  // append: bad length / offsets, or a page id outside the pool
