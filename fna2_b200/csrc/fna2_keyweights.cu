@@ -16,9 +16,10 @@
 //   warps 0-3 / 4-7  sum key tile 0 / 1 (thread t = key t = TMEM lane t)
 //   warp 8           draws items, TMA producer (K and R_k page by page, as in
 //                    fna2_paged_many.cu)
-//   warp 9           TMEM allocation, MMA issue; S^T of key tile i alternates between
-//                    two TMEM buffers, so a tile's MMAs run while the previous one
-//                    is summed
+//   warp 9           TMEM allocation, MMA issue; each key tile has 256 / QT TMEM
+//                    buffers, so its next MMAs run while a unit is summed
+// The LSE has a ring of its own: with it in the operands' stages, a unit's loads
+// waited for the sums two units before (4200 clk per unit at QT = 128).
 // A small kernel first writes R~_q hi / lo rows and the log2-domain LSE.
 // Bound: one exp2 per (key, query, head), 16 per clock and SM: 2 x 128 x 128 of them
 // take 2048 clk per unit, the 2 x (D + 2 r_pad)/16 MMAs about 1300.
@@ -80,11 +81,13 @@ struct KwSmem {
   static constexpr int kQChunk = QT * 128;
   static constexpr int kKStages = QT == 64 ? 2 : 1;
   static constexpr int oK = 0;                                // kKStages x key tiles 0, 1
-  static constexpr int oStage = oK + kKStages * 2 * kTile;    // 2 x [Q | R_k 0, 1 | R~_q hi, lo | -LSE]
-  static constexpr int sQ = 0, sRk = kQTile, sRq = sRk + 2 * kRTile, sLse = sRq + 2 * kRqTile;
-  static constexpr int kStage = sLse + 1024;
-  static constexpr int oBar = oStage + 2 * kStage;
-  static constexpr int oMisc = oBar + 20 * 8;
+  static constexpr int oStage = oK + kKStages * 2 * kTile;    // 2 x [Q | R_k 0, 1 | R~_q hi, lo]
+  static constexpr int sQ = 0, sRk = kQTile, sRq = sRk + 2 * kRTile;
+  static constexpr int kStage = sRq + 2 * kRqTile;
+  static constexpr int kBufs = 256 / QT;                      // TMEM buffers per key tile
+  static constexpr int oLse = oStage + 2 * kStage;            // 4 x -LSE of a unit
+  static constexpr int oBar = oLse + 4 * QT * 4;
+  static constexpr int oMisc = oBar + 32 * 8;
   static constexpr int oItem = oMisc + 16;                    // kKStages x KwItem
   static constexpr int kUsed = oItem + kKStages * 32;
   static constexpr int kTotal = kUsed + 1024;
@@ -96,9 +99,11 @@ enum KwBar {
   kWbKFull = 0,    // +K stage: K and the item's description
   kWbKEmpty = 2,   // +K stage: its MMAs are done, every sum warp has left the item (1 + 8 arrivals)
   kWbFull = 4,     // +stage: the unit's operands
-  kWbEmpty = 6,    // +stage: MMAs that read it are done, and its LSE has been read (1 + 8 arrivals)
-  kWbSFull = 8,    // +2 tile + buffer
-  kWbSEmpty = 12,  // +2 tile + buffer (one arrival per warp)
+  kWbEmpty = 6,    // +stage: MMAs that read it are done
+  kWbLFull = 8,    // +LSE slot
+  kWbLEmpty = 12,  // +LSE slot (8 arrivals)
+  kWbSFull = 16,   // +4 tile + buffer
+  kWbSEmpty = 24,  // +4 tile + buffer (one arrival per warp)
 };
 
 struct KwItem {
@@ -146,6 +151,38 @@ __device__ __forceinline__ KwItem kw_item(const KeyWeightsParams& p, int idx, in
   return it;
 }
 
+// Sum over the QT columns of this thread's lane of 2^(sl2 S - LSE); MASK: of columns [lo, hi) only.
+// (Two copies: masks cost 5 instructions per column.)
+template <int QT, bool MASK>
+__device__ __forceinline__ float kw_sum(uint32_t t_addr, const float4* lse4, float2 sl2, int lo, int hi) {
+  float2 a[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+  uint32_t r[2][32];
+  tmem_ld32(t_addr, r[0]);
+#pragma unroll
+  for (int c = 0; c < QT / 32; ++c) {
+    uint32_t* x = r[c & 1];
+    tmem_ld_wait32(x);
+    if (c + 1 < QT / 32) tmem_ld32(t_addr + 32 * (c + 1), r[(c + 1) & 1]);
+#pragma unroll
+    for (int k = 0; k < 32; k += 4) {
+      const float4 l = lse4[8 * c + k / 4];
+      const float2 y0 = __ffma2_rn(f32x2(x[k], x[k + 1]), sl2, make_float2(l.x, l.y));
+      const float2 y1 = __ffma2_rn(f32x2(x[k + 2], x[k + 3]), sl2, make_float2(l.z, l.w));
+      float2 e0 = make_float2(ex2(y0.x), ex2(y0.y)), e1 = make_float2(ex2(y1.x), ex2(y1.y));
+      if (MASK) {
+        const int col = 32 * c + k;
+        e0.x = col >= lo && col < hi ? e0.x : 0.f;
+        e0.y = col + 1 >= lo && col + 1 < hi ? e0.y : 0.f;
+        e1.x = col + 2 >= lo && col + 2 < hi ? e1.x : 0.f;
+        e1.y = col + 3 >= lo && col + 3 < hi ? e1.y : 0.f;
+      }
+      a[0] = __fadd2_rn(a[0], e0);
+      a[1] = __fadd2_rn(a[1], e1);
+    }
+  }
+  return (a[0].x + a[0].y) + (a[1].x + a[1].y);
+}
+
 template <int D, int RP, int QT>
 __global__ void __launch_bounds__(kKwThreads, 1)
     fna2_key_weights_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
@@ -166,9 +203,13 @@ __global__ void __launch_bounds__(kKwThreads, 1)
       mbar_init(&bars[kWbKFull + s], 1);
       mbar_init(&bars[kWbKEmpty + s], 9);
       mbar_init(&bars[kWbFull + s], 1);
-      mbar_init(&bars[kWbEmpty + s], 9);
+      mbar_init(&bars[kWbEmpty + s], 1);
     }
     for (int s = 0; s < 4; ++s) {
+      mbar_init(&bars[kWbLFull + s], 1);
+      mbar_init(&bars[kWbLEmpty + s], 8);
+    }
+    for (int s = 0; s < 8; ++s) {
       mbar_init(&bars[kWbSFull + s], 1);
       mbar_init(&bars[kWbSEmpty + s], 4);
     }
@@ -235,13 +276,16 @@ __global__ void __launch_bounds__(kKwThreads, 1)
           const int i = lane + 32 * k;
           lse[k] = i0 + i < it.n ? p.lse2[static_cast<int64_t>(h) * p.bd.T + tok + i] : -INFINITY;
         }
-        const bool room = gu < 2 || mbar_wait(&bars[kWbEmpty + s], ((gu >> 1) - 1) & 1, abort_flag, 121);
+        const bool room = (gu < 4 || mbar_wait(&bars[kWbLEmpty + (gu & 3)], ((gu >> 2) - 1) & 1, abort_flag, 122)) &&
+                          (gu < 2 || mbar_wait(&bars[kWbEmpty + s], ((gu >> 1) - 1) & 1, abort_flag, 121));
         ok = __all_sync(0xffffffffu, room);
         if (!ok) break;
 #pragma unroll
-        for (int k = 0; k < QT / 32; ++k) reinterpret_cast<float*>(st + L::sLse)[lane + 32 * k] = lse[k];
+        for (int k = 0; k < QT / 32; ++k)
+          reinterpret_cast<float*>(smem + L::oLse)[(gu & 3) * QT + lane + 32 * k] = lse[k];
         __syncwarp();
-        if (lane == 0) {  // (the arrival also publishes the LSE)
+        if (lane == 0) {
+          mbar_arrive(&bars[kWbLFull + (gu & 3)]);
           mbar_expect_tx(&bars[kWbFull + s], QT * (D + (graph ? 2 * RP : 0)) * 2 + (graph ? boxes * bk * RP * 2 : 0));
 #pragma unroll
           for (int c = 0; c < D / 64; ++c)
@@ -263,6 +307,7 @@ __global__ void __launch_bounds__(kKwThreads, 1)
     constexpr uint32_t idesc = make_idesc_bf16(kBlockN, QT, 0, 0);
     constexpr uint32_t r_layout = RP == 16 ? kSwizzle32B : kSwizzle64B;
     constexpr uint32_t r_sbo = 8 * RP * 2;
+    constexpr int NB = L::kBufs;
     int gu = 0, used[2] = {0, 0};
     bool ok = true;
     for (int n = 0; ok; ++n) {
@@ -282,15 +327,15 @@ __global__ void __launch_bounds__(kKwThreads, 1)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           if (i >= tiles) continue;
-          const int buf = 2 * i + (used[i] & 1);
-          if (used[i] >= 2 && !mbar_wait_spin(&bars[kWbSEmpty + buf], ((used[i] >> 1) - 1) & 1, abort_flag, 223)) {
+          const int buf = used[i] % NB;
+          if (used[i] >= NB && !mbar_wait_spin(&bars[kWbSEmpty + 4 * i + buf], (used[i] / NB - 1) & 1, abort_flag, 223)) {
             ok = false;
             break;
           }
           ++used[i];
           tc_fence_after();
           if (elect_one()) {
-            const uint32_t tS = tmem + 128 * buf;
+            const uint32_t tS = tmem + 256 * i + QT * buf;
             const uint32_t sK = smem_u32(smem + L::oK + (2 * ks + i) * L::kTile);
 #pragma unroll
             for (int kk = 0; kk < D / 16; ++kk)
@@ -305,7 +350,7 @@ __global__ void __launch_bounds__(kKwThreads, 1)
                 mma_ss(tS, rk, make_sdesc(st + L::sRq + L::kRqTile + kk * 32, 16, r_sbo, r_layout), idesc, 1);
               }
             }
-            mma_commit(&bars[kWbSFull + buf]);
+            mma_commit(&bars[kWbSFull + 4 * i + buf]);
             if (i == tiles - 1) mma_commit(&bars[kWbEmpty + s]);
           }
           __syncwarp();
@@ -331,9 +376,9 @@ __global__ void __launch_bounds__(kKwThreads, 1)
       float* dst = p.kw + items[ks].b * p.kw_sb + items[ks].kh * p.kw_sh + j;
       float w = mine && j < len ? *dst : 0.f;
       for (int u = 0; u < n_units; ++u, ++gu) {
-        const int s = gu & 1, buf = used & 1;
-        if (!mbar_wait(&bars[kWbFull + s], (gu >> 1) & 1, abort_flag, 321) ||
-            (mine && !mbar_wait(&bars[kWbSFull + 2 * wi + buf], (used >> 1) & 1, abort_flag, 322))) {
+        const int ls = gu & 3, buf = used % L::kBufs;
+        if (!mbar_wait(&bars[kWbLFull + ls], (gu >> 2) & 1, abort_flag, 321) ||
+            (mine && !mbar_wait(&bars[kWbSFull + 4 * wi + buf], (used / L::kBufs) & 1, abort_flag, 322))) {
           ok = false;
           break;
         }
@@ -341,43 +386,19 @@ __global__ void __launch_bounds__(kKwThreads, 1)
           ++used;
           tc_fence_after();
           const int i0 = (u0 + u % per_head) * QT;
-          const float4* lse4 = reinterpret_cast<const float4*>(smem + L::oStage + s * L::kStage + L::sLse);
+          const float4* lse4 = reinterpret_cast<const float4*>(smem + L::oLse + ls * QT * 4);
           // columns [first, nq - i0) belong to queries that see the key; a NaN score of another sequence's
           // query is never read into a sum
           const int first = p.causal ? j - past - i0 : 0;
           const bool whole = (!p.causal || tile0 + kBlockN - 1 <= past + i0) && i0 + QT <= nq;
-          float2 a[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-          uint32_t r[2][32];
-          tmem_ld32(t_lane + 128 * buf, r[0]);
-#pragma unroll
-          for (int c = 0; c < QT / 32; ++c) {
-            uint32_t* x = r[c & 1];
-            tmem_ld_wait32(x);
-            if (c + 1 < QT / 32) tmem_ld32(t_lane + 128 * buf + 32 * (c + 1), r[(c + 1) & 1]);
-            const int lo = first - 32 * c, hi = nq - i0 - 32 * c;
-#pragma unroll
-            for (int k = 0; k < 32; k += 4) {
-              const float4 l = lse4[8 * c + k / 4];
-              const float2 y0 = __ffma2_rn(f32x2(x[k], x[k + 1]), sl2, make_float2(l.x, l.y));
-              const float2 y1 = __ffma2_rn(f32x2(x[k + 2], x[k + 3]), sl2, make_float2(l.z, l.w));
-              float2 e0 = make_float2(ex2(y0.x), ex2(y0.y)), e1 = make_float2(ex2(y1.x), ex2(y1.y));
-              if (!whole) {
-                e0.x = k >= lo && k < hi ? e0.x : 0.f;
-                e0.y = k + 1 >= lo && k + 1 < hi ? e0.y : 0.f;
-                e1.x = k + 2 >= lo && k + 2 < hi ? e1.x : 0.f;
-                e1.y = k + 3 >= lo && k + 3 < hi ? e1.y : 0.f;
-              }
-              a[0] = __fadd2_rn(a[0], e0);
-              a[1] = __fadd2_rn(a[1], e1);
-            }
-          }
-          w += (a[0].x + a[0].y) + (a[1].x + a[1].y);
+          w += whole ? kw_sum<QT, false>(t_lane + QT * buf, lse4, sl2, 0, 0)
+                     : kw_sum<QT, true>(t_lane + QT * buf, lse4, sl2, first, nq - i0);
           tc_fence_before();
         }
         __syncwarp();
         if (lane == 0) {
-          if (mine) mbar_arrive(&bars[kWbSEmpty + 2 * wi + buf]);
-          mbar_arrive(&bars[kWbEmpty + s]);
+          if (mine) mbar_arrive(&bars[kWbSEmpty + 4 * wi + buf]);
+          mbar_arrive(&bars[kWbLEmpty + ls]);
         }
       }
       if (ok && mine && j < len) *dst = w;
