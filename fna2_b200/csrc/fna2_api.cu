@@ -770,6 +770,9 @@ struct PagedPlan {
 
 size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 
+// Workspace of the key weights: the R~_q hi / lo and LSE columns, and the item counter.
+size_t kw_workspace_bytes(int64_t T, int H, int RP) { return up256(static_cast<size_t>(T) * H * (2 * RP + 16) * 2) + 256; }
+
 // Splits of the tensor-core kernel's keys: `base` CTAs without splits, `tiles` key tiles each.  One
 // CTA runs per SM; a tile takes about 2 us, a CTA's start and end 6 us, and the join moves 8 D bytes
 // per row and split.  Takes the count with the least estimated time.
@@ -847,7 +850,7 @@ int paged_plan(const Fna2PagedKV* kv, const Fna2PagedAttnArgs* a, PagedAttnParam
   l->logit = take(l->logits, static_cast<size_t>(p->bd.B) * p->kv.hkv * max_rows * p->logit_sr * 4);
   l->lse2 = take(l->logits, th * 4);
   l->lse = take(p->kw && !l->logits && !a->lse, th * 4);
-  l->kw = take(p->kw && !l->logits, up256(th * 4) + up256(static_cast<size_t>(p->bd.T) * p->kv.hg * 4 * p->RP) + 256);
+  l->kw = take(p->kw && !l->logits, kw_workspace_bytes(p->bd.T, p->H, p->RP));
   l->total = at;
   return FNA2_OK;
 }
@@ -884,28 +887,22 @@ int many_maps(const PagedAttnParams& p, int D, ManyMaps* m) {
   return FNA2_OK;
 }
 
-// Workspace of the key weights: R~_q hi / lo rows and the log2-domain LSE.
-size_t kw_rq2_bytes(const KeyWeightsParams& p) { return up256(static_cast<size_t>(p.bd.T) * p.kv.hg * 2 * p.RP * 2); }
-size_t kw_workspace_bytes(const KeyWeightsParams& p) {
-  return kw_rq2_bytes(p) + up256(static_cast<size_t>(p.bd.T) * p.H * 4) + 256;
-}
-
 int run_key_weights(KeyWeightsParams& p, int D, uint8_t* ws, cudaStream_t st) {
   p.rq2 = reinterpret_cast<__nv_bfloat16*>(ws);
-  p.lse2 = reinterpret_cast<float*>(ws + kw_rq2_bytes(p));
-  p.next = reinterpret_cast<int*>(ws + kw_workspace_bytes(p) - 256);
+  p.next = reinterpret_cast<int*>(ws + kw_workspace_bytes(p.bd.T, p.H, p.RP) - 256);
   const int qt = kw_query_tile(p);
-  FNA2_CHECK(static_cast<int64_t>(p.bd.B) * p.kv.hkv * ((p.bd.max_k + 255) / 256) < (1ll << 30), "too many key tiles");
+  FNA2_CHECK(static_cast<int64_t>(p.bd.B) * p.kv.hkv * ((p.bd.max_k + 127) / 128) < (1ll << 30), "too many key tiles");
   const CUtensorMapSwizzle r_swz = p.RP == 16 ? CU_TENSOR_MAP_SWIZZLE_32B : CU_TENSOR_MAP_SWIZZLE_64B;
   KwMaps m;
   if (int rc = make_map(&m.q, p.q, D, p.bd.T, p.H, 1, p.q_st, p.q_sh, 0, 64, qt, CU_TENSOR_MAP_SWIZZLE_128B, "q"))
     return rc;
   if (int rc = map_pages(&m.k, p.kv.k, D, p.kv.hkv, p.kv, 64, kBlockN, CU_TENSOR_MAP_SWIZZLE_128B, "k pages")) return rc;
+  const int64_t w = 2 * p.RP + 16;
+  if (int rc = make_map(&m.l, p.rq2, w, p.bd.T, p.H, 1, p.H * w, w, 0, 16, qt, CU_TENSOR_MAP_SWIZZLE_32B, "lse columns"))
+    return rc;
   m.rq = m.q, m.rk = m.k;  // never dereferenced without graph heads
   if (p.kv.hg > 0) {
-    const int64_t w = 2 * p.RP;
-    if (int rc = make_map(&m.rq, p.rq2, w, p.bd.T, p.kv.hg, 1, p.kv.hg * w, w, 0, p.RP, qt, r_swz, "r_q hi, lo"))
-      return rc;
+    if (int rc = make_map(&m.rq, p.rq2, w, p.bd.T, p.H, 1, p.H * w, w, 0, p.RP, qt, r_swz, "r_q hi, lo")) return rc;
     if (int rc = map_pages(&m.rk, p.kv.rk, p.kv.rank, p.kv.hg, p.kv, p.RP, kBlockN, r_swz, "rk pages")) return rc;
   }
   FNA2_CUDA(launch_key_weights(m, p, D, st));
@@ -1017,7 +1014,7 @@ extern "C" size_t fna2_key_weights_workspace_size(const Fna2PagedKV* kv, const F
   g_last_error.clear();
   KeyWeightsParams p{};
   if (paged_queries(kv, a, &p)) return 0;
-  return kw_workspace_bytes(p);
+  return kw_workspace_bytes(p.bd.T, p.H, p.RP);
 }
 
 extern "C" int fna2_key_weights(const Fna2PagedKV* kv, const Fna2PagedAttnArgs* a, void* workspace,
@@ -1027,7 +1024,7 @@ extern "C" int fna2_key_weights(const Fna2PagedKV* kv, const Fna2PagedAttnArgs* 
   if (int rc = paged_queries(kv, a, &p)) return rc;
   FNA2_CHECK(a->key_weights != nullptr && (a->lse != nullptr || a->total_q == 0), "key weights need lse and key_weights");
   if (p.bd.B == 0 || p.bd.T == 0 || p.bd.max_k == 0) return FNA2_OK;
-  const size_t need = kw_workspace_bytes(p);
+  const size_t need = kw_workspace_bytes(p.bd.T, p.H, p.RP);
   if (workspace == nullptr || workspace_bytes < need)
     return fail(FNA2_ERR_WORKSPACE, "key weights workspace: need %zu bytes, got %zu", need, workspace_bytes);
   FNA2_CHECK((reinterpret_cast<uintptr_t>(workspace) & 255u) == 0, "workspace must be 256-byte aligned");

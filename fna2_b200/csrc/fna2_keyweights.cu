@@ -3,26 +3,30 @@
 //                  see key j of exp(S[h,i,j] - LSE[h,i])
 // with S and LSE as in the paged attention (fna2_paged.cu).
 //
-// Key-stationary on the tensor cores: the transposed scores S^T = [K | R_k | R_k]
-// [Q | R~_q hi | R~_q lo]^T put a key on every TMEM lane, so the thread that owns
-// a key sums its weights over the columns in a register: no reduction between
-// threads, no atomics on the result, which does not depend on timing.  An item is a
-// pair of 128-key tiles of one (sequence, KV head); its units are the (query head,
-// tile of QT queries) that see it.  One persistent CTA per SM draws items from a
-// counter and streams their units through a two-stage ring: Q, R~_q hi and lo, and
-// the R_k rows of that head for its keys.  QT is 64 when no sequence has more
-// queries (K is then double-buffered: an item is only as many units as there are
-// heads), else 128.
-//   warps 0-3 / 4-7  sum key tile 0 / 1 (thread t = key t = TMEM lane t)
+// Key-stationary on the tensor cores: the transposed scores
+//   S^T - LSE/scale = [K | R_k | R_k | 1] [Q | R~_q hi | R~_q lo | -LSE/scale]^T
+// put a key on every TMEM lane, so the thread that owns a key sums its weights over
+// the columns in a register: no reduction between threads (but one addition, below),
+// no atomics on the result, which does not depend on timing.  The LSE is one more
+// K slice, three bf16 terms that hold its 24 bits, so that a column costs the sum
+// warps one exp2, half a multiplication and half an addition (packed pairs).  One
+// persistent CTA per SM draws items (key tiles of a sequence and KV head) from a
+// counter and streams their units of 128 columns through a two-stage ring.
+//   QT = 128  an item is a pair of 128-key tiles, a unit 128 queries of one head;
+//             warpgroup i sums key tile i, and every Q tile serves both
+//   QT = 64   (no sequence has more than 64 queries) an item is one key tile, K is
+//             double-buffered, a unit is the queries of two heads side by side (one
+//             N = 128 product with K, then each head's R_k against its half);
+//             warpgroup i sums head i's half and the two are added at the end
+//   warps 0-3 / 4-7  sums (thread t = key t = TMEM lane t)
 //   warp 8           draws items, TMA producer (K and R_k page by page, as in
-//                    fna2_paged_many.cu)
-//   warp 9           TMEM allocation, MMA issue; each key tile has 256 / QT TMEM
-//                    buffers, so its next MMAs run while a unit is summed
-// The LSE has a ring of its own: with it in the operands' stages, a unit's loads
-// waited for the sums two units before (4200 clk per unit at QT = 128).
-// A small kernel first writes R~_q hi / lo rows and the log2-domain LSE.
-// Bound: one exp2 per (key, query, head), 16 per clock and SM: 2 x 128 x 128 of them
-// take 2048 clk per unit, the 2 x (D + 2 r_pad)/16 MMAs about 1300.
+//                    fna2_paged_many.cu; R_k only when the unit's heads change)
+//   warp 9           TMEM allocation, MMA issue
+//   warp 10          waits for warp 9 (a wait by the warp that issued MMAs returns only
+//                    when its own MMAs have drained; a named barrier does not)
+// A small kernel first writes the R~_q hi / lo and LSE columns.
+// Bound: exp2, 16 per clock and SM (2048 clk for the 2 x 128 x 128 of a QT = 128
+// unit), beside about 100 clk per MMA and the operands' way from L2 (48 KB a unit).
 #include "fna2_paged.cuh"
 
 namespace fna2 {
@@ -41,55 +45,59 @@ struct KeyWeightsParams {
   int64_t lse_sh;
   float* kw;
   int64_t kw_sb, kw_sh;
-  __nv_bfloat16* rq2;  // workspace: [T][H_G][2 RP] R~_q hi, lo
-  float* lse2;         // workspace: [H][T] -LSE * log2(e), -inf for a row without weight
+  __nv_bfloat16* rq2;  // workspace: [T][H][2 RP + 16]: R~_q hi, lo (graph heads), -LSE/scale as three terms
   int* next;           // workspace: item counter, zeroed by the prep kernel
 };
 
-// R~_q = gs/scale * R_q as hi + lo, columns [rank, RP) zero; -LSE in the log2 domain.
+// R~_q = gs/scale * R_q as hi + lo, columns [rank, RP) zero, and -LSE/scale = l1 + l2 + l3 (a row
+// without weight: -1e38, whose weights are 0).
 __global__ void __launch_bounds__(256) fna2_key_weights_prep_kernel(const KeyWeightsParams p) {
   const int64_t e = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
   if (e == 0) *p.next = 0;
-  const int r8 = p.RP / 8;
-  const int64_t n_r = static_cast<int64_t>(p.bd.T) * p.kv.hg * r8, n_l = static_cast<int64_t>(p.bd.T) * p.H;
-  if (e < n_r) {
-    const int c = static_cast<int>(e % r8) * 8, h = static_cast<int>(e / r8 % p.kv.hg);
-    const int64_t t = e / r8 / p.kv.hg;
+  const int r8 = p.RP / 8, per = r8 + 1;  // pieces of a row: R_q's, then the LSE's
+  if (e >= static_cast<int64_t>(p.bd.T) * p.H * per) return;
+  const int x = static_cast<int>(e % per), h = static_cast<int>(e / per % p.H);
+  const int64_t t = e / per / p.H;
+  __nv_bfloat16* dst = p.rq2 + (t * p.H + h) * (2 * p.RP + 16);
+  if (x == r8) {
+    const float lse = p.lse[h * p.lse_sh + t];
+    const float c = lse == -INFINITY ? -1e38f : -lse / p.scale;
+    const float l1 = __bfloat162float(__float2bfloat16_rn(c)), l2 = __bfloat162float(__float2bfloat16_rn(c - l1));
+    *reinterpret_cast<uint4*>(dst + 2 * p.RP) = make_uint4(pack_bf16(l1, l2), pack_bf16(c - l1 - l2, 0.f), 0, 0);
+    *reinterpret_cast<uint4*>(dst + 2 * p.RP + 8) = make_uint4(0, 0, 0, 0);
+  } else if (h < p.kv.hg) {
     uint32_t hi[4] = {0, 0, 0, 0}, lo[4] = {0, 0, 0, 0};
-    if (c < p.kv.rank)
-      split_bias(*reinterpret_cast<const uint4*>(p.rq + t * p.rq_st + h * p.rq_sh + c), __ldg(p.gs + h) / p.scale, hi, lo);
-    __nv_bfloat16* dst = p.rq2 + (t * p.kv.hg + h) * 2 * p.RP + c;
-    *reinterpret_cast<uint4*>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-    *reinterpret_cast<uint4*>(dst + p.RP) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-  }
-  if (e < n_l) {
-    const int64_t h = e / p.bd.T, t = e % p.bd.T;
-    const float v = p.lse[h * p.lse_sh + t];
-    p.lse2[e] = v == -INFINITY ? v : -v * kLog2e;
+    if (8 * x < p.kv.rank)
+      split_bias(*reinterpret_cast<const uint4*>(p.rq + t * p.rq_st + h * p.rq_sh + 8 * x), __ldg(p.gs + h) / p.scale,
+                 hi, lo);
+    *reinterpret_cast<uint4*>(dst + 8 * x) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+    *reinterpret_cast<uint4*>(dst + p.RP + 8 * x) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
   }
 }
 
-constexpr int kKwThreads = 320;
+constexpr int kKwThreads = 352;
 
 template <int D, int RP, int QT>
 struct KwSmem {
-  static constexpr int kTile = 128 * D * 2;    // K tile
-  static constexpr int kRTile = 128 * RP * 2;  // R_k of a key tile
-  static constexpr int kQTile = QT * D * 2;
-  static constexpr int kRqTile = QT * RP * 2;  // R~_q hi or lo
-  static constexpr int kChunk = 128 * 128;     // 64 columns of a 128-row tile
-  static constexpr int kQChunk = QT * 128;
-  static constexpr int kKStages = QT == 64 ? 2 : 1;
-  static constexpr int oK = 0;                                // kKStages x key tiles 0, 1
-  static constexpr int oStage = oK + kKStages * 2 * kTile;    // 2 x [Q | R_k 0, 1 | R~_q hi, lo]
-  static constexpr int sQ = 0, sRk = kQTile, sRq = sRk + 2 * kRTile;
-  static constexpr int kStage = sRq + 2 * kRqTile;
-  static constexpr int kBufs = 256 / QT;                      // TMEM buffers per key tile
-  static constexpr int oLse = oStage + 2 * kStage;            // 4 x -LSE of a unit
-  static constexpr int oBar = oLse + 4 * QT * 4;
+  static constexpr int kTiles = QT == 128 ? 2 : 1;     // key tiles of an item
+  static constexpr int kHeads = QT == 128 ? 1 : 2;     // heads of a unit
+  static constexpr int kKStages = QT == 128 ? 1 : 2;
+  static constexpr int kBufs = 4 / kTiles;             // 128-column TMEM buffers per key tile
+  static constexpr int kTile = 128 * D * 2;            // K tile, Q of a unit
+  static constexpr int kRTile = 128 * RP * 2;          // R_k of a key tile and head, R~_q hi or lo of a unit
+  static constexpr int kChunk = 128 * 128;             // 64 columns of a 128-row tile
+  static constexpr int oK = 0;                                     // kKStages x key tiles
+  static constexpr int kLTile = 128 * 32;              // the LSE's K slice of a unit, the ones against it
+  static constexpr int oStage = oK + kKStages * kTiles * kTile;    // 2 x [Q | R~_q hi, lo | LSE]
+  static constexpr int sQ = 0, sRq = kTile, sL = sRq + 2 * kRTile;
+  static constexpr int kStage = sL + kLTile;
+  static constexpr int oRk = oStage + 2 * kStage;                  // 2 x R_k of (head, tile): unit's heads
+  static constexpr int oOne = oRk + 2 * 2 * kRTile;
+  static constexpr int oPart = oOne + kLTile;                      // QT = 64: 2 x warpgroup 1's sums
+  static constexpr int oBar = oPart + 2 * 512;
   static constexpr int oMisc = oBar + 32 * 8;
-  static constexpr int oItem = oMisc + 16;                    // kKStages x KwItem
-  static constexpr int kUsed = oItem + kKStages * 32;
+  static constexpr int oItem = oMisc + 16;                         // kKStages x KwItem
+  static constexpr int kUsed = oItem + kKStages * 48;
   static constexpr int kTotal = kUsed + 1024;
   static_assert(kTotal <= kMaxDynamicSmem, "shared memory budget");
   static_assert(kStage % 1024 == 0, "swizzle atoms stay aligned");
@@ -100,19 +108,19 @@ enum KwBar {
   kWbKEmpty = 2,   // +K stage: its MMAs are done, every sum warp has left the item (1 + 8 arrivals)
   kWbFull = 4,     // +stage: the unit's operands
   kWbEmpty = 6,    // +stage: MMAs that read it are done
-  kWbLFull = 8,    // +LSE slot
-  kWbLEmpty = 12,  // +LSE slot (8 arrivals)
-  kWbSFull = 16,   // +4 tile + buffer
-  kWbSEmpty = 24,  // +4 tile + buffer (one arrival per warp)
+  kWbSFull = 8,    // +buffer (of key tile i: from kBufs i)
+  kWbSEmpty = 12,  // +buffer (one arrival per warp that reads it)
+  kWbPart = 16,    // +item parity: warpgroup 1's sums (QT = 64, 4 arrivals)
 };
 
 struct KwItem {
-  int b, kh, k0, len, n, u0, per_head, n_units;  // n_units < 0: no more items; u0: first query tile
+  int b, kh, k0, len, n, q0, u0, per_head, n_units;  // n_units < 0: no more items; u0: first query tile that sees keys
 };
 
-// Item `idx`: (pair of key tiles, KV head) of the sequences in packing order, KV heads of a pair
+// Item `idx`: (key tiles, KV head) of the sequences in packing order, the KV heads of the same keys
 // together, early keys (which the most queries see) first.  Called by a whole warp.
-__device__ __forceinline__ KwItem kw_item(const KeyWeightsParams& p, int idx, int lane, int QT) {
+template <int QT, int KEYS>
+__device__ __forceinline__ KwItem kw_item(const KeyWeightsParams& p, int idx, int lane) {
   KwItem it;
   it.n_units = -1;
   int carry = 0;
@@ -123,7 +131,7 @@ __device__ __forceinline__ KwItem kw_item(const KeyWeightsParams& p, int idx, in
     if (b < p.bd.B) {
       s = paged_seq(p.bd, b);
       if (!s.ok) atomicCAS(&g_device_error, 0, kStatusBadSeqPaged);
-      if (s.n > 0) cnt = (s.len + 2 * kBlockN - 1) / (2 * kBlockN) * p.kv.hkv;
+      if (s.n > 0) cnt = (s.len + KEYS - 1) / KEYS * p.kv.hkv;
     }
     int incl = cnt;
 #pragma unroll
@@ -137,13 +145,14 @@ __device__ __forceinline__ KwItem kw_item(const KeyWeightsParams& p, int idx, in
       const int local = idx - carry - (__shfl_sync(0xffffffffu, incl, src) - __shfl_sync(0xffffffffu, cnt, src));
       it.b = base + src;
       it.kh = local % p.kv.hkv;
-      it.k0 = local / p.kv.hkv * 2 * kBlockN;
+      it.k0 = local / p.kv.hkv * KEYS;
       it.len = __shfl_sync(0xffffffffu, s.len, src);
       it.n = __shfl_sync(0xffffffffu, s.n, src);
+      it.q0 = __shfl_sync(0xffffffffu, s.q0, src);
       const int n_qt = (it.n + QT - 1) / QT;
       it.u0 = p.causal ? min(n_qt, max(0, it.k0 - (it.len - it.n)) / QT) : 0;  // earlier tokens see none of these keys
       it.per_head = n_qt - it.u0;
-      it.n_units = it.per_head * p.G;
+      it.n_units = QT == 128 ? it.per_head * p.G : it.per_head * ((p.G + 1) / 2);
       return it;
     }
     carry += __shfl_sync(0xffffffffu, incl, 31);
@@ -151,10 +160,10 @@ __device__ __forceinline__ KwItem kw_item(const KeyWeightsParams& p, int idx, in
   return it;
 }
 
-// Sum over the QT columns of this thread's lane of 2^(sl2 S - LSE); MASK: of columns [lo, hi) only.
+// Sum over the QT columns of this thread's lane of 2^(sl2 S); MASK: of columns [lo, hi) only.
 // (Two copies: masks cost 5 instructions per column.)
 template <int QT, bool MASK>
-__device__ __forceinline__ float kw_sum(uint32_t t_addr, const float4* lse4, float2 sl2, int lo, int hi) {
+__device__ __forceinline__ float kw_sum(uint32_t t_addr, float2 sl2, int lo, int hi) {
   float2 a[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
   uint32_t r[2][32];
   tmem_ld32(t_addr, r[0]);
@@ -164,20 +173,15 @@ __device__ __forceinline__ float kw_sum(uint32_t t_addr, const float4* lse4, flo
     tmem_ld_wait32(x);
     if (c + 1 < QT / 32) tmem_ld32(t_addr + 32 * (c + 1), r[(c + 1) & 1]);
 #pragma unroll
-    for (int k = 0; k < 32; k += 4) {
-      const float4 l = lse4[8 * c + k / 4];
-      const float2 y0 = __ffma2_rn(f32x2(x[k], x[k + 1]), sl2, make_float2(l.x, l.y));
-      const float2 y1 = __ffma2_rn(f32x2(x[k + 2], x[k + 3]), sl2, make_float2(l.z, l.w));
-      float2 e0 = make_float2(ex2(y0.x), ex2(y0.y)), e1 = make_float2(ex2(y1.x), ex2(y1.y));
+    for (int k = 0; k < 32; k += 2) {
+      const float2 y = __fmul2_rn(f32x2(x[k], x[k + 1]), sl2);
+      float2 e = make_float2(ex2(y.x), ex2(y.y));
       if (MASK) {
         const int col = 32 * c + k;
-        e0.x = col >= lo && col < hi ? e0.x : 0.f;
-        e0.y = col + 1 >= lo && col + 1 < hi ? e0.y : 0.f;
-        e1.x = col + 2 >= lo && col + 2 < hi ? e1.x : 0.f;
-        e1.y = col + 3 >= lo && col + 3 < hi ? e1.y : 0.f;
+        e.x = col >= lo && col < hi ? e.x : 0.f;
+        e.y = col + 1 >= lo && col + 1 < hi ? e.y : 0.f;
       }
-      a[0] = __fadd2_rn(a[0], e0);
-      a[1] = __fadd2_rn(a[1], e1);
+      a[k / 2 & 1] = __fadd2_rn(a[k / 2 & 1], e);
     }
   }
   return (a[0].x + a[0].y) + (a[1].x + a[1].y);
@@ -187,9 +191,9 @@ template <int D, int RP, int QT>
 __global__ void __launch_bounds__(kKwThreads, 1)
     fna2_key_weights_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                             const __grid_constant__ CUtensorMap tmRq, const __grid_constant__ CUtensorMap tmRk,
-                            const KeyWeightsParams p) {
+                            const __grid_constant__ CUtensorMap tmL, const KeyWeightsParams p) {
   using L = KwSmem<D, RP, QT>;
-  constexpr int KS = L::kKStages;
+  constexpr int KS = L::kKStages, NT = L::kTiles, NH = L::kHeads, NB = L::kBufs;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::oBar);
@@ -204,18 +208,20 @@ __global__ void __launch_bounds__(kKwThreads, 1)
       mbar_init(&bars[kWbKEmpty + s], 9);
       mbar_init(&bars[kWbFull + s], 1);
       mbar_init(&bars[kWbEmpty + s], 1);
+      mbar_init(&bars[kWbPart + s], 4);
     }
     for (int s = 0; s < 4; ++s) {
-      mbar_init(&bars[kWbLFull + s], 1);
-      mbar_init(&bars[kWbLEmpty + s], 8);
-    }
-    for (int s = 0; s < 8; ++s) {
       mbar_init(&bars[kWbSFull + s], 1);
-      mbar_init(&bars[kWbSEmpty + s], 4);
+      mbar_init(&bars[kWbSEmpty + s], 8 / NT);
     }
     *abort_flag = 0;
     fence_mbar_init();
   }
+  // the ones against the LSE's three terms: columns 0-2 of 16, 32-byte swizzled rows
+  for (int e = tid; e < 256; e += kKwThreads)
+    *reinterpret_cast<uint4*>(smem + L::oOne + e * 16) =
+        (e & 1) == ((e >> 3) & 1) ? make_uint4(0x3f803f80u, 0x00003f80u, 0, 0) : make_uint4(0, 0, 0, 0);
+  fence_proxy_async_smem();
   if (warp == 9) {
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
@@ -232,20 +238,29 @@ __global__ void __launch_bounds__(kKwThreads, 1)
       tma_prefetch_desc(&tmK);
     }
     const int lg = p.kv.page_log2, mask = (1 << lg) - 1;
-    const int bk = min(1 << lg, kBlockN);  // rows of a box; lane l owns box l of the two key tiles (at most 16)
+    const int bk = min(1 << lg, kBlockN);  // rows of a box; lane l owns box l of the key tiles (at most 16)
     const int tile = lane * bk / kBlockN, row = lane * bk % kBlockN;
-    int gu = 0;  // units so far
-    for (int n = 0;; ++n) {
-      const int ks = n % KS;
+    // Items are drawn and their pages looked up while earlier units wait for room.
+    auto draw = [&]() {
       int idx = 0;
       if (lane == 0) idx = atomicAdd(p.next, 1);
-      idx = __shfl_sync(0xffffffffu, idx, 0);
-      const KwItem it = kw_item(p, idx, lane, QT);
+      return kw_item<QT, NT * kBlockN>(p, __shfl_sync(0xffffffffu, idx, 0), lane);
+    };
+    auto page_of = [&](const KwItem& it) {
+      const int key = it.k0 + lane * bk;
+      return it.n_units >= 0 && lane * bk < NT * kBlockN && key < it.len
+                 ? __ldg(p.kv.table + it.b * p.kv.table_sb + (key >> lg))
+                 : -1;
+    };
+    KwItem it = draw(), next = it;
+    int page = page_of(it), next_page = -1;
+    int gu = 0, rs = 1;  // units so far, R_k slot
+    for (int n = 0;; ++n) {
+      const int ks = n % KS;
       const bool free = n < KS || mbar_wait(&bars[kWbKEmpty + ks], (n / KS - 1) & 1, abort_flag, 120);
       if (!__all_sync(0xffffffffu, free)) break;
       const int key = it.k0 + lane * bk;
-      const bool mine = it.n_units >= 0 && lane * bk < 2 * kBlockN && key < it.len;
-      const int page = mine ? __ldg(p.kv.table + it.b * p.kv.table_sb + (key >> lg)) : 0;
+      const bool mine = it.n_units >= 0 && lane * bk < NT * kBlockN && key < it.len;
       const int boxes = __popc(__ballot_sync(0xffffffffu, mine));
       if (lane == 0) {  // (the arrival also publishes the description)
         volatile KwItem* d = items + ks;
@@ -258,150 +273,166 @@ __global__ void __launch_bounds__(kKwThreads, 1)
       if (mine) {
 #pragma unroll
         for (int c = 0; c < D / 64; ++c)
-          tma_load_4d(smem + L::oK + (2 * ks + tile) * L::kTile + c * L::kChunk + row * 128, &tmK,
+          tma_load_4d(smem + L::oK + (NT * ks + tile) * L::kTile + c * L::kChunk + row * 128, &tmK,
                       &bars[kWbKFull + ks], c * 64, key & mask, it.kh, page);
       }
       __syncwarp();
-      const int q0 = __ldg(p.bd.cu + it.b);
+      auto fetch = [&]() {
+        next = draw();
+        next_page = page_of(next);
+      };
+      if (it.n_units == 0) fetch();
       bool ok = true;
       for (int u = 0; u < it.n_units; ++u, ++gu) {
-        const int s = gu & 1, h = it.kh * p.G + u / it.per_head;
-        const int i0 = (it.u0 + u % it.per_head) * QT, tok = q0 + i0;
-        const bool graph = h < p.kv.hg;
+        const int s = gu & 1;
+        const int h0 = it.kh * p.G + (QT == 128 ? u / it.per_head : 2 * u), nh = min(NH, (it.kh + 1) * p.G - h0);
+        const int tok = it.q0 + (QT == 128 ? (it.u0 + u % it.per_head) * QT : 0);
+        const int ng = max(0, min(nh, p.kv.hg - h0));  // heads of the unit that carry the bias
         uint8_t* st = smem + L::oStage + s * L::kStage;
-        // this unit's -LSE (columns past the end: -inf, which adds 0)
-        float lse[QT / 32];
-#pragma unroll
-        for (int k = 0; k < QT / 32; ++k) {
-          const int i = lane + 32 * k;
-          lse[k] = i0 + i < it.n ? p.lse2[static_cast<int64_t>(h) * p.bd.T + tok + i] : -INFINITY;
-        }
-        const bool room = (gu < 4 || mbar_wait(&bars[kWbLEmpty + (gu & 3)], ((gu >> 2) - 1) & 1, abort_flag, 122)) &&
-                          (gu < 2 || mbar_wait(&bars[kWbEmpty + s], ((gu >> 1) - 1) & 1, abort_flag, 121));
+        // R_k: unless this unit's head is the last one's.  The slot's former readers are done: the unit before
+        // the last one is, and at least one unit has used the other slot since.
+        const bool fresh = QT == 64 || u % it.per_head == 0;
+        if (fresh) rs ^= 1;
+        const bool room = gu < 2 || mbar_wait(&bars[kWbEmpty + s], ((gu >> 1) - 1) & 1, abort_flag, 121);
         ok = __all_sync(0xffffffffu, room);
         if (!ok) break;
-#pragma unroll
-        for (int k = 0; k < QT / 32; ++k)
-          reinterpret_cast<float*>(smem + L::oLse)[(gu & 3) * QT + lane + 32 * k] = lse[k];
+        if (lane == 0)
+          mbar_expect_tx(&bars[kWbFull + s], QT * (nh * (D + 16) + ng * 2 * RP) * 2 + (fresh ? ng * boxes * bk * RP * 2 : 0));
         __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(&bars[kWbLFull + (gu & 3)]);
-          mbar_expect_tx(&bars[kWbFull + s], QT * (D + (graph ? 2 * RP : 0)) * 2 + (graph ? boxes * bk * RP * 2 : 0));
-#pragma unroll
-          for (int c = 0; c < D / 64; ++c)
-            tma_load_4d(st + L::sQ + c * L::kQChunk, &tmQ, &bars[kWbFull + s], c * 64, tok, h, 0);
-          if (graph) {
-            tma_load_4d(st + L::sRq, &tmRq, &bars[kWbFull + s], 0, tok, h, 0);
-            tma_load_4d(st + L::sRq + L::kRqTile, &tmRq, &bars[kWbFull + s], RP, tok, h, 0);
-          }
+        // lanes 16 + (0 .. 2 D/64): Q chunks; lanes 24 + (0 .. 4): R~_q hi, lo; lanes 28 + (0, 1): LSE; a head each
+        // in turn
+        const int x = lane - 16, y = lane - 24, z = lane - 28, g_q = x / (D / 64), g_r = y / 2;
+        const bool is_q = x >= 0 && x < 8 && g_q < nh, is_r = y >= 0 && y < 4 && g_r < ng, is_l = z >= 0 && z < nh;
+        if (is_q || is_r || is_l) {
+          uint8_t* dst = st + (is_q   ? L::sQ + x % (D / 64) * L::kChunk + g_q * QT * 128
+                               : is_r ? L::sRq + y % 2 * L::kRTile + g_r * QT * RP * 2
+                                      : L::sL + z * QT * 32);
+          tma_load_4d(dst, is_q ? &tmQ : is_r ? &tmRq : &tmL, &bars[kWbFull + s],
+                      is_q ? x % (D / 64) * 64 : is_r ? y % 2 * RP : 2 * RP, tok, h0 + (is_q ? g_q : is_r ? g_r : z), 0);
         }
+        if (mine && fresh)
+          for (int g = 0; g < ng; ++g)
+            tma_load_4d(smem + L::oRk + (2 * rs + g * NT + tile) * L::kRTile + row * RP * 2, &tmRk, &bars[kWbFull + s], 0,
+                        key & mask, h0 + g, page);
         __syncwarp();
-        if (mine && graph)
-          tma_load_4d(st + L::sRk + tile * L::kRTile + row * RP * 2, &tmRk, &bars[kWbFull + s], 0, key & mask, h, page);
-        __syncwarp();
+        if (u == max(0, it.n_units - 2)) fetch();  // not earlier: who draws early gets work before it is free
       }
       if (!ok) break;
+      it = next, page = next_page;
     }
-  } else if (warp == 9) {
-    // ------------------------------------------------------------ MMA issuer
-    constexpr uint32_t idesc = make_idesc_bf16(kBlockN, QT, 0, 0);
+  } else if (warp >= 9) {
+    // ------------------------------------------------------------ MMA issuer (9) and its waiter (10)
+    constexpr uint32_t idesc = make_idesc_bf16(kBlockN, 128, 0, 0), idesc_r = make_idesc_bf16(kBlockN, QT, 0, 0);
     constexpr uint32_t r_layout = RP == 16 ? kSwizzle32B : kSwizzle64B;
     constexpr uint32_t r_sbo = 8 * RP * 2;
-    constexpr int NB = L::kBufs;
-    int gu = 0, used[2] = {0, 0};
+    const bool issuer = warp == 9;
+    int gu = 0, rs = 1, used[NT] = {};
     bool ok = true;
     for (int n = 0; ok; ++n) {
       const int ks = n % KS;
-      if (!mbar_wait(&bars[kWbKFull + ks], (n / KS) & 1, abort_flag, 221)) break;
-      const int n_units = items[ks].n_units, per_head = items[ks].per_head, h0 = items[ks].kh * p.G;
-      const int tiles = items[ks].k0 + kBlockN < items[ks].len ? 2 : 1;
+      ok = issuer || mbar_wait(&bars[kWbKFull + ks], (n / KS) & 1, abort_flag, 221);
+      ok = pair_rendezvous(1, ok);
+      if (!ok) break;
+      const int n_units = items[ks].n_units, per_head = items[ks].per_head, kh = items[ks].kh;
+      const int tiles = items[ks].k0 + kBlockN < items[ks].len ? NT : 1;
       if (n_units < 0) break;
       for (int u = 0; ok && u < n_units; ++u, ++gu) {
         const int s = gu & 1;
-        const bool graph = h0 + u / per_head < p.kv.hg;
-        if (!mbar_wait_spin(&bars[kWbFull + s], (gu >> 1) & 1, abort_flag, 222)) {
-          ok = false;
-          break;
-        }
+        const int h0 = kh * p.G + (QT == 128 ? u / per_head : 2 * u), nh = min(NH, (kh + 1) * p.G - h0);
         const uint32_t st = smem_u32(smem + L::oStage + s * L::kStage);
+        if (QT == 64 || u % per_head == 0) rs ^= 1;
+        if (!issuer) ok = mbar_wait(&bars[kWbFull + s], (gu >> 1) & 1, abort_flag, 222);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < NT; ++i) {
           if (i >= tiles) continue;
-          const int buf = used[i] % NB;
-          if (used[i] >= NB && !mbar_wait_spin(&bars[kWbSEmpty + 4 * i + buf], (used[i] / NB - 1) & 1, abort_flag, 223)) {
-            ok = false;
-            break;
-          }
+          const int buf = NB * i + used[i] % NB;
+          if (!issuer && ok && used[i] >= NB)
+            ok = mbar_wait(&bars[kWbSEmpty + buf], (used[i] / NB - 1) & 1, abort_flag, 223);
           ++used[i];
+          ok = pair_rendezvous(1, ok);
+          if (!ok) break;
+          if (!issuer) continue;
           tc_fence_after();
           if (elect_one()) {
-            const uint32_t tS = tmem + 256 * i + QT * buf;
-            const uint32_t sK = smem_u32(smem + L::oK + (2 * ks + i) * L::kTile);
+            const uint32_t tS = tmem + 128 * buf;
+            const uint32_t sK = smem_u32(smem + L::oK + (NT * ks + i) * L::kTile);
 #pragma unroll
-            for (int kk = 0; kk < D / 16; ++kk)
-              mma_ss(tS, make_sdesc(sK + (kk >> 2) * L::kChunk + (kk & 3) * 32, 16, 1024, kSwizzle128B),
-                     make_sdesc(st + L::sQ + (kk >> 2) * L::kQChunk + (kk & 3) * 32, 16, 1024, kSwizzle128B), idesc,
-                     kk > 0);
-            if (graph) {
+            for (int kk = 0; kk < D / 16; ++kk) {
+              const uint32_t off = (kk >> 2) * L::kChunk + (kk & 3) * 32;
+              mma_ss(tS, make_sdesc(sK + off, 16, 1024, kSwizzle128B),
+                     make_sdesc(st + L::sQ + off, 16, 1024, kSwizzle128B), idesc, kk > 0);
+            }
+            mma_ss(tS, make_sdesc(smem_u32(smem + L::oOne), 16, 256, kSwizzle32B),
+                   make_sdesc(st + L::sL, 16, 256, kSwizzle32B), idesc, 1);
+#pragma unroll
+            for (int g = 0; g < NH; ++g) {
+              if (g >= nh || h0 + g >= p.kv.hg) continue;
+              const uint32_t sRk = smem_u32(smem + L::oRk + (2 * rs + g * NT + i) * L::kRTile);
 #pragma unroll
               for (int kk = 0; kk < RP / 16; ++kk) {
-                const uint64_t rk = make_sdesc(st + L::sRk + i * L::kRTile + kk * 32, 16, r_sbo, r_layout);
-                mma_ss(tS, rk, make_sdesc(st + L::sRq + kk * 32, 16, r_sbo, r_layout), idesc, 1);
-                mma_ss(tS, rk, make_sdesc(st + L::sRq + L::kRqTile + kk * 32, 16, r_sbo, r_layout), idesc, 1);
+                const uint32_t hi = st + L::sRq + g * QT * RP * 2 + kk * 32;
+                const uint64_t rk = make_sdesc(sRk + kk * 32, 16, r_sbo, r_layout);
+                mma_ss(tS + g * QT, rk, make_sdesc(hi, 16, r_sbo, r_layout), idesc_r, 1);
+                mma_ss(tS + g * QT, rk, make_sdesc(hi + L::kRTile, 16, r_sbo, r_layout), idesc_r, 1);
               }
             }
-            mma_commit(&bars[kWbSFull + 4 * i + buf]);
+            mma_commit(&bars[kWbSFull + buf]);
             if (i == tiles - 1) mma_commit(&bars[kWbEmpty + s]);
           }
           __syncwarp();
         }
       }
-      if (ok && elect_one()) mma_commit(&bars[kWbKEmpty + ks]);
+      if (ok && issuer && elect_one()) mma_commit(&bars[kWbKEmpty + ks]);
       __syncwarp();
     }
   } else {
-    // ------------------------------------------------------------ sums (warpgroup i = key tile i)
-    const int wi = warp >> 2;
-    const uint32_t t_lane = tmem + 256 * wi + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+    // ------------------------------------------------------------ sums
+    const int wi = warp >> 2, ti = NT == 2 ? wi : 0, gi = NT == 2 ? 0 : wi;  // key tile, head of the unit
+    const uint32_t t_lane = tmem + 128 * NB * ti + gi * QT + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     const float2 sl2 = make_float2(p.scale_log2, p.scale_log2);
-    int gu = 0, used = 0;
+    int used = 0;
     bool ok = true;
     for (int n = 0; ok; ++n) {
       const int ks = n % KS;
       if (!mbar_wait(&bars[kWbKFull + ks], (n / KS) & 1, abort_flag, 320)) break;
       const int n_units = items[ks].n_units, per_head = items[ks].per_head, u0 = items[ks].u0, nq = items[ks].n;
-      const int len = items[ks].len, tile0 = items[ks].k0 + wi * kBlockN, j = tile0 + (tid & 127), past = len - nq;
+      const int len = items[ks].len, tile0 = items[ks].k0 + ti * kBlockN, j = tile0 + (tid & 127), past = len - nq;
       if (n_units < 0) break;
-      const bool mine = tile0 < len;
+      const bool mine = tile0 < len;  // this key tile has keys
       float* dst = p.kw + items[ks].b * p.kw_sb + items[ks].kh * p.kw_sh + j;
-      float w = mine && j < len ? *dst : 0.f;
-      for (int u = 0; u < n_units; ++u, ++gu) {
-        const int ls = gu & 3, buf = used % L::kBufs;
-        if (!mbar_wait(&bars[kWbLFull + ls], (gu >> 2) & 1, abort_flag, 321) ||
-            (mine && !mbar_wait(&bars[kWbSFull + 4 * wi + buf], (used / L::kBufs) & 1, abort_flag, 322))) {
+      float w = gi == 0 && mine && j < len ? *dst : 0.f;
+      for (int u = 0; u < n_units; ++u) {
+        const int buf = NB * ti + used % NB;
+        if (!mine) continue;
+        if (!mbar_wait(&bars[kWbSFull + buf], (used / NB) & 1, abort_flag, 322)) {
           ok = false;
           break;
         }
-        if (mine) {
-          ++used;
-          tc_fence_after();
-          const int i0 = (u0 + u % per_head) * QT;
-          const float4* lse4 = reinterpret_cast<const float4*>(smem + L::oLse + ls * QT * 4);
-          // columns [first, nq - i0) belong to queries that see the key; a NaN score of another sequence's
-          // query is never read into a sum
-          const int first = p.causal ? j - past - i0 : 0;
-          const bool whole = (!p.causal || tile0 + kBlockN - 1 <= past + i0) && i0 + QT <= nq;
-          w += whole ? kw_sum<QT, false>(t_lane + QT * buf, lse4, sl2, 0, 0)
-                     : kw_sum<QT, true>(t_lane + QT * buf, lse4, sl2, first, nq - i0);
-          tc_fence_before();
-        }
+        tc_fence_after();
+        const int i0 = QT == 128 ? (u0 + u % per_head) * QT : 0;
+        // columns [first, nq - i0) belong to queries that see the key; the score of another sequence's
+        // query or of a head that the unit lacks is never read into a sum
+        const int first = p.causal ? j - past - i0 : 0;
+        const bool whole = (!p.causal || tile0 + kBlockN - 1 <= past + i0) && i0 + QT <= nq;
+        const uint32_t at = t_lane + 128 * (used % NB);
+        if (NH == 1 || 2 * u + gi < p.G)
+          w += whole ? kw_sum<QT, false>(at, sl2, 0, 0) : kw_sum<QT, true>(at, sl2, first, nq - i0);
+        ++used;
+        tc_fence_before();
         __syncwarp();
-        if (lane == 0) {
-          if (mine) mbar_arrive(&bars[kWbSEmpty + 4 * wi + buf]);
-          mbar_arrive(&bars[kWbLEmpty + ls]);
+        if (lane == 0) mbar_arrive(&bars[kWbSEmpty + buf]);
+      }
+      if (NT == 1) {  // add the two heads' halves (a slot is written again only after everyone left its item)
+        float* part = reinterpret_cast<float*>(smem + L::oPart) + (n & 1) * 128 + (tid & 127);
+        if (wi == 1) {
+          *part = w;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bars[kWbPart + (n & 1)]);
+        } else if (ok && (ok = mbar_wait(&bars[kWbPart + (n & 1)], (n >> 1) & 1, abort_flag, 323))) {
+          w += *part;
         }
       }
-      if (ok && mine && j < len) *dst = w;
+      if (ok && gi == 0 && mine && j < len) *dst = w;
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars[kWbKEmpty + ks]);
     }
@@ -416,7 +447,7 @@ __global__ void __launch_bounds__(kKwThreads, 1)
 }
 
 struct KwMaps {
-  CUtensorMap q, k, rq, rk;
+  CUtensorMap q, k, rq, rk, l;
 };
 
 // Queries per unit.
@@ -429,11 +460,11 @@ cudaError_t launch_key_weights_t(const KwMaps& m, const KeyWeightsParams& p, cud
   static std::atomic<uint64_t> allowed{0};
   cudaError_t e = allow_smem(reinterpret_cast<const void*>(kern), allowed);
   if (e != cudaSuccess) return e;
-  const int64_t n = static_cast<int64_t>(p.bd.T) * std::max<int64_t>(p.H, static_cast<int64_t>(p.kv.hg) * p.RP / 8);
+  const int64_t n = static_cast<int64_t>(p.bd.T) * p.H * (p.RP / 8 + 1);
   fna2_key_weights_prep_kernel<<<static_cast<unsigned>((n + 255) / 256), 256, 0, stream>>>(p);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
-  const int64_t items = static_cast<int64_t>(p.bd.B) * p.kv.hkv * ((p.bd.max_k + 2 * kBlockN - 1) / (2 * kBlockN));
-  kern<<<static_cast<unsigned>(std::min<int64_t>(items, kSms)), kKwThreads, L::kTotal, stream>>>(m.q, m.k, m.rq, m.rk, p);
+  const int64_t items = static_cast<int64_t>(p.bd.B) * p.kv.hkv * ((p.bd.max_k + L::kTiles * kBlockN - 1) / (L::kTiles * kBlockN));
+  kern<<<static_cast<unsigned>(std::min<int64_t>(items, kSms)), kKwThreads, L::kTotal, stream>>>(m.q, m.k, m.rq, m.rk, m.l, p);
   return cudaGetLastError();
 }
 
