@@ -3,30 +3,30 @@
 //                  see key j of exp(S[h,i,j] - LSE[h,i])
 // with S and LSE as in the paged attention (fna2_paged.cu).
 //
-// Key-stationary on the tensor cores: the transposed scores
+// On the tensor cores, the transposed scores
 //   S^T - LSE/scale = [K | R_k | R_k | 1] [Q | R~_q hi | R~_q lo | -LSE/scale]^T
 // put a key on every TMEM lane, so the thread that owns a key sums its weights over
 // the columns in a register: no reduction between threads (but one addition, below),
 // no atomics on the result, which does not depend on timing.  The LSE is one more
 // K slice, three bf16 terms that hold its 24 bits, so that a column costs the sum
-// warps one exp2, half a multiplication and half an addition (packed pairs).  One
-// persistent CTA per SM draws items (key tiles of a sequence and KV head) from a
-// counter and streams their units of 128 columns through a two-stage ring.
-//   QT = 128  an item is a pair of 128-key tiles, a unit 128 queries of one head;
-//             warpgroup i sums key tile i, and every Q tile serves both
-//   QT = 64   (no sequence has more than 64 queries) an item is one key tile, K is
-//             double-buffered, a unit is the queries of two heads side by side (one
-//             N = 128 product with K, then each head's R_k against its half);
-//             warpgroup i sums head i's half and the two are added at the end
-//   warps 0-3 / 4-7  sums (thread t = key t = TMEM lane t)
-//   warp 8           draws items, TMA producer (K and R_k page by page, as in
-//                    fna2_paged_many.cu; R_k only when the unit's heads change)
-//   warp 9           TMEM allocation, MMA issue
-//   warp 10          waits for warp 9 (a wait by the warp that issued MMAs returns only
-//                    when its own MMAs have drained; a named barrier does not)
-// A small kernel first writes the R~_q hi / lo and LSE columns.
-// Bound: exp2, 16 per clock and SM (2048 clk for the 2 x 128 x 128 of a QT = 128
-// unit), beside about 100 clk per MMA and the operands' way from L2 (48 KB a unit).
+// warps one exp2, half a multiplication and half an addition (packed pairs).  A small
+// kernel first writes the R~_q hi / lo and LSE columns.  Persistent CTAs, one per SM,
+// draw items from a counter and work on units of 128 columns:
+//   fna2_key_weights_kernel         key-stationary: an item is a pair of 128-key tiles
+//     of a (sequence, KV head), a unit 128 queries of one head; warpgroup i sums key
+//     tile i, every Q tile serves both.
+//   fna2_key_weights_window_kernel  query-stationary, when no sequence has more than
+//     64 queries: an item is a run of key tiles, the queries of up to four heads stay
+//     in shared memory while K and R_k stream (streaming Q past each key tile instead
+//     took 128 KB per tile from L2 where this takes 48, and ran at its rate); a unit
+//     is two heads side by side (one N = 128 product with K, then each head's R_k
+//     against its half), warpgroup i sums head i's half, and the two are added.
+// Warps 0-7: sums (thread t = key t = TMEM lane t); warp 8: draws items, TMA (K and R_k
+// page by page, as in fna2_paged_many.cu); warp 9: TMEM allocation, MMA issue; warp 10:
+// waits for warp 9 (a wait by the warp that issued MMAs returns only when its own MMAs
+// have drained; a named barrier does not).
+// Bound: exp2, 16 per clock and SM (2048 clk for the 2 x 128 x 128 of a key-stationary
+// unit), beside about 100 clk per MMA and the operands' way from L2.
 #include "fna2_paged.cuh"
 
 namespace fna2 {
@@ -47,6 +47,7 @@ struct KeyWeightsParams {
   int64_t kw_sb, kw_sh;
   __nv_bfloat16* rq2;  // workspace: [T][H][2 RP + 16]: R~_q hi, lo (graph heads), -LSE/scale as three terms
   int* next;           // workspace: item counter, zeroed by the prep kernel
+  int run_tiles;       // key tiles per item
 };
 
 // R~_q = gs/scale * R_q as hi + lo, columns [rank, RP) zero, and -LSE/scale = l1 + l2 + l3 (a row
@@ -77,50 +78,43 @@ __global__ void __launch_bounds__(256) fna2_key_weights_prep_kernel(const KeyWei
 
 constexpr int kKwThreads = 352;
 
-template <int D, int RP, int QT>
+template <int D, int RP>
 struct KwSmem {
-  static constexpr int kTiles = QT == 128 ? 2 : 1;     // key tiles of an item
-  static constexpr int kHeads = QT == 128 ? 1 : 2;     // heads of a unit
-  static constexpr int kKStages = QT == 128 ? 1 : 2;
-  static constexpr int kBufs = 4 / kTiles;             // 128-column TMEM buffers per key tile
   static constexpr int kTile = 128 * D * 2;            // K tile, Q of a unit
-  static constexpr int kRTile = 128 * RP * 2;          // R_k of a key tile and head, R~_q hi or lo of a unit
+  static constexpr int kRTile = 128 * RP * 2;          // R_k of a key tile, R~_q hi or lo of a unit
   static constexpr int kChunk = 128 * 128;             // 64 columns of a 128-row tile
-  static constexpr int oK = 0;                                     // kKStages x key tiles
   static constexpr int kLTile = 128 * 32;              // the LSE's K slice of a unit, the ones against it
-  static constexpr int oStage = oK + kKStages * kTiles * kTile;    // 2 x [Q | R~_q hi, lo | LSE]
+  static constexpr int oK = 0;                         // key tiles 0, 1
+  static constexpr int oStage = oK + 2 * kTile;        // 2 x [Q | R~_q hi, lo | LSE]
   static constexpr int sQ = 0, sRq = kTile, sL = sRq + 2 * kRTile;
   static constexpr int kStage = sL + kLTile;
-  static constexpr int oRk = oStage + 2 * kStage;                  // 2 x R_k of (head, tile): unit's heads
+  static constexpr int oRk = oStage + 2 * kStage;      // 2 x R_k of key tiles 0, 1 and the unit's head
   static constexpr int oOne = oRk + 2 * 2 * kRTile;
-  static constexpr int oPart = oOne + kLTile;                      // QT = 64: 2 x warpgroup 1's sums
-  static constexpr int oBar = oPart + 2 * 512;
+  static constexpr int oBar = oOne + kLTile;
   static constexpr int oMisc = oBar + 32 * 8;
-  static constexpr int oItem = oMisc + 16;                         // kKStages x KwItem
-  static constexpr int kUsed = oItem + kKStages * 48;
+  static constexpr int oItem = oMisc + 16;
+  static constexpr int kUsed = oItem + 64;
   static constexpr int kTotal = kUsed + 1024;
   static_assert(kTotal <= kMaxDynamicSmem, "shared memory budget");
   static_assert(kStage % 1024 == 0, "swizzle atoms stay aligned");
 };
 
 enum KwBar {
-  kWbKFull = 0,    // +K stage: K and the item's description
-  kWbKEmpty = 2,   // +K stage: its MMAs are done, every sum warp has left the item (1 + 8 arrivals)
+  kWbKFull = 0,    // K and the item's description
+  kWbKEmpty = 1,   // its MMAs are done, every sum warp has left the item (1 + 8 arrivals)
   kWbFull = 4,     // +stage: the unit's operands
   kWbEmpty = 6,    // +stage: MMAs that read it are done
-  kWbSFull = 8,    // +buffer (of key tile i: from kBufs i)
-  kWbSEmpty = 12,  // +buffer (one arrival per warp that reads it)
-  kWbPart = 16,    // +item parity: warpgroup 1's sums (QT = 64, 4 arrivals)
+  kWbSFull = 8,    // +2 tile + buffer
+  kWbSEmpty = 12,  // +2 tile + buffer (one arrival per warp)
 };
 
 struct KwItem {
   int b, kh, k0, len, n, q0, u0, per_head, n_units;  // n_units < 0: no more items; u0: first query tile that sees keys
 };
 
-// Item `idx`: (key tiles, KV head) of the sequences in packing order, the KV heads of the same keys
+// Item `idx`: (`keys` keys, KV head) of the sequences in packing order, the KV heads of the same keys
 // together, early keys (which the most queries see) first.  Called by a whole warp.
-template <int QT, int KEYS>
-__device__ __forceinline__ KwItem kw_item(const KeyWeightsParams& p, int idx, int lane) {
+__device__ __forceinline__ KwItem kw_item(const KeyWeightsParams& p, int idx, int keys, int lane) {
   KwItem it;
   it.n_units = -1;
   int carry = 0;
@@ -131,7 +125,7 @@ __device__ __forceinline__ KwItem kw_item(const KeyWeightsParams& p, int idx, in
     if (b < p.bd.B) {
       s = paged_seq(p.bd, b);
       if (!s.ok) atomicCAS(&g_device_error, 0, kStatusBadSeqPaged);
-      if (s.n > 0) cnt = (s.len + KEYS - 1) / KEYS * p.kv.hkv;
+      if (s.n > 0) cnt = (s.len + keys - 1) / keys * p.kv.hkv;
     }
     int incl = cnt;
 #pragma unroll
@@ -145,19 +139,27 @@ __device__ __forceinline__ KwItem kw_item(const KeyWeightsParams& p, int idx, in
       const int local = idx - carry - (__shfl_sync(0xffffffffu, incl, src) - __shfl_sync(0xffffffffu, cnt, src));
       it.b = base + src;
       it.kh = local % p.kv.hkv;
-      it.k0 = local / p.kv.hkv * KEYS;
+      it.k0 = local / p.kv.hkv * keys;
       it.len = __shfl_sync(0xffffffffu, s.len, src);
       it.n = __shfl_sync(0xffffffffu, s.n, src);
       it.q0 = __shfl_sync(0xffffffffu, s.q0, src);
-      const int n_qt = (it.n + QT - 1) / QT;
-      it.u0 = p.causal ? min(n_qt, max(0, it.k0 - (it.len - it.n)) / QT) : 0;  // earlier tokens see none of these keys
+      const int n_qt = (it.n + kBlockM - 1) / kBlockM;
+      it.u0 = p.causal ? min(n_qt, max(0, it.k0 - (it.len - it.n)) / kBlockM) : 0;  // earlier tokens see none of these keys
       it.per_head = n_qt - it.u0;
-      it.n_units = QT == 128 ? it.per_head * p.G : it.per_head * ((p.G + 1) / 2);
+      it.n_units = it.per_head * p.G;
       return it;
     }
     carry += __shfl_sync(0xffffffffu, incl, 31);
   }
   return it;
+}
+
+// The ones against the LSE's three terms: 128 rows of 16 columns, of which 0-2, 32-byte swizzled.
+__device__ __forceinline__ void kw_write_ones(uint8_t* dst) {
+  for (int e = threadIdx.x; e < 256; e += kKwThreads)
+    *reinterpret_cast<uint4*>(dst + e * 16) =
+        (e & 1) == ((e >> 3) & 1) ? make_uint4(0x3f803f80u, 0x00003f80u, 0, 0) : make_uint4(0, 0, 0, 0);
+  fence_proxy_async_smem();
 }
 
 // Sum over the QT columns of this thread's lane of 2^(sl2 S); MASK: of columns [lo, hi) only.
@@ -187,13 +189,13 @@ __device__ __forceinline__ float kw_sum(uint32_t t_addr, float2 sl2, int lo, int
   return (a[0].x + a[0].y) + (a[1].x + a[1].y);
 }
 
-template <int D, int RP, int QT>
+template <int D, int RP>
 __global__ void __launch_bounds__(kKwThreads, 1)
     fna2_key_weights_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                             const __grid_constant__ CUtensorMap tmRq, const __grid_constant__ CUtensorMap tmRk,
                             const __grid_constant__ CUtensorMap tmL, const KeyWeightsParams p) {
-  using L = KwSmem<D, RP, QT>;
-  constexpr int KS = L::kKStages, NT = L::kTiles, NH = L::kHeads, NB = L::kBufs;
+  using L = KwSmem<D, RP>;
+  constexpr int QT = 128;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::oBar);
@@ -203,25 +205,20 @@ __global__ void __launch_bounds__(kKwThreads, 1)
   const int warp = warp_id(), lane = lane_id(), tid = threadIdx.x;
 
   if (tid == 0) {
+    mbar_init(&bars[kWbKFull], 1);
+    mbar_init(&bars[kWbKEmpty], 9);
     for (int s = 0; s < 2; ++s) {
-      mbar_init(&bars[kWbKFull + s], 1);
-      mbar_init(&bars[kWbKEmpty + s], 9);
       mbar_init(&bars[kWbFull + s], 1);
       mbar_init(&bars[kWbEmpty + s], 1);
-      mbar_init(&bars[kWbPart + s], 4);
     }
     for (int s = 0; s < 4; ++s) {
       mbar_init(&bars[kWbSFull + s], 1);
-      mbar_init(&bars[kWbSEmpty + s], 8 / NT);
+      mbar_init(&bars[kWbSEmpty + s], 4);
     }
     *abort_flag = 0;
     fence_mbar_init();
   }
-  // the ones against the LSE's three terms: columns 0-2 of 16, 32-byte swizzled rows
-  for (int e = tid; e < 256; e += kKwThreads)
-    *reinterpret_cast<uint4*>(smem + L::oOne + e * 16) =
-        (e & 1) == ((e >> 3) & 1) ? make_uint4(0x3f803f80u, 0x00003f80u, 0, 0) : make_uint4(0, 0, 0, 0);
-  fence_proxy_async_smem();
+  kw_write_ones(smem + L::oOne);
   if (warp == 9) {
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
@@ -244,11 +241,11 @@ __global__ void __launch_bounds__(kKwThreads, 1)
     auto draw = [&]() {
       int idx = 0;
       if (lane == 0) idx = atomicAdd(p.next, 1);
-      return kw_item<QT, NT * kBlockN>(p, __shfl_sync(0xffffffffu, idx, 0), lane);
+      return kw_item(p, __shfl_sync(0xffffffffu, idx, 0), 2 * kBlockN, lane);
     };
     auto page_of = [&](const KwItem& it) {
       const int key = it.k0 + lane * bk;
-      return it.n_units >= 0 && lane * bk < NT * kBlockN && key < it.len
+      return it.n_units >= 0 && lane * bk < 2 * kBlockN && key < it.len
                  ? __ldg(p.kv.table + it.b * p.kv.table_sb + (key >> lg))
                  : -1;
     };
@@ -256,25 +253,24 @@ __global__ void __launch_bounds__(kKwThreads, 1)
     int page = page_of(it), next_page = -1;
     int gu = 0, rs = 1;  // units so far, R_k slot
     for (int n = 0;; ++n) {
-      const int ks = n % KS;
-      const bool free = n < KS || mbar_wait(&bars[kWbKEmpty + ks], (n / KS - 1) & 1, abort_flag, 120);
+      const bool free = n < 1 || mbar_wait(&bars[kWbKEmpty], (n - 1) & 1, abort_flag, 120);
       if (!__all_sync(0xffffffffu, free)) break;
       const int key = it.k0 + lane * bk;
-      const bool mine = it.n_units >= 0 && lane * bk < NT * kBlockN && key < it.len;
+      const bool mine = it.n_units >= 0 && lane * bk < 2 * kBlockN && key < it.len;
       const int boxes = __popc(__ballot_sync(0xffffffffu, mine));
       if (lane == 0) {  // (the arrival also publishes the description)
-        volatile KwItem* d = items + ks;
+        volatile KwItem* d = items;
         d->b = it.b, d->kh = it.kh, d->k0 = it.k0, d->len = it.len, d->n = it.n, d->u0 = it.u0;
         d->per_head = it.per_head, d->n_units = it.n_units;
-        mbar_expect_tx(&bars[kWbKFull + ks], boxes * bk * D * 2);
+        mbar_expect_tx(&bars[kWbKFull], boxes * bk * D * 2);
       }
       __syncwarp();
       if (it.n_units < 0) break;
       if (mine) {
 #pragma unroll
         for (int c = 0; c < D / 64; ++c)
-          tma_load_4d(smem + L::oK + (NT * ks + tile) * L::kTile + c * L::kChunk + row * 128, &tmK,
-                      &bars[kWbKFull + ks], c * 64, key & mask, it.kh, page);
+          tma_load_4d(smem + L::oK + tile * L::kTile + c * L::kChunk + row * 128, &tmK,
+                      &bars[kWbKFull], c * 64, key & mask, it.kh, page);
       }
       __syncwarp();
       auto fetch = [&]() {
@@ -285,35 +281,30 @@ __global__ void __launch_bounds__(kKwThreads, 1)
       bool ok = true;
       for (int u = 0; u < it.n_units; ++u, ++gu) {
         const int s = gu & 1;
-        const int h0 = it.kh * p.G + (QT == 128 ? u / it.per_head : 2 * u), nh = min(NH, (it.kh + 1) * p.G - h0);
-        const int tok = it.q0 + (QT == 128 ? (it.u0 + u % it.per_head) * QT : 0);
-        const int ng = max(0, min(nh, p.kv.hg - h0));  // heads of the unit that carry the bias
+        const int h = it.kh * p.G + u / it.per_head, tok = it.q0 + (it.u0 + u % it.per_head) * QT;
+        const bool graph = h < p.kv.hg;
         uint8_t* st = smem + L::oStage + s * L::kStage;
         // R_k: unless this unit's head is the last one's.  The slot's former readers are done: the unit before
         // the last one is, and at least one unit has used the other slot since.
-        const bool fresh = QT == 64 || u % it.per_head == 0;
+        const bool fresh = u % it.per_head == 0;
         if (fresh) rs ^= 1;
         const bool room = gu < 2 || mbar_wait(&bars[kWbEmpty + s], ((gu >> 1) - 1) & 1, abort_flag, 121);
         ok = __all_sync(0xffffffffu, room);
         if (!ok) break;
         if (lane == 0)
-          mbar_expect_tx(&bars[kWbFull + s], QT * (nh * (D + 16) + ng * 2 * RP) * 2 + (fresh ? ng * boxes * bk * RP * 2 : 0));
+          mbar_expect_tx(&bars[kWbFull + s],
+                         QT * (D + 16 + (graph ? 2 * RP : 0)) * 2 + (fresh && graph ? boxes * bk * RP * 2 : 0));
         __syncwarp();
-        // lanes 16 + (0 .. 2 D/64): Q chunks; lanes 24 + (0 .. 4): R~_q hi, lo; lanes 28 + (0, 1): LSE; a head each
-        // in turn
-        const int x = lane - 16, y = lane - 24, z = lane - 28, g_q = x / (D / 64), g_r = y / 2;
-        const bool is_q = x >= 0 && x < 8 && g_q < nh, is_r = y >= 0 && y < 4 && g_r < ng, is_l = z >= 0 && z < nh;
-        if (is_q || is_r || is_l) {
-          uint8_t* dst = st + (is_q   ? L::sQ + x % (D / 64) * L::kChunk + g_q * QT * 128
-                               : is_r ? L::sRq + y % 2 * L::kRTile + g_r * QT * RP * 2
-                                      : L::sL + z * QT * 32);
-          tma_load_4d(dst, is_q ? &tmQ : is_r ? &tmRq : &tmL, &bars[kWbFull + s],
-                      is_q ? x % (D / 64) * 64 : is_r ? y % 2 * RP : 2 * RP, tok, h0 + (is_q ? g_q : is_r ? g_r : z), 0);
-        }
-        if (mine && fresh)
-          for (int g = 0; g < ng; ++g)
-            tma_load_4d(smem + L::oRk + (2 * rs + g * NT + tile) * L::kRTile + row * RP * 2, &tmRk, &bars[kWbFull + s], 0,
-                        key & mask, h0 + g, page);
+        // lanes 16, 17: Q chunks; 24, 25: R~_q hi, lo; 28: LSE
+        const int x = lane - 16, y = lane - 24;
+        const bool is_q = x >= 0 && x < D / 64, is_r = graph && y >= 0 && y < 2;
+        if (is_q || is_r || lane == 28)
+          tma_load_4d(st + (is_q ? L::sQ + x * L::kChunk : is_r ? L::sRq + y * L::kRTile : L::sL),
+                      is_q ? &tmQ : is_r ? &tmRq : &tmL, &bars[kWbFull + s], is_q ? x * 64 : is_r ? y * RP : 2 * RP, tok, h,
+                      0);
+        if (mine && fresh && graph)
+          tma_load_4d(smem + L::oRk + (2 * rs + tile) * L::kRTile + row * RP * 2, &tmRk, &bars[kWbFull + s], 0, key & mask,
+                      h, page);
         __syncwarp();
         if (u == max(0, it.n_units - 2)) fetch();  // not earlier: who draws early gets work before it is free
       }
@@ -322,32 +313,31 @@ __global__ void __launch_bounds__(kKwThreads, 1)
     }
   } else if (warp >= 9) {
     // ------------------------------------------------------------ MMA issuer (9) and its waiter (10)
-    constexpr uint32_t idesc = make_idesc_bf16(kBlockN, 128, 0, 0), idesc_r = make_idesc_bf16(kBlockN, QT, 0, 0);
+    constexpr uint32_t idesc = make_idesc_bf16(kBlockN, 128, 0, 0);
     constexpr uint32_t r_layout = RP == 16 ? kSwizzle32B : kSwizzle64B;
     constexpr uint32_t r_sbo = 8 * RP * 2;
     const bool issuer = warp == 9;
-    int gu = 0, rs = 1, used[NT] = {};
+    int gu = 0, rs = 1, used[2] = {};
     bool ok = true;
     for (int n = 0; ok; ++n) {
-      const int ks = n % KS;
-      ok = issuer || mbar_wait(&bars[kWbKFull + ks], (n / KS) & 1, abort_flag, 221);
+      ok = issuer || mbar_wait(&bars[kWbKFull], n & 1, abort_flag, 221);
       ok = pair_rendezvous(1, ok);
       if (!ok) break;
-      const int n_units = items[ks].n_units, per_head = items[ks].per_head, kh = items[ks].kh;
-      const int tiles = items[ks].k0 + kBlockN < items[ks].len ? NT : 1;
+      const int n_units = items[0].n_units, per_head = items[0].per_head, kh = items[0].kh;
+      const int tiles = items[0].k0 + kBlockN < items[0].len ? 2 : 1;
       if (n_units < 0) break;
       for (int u = 0; ok && u < n_units; ++u, ++gu) {
         const int s = gu & 1;
-        const int h0 = kh * p.G + (QT == 128 ? u / per_head : 2 * u), nh = min(NH, (kh + 1) * p.G - h0);
+        const bool graph = kh * p.G + u / per_head < p.kv.hg;
         const uint32_t st = smem_u32(smem + L::oStage + s * L::kStage);
-        if (QT == 64 || u % per_head == 0) rs ^= 1;
+        if (u % per_head == 0) rs ^= 1;
         if (!issuer) ok = mbar_wait(&bars[kWbFull + s], (gu >> 1) & 1, abort_flag, 222);
 #pragma unroll
-        for (int i = 0; i < NT; ++i) {
+        for (int i = 0; i < 2; ++i) {
           if (i >= tiles) continue;
-          const int buf = NB * i + used[i] % NB;
-          if (!issuer && ok && used[i] >= NB)
-            ok = mbar_wait(&bars[kWbSEmpty + buf], (used[i] / NB - 1) & 1, abort_flag, 223);
+          const int buf = 2 * i + used[i] % 2;
+          if (!issuer && ok && used[i] >= 2)
+            ok = mbar_wait(&bars[kWbSEmpty + buf], (used[i] / 2 - 1) & 1, abort_flag, 223);
           ++used[i];
           ok = pair_rendezvous(1, ok);
           if (!ok) break;
@@ -355,7 +345,7 @@ __global__ void __launch_bounds__(kKwThreads, 1)
           tc_fence_after();
           if (elect_one()) {
             const uint32_t tS = tmem + 128 * buf;
-            const uint32_t sK = smem_u32(smem + L::oK + (NT * ks + i) * L::kTile);
+            const uint32_t sK = smem_u32(smem + L::oK + i * L::kTile);
 #pragma unroll
             for (int kk = 0; kk < D / 16; ++kk) {
               const uint32_t off = (kk >> 2) * L::kChunk + (kk & 3) * 32;
@@ -364,16 +354,13 @@ __global__ void __launch_bounds__(kKwThreads, 1)
             }
             mma_ss(tS, make_sdesc(smem_u32(smem + L::oOne), 16, 256, kSwizzle32B),
                    make_sdesc(st + L::sL, 16, 256, kSwizzle32B), idesc, 1);
-#pragma unroll
-            for (int g = 0; g < NH; ++g) {
-              if (g >= nh || h0 + g >= p.kv.hg) continue;
-              const uint32_t sRk = smem_u32(smem + L::oRk + (2 * rs + g * NT + i) * L::kRTile);
+            if (graph) {
+              const uint32_t sRk = smem_u32(smem + L::oRk + (2 * rs + i) * L::kRTile);
 #pragma unroll
               for (int kk = 0; kk < RP / 16; ++kk) {
-                const uint32_t hi = st + L::sRq + g * QT * RP * 2 + kk * 32;
                 const uint64_t rk = make_sdesc(sRk + kk * 32, 16, r_sbo, r_layout);
-                mma_ss(tS + g * QT, rk, make_sdesc(hi, 16, r_sbo, r_layout), idesc_r, 1);
-                mma_ss(tS + g * QT, rk, make_sdesc(hi + L::kRTile, 16, r_sbo, r_layout), idesc_r, 1);
+                mma_ss(tS, rk, make_sdesc(st + L::sRq + kk * 32, 16, r_sbo, r_layout), idesc, 1);
+                mma_ss(tS, rk, make_sdesc(st + L::sRq + L::kRTile + kk * 32, 16, r_sbo, r_layout), idesc, 1);
               }
             }
             mma_commit(&bars[kWbSFull + buf]);
@@ -382,59 +369,322 @@ __global__ void __launch_bounds__(kKwThreads, 1)
           __syncwarp();
         }
       }
-      if (ok && issuer && elect_one()) mma_commit(&bars[kWbKEmpty + ks]);
+      if (ok && issuer && elect_one()) mma_commit(&bars[kWbKEmpty]);
       __syncwarp();
     }
   } else {
     // ------------------------------------------------------------ sums
-    const int wi = warp >> 2, ti = NT == 2 ? wi : 0, gi = NT == 2 ? 0 : wi;  // key tile, head of the unit
-    const uint32_t t_lane = tmem + 128 * NB * ti + gi * QT + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+    const int wi = warp >> 2;
+    const uint32_t t_lane = tmem + 256 * wi + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     const float2 sl2 = make_float2(p.scale_log2, p.scale_log2);
     int used = 0;
     bool ok = true;
     for (int n = 0; ok; ++n) {
-      const int ks = n % KS;
-      if (!mbar_wait(&bars[kWbKFull + ks], (n / KS) & 1, abort_flag, 320)) break;
-      const int n_units = items[ks].n_units, per_head = items[ks].per_head, u0 = items[ks].u0, nq = items[ks].n;
-      const int len = items[ks].len, tile0 = items[ks].k0 + ti * kBlockN, j = tile0 + (tid & 127), past = len - nq;
+      if (!mbar_wait(&bars[kWbKFull], n & 1, abort_flag, 320)) break;
+      const int n_units = items[0].n_units, per_head = items[0].per_head, u0 = items[0].u0, nq = items[0].n;
+      const int len = items[0].len, tile0 = items[0].k0 + wi * kBlockN, j = tile0 + (tid & 127), past = len - nq;
       if (n_units < 0) break;
       const bool mine = tile0 < len;  // this key tile has keys
-      float* dst = p.kw + items[ks].b * p.kw_sb + items[ks].kh * p.kw_sh + j;
-      float w = gi == 0 && mine && j < len ? *dst : 0.f;
+      float* dst = p.kw + items[0].b * p.kw_sb + items[0].kh * p.kw_sh + j;
+      float w = mine && j < len ? *dst : 0.f;
       for (int u = 0; u < n_units; ++u) {
-        const int buf = NB * ti + used % NB;
+        const int buf = 2 * wi + used % 2;
         if (!mine) continue;
-        if (!mbar_wait(&bars[kWbSFull + buf], (used / NB) & 1, abort_flag, 322)) {
+        if (!mbar_wait(&bars[kWbSFull + buf], (used / 2) & 1, abort_flag, 322)) {
           ok = false;
           break;
         }
         tc_fence_after();
-        const int i0 = QT == 128 ? (u0 + u % per_head) * QT : 0;
+        const int i0 = (u0 + u % per_head) * QT;
         // columns [first, nq - i0) belong to queries that see the key; the score of another sequence's
-        // query or of a head that the unit lacks is never read into a sum
+        // query is never read into a sum
         const int first = p.causal ? j - past - i0 : 0;
         const bool whole = (!p.causal || tile0 + kBlockN - 1 <= past + i0) && i0 + QT <= nq;
-        const uint32_t at = t_lane + 128 * (used % NB);
-        if (NH == 1 || 2 * u + gi < p.G)
-          w += whole ? kw_sum<QT, false>(at, sl2, 0, 0) : kw_sum<QT, true>(at, sl2, first, nq - i0);
+        const uint32_t at = t_lane + 128 * (used % 2);
+        w += whole ? kw_sum<QT, false>(at, sl2, 0, 0) : kw_sum<QT, true>(at, sl2, first, nq - i0);
         ++used;
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars[kWbSEmpty + buf]);
       }
-      if (NT == 1) {  // add the two heads' halves (a slot is written again only after everyone left its item)
-        float* part = reinterpret_cast<float*>(smem + L::oPart) + (n & 1) * 128 + (tid & 127);
-        if (wi == 1) {
-          *part = w;
+      if (ok && mine && j < len) *dst = w;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars[kWbKEmpty]);
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// query-stationary form: at most 64 queries per sequence
+// ---------------------------------------------------------------------------
+template <int D, int RP>
+struct KwwSmem {
+  static constexpr int kPairs = D == 128 && RP == 32 ? 1 : 2;  // head pairs whose queries stay
+  static constexpr int kHeads = 2 * kPairs;
+  static constexpr int kTile = 128 * D * 2;                    // K tile, Q of a head pair
+  static constexpr int kRTile = 128 * RP * 2;                  // R_k of a head, R~_q hi or lo of a head pair
+  static constexpr int kChunk = 128 * 128;
+  static constexpr int kLTile = 128 * 32;
+  static constexpr int sRq = kTile, sL = sRq + 2 * kRTile, kPair = sL + kLTile;  // [Q | R~_q hi, lo | LSE] of a pair
+  static constexpr int oQ = 0;
+  static constexpr int oK = oQ + kPairs * kPair;               // 2 x [K | R_k of each head]
+  static constexpr int kStage = kTile + kHeads * kRTile;
+  static constexpr int oOne = oK + 2 * kStage;
+  static constexpr int oPart = oOne + kLTile;                  // 2 x warpgroup 1's sums
+  static constexpr int oBar = oPart + 2 * 512;
+  static constexpr int oMisc = oBar + 32 * 8;
+  static constexpr int oItem = oMisc + 16;
+  static constexpr int kUsed = oItem + 64;
+  static constexpr int kTotal = kUsed + 1024;
+  static_assert(kTotal <= kMaxDynamicSmem, "shared memory budget");
+  static_assert(kPair % 1024 == 0 && kStage % 1024 == 0, "swizzle atoms stay aligned");
+};
+
+enum KwwBar {
+  kVbQFull = 0,    // the queries and the step's description
+  kVbQEmpty = 1,   // the step's MMAs are done, every sum warp has read its description (1 + 8 arrivals)
+  kVbFull = 2,     // +stage: K and R_k of a key tile
+  kVbEmpty = 4,    // +stage
+  kVbSFull = 6,    // +buffer
+  kVbSEmpty = 10,  // +buffer (8 arrivals)
+  kVbPFull = 14,   // +tile parity: warpgroup 1's sums (4 arrivals)
+  kVbPEmpty = 16,  // +tile parity (4 arrivals)
+};
+
+// A step: `tiles` key tiles from key k0 on against heads [h0, h0 + heads) of one KV head.
+struct KwwStep {
+  int b, kh, k0, len, n, tiles, h0, heads;  // tiles < 0: no more steps
+};
+
+template <int D, int RP>
+__global__ void __launch_bounds__(kKwThreads, 1)
+    fna2_key_weights_window_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                                   const __grid_constant__ CUtensorMap tmRq, const __grid_constant__ CUtensorMap tmRk,
+                                   const __grid_constant__ CUtensorMap tmL, const KeyWeightsParams p) {
+  using L = KwwSmem<D, RP>;
+  constexpr int QT = 64, NB = 4;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::oBar);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::oMisc);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::oMisc + 4);
+  volatile KwwStep* step = reinterpret_cast<volatile KwwStep*>(smem + L::oItem);
+  const int warp = warp_id(), lane = lane_id(), tid = threadIdx.x;
+
+  if (tid == 0) {
+    mbar_init(&bars[kVbQFull], 1);
+    mbar_init(&bars[kVbQEmpty], 9);
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&bars[kVbFull + s], 1);
+      mbar_init(&bars[kVbEmpty + s], 1);
+      mbar_init(&bars[kVbPFull + s], 4);
+      mbar_init(&bars[kVbPEmpty + s], 4);
+    }
+    for (int s = 0; s < NB; ++s) {
+      mbar_init(&bars[kVbSFull + s], 1);
+      mbar_init(&bars[kVbSEmpty + s], 8);
+    }
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  kw_write_ones(smem + L::oOne);
+  if (warp == 9) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp == 8) {
+    // ------------------------------------------------------------ producer
+    if (lane == 0) {
+      tma_prefetch_desc(&tmQ);
+      tma_prefetch_desc(&tmK);
+    }
+    const int lg = p.kv.page_log2, mask = (1 << lg) - 1;
+    const int bk = min(1 << lg, kBlockN), row = lane * bk;  // lane l owns box l of a key tile (at most 8)
+    auto draw = [&]() {
+      int idx = 0;
+      if (lane == 0) idx = atomicAdd(p.next, 1);
+      return kw_item(p, __shfl_sync(0xffffffffu, idx, 0), p.run_tiles * kBlockN, lane);
+    };
+    KwItem it = draw(), next = it;
+    int gt = 0;  // key tiles so far
+    bool ok = true;
+    for (int n = 0; ok; ++n) {
+      const bool last = it.n_units < 0;
+      const int tiles = last ? -1 : min(p.run_tiles, (it.len - it.k0 + kBlockN - 1) / kBlockN);
+      for (int g0 = 0; ok && g0 < p.G; g0 += L::kHeads) {
+        const int h0 = it.kh * p.G + g0, nh = min(L::kHeads, p.G - g0), ng = max(0, min(nh, p.kv.hg - h0));
+        const bool free = n == 0 || mbar_wait(&bars[kVbQEmpty], (n - 1) & 1, abort_flag, 125);
+        if (!(ok = __all_sync(0xffffffffu, free))) break;
+        if (lane == 0) {  // (the arrival also publishes the description)
+          step->b = it.b, step->kh = it.kh, step->k0 = it.k0, step->len = it.len, step->n = it.n, step->tiles = tiles;
+          step->h0 = h0, step->heads = nh;
+          mbar_expect_tx(&bars[kVbQFull], last ? 0 : QT * (nh * (D + 16) + ng * 2 * RP) * 2);
+        }
+        __syncwarp();
+        if (last) break;
+        // lane 8 g + x of head g: x = 0, 1: Q chunks; 2, 3: R~_q hi, lo; 4: LSE
+        const int g = lane / 8, x = lane % 8;
+        if (g < nh && (x < D / 64 || x == 4 || (x / 2 == 1 && g < ng))) {
+          uint8_t* dst = smem + L::oQ + g / 2 * L::kPair +
+                         (x < D / 64 ? x * L::kChunk + g % 2 * QT * 128
+                          : x == 4   ? L::sL + g % 2 * QT * 32
+                                     : L::sRq + (x - 2) * L::kRTile + g % 2 * QT * RP * 2);
+          tma_load_4d(dst, x < D / 64 ? &tmQ : x == 4 ? &tmL : &tmRq, &bars[kVbQFull],
+                      x < D / 64 ? x * 64 : x == 4 ? 2 * RP : (x - 2) * RP, it.q0, h0 + g, 0);
+        }
+        __syncwarp();
+        for (int t = 0; t < tiles; ++t, ++gt) {
+          const int s = gt & 1, key = it.k0 + t * kBlockN + row;
+          const bool mine = row < kBlockN && key < it.len;
+          const int page = mine ? __ldg(p.kv.table + it.b * p.kv.table_sb + (key >> lg)) : 0;
+          const bool room = gt < 2 || mbar_wait(&bars[kVbEmpty + s], ((gt >> 1) - 1) & 1, abort_flag, 126);
+          if (!(ok = __all_sync(0xffffffffu, room))) break;
+          const int boxes = __popc(__ballot_sync(0xffffffffu, mine));
+          if (lane == 0) mbar_expect_tx(&bars[kVbFull + s], boxes * bk * (D + ng * RP) * 2);
           __syncwarp();
-          if (lane == 0) mbar_arrive(&bars[kWbPart + (n & 1)]);
-        } else if (ok && (ok = mbar_wait(&bars[kWbPart + (n & 1)], (n >> 1) & 1, abort_flag, 323))) {
-          w += *part;
+          uint8_t* st = smem + L::oK + s * L::kStage;
+          if (mine) {
+#pragma unroll
+            for (int c = 0; c < D / 64; ++c)
+              tma_load_4d(st + c * L::kChunk + row * 128, &tmK, &bars[kVbFull + s], c * 64, key & mask, it.kh, page);
+            for (int hh = 0; hh < ng; ++hh)
+              tma_load_4d(st + L::kTile + hh * L::kRTile + row * RP * 2, &tmRk, &bars[kVbFull + s], 0, key & mask, h0 + hh,
+                          page);
+          }
+          __syncwarp();
+          // not earlier: who draws early gets work before it is free
+          if (g0 + L::kHeads >= p.G && t == max(0, tiles - 2)) next = draw();
+        }
+        if (g0 + L::kHeads < p.G) ++n;
+      }
+      if (last) break;
+      it = next;
+    }
+  } else if (warp >= 9) {
+    // ------------------------------------------------------------ MMA issuer (9) and its waiter (10)
+    constexpr uint32_t idesc = make_idesc_bf16(kBlockN, 128, 0, 0), idesc_r = make_idesc_bf16(kBlockN, QT, 0, 0);
+    constexpr uint32_t r_layout = RP == 16 ? kSwizzle32B : kSwizzle64B;
+    constexpr uint32_t r_sbo = 8 * RP * 2;
+    const bool issuer = warp == 9;
+    int gt = 0, used = 0;
+    bool ok = true;
+    for (int n = 0; ok; ++n) {
+      ok = issuer || mbar_wait(&bars[kVbQFull], n & 1, abort_flag, 225);
+      ok = pair_rendezvous(1, ok);
+      if (!ok) break;
+      const int tiles = step->tiles, h0 = step->h0, heads = step->heads;
+      if (tiles < 0) break;
+      for (int t = 0; ok && t < tiles; ++t, ++gt) {
+        const int s = gt & 1;
+        const uint32_t sK = smem_u32(smem + L::oK + s * L::kStage);
+        if (!issuer) ok = mbar_wait(&bars[kVbFull + s], (gt >> 1) & 1, abort_flag, 226);
+#pragma unroll
+        for (int u = 0; u < L::kPairs; ++u) {
+          if (2 * u >= heads) continue;
+          const int buf = used % NB;
+          if (!issuer && ok && used >= NB) ok = mbar_wait(&bars[kVbSEmpty + buf], (used / NB - 1) & 1, abort_flag, 227);
+          ++used;
+          ok = pair_rendezvous(1, ok);
+          if (!ok) break;
+          if (!issuer) continue;
+          tc_fence_after();
+          if (elect_one()) {
+            const uint32_t tS = tmem + 128 * buf;
+            const uint32_t sQ = smem_u32(smem + L::oQ + u * L::kPair);
+#pragma unroll
+            for (int kk = 0; kk < D / 16; ++kk) {
+              const uint32_t off = (kk >> 2) * L::kChunk + (kk & 3) * 32;
+              mma_ss(tS, make_sdesc(sK + off, 16, 1024, kSwizzle128B), make_sdesc(sQ + off, 16, 1024, kSwizzle128B), idesc,
+                     kk > 0);
+            }
+            mma_ss(tS, make_sdesc(smem_u32(smem + L::oOne), 16, 256, kSwizzle32B),
+                   make_sdesc(sQ + L::sL, 16, 256, kSwizzle32B), idesc, 1);
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+              if (2 * u + g >= heads || h0 + 2 * u + g >= p.kv.hg) continue;
+              const uint32_t sRk = sK + L::kTile + (2 * u + g) * L::kRTile;
+#pragma unroll
+              for (int kk = 0; kk < RP / 16; ++kk) {
+                const uint32_t hi = sQ + L::sRq + g * QT * RP * 2 + kk * 32;
+                const uint64_t rk = make_sdesc(sRk + kk * 32, 16, r_sbo, r_layout);
+                mma_ss(tS + g * QT, rk, make_sdesc(hi, 16, r_sbo, r_layout), idesc_r, 1);
+                mma_ss(tS + g * QT, rk, make_sdesc(hi + L::kRTile, 16, r_sbo, r_layout), idesc_r, 1);
+              }
+            }
+            mma_commit(&bars[kVbSFull + buf]);
+            if (2 * u + 2 >= heads) mma_commit(&bars[kVbEmpty + s]);
+          }
+          __syncwarp();
         }
       }
-      if (ok && gi == 0 && mine && j < len) *dst = w;
+      if (ok && issuer && elect_one()) mma_commit(&bars[kVbQEmpty]);
       __syncwarp();
-      if (lane == 0) mbar_arrive(&bars[kWbKEmpty + ks]);
+    }
+  } else {
+    // ------------------------------------------------------------ sums (warpgroup i: head i of each pair)
+    const int wi = warp >> 2;
+    const uint32_t t_lane = tmem + QT * wi + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+    const float2 sl2 = make_float2(p.scale_log2, p.scale_log2);
+    int used = 0, gt = 0;
+    bool ok = true;
+    for (int n = 0; ok; ++n) {
+      if (!mbar_wait(&bars[kVbQFull], n & 1, abort_flag, 325)) break;
+      const int tiles = step->tiles, heads = step->heads, nq = step->n, len = step->len, k0 = step->k0;
+      float* dst = p.kw + step->b * p.kw_sb + step->kh * p.kw_sh + k0 + (tid & 127);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars[kVbQEmpty]);
+      if (tiles < 0) break;
+      const int past = len - nq;
+      for (int t = 0; ok && t < tiles; ++t, ++gt) {
+        const int tile0 = k0 + t * kBlockN, j = tile0 + (tid & 127);
+        const bool store = wi == 0 && j < len;
+        const float before = store ? dst[t * kBlockN] : 0.f;
+        float w = 0.f;
+        for (int u = 0; 2 * u < heads; ++u) {
+          const int buf = used % NB;
+          if (!mbar_wait(&bars[kVbSFull + buf], (used / NB) & 1, abort_flag, 326)) {
+            ok = false;
+            break;
+          }
+          ++used;
+          tc_fence_after();
+          // columns [first, nq) belong to queries that see the key; the score of another sequence's query
+          // or of a head that the pair lacks is never read into a sum
+          const bool whole = (!p.causal || tile0 + kBlockN - 1 <= past) && nq == QT;
+          if (2 * u + wi < heads)
+            w += whole ? kw_sum<QT, false>(t_lane + 128 * buf, sl2, 0, 0)
+                       : kw_sum<QT, true>(t_lane + 128 * buf, sl2, p.causal ? j - past : 0, nq);
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bars[kVbSEmpty + buf]);
+        }
+        if (!ok) break;
+        float* part = reinterpret_cast<float*>(smem + L::oPart) + (gt & 1) * 128 + (tid & 127);
+        if (wi == 1) {
+          if (gt >= 2 && !(ok = mbar_wait(&bars[kVbPEmpty + (gt & 1)], ((gt >> 1) - 1) & 1, abort_flag, 327))) break;
+          *part = w;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bars[kVbPFull + (gt & 1)]);
+        } else {
+          if (!(ok = mbar_wait(&bars[kVbPFull + (gt & 1)], (gt >> 1) & 1, abort_flag, 328))) break;
+          w += *part;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bars[kVbPEmpty + (gt & 1)]);
+          if (store) dst[t * kBlockN] = before + w;
+        }
+      }
     }
   }
 
@@ -450,33 +700,31 @@ struct KwMaps {
   CUtensorMap q, k, rq, rk, l;
 };
 
-// Queries per unit.
+// Queries per unit: which of the two kernels runs.
 inline int kw_query_tile(const KeyWeightsParams& p) { return p.bd.max_q <= 64 ? 64 : 128; }
 
-template <int D, int RP, int QT>
-cudaError_t launch_key_weights_t(const KwMaps& m, const KeyWeightsParams& p, cudaStream_t stream) {
-  using L = KwSmem<D, RP, QT>;
-  auto kern = fna2_key_weights_kernel<D, RP, QT>;
-  static std::atomic<uint64_t> allowed{0};
-  cudaError_t e = allow_smem(reinterpret_cast<const void*>(kern), allowed);
+template <int D, int RP>
+cudaError_t launch_key_weights_t(const KwMaps& m, KeyWeightsParams& p, cudaStream_t stream) {
+  const bool window = kw_query_tile(p) == 64;
+  auto kern = window ? fna2_key_weights_window_kernel<D, RP> : fna2_key_weights_kernel<D, RP>;
+  static std::atomic<uint64_t> allowed[2];
+  cudaError_t e = allow_smem(reinterpret_cast<const void*>(kern), allowed[window]);
   if (e != cudaSuccess) return e;
   const int64_t n = static_cast<int64_t>(p.bd.T) * p.H * (p.RP / 8 + 1);
   fna2_key_weights_prep_kernel<<<static_cast<unsigned>((n + 255) / 256), 256, 0, stream>>>(p);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
-  const int64_t items = static_cast<int64_t>(p.bd.B) * p.kv.hkv * ((p.bd.max_k + L::kTiles * kBlockN - 1) / (L::kTiles * kBlockN));
-  kern<<<static_cast<unsigned>(std::min<int64_t>(items, kSms)), kKwThreads, L::kTotal, stream>>>(m.q, m.k, m.rq, m.rk, m.l, p);
+  const int64_t tiles = (p.bd.max_k + kBlockN - 1) / kBlockN, seqs = static_cast<int64_t>(p.bd.B) * p.kv.hkv;
+  // key tiles per item: a pair, or runs (about three per CTA when all sequences are the longest)
+  p.run_tiles = window ? static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(16, seqs * tiles / (3 * kSms)))) : 2;
+  const int64_t items = seqs * ((tiles + p.run_tiles - 1) / p.run_tiles);
+  kern<<<static_cast<unsigned>(std::min<int64_t>(items, kSms)), kKwThreads,
+         window ? KwwSmem<D, RP>::kTotal : KwSmem<D, RP>::kTotal, stream>>>(m.q, m.k, m.rq, m.rk, m.l, p);
   return cudaGetLastError();
 }
 
-template <int D, int RP>
-cudaError_t launch_key_weights_r(const KwMaps& m, const KeyWeightsParams& p, cudaStream_t stream) {
-  return kw_query_tile(p) == 64 ? launch_key_weights_t<D, RP, 64>(m, p, stream)
-                                : launch_key_weights_t<D, RP, 128>(m, p, stream);
-}
-
-inline cudaError_t launch_key_weights(const KwMaps& m, const KeyWeightsParams& p, int D, cudaStream_t stream) {
-  if (D == 64) return p.RP == 16 ? launch_key_weights_r<64, 16>(m, p, stream) : launch_key_weights_r<64, 32>(m, p, stream);
-  return p.RP == 16 ? launch_key_weights_r<128, 16>(m, p, stream) : launch_key_weights_r<128, 32>(m, p, stream);
+inline cudaError_t launch_key_weights(const KwMaps& m, KeyWeightsParams& p, int D, cudaStream_t stream) {
+  if (D == 64) return p.RP == 16 ? launch_key_weights_t<64, 16>(m, p, stream) : launch_key_weights_t<64, 32>(m, p, stream);
+  return p.RP == 16 ? launch_key_weights_t<128, 16>(m, p, stream) : launch_key_weights_t<128, 32>(m, p, stream);
 }
 
 }  // namespace fna2
