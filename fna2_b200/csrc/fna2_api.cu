@@ -798,11 +798,11 @@ int paged_plan(const Fna2PagedKV* kv, const Fna2PagedAttnArgs* a, PagedAttnParam
   for (;; l->RW /= 2) {
     p->ng_max = std::min({p->G, 16 * l->RW, p->kv.hg});
     p->nh_max = std::min({p->G, 16, p->kv.hg});
-    // ring depth: about 64 KB of tiles per CTA, at most 8 and at least 2 of them
+    // ring depth: about 64 KB of tiles per CTA, at most 4 and at least 2 of them
     const FewSmem one(D, l->RW, p->ng_max, p->nh_max, p->RP, 1, p->few_rows);
-    p->stages = std::max(2, std::min(8, 72 * 1024 / ((one.kv_stage + one.r_stage) * (4 / l->RW))));
+    p->stages = std::max(2, std::min(4, 72 * 1024 / ((one.kv_stage + one.r_stage) * (4 / l->RW))));
     l->smem = FewSmem(D, l->RW, p->ng_max, p->nh_max, p->RP, p->stages, p->few_rows).total;
-    if ((l->smem <= kMaxDynamicSmem && 2 * D / 64 + p->ng_max <= 32) || l->RW == 1) break;  // a lane per box
+    if (l->smem <= kMaxDynamicSmem || l->RW == 1) break;
   }
   FNA2_CHECK(l->smem <= kMaxDynamicSmem, "heads per KV head and rank need too much shared memory");
   p->block_rows = 16 * l->RW;
@@ -861,15 +861,6 @@ int map_pages(CUtensorMap* m, const PagedRows& r, int cols, int heads, const Pag
   const int page = 1 << kv.page_log2;
   return make_map(m, r.ptr, cols, page, heads, kv.pages, r.st, r.sh, r.sp, box_cols,
                   std::min<uint32_t>(page, max_rows), swz, what);
-}
-
-int few_maps(const PagedAttnParams& p, int D, FewMaps* m) {
-  if (int rc = map_pages(&m->k, p.kv.k, D, p.kv.hkv, p.kv, 64, kFewKeys, CU_TENSOR_MAP_SWIZZLE_128B, "k pages")) return rc;
-  if (int rc = map_pages(&m->v, p.kv.v, D, p.kv.hkv, p.kv, 64, kFewKeys, CU_TENSOR_MAP_SWIZZLE_128B, "v pages")) return rc;
-  m->rk = m->k;  // never dereferenced without graph heads
-  if (p.kv.hg == 0) return FNA2_OK;
-  return map_pages(&m->rk, p.kv.rk, p.kv.rank, p.kv.hg, p.kv, p.RP, kFewKeys,
-                   p.RP == 16 ? CU_TENSOR_MAP_SWIZZLE_32B : CU_TENSOR_MAP_SWIZZLE_64B, "rk pages");
 }
 
 int many_maps(const PagedAttnParams& p, int D, ManyMaps* m) {
@@ -967,6 +958,7 @@ extern "C" int fna2_paged_attn(const Fna2PagedKV* kv, const Fna2PagedAttnArgs* a
   PagedAttnParams p{};
   PagedPlan l;
   if (int rc = paged_queries(kv, a, &p)) return rc;
+  p.inv_scale = 1.f / p.scale;
   if (int rc = paged_plan(kv, a, &p, &l)) return rc;
   if (p.bd.B == 0 || p.bd.T == 0) return FNA2_OK;
   FNA2_CHECK(a->out != nullptr && aligned16(a->out) && strides_ok({a->out_token_stride, a->out_head_stride}),
@@ -993,11 +985,7 @@ extern "C" int fna2_paged_attn(const Fna2PagedKV* kv, const Fna2PagedAttnArgs* a
     if (int rc = many_maps(p, kv->head_dim, &m)) return rc;
     FNA2_CUDA(launch_paged_many(m, p, kv->head_dim, st));
   }
-  if (l.few) {
-    FewMaps m;
-    if (int rc = few_maps(p, kv->head_dim, &m)) return rc;
-    FNA2_CUDA(launch_paged_few(m, p, kv->head_dim, l.RW, l.smem, st));
-  }
+  if (l.few) FNA2_CUDA(launch_paged_few(p, kv->head_dim, l.RW, l.smem, st));
   if (l.many_join) FNA2_CUDA(launch_paged_many_join(p, kv->head_dim, st));
   if (l.few_join) FNA2_CUDA(launch_paged_few_join(p, kv->head_dim, st));
   if (l.logits && p.bd.max_k > 0) FNA2_CUDA(launch_logit_weights(p, st));

@@ -25,14 +25,14 @@
 // cut.  A query row is (query head of the KV group, new token), head-major,
 // so that the 16 rows of a warp span few heads.  4 warps: RW row blocks x 4/RW key
 // groups; a key group streams its own 16-key tiles through a ring in shared memory
-// that its RW warps read together (mma.sync m16n8k16, fp32 accumulation, online
-// softmax in registers).  16 keys never cross a page, so a tile is one TMA box per
-// 64 columns of K and V and one per head of R_k, issued by as many lanes; 128-byte
-// (R_k: 32- or 64-byte) swizzled rows give conflict-free ldmatrix reads.
-// Bound: HBM; each cached key is read once per row block.  A warp takes about 1600
-// clk per tile, latency rather than issue (313 instructions), so an SM needs its 8
-// warps; about 140 KB of loads in flight per SM suffice (deeper rings measured the
-// same or slower).
+// that its RW warps fill with asynchronous copies (16 bytes a lane, whole rows an
+// instruction, rows swizzled for conflict-free ldmatrix) and read together
+// (mma.sync m16n8k16, fp32 accumulation, online softmax in registers).  16 keys never
+// cross a page, so a tile needs one page lookup and a lane's addresses are one base
+// and constant steps.  (One TMA box per 64 columns and head instead: each costs the
+// issuing warp about 110 clk, 580 of the 1800 clk of a tile; a general address per
+// copy: 820 instructions a tile.)
+// Bound: HBM; each cached key is read once per row block.
 #include "fna2_paged.cuh"
 
 namespace fna2 {
@@ -43,7 +43,7 @@ struct PagedAttnParams {
   int H, G;       // query heads, query heads per KV head
   int RP;         // rank rounded up to 16 or 32
   int causal;
-  float scale, scale_log2;
+  float scale, scale_log2, inv_scale;
   const __nv_bfloat16* q;
   int64_t q_st, q_sh;
   const __nv_bfloat16* rq;
@@ -101,8 +101,8 @@ constexpr int kFewThreads = 128;
 constexpr int kFewKeys = 16;  // keys per tile
 
 // Shared-memory geometry (host and device agree on it): [A of the RW row blocks | K and V ring of
-// the key groups | R_k ring | m, l and accumulators of the key groups | barriers]; ng: graph heads of a block's rows, nh: heads that the 16
-// rows of one warp span.
+// the key groups | R_k ring | m, l and accumulators of the key groups | scan]; ng: graph heads
+// of a block's rows, nh: heads that the 16 rows of one warp span.
 struct FewSmem {
   int a_stride, kv_stage, r_head, r_stage, o_kv, o_r, o_join, o_bar, total;
   // (of the row block's rows only `rows`, its bound, are joined)
@@ -116,9 +116,26 @@ struct FewSmem {
     o_r = o_kv + rings * kv_stage;
     o_join = o_r + (rings * r_stage + 1023) / 1024 * 1024;
     o_bar = o_join + 512 + 4 / RW * (rows < 16 * RW ? rows : 16 * RW) * D * 4;
-    total = o_bar + 2 * rings * 8 + 64;
+    total = o_bar + 80;
   }
 };
+
+// Rendezvous of the RW warps of a key group (named barrier 1 + group).
+template <int RW>
+__device__ __forceinline__ void group_sync(int kg) {
+  if (RW == 1)
+    __syncwarp();
+  else
+    asm volatile("bar.sync %0, %1;" ::"r"(kg + 1), "n"(32 * RW) : "memory");
+}
+
+// 16 bytes to shared memory, or zeros.
+__device__ __forceinline__ void few_cp16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void few_cp16(uint32_t dst, const void* src, bool valid) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
+}
 
 // Four columns of a finished row: O = acc / (l + 1e-6), LSE = m + log(l + 1e-6).
 template <int D>
@@ -135,77 +152,85 @@ __device__ __forceinline__ void few_store(const PagedAttnParams& p, int64_t tok,
 }
 
 template <int D, int RW>
-__global__ void __launch_bounds__(kFewThreads, 2)
-    fna2_paged_few_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
-                          const __grid_constant__ CUtensorMap tmRk, const PagedAttnParams p) {
+__global__ void __launch_bounds__(kFewThreads, 2) fna2_paged_few_kernel(const PagedAttnParams p) {
   constexpr int KW = 4 / RW;  // key groups per CTA
-  constexpr int DC = D / 64;  // 64-column chunks of a K or V row
-  extern __shared__ __align__(1024) uint8_t dsm[];
-  if (smem_u32(dsm) & 1023u) {  // the swizzled layouts need it
-    if (threadIdx.x == 0) atomicCAS(&g_device_error, 0, kStatusSmemBase);
-    return;
-  }
+  extern __shared__ __align__(16) uint8_t dsm[];
   const int cta = blockIdx.x, lanes = p.kv.hkv * p.row_blocks, run = cta / lanes;
   const int kh = cta % lanes / p.row_blocks, r0 = cta % p.row_blocks * (16 * RW);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int rw = warp % RW, kg = warp / RW;
   const FewSmem L(D, RW, p.ng_max, p.nh_max, p.RP, p.stages, p.few_rows);
-  uint64_t* full = reinterpret_cast<uint64_t*>(dsm + L.o_bar) + kg * p.stages;
-  uint64_t* empty = full + KW * p.stages;
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(dsm + L.o_bar + 2 * KW * p.stages * 8);
-  int64_t* s_scan = reinterpret_cast<int64_t*>(dsm + L.o_bar + 2 * KW * p.stages * 8 + 16);  // [4], prefix
-  int* s_first = const_cast<int*>(abort_flag) + 1;
-  if (tid == 0) {
-    for (int s = 0; s < KW * p.stages; ++s) {
-      mbar_init(reinterpret_cast<uint64_t*>(dsm + L.o_bar) + s, 1);
-      mbar_init(reinterpret_cast<uint64_t*>(dsm + L.o_bar) + KW * p.stages + s, RW);
+  int64_t* s_scan = reinterpret_cast<int64_t*>(dsm + L.o_bar);  // [4] warps' sums, [4]: units before the first sequence
+  int* s_first = reinterpret_cast<int*>(s_scan + 5);            // first sequence: b, q0, n, len
+
+  // R_k ring: columns [rank, RP) of every head are zero, and stay so.
+  uint8_t* r_ring = dsm + L.o_r + kg * p.stages * L.r_stage;
+  const int rp8 = p.RP / 8, r8 = p.kv.rank / 8;
+  if (r8 != rp8) {
+    const int n = 4 / RW * p.stages * p.ng_max * 16;  // rows of all rings
+    for (int e = tid; e < n * (rp8 - r8); e += kFewThreads) {
+      const int row = e % n, c = r8 + e / n, sw = p.RP == 16 ? (row >> 2) & 1 : (row >> 1) & 3;
+      *reinterpret_cast<uint4*>(dsm + L.o_r + row * p.RP * 2 + (c ^ sw) * 16) = make_uint4(0, 0, 0, 0);
     }
-    *abort_flag = 0;
-    fence_mbar_init();
   }
 
-  // Number of units, this CTA's run [u, u_end) of them, and the sequence that unit u is in.
-  int64_t U = 0;
-  for (int b = tid; b < p.bd.B; b += kFewThreads) U += few_units(p, paged_seq(p.bd, b));
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) U += __shfl_xor_sync(0xffffffffu, U, o);
-  if (lane == 0) s_scan[warp] = U;
-  __syncthreads();
-  U = s_scan[0] + s_scan[1] + s_scan[2] + s_scan[3];
-  const int C = few_runs(p, U);
-  const int64_t u_beg = few_first(U, C, min(run, C)), u_end = few_first(U, C, min(run + 1, C));
-  int64_t carry = 0;
-  for (int base = 0; base < p.bd.B; base += kFewThreads) {
+  // Number of units U, this CTA's run [u_beg, u_end) of them, and the sequence that its first unit is in:
+  // a scan over the sequences, 128 a round (a second pass over the later rounds when there are more).
+  int64_t U = 0, pre0 = 0;
+  int units0 = 0;
+  PagedSeq sq0{0, 0, 0, false};
+  auto scan = [&](int base, PagedSeq* s, int* units) {
     const int b = base + tid;
-    int units = 0;
+    *units = 0;
     if (b < p.bd.B) {
-      const PagedSeq s = paged_seq(p.bd, b);
-      if (!s.ok && cta == 0) atomicCAS(&g_device_error, 0, kStatusBadSeqPaged);
-      units = few_units(p, s);
+      *s = paged_seq(p.bd, b);
+      if (!s->ok && cta == 0) atomicCAS(&g_device_error, 0, kStatusBadSeqPaged);
+      *units = few_units(p, *s);
     }
-    int64_t incl = units;
+    int64_t incl = *units;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
       if (lane >= o) incl += v;
     }
-    __syncthreads();  // s_scan has been read
     if (lane == 31) s_scan[warp] = incl;
     __syncthreads();
-    int64_t pre = carry + incl - units;
+    int64_t pre = U + incl - *units;
     for (int w = 0; w < warp; ++w) pre += s_scan[w];
-    carry += s_scan[0] + s_scan[1] + s_scan[2] + s_scan[3];
+    U += s_scan[0] + s_scan[1] + s_scan[2] + s_scan[3];
+    __syncthreads();
     if (cta == 0 && b < p.bd.B && p.prefix) p.prefix[b] = pre;
-    if (units > 0 && pre <= u_beg && u_beg < pre + units) *s_first = b, s_scan[4] = pre;
+    return pre;
+  };
+  pre0 = scan(0, &sq0, &units0);
+  const int64_t U0 = U;
+  for (int base = kFewThreads; base < p.bd.B; base += kFewThreads) {
+    PagedSeq s;
+    int units;
+    scan(base, &s, &units);
   }
+  const int C = few_runs(p, U);
+  const int64_t U_all = U, u_beg = few_first(U, C, min(run, C)), u_end = few_first(U, C, min(run + 1, C));
   if (cta == 0 && tid == 0 && p.prefix) p.prefix[p.bd.B] = U;
   if (u_beg == u_end) return;
+  auto found = [&](int b, const PagedSeq& s, int units, int64_t pre) {
+    if (units > 0 && pre <= u_beg && u_beg < pre + units)
+      s_first[0] = b, s_first[1] = s.q0, s_first[2] = s.n, s_first[3] = s.len, s_scan[4] = pre;
+  };
+  found(tid, sq0, units0, pre0);
+  U = U0;
+  for (int base = kFewThreads; base < p.bd.B && U <= u_beg && U < U_all; base += kFewThreads) {
+    PagedSeq s;
+    int units;
+    const int64_t pre = scan(base, &s, &units);
+    found(base + tid, s, units, pre);
+  }
   __syncthreads();
 
   // Current sequence: units [o_beg, o_end) of it.
   int64_t u = u_beg, pre = s_scan[4];
-  int b = *s_first;
-  PagedSeq sq = paged_seq(p.bd, b);
+  int b = s_first[0];
+  PagedSeq sq{s_first[1], s_first[2], s_first[3], true};
   int units = few_units(p, sq), rows, r_last, o_beg, o_end, past, g_lo, ng, k_begin, k_end, n_tiles;
   const int* table;
   auto segment = [&]() {
@@ -232,41 +257,70 @@ __global__ void __launch_bounds__(kFewThreads, 2)
   };
   segment();
 
-  // Ring of the key group: lane l issues box l of a tile (K chunks, V chunks, R_k heads).
+  // Ring of the key group.  K and V: lane l copies 16-byte piece l % PPR of row row0 + k RW RPI, in turn
+  // k; piece c of row r lies at chunk c ^ (r & 7) of its 128 bytes.  R_k: piece x of row lane % 16.
+  constexpr int PPR = D / 8, RPI = 32 / PPR, NI = 16 / (RW * RPI), STEP = RW * RPI;
   uint8_t* kv_ring = dsm + L.o_kv + kg * p.stages * L.kv_stage;
-  uint8_t* r_ring = dsm + L.o_r + kg * p.stages * L.r_stage;
   const int lg = p.kv.page_log2, mask = (1 << lg) - 1;
-  const CUtensorMap* map = lane < DC ? &tmK : lane < 2 * DC ? &tmV : &tmRk;
-  const int box_col = lane < 2 * DC ? lane % DC * 64 : 0;
-  uint8_t* box_dst = lane < 2 * DC ? kv_ring + lane * (kFewKeys * 128) : r_ring + (lane - 2 * DC) * L.r_head;
-  const int box_step = lane < 2 * DC ? L.kv_stage : L.r_stage;
-  int issued = 0, i_stage = 0, i_phase = 1;  // empty barriers: the first round passes
-  int j_next = 0, page_next = 0;
+  const int row0 = rw * RPI + lane / PPR, pc = lane % PPR, r_row = lane % 16, r_lg = p.RP == 16 ? 1 : 2;
+  const uint32_t d_lane = (pc >> 3) * (kFewKeys * 128) + row0 * 128 + ((pc ^ row0) & 7) * 16;
+  const uint32_t dr_lane = r_row * p.RP * 2;
+  const int dr_sw = p.RP == 16 ? (r_row >> 2) & 1 : (r_row >> 1) & 3;
+  const __nv_bfloat16* k_lane = p.kv.k.ptr + kh * p.kv.k.sh + row0 * p.kv.k.st + pc * 8;
+  const __nv_bfloat16* v_lane = p.kv.v.ptr + kh * p.kv.v.sh + row0 * p.kv.v.st + pc * 8;
+  int issued = 0, i_stage = 0, j_next = 0, page_next = 0;
   auto issue = [&]() {
-    if (issued >= n_tiles) return;
-    const int page = page_next, slot = j_next & mask;
-    j_next += KW * kFewKeys;
-    ++issued;
-    if (issued < n_tiles) page_next = __ldg(table + (j_next >> lg));
-    if (RW > 1) mbar_wait(empty + i_stage, i_phase, abort_flag, 131);
-    if (lane == 0) mbar_expect_tx(full + i_stage, L.kv_stage + ng * L.r_head);
-    __syncwarp();
-    if (lane < 2 * DC + ng)
-      tma_load_4d(box_dst + i_stage * box_step, map, full + i_stage, box_col, slot,
-                  lane < 2 * DC ? kh : kh * p.G + g_lo + lane - 2 * DC, page);
-    if (++i_stage == p.stages) i_stage = 0, i_phase ^= 1;
+    if (issued < n_tiles) {
+      const int page = page_next, slot = j_next & mask, j0 = j_next;
+      j_next += KW * kFewKeys;
+      if (++issued < n_tiles) page_next = __ldg(table + (j_next >> lg));
+      const uint32_t dk = smem_u32(kv_ring + i_stage * L.kv_stage) + d_lane;
+      const uint32_t dr = smem_u32(r_ring + i_stage * L.r_stage) + dr_lane;
+      // rows past the sequence's end are zero-filled: what a page holds there is never used
+      const int nv = page >= 0 && page < p.kv.pages ? min(kFewKeys, sq.len - j0) : 0;
+      const int64_t pg = nv > 0 ? page : 0;
+      const __nv_bfloat16* ks = k_lane + pg * p.kv.k.sp + slot * p.kv.k.st;
+      const __nv_bfloat16* vs = v_lane + pg * p.kv.v.sp + slot * p.kv.v.st;
+      if (nv == kFewKeys) {
+#pragma unroll
+        for (int k = 0; k < NI; ++k) {
+          const uint32_t d = (dk ^ ((k * STEP & 7) * 16)) + k * STEP * 128;
+          few_cp16(d, ks);
+          few_cp16(d + kFewKeys * D * 2, vs);
+          ks += STEP * p.kv.k.st, vs += STEP * p.kv.v.st;
+        }
+      } else {
+        for (int k = 0; k < NI; ++k) {
+          const uint32_t d = (dk ^ ((k * STEP & 7) * 16)) + k * STEP * 128;
+          const bool valid = row0 + k * STEP < nv;
+          few_cp16(d, valid ? ks : p.kv.k.ptr, valid);
+          few_cp16(d + kFewKeys * D * 2, valid ? vs : p.kv.v.ptr, valid);
+          ks += STEP * p.kv.k.st, vs += STEP * p.kv.v.st;
+        }
+      }
+      if (ng > 0) {
+        const bool valid = r_row < nv;
+        const __nv_bfloat16* rs = p.kv.rk.ptr + (kh * p.G + g_lo) * p.kv.rk.sh + pg * p.kv.rk.sp + (slot + r_row) * p.kv.rk.st;
+        for (int x = lane / 16 + 2 * rw; x < ng << r_lg; x += 2 * RW) {
+          const int hh = x >> r_lg, c = x & (rp8 - 1);
+          if (c < r8)
+            few_cp16(dr + hh * L.r_head + (c ^ dr_sw) * 16, valid ? rs + hh * p.kv.rk.sh + c * 8 : p.kv.rk.ptr, valid);
+        }
+      }
+      if (++i_stage == p.stages) i_stage = 0;
+    }
+    dec_commit();
   };
   // The first tiles of a sequence; the ring is empty here.
   auto start = [&]() {
-    if (rw != 0 || n_tiles == 0) return;
     issued = 0;
     j_next = k_begin + kg * kFewKeys;
-    page_next = __ldg(table + (j_next >> lg));
+    if (n_tiles > 0) page_next = __ldg(table + (j_next >> lg));
     for (int s = 0; s < p.stages - 1; ++s) issue();
   };
   start();
 
-  int stage = 0, phase = 0;
+  int stage = 0;
   while (true) {
   // A = [q | R~_q hi, lo of the warp's heads] of the row blocks' 16 rows each (rows past the end are zero)
   const int wr0 = r0 + rw * 16;
@@ -274,27 +328,30 @@ __global__ void __launch_bounds__(kFewThreads, 2)
   const int wn = wr0 < rows ? max(0, wg_hi - wg_lo + 1) : 0;
   uint8_t* sa = dsm + rw * 16 * L.a_stride;
   {
-    const int part = kg * 32 + lane;  // of 32 KW threads
-    for (int e = part; e < 16 * (D / 8); e += 32 * KW) {
-      const int row = e / (D / 8), c = e % (D / 8) * 8, r = wr0 + row;
-      uint4 v = make_uint4(0, 0, 0, 0);
-      if (r < rows)
-        v = *reinterpret_cast<const uint4*>(p.q + (sq.q0 + r % sq.n) * p.q_st + (kh * p.G + r / sq.n) * p.q_sh + c);
-      *reinterpret_cast<uint4*>(sa + row * L.a_stride + c * 2) = v;
-    }
-    const int rp8 = p.RP / 8;
-    for (int e = part; e < 16 * wn * rp8; e += 32 * KW) {
-      const int row = e / (wn * rp8), g = e / rp8 % wn, c = e % rp8 * 8, r = wr0 + row;
+    constexpr int TPR = 2 * KW;  // threads per row
+    const int part = kg * 32 + lane, row = part / TPR, sub = part % TPR, r = wr0 + row;
+    const bool real = r < rows;
+    const int hh = real ? r / sq.n : 0, h = kh * p.G + hh;
+    const int64_t tok = sq.q0 + (r - hh * sq.n);
+    uint4 v[D / 8 / TPR];
+#pragma unroll
+    for (int k = 0; k < D / 8 / TPR; ++k)
+      v[k] = real ? *reinterpret_cast<const uint4*>(p.q + tok * p.q_st + h * p.q_sh + (sub + k * TPR) * 8)
+                  : make_uint4(0, 0, 0, 0);
+    // block-diagonal: a row holds its own head's R~_q
+    const bool graph = real && h < p.kv.hg;
+    const float f = graph ? __ldg(p.gs + h) * p.inv_scale : 0.f;
+    for (int x = sub; x < wn * 2 * rp8; x += TPR) {
+      const int gg = x / (2 * rp8), c = x % rp8;
       uint32_t hi[4] = {0, 0, 0, 0}, lo[4] = {0, 0, 0, 0};
-      if (r < rows && r / sq.n == wg_lo + g && c < p.kv.rank) {  // block-diagonal: a row holds its own head's R~_q
-        const int h = kh * p.G + wg_lo + g;
-        split_bias(*reinterpret_cast<const uint4*>(p.rq + (sq.q0 + r % sq.n) * p.rq_st + h * p.rq_sh + c),
-                   __ldg(p.gs + h) / p.scale, hi, lo);
-      }
-      uint8_t* dst = sa + row * L.a_stride + (D + 2 * g * p.RP + c) * 2;
-      *reinterpret_cast<uint4*>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-      *reinterpret_cast<uint4*>(dst + p.RP * 2) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+      if (graph && hh == wg_lo + gg && c < r8)
+        split_bias(*reinterpret_cast<const uint4*>(p.rq + tok * p.rq_st + h * p.rq_sh + c * 8), f, hi, lo);
+      const bool is_lo = x % (2 * rp8) >= rp8;
+      *reinterpret_cast<uint4*>(sa + row * L.a_stride + (D + x * 8) * 2) =
+          is_lo ? make_uint4(lo[0], lo[1], lo[2], lo[3]) : make_uint4(hi[0], hi[1], hi[2], hi[3]);
     }
+#pragma unroll
+    for (int k = 0; k < D / 8 / TPR; ++k) *reinterpret_cast<uint4*>(sa + row * L.a_stride + (sub + k * TPR) * 16) = v[k];
   }
   __syncthreads();
 
@@ -329,22 +386,13 @@ __global__ void __launch_bounds__(kFewThreads, 2)
   }
 
   for (int tt = 0; tt < n_tiles; ++tt) {
-    __syncwarp();  // (RW == 1) every lane is done with the stage that this issue refills
-    if (rw == 0) issue();
-    if (!mbar_wait(full + stage, phase, abort_flag, 132)) break;
-    uint8_t* kv = kv_ring + stage * L.kv_stage;
-    const uint32_t kv_addr = smem_u32(kv);
+    group_sync<RW>(kg);      // everyone is done with the stage that this issue refills
+    issue();
+    dec_wait(p.stages - 1);  // this thread's pieces of tile tt have landed
+    group_sync<RW>(kg);      // and so have the others'
+    const uint32_t kv_addr = smem_u32(kv_ring + stage * L.kv_stage);
     const uint32_t rk_addr = smem_u32(r_ring + stage * L.r_stage) + (wg_lo - g_lo) * L.r_head + r_off;
     const int j0 = k_begin + (kg + tt * KW) * kFewKeys;
-    if (j0 + kFewKeys > sq.len) {
-      // past the sequence's end a page holds anything: V rows become zero (P is 0 there, but 0 * NaN
-      // is not); K rows only reach logits that are masked.  The RW warps write the same zeros.
-      for (int e = lane; e < (j0 + kFewKeys - sq.len) * 8 * DC; e += 32)
-        *reinterpret_cast<uint4*>(kv + kFewKeys * D * 2 + e % DC * (kFewKeys * 128) +
-                                  (sq.len - j0) * 128 + e / DC * 16) = make_uint4(0, 0, 0, 0);
-      fence_proxy_async_smem();  // a later segment's tile is loaded into this stage
-      __syncwarp();
-    }
     float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int ks = 0; ks < D / 16; ++ks) {
@@ -413,11 +461,7 @@ __global__ void __launch_bounds__(kFewThreads, 2)
       mma_bf16(acc[2 * d16], pa, vb[0], vb[1]);
       mma_bf16(acc[2 * d16 + 1], pa, vb[2], vb[3]);
     }
-    if (RW > 1) {
-      __syncwarp();
-      if (lane == 0) mbar_arrive(empty + stage);
-    }
-    if (++stage == p.stages) stage = 0, phase ^= 1;
+    if (++stage == p.stages) stage = 0;
   }
   // sums and the true maximum over the row's four lanes; everything relative to that maximum
 #pragma unroll
@@ -460,6 +504,7 @@ __global__ void __launch_bounds__(kFewThreads, 2)
       units = few_units(p, sq);
     }
     segment();
+    group_sync<RW>(kg);  // everyone is done with the ring
     start();
   }
   __syncthreads();
@@ -638,30 +683,25 @@ __global__ void __launch_bounds__(128) fna2_paged_many_join_kernel(const PagedAt
 // ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
-struct FewMaps {
-  CUtensorMap k, v, rk;
-};
-
 template <int D, int RW>
-cudaError_t launch_paged_few_t(const FewMaps& m, const PagedAttnParams& p, size_t smem, cudaStream_t stream) {
+cudaError_t launch_paged_few_t(const PagedAttnParams& p, size_t smem, cudaStream_t stream) {
   auto kern = fna2_paged_few_kernel<D, RW>;
   static std::atomic<uint64_t> allowed{0};
   cudaError_t e = allow_smem(reinterpret_cast<const void*>(kern), allowed);
   if (e != cudaSuccess) return e;
-  kern<<<p.runs * p.kv.hkv * p.row_blocks, kFewThreads, smem, stream>>>(m.k, m.v, m.rk, p);
+  kern<<<p.runs * p.kv.hkv * p.row_blocks, kFewThreads, smem, stream>>>(p);
   return cudaGetLastError();
 }
 
 template <int D>
-cudaError_t launch_paged_few_d(const FewMaps& m, const PagedAttnParams& p, int RW, size_t smem, cudaStream_t stream) {
-  return RW == 1   ? launch_paged_few_t<D, 1>(m, p, smem, stream)
-         : RW == 2 ? launch_paged_few_t<D, 2>(m, p, smem, stream)
-                   : launch_paged_few_t<D, 4>(m, p, smem, stream);
+cudaError_t launch_paged_few_d(const PagedAttnParams& p, int RW, size_t smem, cudaStream_t stream) {
+  return RW == 1   ? launch_paged_few_t<D, 1>(p, smem, stream)
+         : RW == 2 ? launch_paged_few_t<D, 2>(p, smem, stream)
+                   : launch_paged_few_t<D, 4>(p, smem, stream);
 }
 
-inline cudaError_t launch_paged_few(const FewMaps& m, const PagedAttnParams& p, int D, int RW, size_t smem,
-                                    cudaStream_t stream) {
-  return D == 128 ? launch_paged_few_d<128>(m, p, RW, smem, stream) : launch_paged_few_d<64>(m, p, RW, smem, stream);
+inline cudaError_t launch_paged_few(const PagedAttnParams& p, int D, int RW, size_t smem, cudaStream_t stream) {
+  return D == 128 ? launch_paged_few_d<128>(p, RW, smem, stream) : launch_paged_few_d<64>(p, RW, smem, stream);
 }
 
 inline cudaError_t launch_paged_few_join(const PagedAttnParams& p, int D, cudaStream_t stream) {
