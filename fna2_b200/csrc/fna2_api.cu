@@ -985,7 +985,7 @@ extern "C" int fna2_paged_attn(const Fna2PagedKV* kv, const Fna2PagedAttnArgs* a
     if (int rc = many_maps(p, kv->head_dim, &m)) return rc;
     FNA2_CUDA(launch_paged_many(m, p, kv->head_dim, st));
   }
-  if (l.few) FNA2_CUDA(launch_paged_few(p, kv->head_dim, l.RW, l.smem, st));
+  if (l.few) FNA2_CUDA(launch_paged_few(p, kv->head_dim, l.RW, l.smem, l.many, st));
   if (l.many_join) FNA2_CUDA(launch_paged_many_join(p, kv->head_dim, st));
   if (l.few_join) FNA2_CUDA(launch_paged_few_join(p, kv->head_dim, st));
   if (l.logits && p.bd.max_k > 0) FNA2_CUDA(launch_logit_weights(p, st));

@@ -115,6 +115,7 @@ __global__ void __launch_bounds__(kSelThreads) fna2_evict_select_kernel(const Ev
   __shared__ int s_warp[2][32];
   __shared__ int s_digit, s_above;
   const int kh = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  pdl_trigger();
   int len = __ldg(p.lens + b);
   if (len < 0 || len > p.max_k) {
     if (tid == 0) atomicCAS(&g_device_error, 0, kStatusBadSeqEvict);
@@ -213,6 +214,7 @@ constexpr int kMoveRows = 32;
 
 __global__ void __launch_bounds__(kMoveThreads) fna2_evict_move_kernel(const EvictParams p) {
   __shared__ RowPlace s_at[kMoveRows];
+  pdl_wait();
   move_rows<kMoveThreads, kMoveRows>(p, blockIdx.z, blockIdx.y, blockIdx.x * kMoveRows, s_at);
 }
 
@@ -229,8 +231,8 @@ inline cudaError_t launch_evict(const EvictParams& p, cudaStream_t stream) {
   fna2_evict_select_kernel<false><<<heads, kSelThreads, 0, stream>>>(p);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return e;
-  fna2_evict_move_kernel<<<dim3((p.budget + kMoveRows - 1) / kMoveRows, p.kv.hkv, p.B), kMoveThreads, 0, stream>>>(p);
-  return cudaGetLastError();
+  return launch_dependent(fna2_evict_move_kernel, dim3((p.budget + kMoveRows - 1) / kMoveRows, p.kv.hkv, p.B),
+                          kMoveThreads, 0, stream, p);
 }
 
 }  // namespace fna2

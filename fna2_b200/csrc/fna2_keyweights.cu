@@ -53,6 +53,7 @@ struct KeyWeightsParams {
 // R~_q = gs/scale * R_q as hi + lo, columns [rank, RP) zero, and -LSE/scale = l1 + l2 + l3 (a row
 // without weight: -1e38, whose weights are 0).
 __global__ void __launch_bounds__(256) fna2_key_weights_prep_kernel(const KeyWeightsParams p) {
+  pdl_trigger();
   const int64_t e = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
   if (e == 0) *p.next = 0;
   const int r8 = p.RP / 8, per = r8 + 1;  // pieces of a row: R_q's, then the LSE's
@@ -227,6 +228,7 @@ __global__ void __launch_bounds__(kKwThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  pdl_wait();
 
   if (warp == 8) {
     // ------------------------------------------------------------ producer
@@ -503,6 +505,7 @@ __global__ void __launch_bounds__(kKwThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  pdl_wait();
 
   if (warp == 8) {
     // ------------------------------------------------------------ producer
@@ -717,9 +720,8 @@ cudaError_t launch_key_weights_t(const KwMaps& m, KeyWeightsParams& p, cudaStrea
   // key tiles per item: a pair, or runs (about three per CTA when all sequences are the longest)
   p.run_tiles = window ? static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(16, seqs * tiles / (3 * kSms)))) : 2;
   const int64_t items = seqs * ((tiles + p.run_tiles - 1) / p.run_tiles);
-  kern<<<static_cast<unsigned>(std::min<int64_t>(items, kSms)), kKwThreads,
-         window ? KwwSmem<D, RP>::kTotal : KwSmem<D, RP>::kTotal, stream>>>(m.q, m.k, m.rq, m.rk, m.l, p);
-  return cudaGetLastError();
+  return launch_dependent(kern, static_cast<unsigned>(std::min<int64_t>(items, kSms)), kKwThreads,
+                          window ? KwwSmem<D, RP>::kTotal : KwSmem<D, RP>::kTotal, stream, m.q, m.k, m.rq, m.rk, m.l, p);
 }
 
 inline cudaError_t launch_key_weights(const KwMaps& m, KeyWeightsParams& p, int D, cudaStream_t stream) {

@@ -154,6 +154,7 @@ __device__ __forceinline__ void few_store(const PagedAttnParams& p, int64_t tok,
 template <int D, int RW>
 __global__ void __launch_bounds__(kFewThreads, 2) fna2_paged_few_kernel(const PagedAttnParams p) {
   constexpr int KW = 4 / RW;  // key groups per CTA
+  pdl_trigger();
   extern __shared__ __align__(16) uint8_t dsm[];
   const int cta = blockIdx.x, lanes = p.kv.hkv * p.row_blocks, run = cta / lanes;
   const int kh = cta % lanes / p.row_blocks, r0 = cta % p.row_blocks * (16 * RW);
@@ -212,7 +213,10 @@ __global__ void __launch_bounds__(kFewThreads, 2) fna2_paged_few_kernel(const Pa
   const int C = few_runs(p, U);
   const int64_t U_all = U, u_beg = few_first(U, C, min(run, C)), u_end = few_first(U, C, min(run + 1, C));
   if (cta == 0 && tid == 0 && p.prefix) p.prefix[p.bd.B] = U;
-  if (u_beg == u_end) return;
+  if (u_beg == u_end) {
+    pdl_wait();
+    return;
+  }
   auto found = [&](int b, const PagedSeq& s, int units, int64_t pre) {
     if (units > 0 && pre <= u_beg && u_beg < pre + units)
       s_first[0] = b, s_first[1] = s.q0, s_first[2] = s.n, s_first[3] = s.len, s_scan[4] = pre;
@@ -533,6 +537,7 @@ __global__ void __launch_bounds__(kFewThreads, 2) fna2_paged_few_kernel(const Pa
   }
   if (!more) break;
   }
+  pdl_wait();  // (a tensor-core kernel before this one has nothing that this one reads)
 }
 
 // Joins the sequences that were cut: a warp per (KV head, query row) rescales the
@@ -581,6 +586,8 @@ template <int D>
 __global__ void __launch_bounds__(kTailThreads) fna2_paged_few_join_kernel(const PagedAttnParams p) {
   const int kh = blockIdx.y, b = blockIdx.z, lane = threadIdx.x & 31;
   const int r = blockIdx.x * kTailRows + (threadIdx.x >> 5);
+  pdl_trigger();
+  pdl_wait();
   const PagedSeq sq = paged_seq(p.bd, b);
   const int units = few_units(p, sq);
   if (units == 0 || r >= sq.n * p.G) return;
@@ -613,6 +620,7 @@ constexpr int kLogitKeys = 4 * kTailThreads;
 
 __global__ void __launch_bounds__(kTailThreads) fna2_paged_logit_weights_kernel(const PagedAttnParams p) {
   __shared__ float s_x[kFewRows];
+  pdl_wait();
   const int kh = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
   const PagedSeq sq = paged_seq(p.bd, b);
   const int rows = sq.n * p.G, past = sq.len - sq.n, j = blockIdx.x * kLogitKeys + 4 * tid;
@@ -646,6 +654,8 @@ __global__ void __launch_bounds__(kTailThreads) fna2_paged_logit_weights_kernel(
 // common max, O = acc / (l + 1e-6), LSE = m + log(l + 1e-6).
 template <int D>
 __global__ void __launch_bounds__(128) fna2_paged_many_join_kernel(const PagedAttnParams p) {
+  pdl_trigger();
+  pdl_wait();
   const int lane = threadIdx.x & 31;
   const int64_t th = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
   const int64_t tok = th / p.H;
@@ -684,49 +694,45 @@ __global__ void __launch_bounds__(128) fna2_paged_many_join_kernel(const PagedAt
 // host side
 // ---------------------------------------------------------------------------
 template <int D, int RW>
-cudaError_t launch_paged_few_t(const PagedAttnParams& p, size_t smem, cudaStream_t stream) {
+cudaError_t launch_paged_few_t(const PagedAttnParams& p, size_t smem, bool after_many, cudaStream_t stream) {
   auto kern = fna2_paged_few_kernel<D, RW>;
   static std::atomic<uint64_t> allowed{0};
   cudaError_t e = allow_smem(reinterpret_cast<const void*>(kern), allowed);
   if (e != cudaSuccess) return e;
-  kern<<<p.runs * p.kv.hkv * p.row_blocks, kFewThreads, smem, stream>>>(p);
+  const unsigned grid = p.runs * p.kv.hkv * p.row_blocks;
+  if (after_many) return launch_dependent(kern, grid, kFewThreads, smem, stream, p);  // fills the SMs it leaves
+  kern<<<grid, kFewThreads, smem, stream>>>(p);
   return cudaGetLastError();
 }
 
 template <int D>
-cudaError_t launch_paged_few_d(const PagedAttnParams& p, int RW, size_t smem, cudaStream_t stream) {
-  return RW == 1   ? launch_paged_few_t<D, 1>(p, smem, stream)
-         : RW == 2 ? launch_paged_few_t<D, 2>(p, smem, stream)
-                   : launch_paged_few_t<D, 4>(p, smem, stream);
+cudaError_t launch_paged_few_d(const PagedAttnParams& p, int RW, size_t smem, bool after_many, cudaStream_t stream) {
+  return RW == 1   ? launch_paged_few_t<D, 1>(p, smem, after_many, stream)
+         : RW == 2 ? launch_paged_few_t<D, 2>(p, smem, after_many, stream)
+                   : launch_paged_few_t<D, 4>(p, smem, after_many, stream);
 }
 
-inline cudaError_t launch_paged_few(const PagedAttnParams& p, int D, int RW, size_t smem, cudaStream_t stream) {
-  return D == 128 ? launch_paged_few_d<128>(p, RW, smem, stream) : launch_paged_few_d<64>(p, RW, smem, stream);
+inline cudaError_t launch_paged_few(const PagedAttnParams& p, int D, int RW, size_t smem, bool after_many,
+                                    cudaStream_t stream) {
+  return D == 128 ? launch_paged_few_d<128>(p, RW, smem, after_many, stream) : launch_paged_few_d<64>(p, RW, smem, after_many, stream);
 }
 
 inline cudaError_t launch_paged_few_join(const PagedAttnParams& p, int D, cudaStream_t stream) {
   const int rows = std::min(p.bd.max_q * p.G, p.few_rows);
   const dim3 grid((rows + kTailRows - 1) / kTailRows, p.kv.hkv, p.bd.B);
-  if (D == 128)
-    fna2_paged_few_join_kernel<128><<<grid, kTailThreads, 0, stream>>>(p);
-  else
-    fna2_paged_few_join_kernel<64><<<grid, kTailThreads, 0, stream>>>(p);
-  return cudaGetLastError();
+  return launch_dependent(D == 128 ? fna2_paged_few_join_kernel<128> : fna2_paged_few_join_kernel<64>, grid, kTailThreads,
+                          0, stream, p);
 }
 
 inline cudaError_t launch_logit_weights(const PagedAttnParams& p, cudaStream_t stream) {
   const dim3 grid((p.bd.max_k + kLogitKeys - 1) / kLogitKeys, p.kv.hkv, p.bd.B);
-  fna2_paged_logit_weights_kernel<<<grid, kTailThreads, 0, stream>>>(p);
-  return cudaGetLastError();
+  return launch_dependent(fna2_paged_logit_weights_kernel, grid, kTailThreads, 0, stream, p);
 }
 
 inline cudaError_t launch_paged_many_join(const PagedAttnParams& p, int D, cudaStream_t stream) {
   const int64_t blocks = (static_cast<int64_t>(p.bd.T) * p.H + 3) / 4;
-  if (D == 128)
-    fna2_paged_many_join_kernel<128><<<static_cast<unsigned>(blocks), 128, 0, stream>>>(p);
-  else
-    fna2_paged_many_join_kernel<64><<<static_cast<unsigned>(blocks), 128, 0, stream>>>(p);
-  return cudaGetLastError();
+  return launch_dependent(D == 128 ? fna2_paged_many_join_kernel<128> : fna2_paged_many_join_kernel<64>,
+                          static_cast<unsigned>(blocks), 128, 0, stream, p);
 }
 
 }  // namespace fna2

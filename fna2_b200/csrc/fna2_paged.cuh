@@ -89,6 +89,28 @@ __device__ __forceinline__ int warp_seq_of(const int* cu, int B, int64_t t, int 
   return lo;
 }
 
+// Programmatic dependent launch: a kernel launched with launch_dependent may start while the kernel
+// before it runs its last CTAs, once all of those have called pdl_trigger or exited; pdl_wait returns
+// when that kernel is complete and its writes are visible.  Every kernel launched this way calls
+// pdl_wait in every thread that returns normally, so work after it in the stream is ordered as usual.
+__device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+template <class... P, class... A>
+cudaError_t launch_dependent(void (*kern)(P...), dim3 grid, int threads, size_t smem, cudaStream_t stream, A&&... args) {
+  cudaLaunchConfig_t c{};
+  c.gridDim = grid;
+  c.blockDim = dim3(threads);
+  c.dynamicSmemBytes = smem;
+  c.stream = stream;
+  cudaLaunchAttribute a{};
+  a.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  a.val.programmaticStreamSerializationAllowed = 1;
+  c.attrs = &a;
+  c.numAttrs = 1;
+  return cudaLaunchKernelEx(&c, kern, static_cast<P>(args)...);
+}
+
 // Lets a kernel use all of the dynamic shared memory, once per device (`done`: a
 // bit per device; the call costs about a microsecond, a small kernel takes five).
 inline cudaError_t allow_smem(const void* kern, std::atomic<uint64_t>& done) {

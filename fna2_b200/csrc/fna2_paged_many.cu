@@ -113,6 +113,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::oMisc);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::oMisc + 4);
   const int warp = warp_id(), lane = lane_id(), tid = threadIdx.x;
+  pdl_trigger();
 
   ManyItem it;
   if (!many_item(p, blockIdx.y, lane, &it)) return;
