@@ -10,7 +10,7 @@
 // Two kernels.  Select: one CTA per (sequence, KV head) finds the K-th largest
 // weight by a radix search over the ordered bits of the fp32 weights (11 + 11 +
 // 10 bits, a shared-memory histogram per pass), then writes the kept indices in
-// order with a block-wide scan.  Move: HBM-bound, 16-byte copies of whole rows.
+// order, a run of keys per warp.  Move: HBM-bound, 16-byte copies of whole rows.
 #include "fna2_paged.cuh"
 
 namespace fna2 {
@@ -107,9 +107,12 @@ __device__ __forceinline__ uint32_t ordered_bits(float x) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// MOVE: the block also copies its rows (short sequences: one launch instead of two).
-template <bool MOVE>
+// MOVE: the block also copies its rows (short sequences: one launch instead of two).  STAGED: the
+// ordered bits of the sequence's weights fit in shared memory and are read from there after the first
+// pass (each pass over 16,384 weights in global memory took 7 us, latency of dependent loads).
+template <bool MOVE, bool STAGED>
 __global__ void __launch_bounds__(kSelThreads) fna2_evict_select_kernel(const EvictParams p) {
+  extern __shared__ uint32_t s_bits[];
   __shared__ int hist[kSelBins];
   __shared__ RowPlace s_at[MOVE ? kSelThreads : 1];
   __shared__ int s_warp[2][32];
@@ -125,20 +128,37 @@ __global__ void __launch_bounds__(kSelThreads) fna2_evict_select_kernel(const Ev
   const int old_end = max(0, len - p.recent), old_beg = min(p.sink, old_end);  // candidates [old_beg, old_end)
   const int need = keep - (len - old_end) - old_beg;                            // >= 0: sink + recent <= budget
   const float* w = p.w + b * p.w_sb + kh * p.w_sh;
+  const bool all = need >= old_end - old_beg, some = !all && need > 0;
+  auto bits = [&](int j) { return STAGED ? s_bits[j] : ordered_bits(__ldg(w + j)); };
   uint32_t prefix = 0;
   int want = need;  // rank of the threshold among the candidates that share the prefix
-  const bool all = need >= old_end - old_beg;
-  if (!all && need > 0) {
+  if (some) {
     int shift = 32;
     for (int pass = 0; pass < 3; ++pass) {
-      const int bits = pass < 2 ? 11 : 10;
+      const int width = pass < 2 ? 11 : 10;
       const uint32_t hi_mask = pass == 0 ? 0u : 0xffffffffu << shift;
-      shift -= bits;
+      shift -= width;
       for (int i = tid; i < kSelBins; i += kSelThreads) hist[i] = 0;
       __syncthreads();
-      for (int j = old_beg + tid; j < old_end; j += kSelThreads) {
-        const uint32_t u = ordered_bits(__ldg(w + j));
-        if ((u & hi_mask) == prefix) atomicAdd(&hist[(u >> shift) & ((1u << bits) - 1)], 1);
+      if (STAGED && pass == 0) {
+        constexpr int U = 8;  // loads in flight
+        for (int j0 = old_beg + tid; j0 < old_end; j0 += U * kSelThreads) {
+          float x[U];
+#pragma unroll
+          for (int i = 0; i < U; ++i) x[i] = j0 + i * kSelThreads < old_end ? __ldg(w + j0 + i * kSelThreads) : 0.f;
+#pragma unroll
+          for (int i = 0; i < U; ++i)
+            if (j0 + i * kSelThreads < old_end) {
+              const uint32_t u = ordered_bits(x[i]);
+              s_bits[j0 + i * kSelThreads] = u;
+              atomicAdd(&hist[u >> shift], 1);
+            }
+        }
+      } else {
+        for (int j = old_beg + tid; j < old_end; j += kSelThreads) {
+          const uint32_t u = bits(j);
+          if ((u & hi_mask) == prefix) atomicAdd(&hist[(u >> shift) & ((1u << width) - 1)], 1);
+        }
       }
       __syncthreads();
       // suffix counts: thread t owns bins 2t and 2t + 1
@@ -163,40 +183,47 @@ __global__ void __launch_bounds__(kSelThreads) fna2_evict_select_kernel(const Ev
       __syncthreads();
     }
   }
-  // prefix: the threshold value; want: how many candidates equal to it are kept (the lowest indices)
+  // prefix: the threshold value; want: how many candidates equal to it are kept (the lowest indices).
+  // Each warp owns a run of the keys: it counts what it takes, then writes from its offset on.
   int* kept = p.kept + (static_cast<int64_t>(b) * p.kv.hkv + kh) * p.budget;
   float* w_out = p.w_out + (static_cast<int64_t>(b) * p.kv.hkv + kh) * p.cap_out;
-  int base = 0, ties = 0;
-  for (int j0 = 0; j0 < len; j0 += kSelThreads) {
-    const int j = j0 + tid;
-    bool take = false, tie = false;
-    float x = 0.f;
-    if (j < len) {
-      x = __ldg(w + j);
-      const uint32_t u = ordered_bits(x);
+  const int run = (len + kSelThreads - 1) / kSelThreads * 32;
+  const int beg = min(len, warp * run), end = min(len, beg + run);
+  auto flags = [&](int j, unsigned* take, unsigned* tie) {
+    bool a = false, e = false;
+    if (j < end) {
       const bool cand = j >= old_beg && j < old_end;
-      take = !cand || all || (need > 0 && u > prefix);
-      tie = cand && !all && need > 0 && u == prefix;
+      a = !cand || all;
+      if (cand && some) {
+        const uint32_t u = bits(j);
+        a = u > prefix, e = u == prefix;
+      }
     }
-    const unsigned mt = __ballot_sync(0xffffffffu, take), me = __ballot_sync(0xffffffffu, tie);
-    if (lane == 0) s_warp[0][warp] = __popc(mt), s_warp[1][warp] = __popc(me);
-    __syncthreads();
-    int take_before = 0, tie_before = 0, take_all = 0, tie_all = 0;
-    for (int i = 0; i < 32; ++i) {
-      const int a = s_warp[0][i], c = s_warp[1][i];
-      if (i < warp) take_before += a, tie_before += c;
-      take_all += a, tie_all += c;
-    }
-    const unsigned lt = (1u << lane) - 1;
-    const int my_ties = ties + tie_before + __popc(me & lt);
-    const int pos = base + take_before + __popc(mt & lt) + min(my_ties, want) - min(ties, want);
-    if (take || (tie && my_ties < want)) {
+    *take = __ballot_sync(0xffffffffu, a);
+    *tie = __ballot_sync(0xffffffffu, e);
+  };
+  int takes = 0, ties = 0;
+  for (int j0 = beg; j0 < end; j0 += 32) {
+    unsigned mt, me;
+    flags(j0 + lane, &mt, &me);
+    takes += __popc(mt), ties += __popc(me);
+  }
+  if (lane == 0) s_warp[0][warp] = takes, s_warp[1][warp] = ties;
+  __syncthreads();
+  int takes_before = 0, ties_before = 0;
+  for (int i = 0; i < warp; ++i) takes_before += s_warp[0][i], ties_before += s_warp[1][i];
+  const unsigned lt = (1u << lane) - 1;
+  for (int j0 = beg; j0 < end; j0 += 32) {
+    const int j = j0 + lane;
+    unsigned mt, me;
+    flags(j, &mt, &me);
+    const int my_ties = ties_before + __popc(me & lt);
+    if ((mt >> lane & 1) || ((me >> lane & 1) && my_ties < want)) {
+      const int pos = takes_before + __popc(mt & lt) + min(my_ties, want);
       kept[pos] = j;
-      w_out[pos] = x;
+      w_out[pos] = __ldg(w + j);
     }
-    base += take_all + min(ties + tie_all, want) - min(ties, want);
-    ties += tie_all;
-    __syncthreads();
+    takes_before += __popc(mt), ties_before += __popc(me);
   }
   for (int i = keep + tid; i < p.budget; i += kSelThreads) kept[i] = -1;
   for (int i = keep + tid; i < p.cap_out; i += kSelThreads) w_out[i] = 0.f;
@@ -222,14 +249,27 @@ __global__ void __launch_bounds__(kMoveThreads) fna2_evict_move_kernel(const Evi
 // second launch.
 constexpr int kFusedBudget = 512;
 
-inline cudaError_t launch_evict(const EvictParams& p, cudaStream_t stream) {
+// Weights whose ordered bits fit in shared memory beside the histogram.
+constexpr int kStagedKeys = 48 * 1024;
+
+template <bool MOVE>
+cudaError_t launch_evict_select(const EvictParams& p, cudaStream_t stream) {
   const dim3 heads(p.kv.hkv, p.B);
-  if (p.budget <= kFusedBudget) {
-    fna2_evict_select_kernel<true><<<heads, kSelThreads, 0, stream>>>(p);
-    return cudaGetLastError();
+  if (p.max_k <= kStagedKeys) {
+    auto kern = fna2_evict_select_kernel<MOVE, true>;
+    static std::atomic<uint64_t> allowed{0};
+    const cudaError_t e = allow_smem(reinterpret_cast<const void*>(kern), allowed, kStagedKeys * 4);
+    if (e != cudaSuccess) return e;
+    kern<<<heads, kSelThreads, p.max_k * 4, stream>>>(p);
+  } else {
+    fna2_evict_select_kernel<MOVE, false><<<heads, kSelThreads, 0, stream>>>(p);
   }
-  fna2_evict_select_kernel<false><<<heads, kSelThreads, 0, stream>>>(p);
-  cudaError_t e = cudaGetLastError();
+  return cudaGetLastError();
+}
+
+inline cudaError_t launch_evict(const EvictParams& p, cudaStream_t stream) {
+  if (p.budget <= kFusedBudget) return launch_evict_select<true>(p, stream);
+  const cudaError_t e = launch_evict_select<false>(p, stream);
   if (e != cudaSuccess) return e;
   return launch_dependent(fna2_evict_move_kernel, dim3((p.budget + kMoveRows - 1) / kMoveRows, p.kv.hkv, p.B),
                           kMoveThreads, 0, stream, p);

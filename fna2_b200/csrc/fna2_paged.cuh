@@ -111,15 +111,15 @@ cudaError_t launch_dependent(void (*kern)(P...), dim3 grid, int threads, size_t 
   return cudaLaunchKernelEx(&c, kern, static_cast<P>(args)...);
 }
 
-// Lets a kernel use all of the dynamic shared memory, once per device (`done`: a
+// Lets a kernel use all of the dynamic shared memory (or `bytes` of it), once per device (`done`: a
 // bit per device; the call costs about a microsecond, a small kernel takes five).
-inline cudaError_t allow_smem(const void* kern, std::atomic<uint64_t>& done) {
+inline cudaError_t allow_smem(const void* kern, std::atomic<uint64_t>& done, int bytes = kMaxDynamicSmem) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   const uint64_t bit = dev < 64 ? 1ull << dev : 0;
   if (bit && (done.load(std::memory_order_relaxed) & bit)) return cudaSuccess;
-  e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxDynamicSmem);
+  e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
   if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
   return e;
 }
