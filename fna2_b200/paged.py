@@ -302,3 +302,132 @@ def naylis_evict(key_weights: torch.Tensor, pool: PagedKV, page_table: torch.Ten
     if rc:
         _lib.check(rc, "fna2_evict")
     return kept, lens_out, w_out
+
+
+class NaylisPagedCache:
+    """The paged cache of one layer: a pool, and per batch slot its pages, length, next rotary
+    position and key weights.
+
+    Lengths are kept on the host (they follow from the calls) and on the device, so no call
+    waits for the device.  A slot's pages are taken from a free list as it grows; evict moves
+    what it keeps to fresh pages and returns the old ones.  All work is ordered by the current
+    stream; pages that are returned are reused by later calls on the same stream.
+
+        cache = NaylisPagedCache(pages, 64, batch, 32768, H, H_KV, D, graph_heads=H_G, rank=R)
+        q = cache.append(q, k, v, new, r_k, q_norm, k_norm, rope)     # new[b] tokens for slot b
+        out = cache.attend(q, r_q, graph_scale)                       # the tokens just appended
+        cache.evict(budget=4096, recent=256, sink=4)
+    """
+
+    def __init__(self, num_pages: int, page_size: int, batch: int, max_len: int, heads: int, kv_heads: int,
+                 head_dim: int, graph_heads: int = 0, rank: int = 16, key_weights: bool = True, device="cuda"):
+        def pages(h, c):
+            return torch.zeros(num_pages, page_size, h, c, device=device, dtype=torch.bfloat16)
+        self.pool = PagedKV(pages(kv_heads, head_dim), pages(kv_heads, head_dim),
+                            pages(graph_heads, rank) if graph_heads else None)
+        self.heads, self.batch, self.page_size = heads, batch, page_size
+        self.max_pages = -(-max_len // page_size)
+        dev = self.pool.device
+        self.page_table = torch.full((batch, self.max_pages), -1, dtype=torch.int32, device=dev)
+        self.seqlens = torch.zeros(batch, dtype=torch.int32, device=dev)
+        self.positions = torch.zeros(batch, dtype=torch.int32, device=dev)
+        self.key_weights = (torch.zeros(batch, kv_heads, self.max_pages * page_size, device=dev) if key_weights
+                            else None)
+        self.lengths: List[int] = [0] * batch
+        self._pages: List[List[int]] = [[] for _ in range(batch)]
+        self._free = list(range(num_pages))[::-1]
+        self._new: List[int] = [0] * batch
+        self._cu = torch.zeros(batch + 1, dtype=torch.int32, device=dev)
+        self._one_each = torch.arange(batch + 1, dtype=torch.int32, device=dev)
+
+    @property
+    def free_pages(self) -> int:
+        return len(self._free)
+
+    def _take(self, n: int) -> List[int]:
+        if n > len(self._free):
+            raise RuntimeError(f"the pool has {len(self._free)} free pages, {n} are needed")
+        taken, self._free = self._free[len(self._free) - n:], self._free[:len(self._free) - n]
+        return taken[::-1]
+
+    def _grow(self, new: Sequence[int]) -> None:
+        """Pages for new[b] more tokens of each slot."""
+        need = [-(-(n + m) // self.page_size) - len(p) for n, m, p in zip(self.lengths, new, self._pages)]
+        for b, (n, m) in enumerate(zip(self.lengths, new)):
+            _want(m >= 0 and -(-(n + m) // self.page_size) <= self.max_pages,
+                  f"slot {b}: {n} + {m} tokens do not fit its {self.max_pages} pages")
+        taken = self._take(sum(max(0, x) for x in need))
+        at = 0
+        for b, x in enumerate(need):
+            if x > 0:
+                first = len(self._pages[b])
+                self._pages[b] += taken[at:at + x]
+                self.page_table[b, first:first + x] = torch.tensor(taken[at:at + x], dtype=torch.int32)
+                at += x
+
+    def append(self, q, k, v, new: Sequence[int], r_k=None, q_norm=None, k_norm=None, rope=None) -> torch.Tensor:
+        """new[b] new tokens of every slot b (0 for none), packed in slot order: q, k through the
+        norms and the rotary embedding, k, v, r_k into the pages (qk_norm_rope_append).  Returns
+        q for attend()."""
+        new = [int(n) for n in new]
+        _want(len(new) == self.batch and sum(new) == q.shape[0], "new must give the tokens of every slot")
+        self._grow(new)
+        ones = all(n == 1 for n in new)
+        if ones:
+            self._cu = self._one_each
+        else:
+            cu = [0]
+            for n in new:
+                cu.append(cu[-1] + n)
+            self._cu = torch.tensor(cu, dtype=torch.int32).to(self.pool.device, non_blocking=True)
+        out = qk_norm_rope_append(q, k, v, self.pool, self.page_table, self.seqlens, self._cu, r_k, self.positions,
+                                  q_norm, k_norm, rope)
+        added = 1 if ones else self._cu[1:] - self._cu[:-1]
+        self.seqlens += added
+        self.positions += added
+        self.lengths = [a + b for a, b in zip(self.lengths, new)]
+        self._new = new
+        return out
+
+    def attend(self, q, r_q=None, graph_scale=None, softmax_scale=None, weigh: bool = True, return_lse: bool = False):
+        """Attention of the tokens of the last append over their slots' keys (flash_naylis_paged);
+        weigh: add the attention weights to key_weights."""
+        return flash_naylis_paged(q, self.pool, self.page_table, self.seqlens, self._cu, max(self._new), r_q,
+                                  graph_scale, softmax_scale, True, self.key_weights if weigh else None, return_lse,
+                                  max(self.lengths))
+
+    def evict(self, budget: int, recent: int = 0, sink: int = 0) -> List[int]:
+        """Cut every slot with more than `budget` keys to `budget` (naylis_evict).  Rotary positions
+        go on from where they were.  Returns the slots that were cut."""
+        _want(self.key_weights is not None, "evict needs a cache with key weights")
+        over = [b for b, n in enumerate(self.lengths) if n > budget]
+        if not over:
+            return over
+        per = -(-budget // self.page_size)
+        fresh = self._take(per * len(over))
+        rows = [fresh[i * per:(i + 1) * per] for i in range(len(over))]
+        dev = self.pool.device
+        idx = torch.tensor(over, device=dev)
+        table_out = torch.tensor(rows, dtype=torch.int32, device=dev)
+        _, lens, w = naylis_evict(self.key_weights[idx], self.pool, self.page_table[idx], self.seqlens[idx], budget,
+                                  table_out, self.heads, recent, sink, max(self.lengths))
+        self.page_table[idx] = -1
+        self.page_table[idx, :per] = table_out
+        self.seqlens[idx] = lens
+        self.key_weights[idx] = 0.0
+        self.key_weights[idx, :, :w.shape[2]] = w
+        for b, row in zip(over, rows):
+            self._free += self._pages[b]
+            self._pages[b] = list(row)
+            self.lengths[b] = budget
+        return over
+
+    def release(self, slot: int) -> None:
+        """Empty a slot; its pages go back to the pool."""
+        self._free += self._pages[slot]
+        self._pages[slot], self.lengths[slot], self._new[slot] = [], 0, 0
+        self.page_table[slot] = -1
+        self.seqlens[slot] = 0
+        self.positions[slot] = 0
+        if self.key_weights is not None:
+            self.key_weights[slot] = 0.0
