@@ -319,6 +319,14 @@ __global__ void __launch_bounds__(kKwThreads, 1)
     constexpr uint32_t r_layout = RP == 16 ? kSwizzle32B : kSwizzle64B;
     constexpr uint32_t r_sbo = 8 * RP * 2;
     const bool issuer = warp == 9;
+    // operand descriptors at their first stage; others differ in the address field only (bytes / 16)
+    const uint32_t s0 = smem_u32(smem);
+    const uint64_t dK0 = make_sdesc(s0 + L::oK, 16, 1024, kSwizzle128B);
+    const uint64_t dQ0 = make_sdesc(s0 + L::oStage + L::sQ, 16, 1024, kSwizzle128B);
+    const uint64_t dOne = make_sdesc(s0 + L::oOne, 16, 256, kSwizzle32B);
+    const uint64_t dL0 = make_sdesc(s0 + L::oStage + L::sL, 16, 256, kSwizzle32B);
+    const uint64_t dRk0 = make_sdesc(s0 + L::oRk, 16, r_sbo, r_layout);
+    const uint64_t dRq0 = make_sdesc(s0 + L::oStage + L::sRq, 16, r_sbo, r_layout);
     int gu = 0, rs = 1, used[2] = {};
     bool ok = true;
     for (int n = 0; ok; ++n) {
@@ -331,7 +339,6 @@ __global__ void __launch_bounds__(kKwThreads, 1)
       for (int u = 0; ok && u < n_units; ++u, ++gu) {
         const int s = gu & 1;
         const bool graph = kh * p.G + u / per_head < p.kv.hg;
-        const uint32_t st = smem_u32(smem + L::oStage + s * L::kStage);
         if (u % per_head == 0) rs ^= 1;
         if (!issuer) ok = mbar_wait(&bars[kWbFull + s], (gu >> 1) & 1, abort_flag, 222);
 #pragma unroll
@@ -347,22 +354,19 @@ __global__ void __launch_bounds__(kKwThreads, 1)
           tc_fence_after();
           if (elect_one()) {
             const uint32_t tS = tmem + 128 * buf;
-            const uint32_t sK = smem_u32(smem + L::oK + i * L::kTile);
+            const uint64_t dK = dK0 + (i * L::kTile >> 4), dQ = dQ0 + (s * L::kStage >> 4);
 #pragma unroll
             for (int kk = 0; kk < D / 16; ++kk) {
-              const uint32_t off = (kk >> 2) * L::kChunk + (kk & 3) * 32;
-              mma_ss(tS, make_sdesc(sK + off, 16, 1024, kSwizzle128B),
-                     make_sdesc(st + L::sQ + off, 16, 1024, kSwizzle128B), idesc, kk > 0);
+              const uint32_t off = ((kk >> 2) * L::kChunk + (kk & 3) * 32) >> 4;
+              mma_ss(tS, dK + off, dQ + off, idesc, kk > 0);
             }
-            mma_ss(tS, make_sdesc(smem_u32(smem + L::oOne), 16, 256, kSwizzle32B),
-                   make_sdesc(st + L::sL, 16, 256, kSwizzle32B), idesc, 1);
+            mma_ss(tS, dOne, dL0 + (s * L::kStage >> 4), idesc, 1);
             if (graph) {
-              const uint32_t sRk = smem_u32(smem + L::oRk + (2 * rs + i) * L::kRTile);
+              const uint64_t dRk = dRk0 + ((2 * rs + i) * L::kRTile >> 4), dRq = dRq0 + (s * L::kStage >> 4);
 #pragma unroll
               for (int kk = 0; kk < RP / 16; ++kk) {
-                const uint64_t rk = make_sdesc(sRk + kk * 32, 16, r_sbo, r_layout);
-                mma_ss(tS, rk, make_sdesc(st + L::sRq + kk * 32, 16, r_sbo, r_layout), idesc, 1);
-                mma_ss(tS, rk, make_sdesc(st + L::sRq + L::kRTile + kk * 32, 16, r_sbo, r_layout), idesc, 1);
+                mma_ss(tS, dRk + kk * 2, dRq + kk * 2, idesc, 1);
+                mma_ss(tS, dRk + kk * 2, dRq + (L::kRTile >> 4) + kk * 2, idesc, 1);
               }
             }
             mma_commit(&bars[kWbSFull + buf]);
@@ -581,6 +585,14 @@ __global__ void __launch_bounds__(kKwThreads, 1)
     constexpr uint32_t r_layout = RP == 16 ? kSwizzle32B : kSwizzle64B;
     constexpr uint32_t r_sbo = 8 * RP * 2;
     const bool issuer = warp == 9;
+    // operand descriptors at their first place; others differ in the address field only (bytes / 16)
+    const uint32_t s0 = smem_u32(smem);
+    const uint64_t dK0 = make_sdesc(s0 + L::oK, 16, 1024, kSwizzle128B);
+    const uint64_t dQ0 = make_sdesc(s0 + L::oQ, 16, 1024, kSwizzle128B);
+    const uint64_t dOne = make_sdesc(s0 + L::oOne, 16, 256, kSwizzle32B);
+    const uint64_t dL0 = make_sdesc(s0 + L::oQ + L::sL, 16, 256, kSwizzle32B);
+    const uint64_t dRk0 = make_sdesc(s0 + L::oK + L::kTile, 16, r_sbo, r_layout);
+    const uint64_t dRq0 = make_sdesc(s0 + L::oQ + L::sRq, 16, r_sbo, r_layout);
     int gt = 0, used = 0;
     bool ok = true;
     for (int n = 0; ok; ++n) {
@@ -591,7 +603,6 @@ __global__ void __launch_bounds__(kKwThreads, 1)
       if (tiles < 0) break;
       for (int t = 0; ok && t < tiles; ++t, ++gt) {
         const int s = gt & 1;
-        const uint32_t sK = smem_u32(smem + L::oK + s * L::kStage);
         if (!issuer) ok = mbar_wait(&bars[kVbFull + s], (gt >> 1) & 1, abort_flag, 226);
 #pragma unroll
         for (int u = 0; u < L::kPairs; ++u) {
@@ -605,25 +616,22 @@ __global__ void __launch_bounds__(kKwThreads, 1)
           tc_fence_after();
           if (elect_one()) {
             const uint32_t tS = tmem + 128 * buf;
-            const uint32_t sQ = smem_u32(smem + L::oQ + u * L::kPair);
+            const uint64_t dK = dK0 + (s * L::kStage >> 4), dQ = dQ0 + (u * L::kPair >> 4);
 #pragma unroll
             for (int kk = 0; kk < D / 16; ++kk) {
-              const uint32_t off = (kk >> 2) * L::kChunk + (kk & 3) * 32;
-              mma_ss(tS, make_sdesc(sK + off, 16, 1024, kSwizzle128B), make_sdesc(sQ + off, 16, 1024, kSwizzle128B), idesc,
-                     kk > 0);
+              const uint32_t off = ((kk >> 2) * L::kChunk + (kk & 3) * 32) >> 4;
+              mma_ss(tS, dK + off, dQ + off, idesc, kk > 0);
             }
-            mma_ss(tS, make_sdesc(smem_u32(smem + L::oOne), 16, 256, kSwizzle32B),
-                   make_sdesc(sQ + L::sL, 16, 256, kSwizzle32B), idesc, 1);
+            mma_ss(tS, dOne, dL0 + (u * L::kPair >> 4), idesc, 1);
 #pragma unroll
             for (int g = 0; g < 2; ++g) {
               if (2 * u + g >= heads || h0 + 2 * u + g >= p.kv.hg) continue;
-              const uint32_t sRk = sK + L::kTile + (2 * u + g) * L::kRTile;
+              const uint64_t dRk = dRk0 + ((s * L::kStage + (2 * u + g) * L::kRTile) >> 4);
+              const uint64_t dRq = dRq0 + ((u * L::kPair + g * QT * RP * 2) >> 4);
 #pragma unroll
               for (int kk = 0; kk < RP / 16; ++kk) {
-                const uint32_t hi = sQ + L::sRq + g * QT * RP * 2 + kk * 32;
-                const uint64_t rk = make_sdesc(sRk + kk * 32, 16, r_sbo, r_layout);
-                mma_ss(tS + g * QT, rk, make_sdesc(hi, 16, r_sbo, r_layout), idesc_r, 1);
-                mma_ss(tS + g * QT, rk, make_sdesc(hi + L::kRTile, 16, r_sbo, r_layout), idesc_r, 1);
+                mma_ss(tS + g * QT, dRk + kk * 2, dRq + kk * 2, idesc_r, 1);
+                mma_ss(tS + g * QT, dRk + kk * 2, dRq + (L::kRTile >> 4) + kk * 2, idesc_r, 1);
               }
             }
             mma_commit(&bars[kVbSFull + buf]);
