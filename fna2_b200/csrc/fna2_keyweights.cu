@@ -46,8 +46,8 @@ struct KeyWeightsParams {
   float* kw;
   int64_t kw_sb, kw_sh;
   __nv_bfloat16* rq2;  // workspace: [T][H][2 RP + 16]: R~_q hi, lo (graph heads), -LSE/scale as three terms
-  int* next;           // workspace: item counter, zeroed by the prep kernel
-  int run_tiles;       // key tiles per item
+  int* next;           // workspace: item counter, set to ctas (whose first items are their own index) by the prep kernel
+  int ctas;
 };
 
 // R~_q = gs/scale * R_q as hi + lo, columns [rank, RP) zero, and -LSE/scale = l1 + l2 + l3 (a row
@@ -55,7 +55,7 @@ struct KeyWeightsParams {
 __global__ void __launch_bounds__(256) fna2_key_weights_prep_kernel(const KeyWeightsParams p) {
   pdl_trigger();
   const int64_t e = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  if (e == 0) *p.next = 0;
+  if (e == 0) *p.next = p.ctas;
   const int r8 = p.RP / 8, per = r8 + 1;  // pieces of a row: R_q's, then the LSE's
   if (e >= static_cast<int64_t>(p.bd.T) * p.H * per) return;
   const int x = static_cast<int>(e % per), h = static_cast<int>(e / per % p.H);
@@ -77,7 +77,8 @@ __global__ void __launch_bounds__(256) fna2_key_weights_prep_kernel(const KeyWei
   }
 }
 
-constexpr int kKwThreads = 352;
+constexpr int kKwThreads = 640;
+constexpr int kKwProducer = 16, kKwIssuer = 17, kKwWaiter = 18;  // warps after the sums; then the one that stores
 
 template <int D, int RP>
 struct KwSmem {
@@ -91,7 +92,8 @@ struct KwSmem {
   static constexpr int kStage = sL + kLTile;
   static constexpr int oRk = oStage + 2 * kStage;      // 2 x R_k of key tiles 0, 1 and the unit's head
   static constexpr int oOne = oRk + 2 * 2 * kRTile;
-  static constexpr int oBar = oOne + kLTile;
+  static constexpr int oPart = oOne + kLTile;          // sums of warpgroup i of key tile i % 2
+  static constexpr int oBar = oPart + 4 * 512;
   static constexpr int oMisc = oBar + 32 * 8;
   static constexpr int oItem = oMisc + 16;
   static constexpr int kUsed = oItem + 64;
@@ -102,7 +104,9 @@ struct KwSmem {
 
 enum KwBar {
   kWbKFull = 0,    // K and the item's description
-  kWbKEmpty = 1,   // its MMAs are done, every sum warp has left the item (1 + 8 arrivals)
+  kWbKEmpty = 1,   // its MMAs are done, every warp has read its description (1 + 17 arrivals)
+  kWbPFull = 2,    // the item's sums (16 arrivals)
+  kWbPEmpty = 3,
   kWbFull = 4,     // +stage: the unit's operands
   kWbEmpty = 6,    // +stage: MMAs that read it are done
   kWbSFull = 8,    // +2 tile + buffer
@@ -168,19 +172,19 @@ __device__ __forceinline__ void kw_write_ones(uint8_t* dst) {
 template <int QT, bool MASK>
 __device__ __forceinline__ float kw_sum(uint32_t t_addr, float2 sl2, int lo, int hi) {
   float2 a[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-  uint32_t r[2][32];
-  tmem_ld32(t_addr, r[0]);
+  uint32_t r[2][16];
+  tmem_ld16(t_addr, r[0]);
 #pragma unroll
-  for (int c = 0; c < QT / 32; ++c) {
+  for (int c = 0; c < QT / 16; ++c) {
     uint32_t* x = r[c & 1];
-    tmem_ld_wait32(x);
-    if (c + 1 < QT / 32) tmem_ld32(t_addr + 32 * (c + 1), r[(c + 1) & 1]);
+    tmem_ld_wait16(x);
+    if (c + 1 < QT / 16) tmem_ld16(t_addr + 16 * (c + 1), r[(c + 1) & 1]);
 #pragma unroll
-    for (int k = 0; k < 32; k += 2) {
+    for (int k = 0; k < 16; k += 2) {
       const float2 y = __fmul2_rn(f32x2(x[k], x[k + 1]), sl2);
       float2 e = make_float2(ex2(y.x), ex2(y.y));
       if (MASK) {
-        const int col = 32 * c + k;
+        const int col = 16 * c + k;
         e.x = col >= lo && col < hi ? e.x : 0.f;
         e.y = col + 1 >= lo && col + 1 < hi ? e.y : 0.f;
       }
@@ -207,7 +211,9 @@ __global__ void __launch_bounds__(kKwThreads, 1)
 
   if (tid == 0) {
     mbar_init(&bars[kWbKFull], 1);
-    mbar_init(&bars[kWbKEmpty], 9);
+    mbar_init(&bars[kWbKEmpty], 18);
+    mbar_init(&bars[kWbPFull], 16);
+    mbar_init(&bars[kWbPEmpty], 1);
     for (int s = 0; s < 2; ++s) {
       mbar_init(&bars[kWbFull + s], 1);
       mbar_init(&bars[kWbEmpty + s], 1);
@@ -220,7 +226,7 @@ __global__ void __launch_bounds__(kKwThreads, 1)
     fence_mbar_init();
   }
   kw_write_ones(smem + L::oOne);
-  if (warp == 9) {
+  if (warp == kKwIssuer) {
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
@@ -228,9 +234,8 @@ __global__ void __launch_bounds__(kKwThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  pdl_wait();
 
-  if (warp == 8) {
+  if (warp == kKwProducer) {
     // ------------------------------------------------------------ producer
     if (lane == 0) {
       tma_prefetch_desc(&tmQ);
@@ -251,7 +256,7 @@ __global__ void __launch_bounds__(kKwThreads, 1)
                  ? __ldg(p.kv.table + it.b * p.kv.table_sb + (key >> lg))
                  : -1;
     };
-    KwItem it = draw(), next = it;
+    KwItem it = kw_item(p, blockIdx.x, 2 * kBlockN, lane), next = it;
     int page = page_of(it), next_page = -1;
     int gu = 0, rs = 1;  // units so far, R_k slot
     for (int n = 0;; ++n) {
@@ -275,6 +280,7 @@ __global__ void __launch_bounds__(kKwThreads, 1)
                       &bars[kWbKFull], c * 64, key & mask, it.kh, page);
       }
       __syncwarp();
+      if (n == 0) pdl_wait();  // the prep kernel writes nothing of what was read so far
       auto fetch = [&]() {
         next = draw();
         next_page = page_of(next);
@@ -313,12 +319,12 @@ __global__ void __launch_bounds__(kKwThreads, 1)
       if (!ok) break;
       it = next, page = next_page;
     }
-  } else if (warp >= 9) {
-    // ------------------------------------------------------------ MMA issuer (9) and its waiter (10)
+  } else if (warp == kKwIssuer || warp == kKwWaiter) {
+    // ------------------------------------------------------------ MMA issuer and its waiter
     constexpr uint32_t idesc = make_idesc_bf16(kBlockN, 128, 0, 0);
     constexpr uint32_t r_layout = RP == 16 ? kSwizzle32B : kSwizzle64B;
     constexpr uint32_t r_sbo = 8 * RP * 2;
-    const bool issuer = warp == 9;
+    const bool issuer = warp == kKwIssuer;
     // operand descriptors at their first stage; others differ in the address field only (bytes / 16)
     const uint32_t s0 = smem_u32(smem);
     const uint64_t dK0 = make_sdesc(s0 + L::oK, 16, 1024, kSwizzle128B);
@@ -340,19 +346,19 @@ __global__ void __launch_bounds__(kKwThreads, 1)
         const int s = gu & 1;
         const bool graph = kh * p.G + u / per_head < p.kv.hg;
         if (u % per_head == 0) rs ^= 1;
-        if (!issuer) ok = mbar_wait(&bars[kWbFull + s], (gu >> 1) & 1, abort_flag, 222);
+        if (!issuer) {
+          ok = mbar_wait(&bars[kWbFull + s], (gu >> 1) & 1, abort_flag, 222);
+          for (int i = 0; ok && i < tiles; ++i)
+            ok = used[i] < 2 || mbar_wait(&bars[kWbSEmpty + 2 * i + used[i] % 2], (used[i] / 2 - 1) & 1, abort_flag, 223);
+        }
+        ok = pair_rendezvous(1, ok);
+        if (!ok) break;
+        if (issuer) tc_fence_after();
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           if (i >= tiles) continue;
-          const int buf = 2 * i + used[i] % 2;
-          if (!issuer && ok && used[i] >= 2)
-            ok = mbar_wait(&bars[kWbSEmpty + buf], (used[i] / 2 - 1) & 1, abort_flag, 223);
-          ++used[i];
-          ok = pair_rendezvous(1, ok);
-          if (!ok) break;
-          if (!issuer) continue;
-          tc_fence_after();
-          if (elect_one()) {
+          const int buf = 2 * i + used[i]++ % 2;
+          if (issuer && elect_one()) {
             const uint32_t tS = tmem + 128 * buf;
             const uint64_t dK = dK0 + (i * L::kTile >> 4), dQ = dQ0 + (s * L::kStage >> 4);
 #pragma unroll
@@ -372,56 +378,76 @@ __global__ void __launch_bounds__(kKwThreads, 1)
             mma_commit(&bars[kWbSFull + buf]);
             if (i == tiles - 1) mma_commit(&bars[kWbEmpty + s]);
           }
-          __syncwarp();
         }
+        __syncwarp();
       }
       if (ok && issuer && elect_one()) mma_commit(&bars[kWbKEmpty]);
       __syncwarp();
     }
-  } else {
-    // ------------------------------------------------------------ sums
-    const int wi = warp >> 2;
-    const uint32_t t_lane = tmem + 256 * wi + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+  } else if (warp < kKwProducer) {
+    // ------------------------------------------------------------ sums: warpgroup i, key tile i % 2, every second unit
+    const int wi = warp >> 2 & 1, half = warp >> 3;
+    const int buf = 2 * wi + half;
+    const uint32_t at = tmem + 128 * buf + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+    float* part = reinterpret_cast<float*>(smem + L::oPart) + (warp >> 2) * 128 + (tid & 127);
     const float2 sl2 = make_float2(p.scale_log2, p.scale_log2);
-    int used = 0;
+    int used = 0;  // units of this key tile so far
     bool ok = true;
     for (int n = 0; ok; ++n) {
       if (!mbar_wait(&bars[kWbKFull], n & 1, abort_flag, 320)) break;
       const int n_units = items[0].n_units, per_head = items[0].per_head, u0 = items[0].u0, nq = items[0].n;
       const int len = items[0].len, tile0 = items[0].k0 + wi * kBlockN, j = tile0 + (tid & 127), past = len - nq;
-      if (n_units < 0) break;
-      const bool mine = tile0 < len;  // this key tile has keys
-      float* dst = p.kw + items[0].b * p.kw_sb + items[0].kh * p.kw_sh + j;
-      float w = mine && j < len ? *dst : 0.f;
-      for (int u = 0; u < n_units; ++u) {
-        const int buf = 2 * wi + used % 2;
-        if (!mine) continue;
-        if (!mbar_wait(&bars[kWbSFull + buf], (used / 2) & 1, abort_flag, 322)) {
-          ok = false;
-          break;
-        }
-        tc_fence_after();
-        const int i0 = (u0 + u % per_head) * QT;
-        // columns [first, nq - i0) belong to queries that see the key; the score of another sequence's
-        // query is never read into a sum
-        const int first = p.causal ? j - past - i0 : 0;
-        const bool whole = (!p.causal || tile0 + kBlockN - 1 <= past + i0) && i0 + QT <= nq;
-        const uint32_t at = t_lane + 128 * (used % 2);
-        w += whole ? kw_sum<QT, false>(at, sl2, 0, 0) : kw_sum<QT, true>(at, sl2, first, nq - i0);
-        ++used;
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&bars[kWbSEmpty + buf]);
-      }
-      if (ok && mine && j < len) *dst = w;
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars[kWbKEmpty]);
+      if (n_units < 0) break;
+      float w = 0.f;
+      if (tile0 < len) {  // this key tile has keys
+        for (int u = (half ^ used) & 1; u < n_units; u += 2) {
+          if (!(ok = mbar_wait(&bars[kWbSFull + buf], ((used + u) >> 1) & 1, abort_flag, 322))) break;
+          tc_fence_after();
+          const int i0 = (u0 + u % per_head) * QT;
+          // columns [first, nq - i0) belong to queries that see the key; the score of another sequence's
+          // query is never read into a sum
+          const int first = p.causal ? j - past - i0 : 0;
+          const bool whole = (!p.causal || tile0 + kBlockN - 1 <= past + i0) && i0 + QT <= nq;
+          w += whole ? kw_sum<QT, false>(at, sl2, 0, 0) : kw_sum<QT, true>(at, sl2, first, nq - i0);
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bars[kWbSEmpty + buf]);
+        }
+        used += n_units;
+      }
+      if (!ok || (n > 0 && !mbar_wait(&bars[kWbPEmpty], (n - 1) & 1, abort_flag, 323))) break;
+      *part = w;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars[kWbPFull]);
+    }
+  } else {
+    // ------------------------------------------------------------ adds the warpgroups' sums and stores
+    const float* part = reinterpret_cast<const float*>(smem + L::oPart) + lane;
+    for (int n = 0;; ++n) {
+      if (!mbar_wait(&bars[kWbKFull], n & 1, abort_flag, 330)) break;
+      const int left = items[0].len - items[0].k0 - lane, n_units = items[0].n_units;
+      float* dst = p.kw + items[0].b * p.kw_sb + items[0].kh * p.kw_sh + items[0].k0 + lane;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars[kWbKEmpty]);
+      if (n_units < 0) break;
+      float w[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) w[k] = 32 * k < left ? dst[32 * k] : 0.f;
+      if (!mbar_wait(&bars[kWbPFull], n & 1, abort_flag, 331)) break;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        if (32 * k < left) dst[32 * k] = w[k] + (part[32 * k] + part[256 + 32 * k]);
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars[kWbPEmpty]);
     }
   }
 
   tc_fence_before();
   __syncthreads();
-  if (warp == 9) {
+  if (warp == kKwIssuer) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
@@ -443,8 +469,8 @@ struct KwwSmem {
   static constexpr int oK = oQ + kPairs * kPair;               // 2 x [K | R_k of each head]
   static constexpr int kStage = kTile + kHeads * kRTile;
   static constexpr int oOne = oK + 2 * kStage;
-  static constexpr int oPart = oOne + kLTile;                  // 2 x warpgroup 1's sums
-  static constexpr int oBar = oPart + 2 * 512;
+  static constexpr int oPart = oOne + kLTile;                  // 2 x sums of four warpgroups
+  static constexpr int oBar = oPart + 2 * 4 * 512;
   static constexpr int oMisc = oBar + 32 * 8;
   static constexpr int oItem = oMisc + 16;
   static constexpr int kUsed = oItem + 64;
@@ -455,19 +481,66 @@ struct KwwSmem {
 
 enum KwwBar {
   kVbQFull = 0,    // the queries and the step's description
-  kVbQEmpty = 1,   // the step's MMAs are done, every sum warp has read its description (1 + 8 arrivals)
+  kVbQEmpty = 1,   // the step's MMAs are done, every warp has read its description (1 + 17 arrivals)
   kVbFull = 2,     // +stage: K and R_k of a key tile
   kVbEmpty = 4,    // +stage
   kVbSFull = 6,    // +buffer
   kVbSEmpty = 10,  // +buffer (8 arrivals)
-  kVbPFull = 14,   // +tile parity: warpgroup 1's sums (4 arrivals)
-  kVbPEmpty = 16,  // +tile parity (4 arrivals)
+  kVbPFull = 14,   // +tile parity: the key tile's sums (16 arrivals)
+  kVbPEmpty = 16,  // +tile parity
 };
 
 // A step: `tiles` key tiles from key k0 on against heads [h0, h0 + heads) of one KV head.
 struct KwwStep {
   int b, kh, k0, len, n, tiles, h0, heads;  // tiles < 0: no more steps
 };
+
+// Up to `most` key tiles of one KV head from position `at` on, in the order: sequences, blocks of key tiles, KV
+// heads, key tiles (the KV heads of the same keys at about the same time: a token's heads lie together).  Blocks of
+// a sequence are equal, of `block` key tiles or a few more, so that a run meets few of them.
+// Called by a whole warp.
+struct KwwRun {
+  int b, kh, k0, len, n, q0, tiles;
+};
+
+__device__ __forceinline__ KwwRun kww_run(const KeyWeightsParams& p, int at, int most, int block, int lane) {
+  KwwRun it{};
+  int carry = 0;
+  for (int base = 0; base < p.bd.B; base += 32) {
+    const int b = base + lane;
+    PagedSeq s{0, 0, 0, false};
+    int cnt = 0;
+    if (b < p.bd.B) {
+      s = paged_seq(p.bd, b);
+      if (s.n > 0) cnt = (s.len + kBlockN - 1) / kBlockN * p.kv.hkv;
+    }
+    int incl = cnt;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += u;
+    }
+    const unsigned hit = __ballot_sync(0xffffffffu, at < carry + incl);
+    if (hit) {
+      const int src = __ffs(hit) - 1;
+      const int local = at - carry - (__shfl_sync(0xffffffffu, incl, src) - __shfl_sync(0xffffffffu, cnt, src));
+      it.b = base + src;
+      it.len = __shfl_sync(0xffffffffu, s.len, src);
+      it.n = __shfl_sync(0xffffffffu, s.n, src);
+      it.q0 = __shfl_sync(0xffffffffu, s.q0, src);
+      const int tiles = (it.len + kBlockN - 1) / kBlockN, blocks = max(1, tiles / block);
+      const int blk = ((local / p.kv.hkv + 1) * static_cast<int64_t>(blocks) - 1) / tiles;
+      const int first = static_cast<int64_t>(blk) * tiles / blocks, in = local - first * p.kv.hkv;
+      const int size = static_cast<int>((blk + 1ll) * tiles / blocks) - first;
+      it.kh = in / size;
+      it.k0 = (first + in % size) * kBlockN;
+      it.tiles = min(most, size - in % size);
+      return it;
+    }
+    carry += __shfl_sync(0xffffffffu, incl, 31);
+  }
+  return it;
+}
 
 template <int D, int RP>
 __global__ void __launch_bounds__(kKwThreads, 1)
@@ -486,12 +559,12 @@ __global__ void __launch_bounds__(kKwThreads, 1)
 
   if (tid == 0) {
     mbar_init(&bars[kVbQFull], 1);
-    mbar_init(&bars[kVbQEmpty], 9);
+    mbar_init(&bars[kVbQEmpty], 18);
     for (int s = 0; s < 2; ++s) {
       mbar_init(&bars[kVbFull + s], 1);
       mbar_init(&bars[kVbEmpty + s], 1);
-      mbar_init(&bars[kVbPFull + s], 4);
-      mbar_init(&bars[kVbPEmpty + s], 4);
+      mbar_init(&bars[kVbPFull + s], 16);
+      mbar_init(&bars[kVbPEmpty + s], 1);
     }
     for (int s = 0; s < NB; ++s) {
       mbar_init(&bars[kVbSFull + s], 1);
@@ -501,7 +574,7 @@ __global__ void __launch_bounds__(kKwThreads, 1)
     fence_mbar_init();
   }
   kw_write_ones(smem + L::oOne);
-  if (warp == 9) {
+  if (warp == kKwIssuer) {
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
@@ -509,9 +582,8 @@ __global__ void __launch_bounds__(kKwThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  pdl_wait();
 
-  if (warp == 8) {
+  if (warp == kKwProducer) {
     // ------------------------------------------------------------ producer
     if (lane == 0) {
       tma_prefetch_desc(&tmQ);
@@ -519,45 +591,34 @@ __global__ void __launch_bounds__(kKwThreads, 1)
     }
     const int lg = p.kv.page_log2, mask = (1 << lg) - 1;
     const int bk = min(1 << lg, kBlockN), row = lane * bk;  // lane l owns box l of a key tile (at most 8)
-    auto draw = [&]() {
-      int idx = 0;
-      if (lane == 0) idx = atomicAdd(p.next, 1);
-      return kw_item(p, __shfl_sync(0xffffffffu, idx, 0), p.run_tiles * kBlockN, lane);
-    };
-    KwItem it = draw(), next = it;
+    int total = 0;  // key tiles of all KV heads
+    for (int base = 0; base < p.bd.B; base += 32) {
+      int cnt = 0;
+      if (base + lane < p.bd.B) {
+        const PagedSeq s = paged_seq(p.bd, base + lane);
+        if (!s.ok) atomicCAS(&g_device_error, 0, kStatusBadSeqPaged);
+        if (s.n > 0) cnt = (s.len + kBlockN - 1) / kBlockN * p.kv.hkv;
+      }
+      total += __reduce_add_sync(0xffffffffu, cnt);
+    }
+    const int C = static_cast<int>(gridDim.x), c = static_cast<int>(blockIdx.x), run = total / C, more = total % C;
+    int at = c * run + min(c, more);
+    const int end = at + run + (c < more);
     int gt = 0;  // key tiles so far
     bool ok = true;
     for (int n = 0; ok; ++n) {
-      const bool last = it.n_units < 0;
-      const int tiles = last ? -1 : min(p.run_tiles, (it.len - it.k0 + kBlockN - 1) / kBlockN);
+      const bool last = at == end;
+      KwwRun it;
+      if (!last) it = kww_run(p, at, end - at, run + (more > 0), lane);
+      const int tiles = last ? -1 : it.tiles;
       for (int g0 = 0; ok && g0 < p.G; g0 += L::kHeads) {
         const int h0 = it.kh * p.G + g0, nh = min(L::kHeads, p.G - g0), ng = max(0, min(nh, p.kv.hg - h0));
-        const bool free = n == 0 || mbar_wait(&bars[kVbQEmpty], (n - 1) & 1, abort_flag, 125);
-        if (!(ok = __all_sync(0xffffffffu, free))) break;
-        if (lane == 0) {  // (the arrival also publishes the description)
-          step->b = it.b, step->kh = it.kh, step->k0 = it.k0, step->len = it.len, step->n = it.n, step->tiles = tiles;
-          step->h0 = h0, step->heads = nh;
-          mbar_expect_tx(&bars[kVbQFull], last ? 0 : QT * (nh * (D + 16) + ng * 2 * RP) * 2);
-        }
-        __syncwarp();
-        if (last) break;
-        // lane 8 g + x of head g: x = 0, 1: Q chunks; 2, 3: R~_q hi, lo; 4: LSE
-        const int g = lane / 8, x = lane % 8;
-        if (g < nh && (x < D / 64 || x == 4 || (x / 2 == 1 && g < ng))) {
-          uint8_t* dst = smem + L::oQ + g / 2 * L::kPair +
-                         (x < D / 64 ? x * L::kChunk + g % 2 * QT * 128
-                          : x == 4   ? L::sL + g % 2 * QT * 32
-                                     : L::sRq + (x - 2) * L::kRTile + g % 2 * QT * RP * 2);
-          tma_load_4d(dst, x < D / 64 ? &tmQ : x == 4 ? &tmL : &tmRq, &bars[kVbQFull],
-                      x < D / 64 ? x * 64 : x == 4 ? 2 * RP : (x - 2) * RP, it.q0, h0 + g, 0);
-        }
-        __syncwarp();
-        for (int t = 0; t < tiles; ++t, ++gt) {
+        auto load = [&](int t) {  // key tile t
           const int s = gt & 1, key = it.k0 + t * kBlockN + row;
           const bool mine = row < kBlockN && key < it.len;
           const int page = mine ? __ldg(p.kv.table + it.b * p.kv.table_sb + (key >> lg)) : 0;
           const bool room = gt < 2 || mbar_wait(&bars[kVbEmpty + s], ((gt >> 1) - 1) & 1, abort_flag, 126);
-          if (!(ok = __all_sync(0xffffffffu, room))) break;
+          if (!(ok = __all_sync(0xffffffffu, room))) return;
           const int boxes = __popc(__ballot_sync(0xffffffffu, mine));
           if (lane == 0) mbar_expect_tx(&bars[kVbFull + s], boxes * bk * (D + ng * RP) * 2);
           __syncwarp();
@@ -571,20 +632,43 @@ __global__ void __launch_bounds__(kKwThreads, 1)
                           page);
           }
           __syncwarp();
-          // not earlier: who draws early gets work before it is free
-          if (g0 + L::kHeads >= p.G && t == max(0, tiles - 2)) next = draw();
+          ++gt;
+        };
+        if (!last) load(0);  // before the queries, which wait for the last step's MMAs
+        if (!ok) break;
+        const bool free = n == 0 || mbar_wait(&bars[kVbQEmpty], (n - 1) & 1, abort_flag, 125);
+        if (!(ok = __all_sync(0xffffffffu, free))) break;
+        if (lane == 0) {  // (the arrival also publishes the description)
+          step->b = it.b, step->kh = it.kh, step->k0 = it.k0, step->len = it.len, step->n = it.n, step->tiles = tiles;
+          step->h0 = h0, step->heads = nh;
+          mbar_expect_tx(&bars[kVbQFull], last ? 0 : QT * (nh * (D + 16) + ng * 2 * RP) * 2);
         }
+        __syncwarp();
+        if (last) break;
+        if (n == 0) pdl_wait();  // the prep kernel writes nothing of what was read so far
+        // lane 8 g + x of head g: x = 0, 1: Q chunks; 2, 3: R~_q hi, lo; 4: LSE
+        const int g = lane / 8, x = lane % 8;
+        if (g < nh && (x < D / 64 || x == 4 || (x / 2 == 1 && g < ng))) {
+          uint8_t* dst = smem + L::oQ + g / 2 * L::kPair +
+                         (x < D / 64 ? x * L::kChunk + g % 2 * QT * 128
+                          : x == 4   ? L::sL + g % 2 * QT * 32
+                                     : L::sRq + (x - 2) * L::kRTile + g % 2 * QT * RP * 2);
+          tma_load_4d(dst, x < D / 64 ? &tmQ : x == 4 ? &tmL : &tmRq, &bars[kVbQFull],
+                      x < D / 64 ? x * 64 : x == 4 ? 2 * RP : (x - 2) * RP, it.q0, h0 + g, 0);
+        }
+        __syncwarp();
+        for (int t = 1; ok && t < tiles; ++t) load(t);
         if (g0 + L::kHeads < p.G) ++n;
       }
       if (last) break;
-      it = next;
+      at += it.tiles;
     }
-  } else if (warp >= 9) {
-    // ------------------------------------------------------------ MMA issuer (9) and its waiter (10)
+  } else if (warp == kKwIssuer || warp == kKwWaiter) {
+    // ------------------------------------------------------------ MMA issuer and its waiter
     constexpr uint32_t idesc = make_idesc_bf16(kBlockN, 128, 0, 0), idesc_r = make_idesc_bf16(kBlockN, QT, 0, 0);
     constexpr uint32_t r_layout = RP == 16 ? kSwizzle32B : kSwizzle64B;
     constexpr uint32_t r_sbo = 8 * RP * 2;
-    const bool issuer = warp == 9;
+    const bool issuer = warp == kKwIssuer;
     // operand descriptors at their first place; others differ in the address field only (bytes / 16)
     const uint32_t s0 = smem_u32(smem);
     const uint64_t dK0 = make_sdesc(s0 + L::oK, 16, 1024, kSwizzle128B);
@@ -603,18 +687,20 @@ __global__ void __launch_bounds__(kKwThreads, 1)
       if (tiles < 0) break;
       for (int t = 0; ok && t < tiles; ++t, ++gt) {
         const int s = gt & 1;
-        if (!issuer) ok = mbar_wait(&bars[kVbFull + s], (gt >> 1) & 1, abort_flag, 226);
+        const int units = (heads + 1) / 2;
+        if (!issuer) {
+          ok = mbar_wait(&bars[kVbFull + s], (gt >> 1) & 1, abort_flag, 226);
+          for (int v = used; ok && v < used + units; ++v)
+            ok = v < NB || mbar_wait(&bars[kVbSEmpty + v % NB], (v / NB - 1) & 1, abort_flag, 227);
+        }
+        ok = pair_rendezvous(1, ok);
+        if (!ok) break;
+        if (issuer) tc_fence_after();
 #pragma unroll
         for (int u = 0; u < L::kPairs; ++u) {
           if (2 * u >= heads) continue;
-          const int buf = used % NB;
-          if (!issuer && ok && used >= NB) ok = mbar_wait(&bars[kVbSEmpty + buf], (used / NB - 1) & 1, abort_flag, 227);
-          ++used;
-          ok = pair_rendezvous(1, ok);
-          if (!ok) break;
-          if (!issuer) continue;
-          tc_fence_after();
-          if (elect_one()) {
+          const int buf = used++ % NB;
+          if (issuer && elect_one()) {
             const uint32_t tS = tmem + 128 * buf;
             const uint64_t dK = dK0 + (s * L::kStage >> 4), dQ = dQ0 + (u * L::kPair >> 4);
 #pragma unroll
@@ -637,71 +723,82 @@ __global__ void __launch_bounds__(kKwThreads, 1)
             mma_commit(&bars[kVbSFull + buf]);
             if (2 * u + 2 >= heads) mma_commit(&bars[kVbEmpty + s]);
           }
-          __syncwarp();
         }
+        __syncwarp();
       }
       if (ok && issuer && elect_one()) mma_commit(&bars[kVbQEmpty]);
       __syncwarp();
     }
-  } else {
-    // ------------------------------------------------------------ sums (warpgroup i: head i of each pair)
-    const int wi = warp >> 2;
+  } else if (warp < kKwProducer) {
+    // ------------------------------------------------------------ sums: warpgroup i, head i % 2 of every second unit
+    const int wi = warp >> 2 & 1, half = warp >> 3;
     const uint32_t t_lane = tmem + QT * wi + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+    float* part = reinterpret_cast<float*>(smem + L::oPart) + (warp >> 2) * 128 + (tid & 127);
     const float2 sl2 = make_float2(p.scale_log2, p.scale_log2);
-    int used = 0, gt = 0;
+    int used = 0, gt = 0;  // units and key tiles so far
     bool ok = true;
     for (int n = 0; ok; ++n) {
       if (!mbar_wait(&bars[kVbQFull], n & 1, abort_flag, 325)) break;
-      const int tiles = step->tiles, heads = step->heads, nq = step->n, len = step->len, k0 = step->k0;
-      float* dst = p.kw + step->b * p.kw_sb + step->kh * p.kw_sh + k0 + (tid & 127);
+      const int tiles = step->tiles, heads = step->heads, nq = step->n, past = step->len - nq, k0 = step->k0;
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars[kVbQEmpty]);
       if (tiles < 0) break;
-      const int past = len - nq;
       for (int t = 0; ok && t < tiles; ++t, ++gt) {
-        const int tile0 = k0 + t * kBlockN, j = tile0 + (tid & 127);
-        const bool store = wi == 0 && j < len;
-        const float before = store ? dst[t * kBlockN] : 0.f;
+        const int tile0 = k0 + t * kBlockN, first = p.causal ? tile0 + (tid & 127) - past : 0;
         float w = 0.f;
-        for (int u = 0; 2 * u < heads; ++u) {
+        for (int u = 0; 2 * u < heads; ++u, ++used) {
+          if ((used & 1) != half) continue;
           const int buf = used % NB;
-          if (!mbar_wait(&bars[kVbSFull + buf], (used / NB) & 1, abort_flag, 326)) {
-            ok = false;
-            break;
-          }
-          ++used;
+          if (!(ok = mbar_wait(&bars[kVbSFull + buf], (used / NB) & 1, abort_flag, 326))) break;
           tc_fence_after();
           // columns [first, nq) belong to queries that see the key; the score of another sequence's query
           // or of a head that the pair lacks is never read into a sum
           const bool whole = (!p.causal || tile0 + kBlockN - 1 <= past) && nq == QT;
           if (2 * u + wi < heads)
             w += whole ? kw_sum<QT, false>(t_lane + 128 * buf, sl2, 0, 0)
-                       : kw_sum<QT, true>(t_lane + 128 * buf, sl2, p.causal ? j - past : 0, nq);
+                       : kw_sum<QT, true>(t_lane + 128 * buf, sl2, first, nq);
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(&bars[kVbSEmpty + buf]);
         }
-        if (!ok) break;
-        float* part = reinterpret_cast<float*>(smem + L::oPart) + (gt & 1) * 128 + (tid & 127);
-        if (wi == 1) {
-          if (gt >= 2 && !(ok = mbar_wait(&bars[kVbPEmpty + (gt & 1)], ((gt >> 1) - 1) & 1, abort_flag, 327))) break;
-          *part = w;
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&bars[kVbPFull + (gt & 1)]);
-        } else {
-          if (!(ok = mbar_wait(&bars[kVbPFull + (gt & 1)], (gt >> 1) & 1, abort_flag, 328))) break;
-          w += *part;
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&bars[kVbPEmpty + (gt & 1)]);
-          if (store) dst[t * kBlockN] = before + w;
+        if (!ok || (gt >= 2 && !(ok = mbar_wait(&bars[kVbPEmpty + (gt & 1)], ((gt >> 1) - 1) & 1, abort_flag, 327)))) break;
+        part[(gt & 1) * 512] = w;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars[kVbPFull + (gt & 1)]);
+      }
+    }
+  } else {
+    // ------------------------------------------------------------ adds the warpgroups' sums and stores
+    const float* part = reinterpret_cast<const float*>(smem + L::oPart) + lane;
+    int gt = 0;
+    bool ok = true;
+    for (int n = 0; ok; ++n) {
+      if (!mbar_wait(&bars[kVbQFull], n & 1, abort_flag, 335)) break;
+      const int tiles = step->tiles;
+      int left = step->len - step->k0 - lane;
+      float* dst = p.kw + step->b * p.kw_sb + step->kh * p.kw_sh + step->k0 + lane;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars[kVbQEmpty]);
+      if (tiles < 0) break;
+      for (int t = 0; t < tiles; ++t, ++gt, left -= kBlockN, dst += kBlockN) {
+        float w[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) w[k] = 32 * k < left ? dst[32 * k] : 0.f;
+        if (!(ok = mbar_wait(&bars[kVbPFull + (gt & 1)], (gt >> 1) & 1, abort_flag, 336))) break;
+        const float* x = part + (gt & 1) * 512;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          if (32 * k < left) dst[32 * k] = w[k] + ((x[32 * k] + x[128 + 32 * k]) + (x[256 + 32 * k] + x[384 + 32 * k]));
         }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars[kVbPEmpty + (gt & 1)]);
       }
     }
   }
 
   tc_fence_before();
   __syncthreads();
-  if (warp == 9) {
+  if (warp == kKwIssuer) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
@@ -722,13 +819,11 @@ cudaError_t launch_key_weights_t(const KwMaps& m, KeyWeightsParams& p, cudaStrea
   cudaError_t e = allow_smem(reinterpret_cast<const void*>(kern), allowed[window]);
   if (e != cudaSuccess) return e;
   const int64_t n = static_cast<int64_t>(p.bd.T) * p.H * (p.RP / 8 + 1);
+  const int64_t tiles = (p.bd.max_k + kBlockN - 1) / kBlockN, seqs = static_cast<int64_t>(p.bd.B) * p.kv.hkv;
+  p.ctas = static_cast<int>(std::min<int64_t>(seqs * (window ? tiles : (tiles + 1) / 2), kSms));
   fna2_key_weights_prep_kernel<<<static_cast<unsigned>((n + 255) / 256), 256, 0, stream>>>(p);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
-  const int64_t tiles = (p.bd.max_k + kBlockN - 1) / kBlockN, seqs = static_cast<int64_t>(p.bd.B) * p.kv.hkv;
-  // key tiles per item: a pair, or runs (about three per CTA when all sequences are the longest)
-  p.run_tiles = window ? static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(16, seqs * tiles / (3 * kSms)))) : 2;
-  const int64_t items = seqs * ((tiles + p.run_tiles - 1) / p.run_tiles);
-  return launch_dependent(kern, static_cast<unsigned>(std::min<int64_t>(items, kSms)), kKwThreads,
+  return launch_dependent(kern, static_cast<unsigned>(p.ctas), kKwThreads,
                           window ? KwwSmem<D, RP>::kTotal : KwSmem<D, RP>::kTotal, stream, m.q, m.k, m.rq, m.rk, m.l, p);
 }
 
