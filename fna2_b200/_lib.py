@@ -199,6 +199,7 @@ class Fna2PagedAttnArgs(ctypes.Structure):
         ("out", ctypes.c_void_p), ("out_token_stride", _I64), ("out_head_stride", _I64),
         ("lse", ctypes.c_void_p), ("lse_head_stride", _I64),
         ("key_weights", ctypes.c_void_p), ("kw_batch_stride", _I64), ("kw_head_stride", _I64),
+        ("kw_clear", _I64),
     ]
 
 

@@ -1011,12 +1011,24 @@ extern "C" int fna2_key_weights(const Fna2PagedKV* kv, const Fna2PagedAttnArgs* 
   KeyWeightsParams p{};
   if (int rc = paged_queries(kv, a, &p)) return rc;
   FNA2_CHECK(a->key_weights != nullptr && (a->lse != nullptr || a->total_q == 0), "key weights need lse and key_weights");
-  if (p.bd.B == 0 || p.bd.T == 0 || p.bd.max_k == 0) return FNA2_OK;
+  FNA2_CHECK(a->kw_clear >= 0 && (a->kw_clear == 0 || a->kw_clear >= p.bd.max_k), "kw_clear (%lld) is below max_seqlen_k",
+             static_cast<long long>(a->kw_clear));
+  FNA2_CHECK(a->kw_clear == 0 || (((a->kw_clear | a->kw_batch_stride | a->kw_head_stride) & 3) == 0 && aligned16(a->key_weights)),
+             "rows of key_weights that are cleared must be 16-byte aligned, kw_clear a multiple of 4");
+  p.clear = a->kw_clear;
+  const bool empty = p.bd.T == 0 || p.bd.max_k == 0;
+  if (p.bd.B == 0 || (empty && p.clear == 0)) return FNA2_OK;
   const size_t need = kw_workspace_bytes(p.bd.T, p.H, p.RP);
   if (workspace == nullptr || workspace_bytes < need)
     return fail(FNA2_ERR_WORKSPACE, "key weights workspace: need %zu bytes, got %zu", need, workspace_bytes);
   FNA2_CHECK((reinterpret_cast<uintptr_t>(workspace) & 255u) == 0, "workspace must be 256-byte aligned");
   p.lse = a->lse, p.lse_sh = a->lse_head_stride;
+  if (empty) {
+    p.bd.T = 0;
+    p.next = static_cast<int*>(workspace);
+    FNA2_CUDA(launch_key_weights_prep(p, static_cast<cudaStream_t>(stream)));
+    return FNA2_OK;
+  }
   return run_key_weights(p, kv->head_dim, static_cast<uint8_t*>(workspace), static_cast<cudaStream_t>(stream));
 }
 

@@ -99,26 +99,25 @@ __device__ __forceinline__ void move_rows(const EvictParams& p, int b, int kh, i
 
 constexpr int kSelThreads = 1024;
 constexpr int kSelBins = 2048;
+constexpr int kHistCopies = 2;  // lanes that count the same bin at once wait for each other: even and odd ones apart
 
 // fp32 bits in an order-preserving unsigned form; -0 equals +0, NaN is lowest.
 __device__ __forceinline__ uint32_t ordered_bits(float x) {
-  if (x != x) return 0u;
-  const uint32_t u = __float_as_uint(x + 0.f);
-  return u & 0x80000000u ? ~u : u | 0x80000000u;
+  const int u = __float_as_int(x + 0.f);
+  return x != x ? 0u : static_cast<uint32_t>(u ^ (u >> 31 | static_cast<int>(0x80000000u)));
 }
 
 // MOVE: the block also copies its rows (short sequences: one launch instead of two).  STAGED: the
-// ordered bits of the sequence's weights fit in shared memory and are read from there after the first
-// pass (each pass over 16,384 weights in global memory took 7 us, latency of dependent loads).
+// sequence's weights fit in shared memory and are read from there after the first pass (each pass over
+// 16,384 weights in global memory took 7 us, latency of dependent loads).
 template <bool MOVE, bool STAGED>
 __global__ void __launch_bounds__(kSelThreads) fna2_evict_select_kernel(const EvictParams p) {
-  extern __shared__ uint32_t s_bits[];
-  __shared__ int hist[kSelBins];
+  extern __shared__ float s_w[];
+  __shared__ int hist[kHistCopies][kSelBins];
   __shared__ RowPlace s_at[MOVE ? kSelThreads : 1];
   __shared__ int s_warp[2][32];
   __shared__ int s_digit, s_above;
   const int kh = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  pdl_trigger();
   int len = __ldg(p.lens + b);
   if (len < 0 || len > p.max_k) {
     if (tid == 0) atomicCAS(&g_device_error, 0, kStatusBadSeqEvict);
@@ -129,40 +128,76 @@ __global__ void __launch_bounds__(kSelThreads) fna2_evict_select_kernel(const Ev
   const int need = keep - (len - old_end) - old_beg;                            // >= 0: sink + recent <= budget
   const float* w = p.w + b * p.w_sb + kh * p.w_sh;
   const bool all = need >= old_end - old_beg, some = !all && need > 0;
-  auto bits = [&](int j) { return STAGED ? s_bits[j] : ordered_bits(__ldg(w + j)); };
+  // weights j .. j + 3 (j a multiple of 4); anything past the candidates
+  auto load4 = [&](int j, float* x) {
+    if (STAGED) {
+      *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(s_w + j);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = j + i < old_end ? __ldg(w + j + i) : 0.f;
+    }
+  };
+  // bit i: key j + i is a candidate below `end`
+  auto candidates = [&](int j, int end) {
+    if (j >= old_beg && j + 3 < end) return 15u;
+    unsigned in = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) in |= static_cast<unsigned>(j + i >= old_beg && j + i < end) << i;
+    return in;
+  };
+  int* my_hist = hist[tid % kHistCopies];
   uint32_t prefix = 0;
   int want = need;  // rank of the threshold among the candidates that share the prefix
+  if (STAGED || some) {
+    for (int i = tid; i < kHistCopies * kSelBins; i += kSelThreads) hist[0][i] = 0;
+    __syncthreads();
+  }
+  if (STAGED) {
+    constexpr int U = 8;  // loads in flight
+    for (int j0 = tid; j0 < len; j0 += U * kSelThreads) {
+      float x[U];
+#pragma unroll
+      for (int i = 0; i < U; ++i) x[i] = j0 + i * kSelThreads < len ? __ldg(w + j0 + i * kSelThreads) : 0.f;
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+        const int j = j0 + i * kSelThreads;
+        if (j < len) {
+          s_w[j] = x[i];
+          if (j >= old_beg && j < old_end) atomicAdd(&my_hist[ordered_bits(x[i]) >> 21], 1);
+        }
+      }
+    }
+    __syncthreads();
+  }
   if (some) {
     int shift = 32;
     for (int pass = 0; pass < 3; ++pass) {
       const int width = pass < 2 ? 11 : 10;
       const uint32_t hi_mask = pass == 0 ? 0u : 0xffffffffu << shift;
       shift -= width;
-      for (int i = tid; i < kSelBins; i += kSelThreads) hist[i] = 0;
-      __syncthreads();
-      if (STAGED && pass == 0) {
-        constexpr int U = 8;  // loads in flight
-        for (int j0 = old_beg + tid; j0 < old_end; j0 += U * kSelThreads) {
-          float x[U];
+      if (!STAGED || pass > 0) {
+        for (int j = (old_beg & ~3) + 4 * tid; j < old_end; j += 4 * kSelThreads) {
+          alignas(16) float x[4];
+          load4(j, x);
+          const unsigned in = candidates(j, old_end);
 #pragma unroll
-          for (int i = 0; i < U; ++i) x[i] = j0 + i * kSelThreads < old_end ? __ldg(w + j0 + i * kSelThreads) : 0.f;
-#pragma unroll
-          for (int i = 0; i < U; ++i)
-            if (j0 + i * kSelThreads < old_end) {
-              const uint32_t u = ordered_bits(x[i]);
-              s_bits[j0 + i * kSelThreads] = u;
-              atomicAdd(&hist[u >> shift], 1);
-            }
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t u = ordered_bits(x[i]);
+            if ((u & hi_mask) == prefix && (in >> i & 1))
+              atomicAdd(&my_hist[(u >> shift) & ((1u << width) - 1)], 1);
+          }
         }
-      } else {
-        for (int j = old_beg + tid; j < old_end; j += kSelThreads) {
-          const uint32_t u = bits(j);
-          if ((u & hi_mask) == prefix) atomicAdd(&hist[(u >> shift) & ((1u << width) - 1)], 1);
-        }
+        __syncthreads();
       }
-      __syncthreads();
       // suffix counts: thread t owns bins 2t and 2t + 1
-      const int c1 = hist[2 * tid + 1], c0 = hist[2 * tid], mine = c0 + c1;
+      int c0 = 0, c1 = 0;
+#pragma unroll
+      for (int i = 0; i < kHistCopies; ++i) {
+        int2* c = reinterpret_cast<int2*>(&hist[i][2 * tid]);
+        c0 += c->x, c1 += c->y;
+        *c = make_int2(0, 0);  // for the next pass
+      }
+      const int mine = c0 + c1;
       int suf = mine;  // inclusive suffix sum within the warp
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -171,8 +206,7 @@ __global__ void __launch_bounds__(kSelThreads) fna2_evict_select_kernel(const Ev
       }
       if (lane == 0) s_warp[0][warp] = suf;
       __syncthreads();
-      int after = 0;
-      for (int i = warp + 1; i < 32; ++i) after += s_warp[0][i];
+      const int after = __reduce_add_sync(0xffffffffu, lane > warp ? s_warp[0][lane] : 0);
       const int above1 = after + suf - mine;  // candidates in bins above 2t + 1
       const int above0 = above1 + c1;
       if (above1 < want && want <= above1 + c1) s_digit = 2 * tid + 1, s_above = above1;
@@ -184,46 +218,69 @@ __global__ void __launch_bounds__(kSelThreads) fna2_evict_select_kernel(const Ev
     }
   }
   // prefix: the threshold value; want: how many candidates equal to it are kept (the lowest indices).
-  // Each warp owns a run of the keys: it counts what it takes, then writes from its offset on.
+  if (all) prefix = 0, want = len;
+  if (!all && !some) prefix = 0xffffffffu;  // above every weight
   int* kept = p.kept + (static_cast<int64_t>(b) * p.kv.hkv + kh) * p.budget;
   float* w_out = p.w_out + (static_cast<int64_t>(b) * p.kv.hkv + kh) * p.cap_out;
-  const int run = (len + kSelThreads - 1) / kSelThreads * 32;
-  const int beg = min(len, warp * run), end = min(len, beg + run);
-  auto flags = [&](int j, unsigned* take, unsigned* tie) {
-    bool a = false, e = false;
-    if (j < end) {
-      const bool cand = j >= old_beg && j < old_end;
-      a = !cand || all;
-      if (cand && some) {
-        const uint32_t u = bits(j);
-        a = u > prefix, e = u == prefix;
-      }
+  for (int j = tid; j < old_beg; j += kSelThreads) kept[j] = j, w_out[j] = STAGED ? s_w[j] : __ldg(w + j);
+  for (int j = old_end + tid; j < len; j += kSelThreads)
+    kept[keep - len + j] = j, w_out[keep - len + j] = STAGED ? s_w[j] : __ldg(w + j);
+  // Each warp owns a run of the keys: it counts the candidates that it takes, then writes from its offset on.
+  const int run = (old_end + 4 * kSelThreads - 1) / (4 * kSelThreads) * 128;
+  const int beg = min(old_end, warp * run), end = min(old_end, beg + run);
+  // Of keys j .. j + 3: bits of those taken for certain, and of those equal to the threshold.
+  auto flags = [&](const float* x, unsigned in, unsigned* take, unsigned* tie) {
+    *take = *tie = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t u = ordered_bits(x[i]);
+      if (u > prefix) *take |= 1u << i;
+      if (u == prefix) *tie |= 1u << i;
     }
-    *take = __ballot_sync(0xffffffffu, a);
-    *tie = __ballot_sync(0xffffffffu, e);
+    *take &= in, *tie &= in;
   };
   int takes = 0, ties = 0;
-  for (int j0 = beg; j0 < end; j0 += 32) {
+  for (int j = beg + 4 * lane; j < end; j += 128) {
+    alignas(16) float x[4];
+    load4(j, x);
     unsigned mt, me;
-    flags(j0 + lane, &mt, &me);
+    flags(x, candidates(j, end), &mt, &me);
     takes += __popc(mt), ties += __popc(me);
   }
+  takes = __reduce_add_sync(0xffffffffu, takes), ties = __reduce_add_sync(0xffffffffu, ties);
   if (lane == 0) s_warp[0][warp] = takes, s_warp[1][warp] = ties;
   __syncthreads();
-  int takes_before = 0, ties_before = 0;
-  for (int i = 0; i < warp; ++i) takes_before += s_warp[0][i], ties_before += s_warp[1][i];
-  const unsigned lt = (1u << lane) - 1;
-  for (int j0 = beg; j0 < end; j0 += 32) {
-    const int j = j0 + lane;
-    unsigned mt, me;
-    flags(j, &mt, &me);
-    const int my_ties = ties_before + __popc(me & lt);
-    if ((mt >> lane & 1) || ((me >> lane & 1) && my_ties < want)) {
-      const int pos = takes_before + __popc(mt & lt) + min(my_ties, want);
-      kept[pos] = j;
-      w_out[pos] = __ldg(w + j);
+  pdl_trigger();
+  int takes_before = old_beg + __reduce_add_sync(0xffffffffu, lane < warp ? s_warp[0][lane] : 0);
+  int ties_before = __reduce_add_sync(0xffffffffu, lane < warp ? s_warp[1][lane] : 0);
+  for (int j0 = beg; j0 < end; j0 += 128) {
+    const int j = j0 + 4 * lane;
+    alignas(16) float x[4];
+    unsigned mt = 0, me = 0;
+    if (j < end) {
+      load4(j, x);
+      flags(x, candidates(j, end), &mt, &me);
     }
-    takes_before += __popc(mt), ties_before += __popc(me);
+    // takes and ties << 16 of the lanes up to this one
+    const int mine = __popc(mt) | __popc(me) << 16;
+    int incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += v;
+    }
+    int a = takes_before + ((incl - mine) & 0xffff), e = ties_before + ((incl - mine) >> 16);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const bool take = mt >> i & 1, tie = me >> i & 1;
+      if (take || (tie && e < want)) {
+        kept[a + min(e, want)] = j + i;
+        w_out[a + min(e, want)] = x[i];
+      }
+      a += take, e += tie;
+    }
+    const int total = __shfl_sync(0xffffffffu, incl, 31);
+    takes_before += total & 0xffff, ties_before += total >> 16;
   }
   for (int i = keep + tid; i < p.budget; i += kSelThreads) kept[i] = -1;
   for (int i = keep + tid; i < p.cap_out; i += kSelThreads) w_out[i] = 0.f;
@@ -260,7 +317,7 @@ cudaError_t launch_evict_select(const EvictParams& p, cudaStream_t stream) {
     static std::atomic<uint64_t> allowed{0};
     const cudaError_t e = allow_smem(reinterpret_cast<const void*>(kern), allowed, kStagedKeys * 4);
     if (e != cudaSuccess) return e;
-    kern<<<heads, kSelThreads, p.max_k * 4, stream>>>(p);
+    kern<<<heads, kSelThreads, (p.max_k + 3) / 4 * 16, stream>>>(p);
   } else {
     fna2_evict_select_kernel<MOVE, false><<<heads, kSelThreads, 0, stream>>>(p);
   }

@@ -48,14 +48,22 @@ struct KeyWeightsParams {
   __nv_bfloat16* rq2;  // workspace: [T][H][2 RP + 16]: R~_q hi, lo (graph heads), -LSE/scale as three terms
   int* next;           // workspace: item counter, set to ctas (whose first items are their own index) by the prep kernel
   int ctas;
+  int64_t clear;       // > 0: the weights are set, not added to; values of each row of kw to write
 };
 
-// R~_q = gs/scale * R_q as hi + lo, columns [rank, RP) zero, and -LSE/scale = l1 + l2 + l3 (a row
+// If weights are set: 0 for the keys that no query sees.  R~_q = gs/scale * R_q as hi + lo, columns [rank, RP) zero, and -LSE/scale = l1 + l2 + l3 (a row
 // without weight: -1e38, whose weights are 0).
 __global__ void __launch_bounds__(256) fna2_key_weights_prep_kernel(const KeyWeightsParams p) {
   pdl_trigger();
   const int64_t e = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
   if (e == 0) *p.next = p.ctas;
+  for (int64_t row = p.clear > 0 ? blockIdx.x : INT64_MAX; row < static_cast<int64_t>(p.bd.B) * p.kv.hkv; row += gridDim.x) {
+    const int b = static_cast<int>(row / p.kv.hkv), kh = static_cast<int>(row % p.kv.hkv);
+    const PagedSeq s = paged_seq(p.bd, b);
+    float* dst = p.kw + b * p.kw_sb + kh * p.kw_sh;
+    for (int64_t x = (s.n > 0 ? s.len / 4 : 0) + threadIdx.x; x < p.clear / 4; x += 256)
+      reinterpret_cast<float4*>(dst)[x] = make_float4(0.f, 0.f, 0.f, 0.f);
+  }
   const int r8 = p.RP / 8, per = r8 + 1;  // pieces of a row: R_q's, then the LSE's
   if (e >= static_cast<int64_t>(p.bd.T) * p.H * per) return;
   const int x = static_cast<int>(e % per), h = static_cast<int>(e / per % p.H);
@@ -346,18 +354,18 @@ __global__ void __launch_bounds__(kKwThreads, 1)
         const int s = gu & 1;
         const bool graph = kh * p.G + u / per_head < p.kv.hg;
         if (u % per_head == 0) rs ^= 1;
-        if (!issuer) {
-          ok = mbar_wait(&bars[kWbFull + s], (gu >> 1) & 1, abort_flag, 222);
-          for (int i = 0; ok && i < tiles; ++i)
-            ok = used[i] < 2 || mbar_wait(&bars[kWbSEmpty + 2 * i + used[i] % 2], (used[i] / 2 - 1) & 1, abort_flag, 223);
-        }
-        ok = pair_rendezvous(1, ok);
-        if (!ok) break;
-        if (issuer) tc_fence_after();
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           if (i >= tiles) continue;
-          const int buf = 2 * i + used[i]++ % 2;
+          const int buf = 2 * i + used[i] % 2;
+          if (!issuer) {
+            ok = used[i] < 2 || mbar_wait(&bars[kWbSEmpty + buf], (used[i] / 2 - 1) & 1, abort_flag, 223);
+            if (ok && i == 0) ok = mbar_wait(&bars[kWbFull + s], (gu >> 1) & 1, abort_flag, 222);
+          }
+          ++used[i];
+          ok = pair_rendezvous(1, ok);
+          if (!ok) break;
+          if (issuer) tc_fence_after();
           if (issuer && elect_one()) {
             const uint32_t tS = tmem + 128 * buf;
             const uint64_t dK = dK0 + (i * L::kTile >> 4), dQ = dQ0 + (s * L::kStage >> 4);
@@ -425,6 +433,7 @@ __global__ void __launch_bounds__(kKwThreads, 1)
   } else {
     // ------------------------------------------------------------ adds the warpgroups' sums and stores
     const float* part = reinterpret_cast<const float*>(smem + L::oPart) + lane;
+    pdl_wait();  // the prep kernel may write up to three weights past those it leaves out
     for (int n = 0;; ++n) {
       if (!mbar_wait(&bars[kWbKFull], n & 1, abort_flag, 330)) break;
       const int left = items[0].len - items[0].k0 - lane, n_units = items[0].n_units;
@@ -434,7 +443,7 @@ __global__ void __launch_bounds__(kKwThreads, 1)
       if (n_units < 0) break;
       float w[8];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) w[k] = 32 * k < left ? dst[32 * k] : 0.f;
+      for (int k = 0; k < 8; ++k) w[k] = 32 * k < left && p.clear == 0 ? dst[32 * k] : 0.f;
       if (!mbar_wait(&bars[kWbPFull], n & 1, abort_flag, 331)) break;
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
@@ -689,9 +698,9 @@ __global__ void __launch_bounds__(kKwThreads, 1)
         const int s = gt & 1;
         const int units = (heads + 1) / 2;
         if (!issuer) {
-          ok = mbar_wait(&bars[kVbFull + s], (gt >> 1) & 1, abort_flag, 226);
           for (int v = used; ok && v < used + units; ++v)
             ok = v < NB || mbar_wait(&bars[kVbSEmpty + v % NB], (v / NB - 1) & 1, abort_flag, 227);
+          if (ok) ok = mbar_wait(&bars[kVbFull + s], (gt >> 1) & 1, abort_flag, 226);
         }
         ok = pair_rendezvous(1, ok);
         if (!ok) break;
@@ -772,10 +781,12 @@ __global__ void __launch_bounds__(kKwThreads, 1)
     const float* part = reinterpret_cast<const float*>(smem + L::oPart) + lane;
     int gt = 0;
     bool ok = true;
+    pdl_wait();  // the prep kernel may write up to three weights past those it leaves out
     for (int n = 0; ok; ++n) {
       if (!mbar_wait(&bars[kVbQFull], n & 1, abort_flag, 335)) break;
       const int tiles = step->tiles;
       int left = step->len - step->k0 - lane;
+      const bool set = p.clear > 0 && step->h0 == step->kh * p.G;  // the KV head's first query heads
       float* dst = p.kw + step->b * p.kw_sb + step->kh * p.kw_sh + step->k0 + lane;
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars[kVbQEmpty]);
@@ -783,7 +794,7 @@ __global__ void __launch_bounds__(kKwThreads, 1)
       for (int t = 0; t < tiles; ++t, ++gt, left -= kBlockN, dst += kBlockN) {
         float w[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) w[k] = 32 * k < left ? dst[32 * k] : 0.f;
+        for (int k = 0; k < 4; ++k) w[k] = 32 * k < left && !set ? dst[32 * k] : 0.f;
         if (!(ok = mbar_wait(&bars[kVbPFull + (gt & 1)], (gt >> 1) & 1, abort_flag, 336))) break;
         const float* x = part + (gt & 1) * 512;
 #pragma unroll
@@ -811,6 +822,14 @@ struct KwMaps {
 // Queries per unit: which of the two kernels runs.
 inline int kw_query_tile(const KeyWeightsParams& p) { return p.bd.max_q <= 64 ? 64 : 128; }
 
+inline cudaError_t launch_key_weights_prep(const KeyWeightsParams& p, cudaStream_t stream) {
+  const int64_t n = static_cast<int64_t>(p.bd.T) * p.H * (p.RP / 8 + 1);
+  const int64_t rows = p.clear > 0 ? static_cast<int64_t>(p.bd.B) * p.kv.hkv : 0;
+  const int64_t blocks = std::max<int64_t>((n + 255) / 256, std::min<int64_t>(std::max<int64_t>(rows, 1), 4 * kSms));
+  fna2_key_weights_prep_kernel<<<static_cast<unsigned>(blocks), 256, 0, stream>>>(p);
+  return cudaGetLastError();
+}
+
 template <int D, int RP>
 cudaError_t launch_key_weights_t(const KwMaps& m, KeyWeightsParams& p, cudaStream_t stream) {
   const bool window = kw_query_tile(p) == 64;
@@ -818,11 +837,10 @@ cudaError_t launch_key_weights_t(const KwMaps& m, KeyWeightsParams& p, cudaStrea
   static std::atomic<uint64_t> allowed[2];
   cudaError_t e = allow_smem(reinterpret_cast<const void*>(kern), allowed[window]);
   if (e != cudaSuccess) return e;
-  const int64_t n = static_cast<int64_t>(p.bd.T) * p.H * (p.RP / 8 + 1);
   const int64_t tiles = (p.bd.max_k + kBlockN - 1) / kBlockN, seqs = static_cast<int64_t>(p.bd.B) * p.kv.hkv;
   p.ctas = static_cast<int>(std::min<int64_t>(seqs * (window ? tiles : (tiles + 1) / 2), kSms));
-  fna2_key_weights_prep_kernel<<<static_cast<unsigned>((n + 255) / 256), 256, 0, stream>>>(p);
-  if ((e = cudaGetLastError()) != cudaSuccess) return e;
+  e = launch_key_weights_prep(p, stream);
+  if (e != cudaSuccess) return e;
   return launch_dependent(kern, static_cast<unsigned>(p.ctas), kKwThreads,
                           window ? KwwSmem<D, RP>::kTotal : KwSmem<D, RP>::kTotal, stream, m.q, m.k, m.rq, m.rk, m.l, p);
 }

@@ -37,7 +37,7 @@ _DT = {torch.float32: _lib.FNA2_DTYPE_F32, torch.bfloat16: _lib.FNA2_DTYPE_BF16}
 
 # The argument blocks of include/fna2.h, packed in one call each: filling a ctypes structure field
 # by field costs several microseconds, as much as a small kernel.
-_ATTN_ARGS = struct.Struct("@8if PqPP PqqPqqP Pqq Pq Pqq".replace(" ", ""))
+_ATTN_ARGS = struct.Struct("@8if PqPP PqqPqqP Pqq Pq Pqqq".replace(" ", ""))
 _APPEND_ARGS = struct.Struct("@6iq PqqPqqPqqPqqPqq Pq PPP PP f P".replace(" ", ""))
 _EVICT_ARGS = struct.Struct("@8i PqPqP Pqq PPP".replace(" ", ""))
 
@@ -181,7 +181,7 @@ def _weights_ok(w: torch.Tensor, B: int, heads: int, keys: int) -> None:
 
 
 def _attention(name, q, pool, page_table, cache_seqlens, cu_seqlens_q, max_seqlen_q, r_q, graph_scale, softmax_scale,
-               is_causal, key_weights, max_seqlen_k, num_splits, out, lse):
+               is_causal, key_weights, max_seqlen_k, num_splits, out, lse, clear=0):
     """Packs the arguments of fna2_paged_attn or fna2_key_weights and calls it."""
     T, H, D = q.shape
     q, q_p, q_0, q_1 = _rows(q, "q", T, H, pool.head_dim, torch.bfloat16)
@@ -210,7 +210,7 @@ def _attention(name, q, pool, page_table, cache_seqlens, cu_seqlens_q, max_seqle
     a = _ATTN_ARGS.pack(B, H, T, int(max_seqlen_q), max_k, max_pages, 1 if is_causal else 0, num_splits,
                         D ** -0.5 if softmax_scale is None else softmax_scale, table.data_ptr(), table.stride(0),
                         lens.data_ptr(), cu.data_ptr(), q_p, q_0, q_1, r_p, r_0, r_1, gs_p,
-                        0 if out is None else out.data_ptr(), H * D, D, l_p, l_0, w_p, w_0, w_1)
+                        0 if out is None else out.data_ptr(), H * D, D, l_p, l_0, w_p, w_0, w_1, clear)
     lib = _lib.load()
     size, call = ((lib.fna2_paged_attn_workspace_size, lib.fna2_paged_attn) if out is not None else
                   (lib.fna2_key_weights_workspace_size, lib.fna2_key_weights))
@@ -262,11 +262,12 @@ def naylis_key_weights(q: torch.Tensor, lse: torch.Tensor, pool: PagedKV, page_t
         raise ValueError(f"lse must be CUDA fp32 [{q.shape[1]}, {q.shape[0]}] (got {lse.dtype} {tuple(lse.shape)})")
     if lse.stride(1) != 1:
         lse = lse.contiguous()
+    clear = 0
     if key_weights is None:
-        key_weights = torch.zeros((page_table.shape[0], pool.kv_heads, page_table.shape[1] * pool.page_size),
-                                  dtype=torch.float32, device=q.device)
+        clear = page_table.shape[1] * pool.page_size
+        key_weights = torch.empty((page_table.shape[0], pool.kv_heads, clear), dtype=torch.float32, device=q.device)
     _attention("fna2_key_weights", q, pool, page_table, cache_seqlens, cu_seqlens_q, max_seqlen_q, r_q, graph_scale,
-               softmax_scale, is_causal, key_weights, max_seqlen_k, 0, None, lse)
+               softmax_scale, is_causal, key_weights, max_seqlen_k, 0, None, lse, clear)
     return key_weights
 
 

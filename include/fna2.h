@@ -315,6 +315,8 @@ typedef struct Fna2PagedAttnArgs {
   void* out;        int64_t out_token_stride, out_head_stride;
   float* lse;       int64_t lse_head_stride;                  /* or NULL */
   float* key_weights; int64_t kw_batch_stride, kw_head_stride; /* or NULL */
+  int64_t kw_clear;            /* fna2_key_weights: if > 0, values of each row set to 0 first: at least max_seqlen_k,
+                                * a multiple of 4 as the strides, rows 16-byte aligned */
 } Fna2PagedAttnArgs;
 size_t fna2_paged_attn_workspace_size(const Fna2PagedKV* kv, const Fna2PagedAttnArgs* args);
 int fna2_paged_attn(const Fna2PagedKV* kv, const Fna2PagedAttnArgs* args, void* workspace, size_t workspace_bytes,

@@ -173,6 +173,41 @@ def test_strides_and_layouts(new):
     _close_lse(lse, rl)
 
 
+@pytest.mark.parametrize("new", [[1] * 150, [2] * 131 + [40] * 3])
+def test_many_sequences(new):
+    """More sequences than a CTA looks through at once, lengths from 0 on; one of many more keys than the rest."""
+    from fna2_b200.paged import flash_naylis_paged, naylis_key_weights
+    lens = [b * 7 % 90 for b in range(len(new))]
+    lens[77] = 5000
+    x = _make(lens, new, 2, 1, 2, 64, 16, 16, 3)
+    d, pool = _dev(x), _pool(x)
+    out, lse = flash_naylis_paged(d["q"], pool, d["table"], d["lens"], d["cu"], max(new), r_q=d["rq"],
+                                  graph_scale=d["gs"], return_lse=True)
+    ro, rl, rw = PO.attention(x, True)
+    _close_out("out", out, ro)
+    _close_lse(lse, rl)
+    _close_w(naylis_key_weights(d["q"], lse, pool, d["table"], d["lens"], d["cu"], max(new), r_q=d["rq"],
+                                graph_scale=d["gs"]), rw)
+    assert _status() == 0
+
+
+@pytest.mark.parametrize("T", [0, 3, 200])
+def test_key_weights_start_from_zero(T):
+    """Fresh weights: also those of keys past a sequence's end, and without a query."""
+    from fna2_b200.paged import naylis_key_weights
+    x = _make([300, 40], [T, 0], 4, 2, 4, 64, 16, 32, 5)
+    d, pool = _dev(x), _pool(x)
+    lse = torch.zeros(4, T, device="cuda")
+    shape = (2, 2, x["table"].shape[1] * 32)
+    dirty = [torch.full(shape, float("nan"), device="cuda") for _ in range(4)]
+    del dirty  # their memory is handed out again
+    w = naylis_key_weights(d["q"], lse, pool, d["table"], d["lens"], d["cu"], T, r_q=d["rq"], graph_scale=d["gs"])
+    w2 = naylis_key_weights(d["q"], lse, pool, d["table"], d["lens"], d["cu"], T, r_q=d["rq"], graph_scale=d["gs"],
+                            key_weights=torch.zeros(shape, device="cuda"))
+    assert torch.equal(w, w2) and (w[1] == 0).all() and (w[0, :, 300:] == 0).all() and (T == 0 or (w[0] > 0).any())
+    assert _status() == 0
+
+
 def test_rows_equal_prefill_and_chunks_agree():
     """A prompt attended in chunks over the pages equals the packed prefill op, row for row."""
     from fna2_b200 import flash_naylis_attn
@@ -260,6 +295,8 @@ EVICT = [
     ([70], 2, 1, 0, 128, 16, 32, 64, 64, 0),   # only the newest
     ([40, 41], 2, 2, 2, 64, 32, 16, 1, 0, 1),  # only the first
     ([5000], 3, 3, 3, 64, 24, 128, 4999, 10, 3),
+    ([50000, 7], 1, 1, 1, 64, 8, 128, 1000, 100, 4),  # weights that do not fit in shared memory
+    ([49500], 2, 1, 1, 64, 8, 128, 500, 10, 0),
 ]
 
 

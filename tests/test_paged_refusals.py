@@ -98,6 +98,14 @@ def test_key_weights_refuse(args):
     _refused(_lib.load().fna2_key_weights(kv, at, None, 0, None), "key_weights")
 
 
+@pytest.mark.parametrize("clear,stride,offset,msg", [(96, 128, 0, "below max_seqlen_k"), (102, 128, 0, "multiple of 4"),
+                                                      (128, 129, 0, "aligned"), (128, 128, 4, "aligned")])
+def test_cleared_key_weights_refuse(args, clear, stride, offset, msg):
+    kv, at, _, _, _ = args
+    at.key_weights, at.kw_batch_stride, at.kw_head_stride, at.kw_clear = at.q + offset, 2 * stride, stride, clear
+    _refused(_lib.load().fna2_key_weights(kv, at, None, 0, None), msg)
+
+
 @pytest.mark.parametrize("field,value,msg", [
     ("in_dtype", 5, "in_dtype"), ("rope_dtype", 7, "rope_dtype"), ("eps", -1.0, "eps"),
     ("cu_seqlens", None, "null sequence"), ("total_tokens", -1, "bad sizes"), ("q_weight", 256, "both RMSNorm"),
