@@ -960,6 +960,7 @@ extern "C" int fna2_paged_attn(const Fna2PagedKV* kv, const Fna2PagedAttnArgs* a
   if (int rc = paged_queries(kv, a, &p)) return rc;
   p.inv_scale = 1.f / p.scale;
   if (int rc = paged_plan(kv, a, &p, &l)) return rc;
+  p.after_many = l.many;
   if (p.bd.B == 0 || p.bd.T == 0) return FNA2_OK;
   FNA2_CHECK(a->out != nullptr && aligned16(a->out) && strides_ok({a->out_token_stride, a->out_head_stride}),
              "out must be 16-byte aligned with strides of multiples of 8 elements");
@@ -985,7 +986,7 @@ extern "C" int fna2_paged_attn(const Fna2PagedKV* kv, const Fna2PagedAttnArgs* a
     if (int rc = many_maps(p, kv->head_dim, &m)) return rc;
     FNA2_CUDA(launch_paged_many(m, p, kv->head_dim, st));
   }
-  if (l.few) FNA2_CUDA(launch_paged_few(p, kv->head_dim, l.RW, l.smem, l.many, st));
+  if (l.few) FNA2_CUDA(launch_paged_few(p, kv->head_dim, l.RW, l.smem, st));
   if (l.many_join) FNA2_CUDA(launch_paged_many_join(p, kv->head_dim, st));
   if (l.few_join) FNA2_CUDA(launch_paged_few_join(p, kv->head_dim, st));
   if (l.logits && p.bd.max_k > 0) FNA2_CUDA(launch_logit_weights(p, st));

@@ -68,6 +68,8 @@ __global__ void __launch_bounds__(kAppendThreads, 10) fna2_append_kernel(const A
   __shared__ float s_cos[D / 2], s_sin[D / 2];
   __shared__ int s_seq[4];  // page id (-1: skip the token), slot, position
   const int t = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, sub = lane % LPR;
+  pdl_wait();
+  pdl_trigger();
   if (warp == 0) {
     const int b = warp_seq_of(p.cu, p.B, t, lane);
     int page = -1, slot = 0, pos = 0;
@@ -177,11 +179,9 @@ __global__ void __launch_bounds__(kAppendThreads, 10) fna2_append_kernel(const A
 }
 
 inline cudaError_t launch_append(const AppendParams& p, int D, int elem_bytes, cudaStream_t stream) {
-  if (D == 128 && elem_bytes == 2) fna2_append_kernel<128, 2><<<p.T, kAppendThreads, 0, stream>>>(p);
-  else if (D == 128) fna2_append_kernel<128, 4><<<p.T, kAppendThreads, 0, stream>>>(p);
-  else if (elem_bytes == 2) fna2_append_kernel<64, 2><<<p.T, kAppendThreads, 0, stream>>>(p);
-  else fna2_append_kernel<64, 4><<<p.T, kAppendThreads, 0, stream>>>(p);
-  return cudaGetLastError();
+  auto kern = D == 128 ? (elem_bytes == 2 ? fna2_append_kernel<128, 2> : fna2_append_kernel<128, 4>)
+                       : (elem_bytes == 2 ? fna2_append_kernel<64, 2> : fna2_append_kernel<64, 4>);
+  return launch_dependent(kern, p.T, kAppendThreads, 0, stream, p);
 }
 
 }  // namespace fna2

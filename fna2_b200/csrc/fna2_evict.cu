@@ -118,6 +118,7 @@ __global__ void __launch_bounds__(kSelThreads) fna2_evict_select_kernel(const Ev
   __shared__ int s_warp[2][32];
   __shared__ int s_digit, s_above;
   const int kh = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  pdl_wait();
   int len = __ldg(p.lens + b);
   if (len < 0 || len > p.max_k) {
     if (tid == 0) atomicCAS(&g_device_error, 0, kStatusBadSeqEvict);
@@ -317,11 +318,9 @@ cudaError_t launch_evict_select(const EvictParams& p, cudaStream_t stream) {
     static std::atomic<uint64_t> allowed{0};
     const cudaError_t e = allow_smem(reinterpret_cast<const void*>(kern), allowed, kStagedKeys * 4);
     if (e != cudaSuccess) return e;
-    kern<<<heads, kSelThreads, (p.max_k + 3) / 4 * 16, stream>>>(p);
-  } else {
-    fna2_evict_select_kernel<MOVE, false><<<heads, kSelThreads, 0, stream>>>(p);
+    return launch_dependent(kern, heads, kSelThreads, (p.max_k + 3) / 4 * 16, stream, p);
   }
-  return cudaGetLastError();
+  return launch_dependent(fna2_evict_select_kernel<MOVE, false>, heads, kSelThreads, 0, stream, p);
 }
 
 inline cudaError_t launch_evict(const EvictParams& p, cudaStream_t stream) {

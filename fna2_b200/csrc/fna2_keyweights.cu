@@ -54,6 +54,7 @@ struct KeyWeightsParams {
 // If weights are set: 0 for the keys that no query sees.  R~_q = gs/scale * R_q as hi + lo, columns [rank, RP) zero, and -LSE/scale = l1 + l2 + l3 (a row
 // without weight: -1e38, whose weights are 0).
 __global__ void __launch_bounds__(256) fna2_key_weights_prep_kernel(const KeyWeightsParams p) {
+  pdl_wait();
   pdl_trigger();
   const int64_t e = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
   if (e == 0) *p.next = p.ctas;
@@ -826,8 +827,7 @@ inline cudaError_t launch_key_weights_prep(const KeyWeightsParams& p, cudaStream
   const int64_t n = static_cast<int64_t>(p.bd.T) * p.H * (p.RP / 8 + 1);
   const int64_t rows = p.clear > 0 ? static_cast<int64_t>(p.bd.B) * p.kv.hkv : 0;
   const int64_t blocks = std::max<int64_t>((n + 255) / 256, std::min<int64_t>(std::max<int64_t>(rows, 1), 4 * kSms));
-  fna2_key_weights_prep_kernel<<<static_cast<unsigned>(blocks), 256, 0, stream>>>(p);
-  return cudaGetLastError();
+  return launch_dependent(fna2_key_weights_prep_kernel, static_cast<unsigned>(blocks), 256, 0, stream, p);
 }
 
 template <int D, int RP>

@@ -76,6 +76,7 @@ struct PagedAttnParams {
   // fna2_paged_many_kernel, the others to fna2_paged_few_kernel; a call launches those it may need.
   int few_rows;
   int chunk_many, many_items;  // keys per split there, upper bound on its (query tile pair, split) items
+  int after_many;  // the few-row kernel runs after the tensor-core kernel, on the SMs that it leaves
 };
 
 // Units of one sequence in the mma.sync kernel: 0 when it is not this kernel's.
@@ -154,6 +155,7 @@ __device__ __forceinline__ void few_store(const PagedAttnParams& p, int64_t tok,
 template <int D, int RW>
 __global__ void __launch_bounds__(kFewThreads, 2) fna2_paged_few_kernel(const PagedAttnParams p) {
   constexpr int KW = 4 / RW;  // key groups per CTA
+  if (!p.after_many) pdl_wait();
   pdl_trigger();
   extern __shared__ __align__(16) uint8_t dsm[];
   const int cta = blockIdx.x, lanes = p.kv.hkv * p.row_blocks, run = cta / lanes;
@@ -537,7 +539,7 @@ __global__ void __launch_bounds__(kFewThreads, 2) fna2_paged_few_kernel(const Pa
   }
   if (!more) break;
   }
-  pdl_wait();  // (a tensor-core kernel before this one has nothing that this one reads)
+  if (p.after_many) pdl_wait();  // (it has nothing that this one reads)
 }
 
 // Joins the sequences that were cut: a warp per (KV head, query row) rescales the
@@ -694,27 +696,24 @@ __global__ void __launch_bounds__(128) fna2_paged_many_join_kernel(const PagedAt
 // host side
 // ---------------------------------------------------------------------------
 template <int D, int RW>
-cudaError_t launch_paged_few_t(const PagedAttnParams& p, size_t smem, bool after_many, cudaStream_t stream) {
+cudaError_t launch_paged_few_t(const PagedAttnParams& p, size_t smem, cudaStream_t stream) {
   auto kern = fna2_paged_few_kernel<D, RW>;
   static std::atomic<uint64_t> allowed{0};
   cudaError_t e = allow_smem(reinterpret_cast<const void*>(kern), allowed);
   if (e != cudaSuccess) return e;
   const unsigned grid = p.runs * p.kv.hkv * p.row_blocks;
-  if (after_many) return launch_dependent(kern, grid, kFewThreads, smem, stream, p);  // fills the SMs it leaves
-  kern<<<grid, kFewThreads, smem, stream>>>(p);
-  return cudaGetLastError();
+  return launch_dependent(kern, grid, kFewThreads, smem, stream, p);
 }
 
 template <int D>
-cudaError_t launch_paged_few_d(const PagedAttnParams& p, int RW, size_t smem, bool after_many, cudaStream_t stream) {
-  return RW == 1   ? launch_paged_few_t<D, 1>(p, smem, after_many, stream)
-         : RW == 2 ? launch_paged_few_t<D, 2>(p, smem, after_many, stream)
-                   : launch_paged_few_t<D, 4>(p, smem, after_many, stream);
+cudaError_t launch_paged_few_d(const PagedAttnParams& p, int RW, size_t smem, cudaStream_t stream) {
+  return RW == 1   ? launch_paged_few_t<D, 1>(p, smem, stream)
+         : RW == 2 ? launch_paged_few_t<D, 2>(p, smem, stream)
+                   : launch_paged_few_t<D, 4>(p, smem, stream);
 }
 
-inline cudaError_t launch_paged_few(const PagedAttnParams& p, int D, int RW, size_t smem, bool after_many,
-                                    cudaStream_t stream) {
-  return D == 128 ? launch_paged_few_d<128>(p, RW, smem, after_many, stream) : launch_paged_few_d<64>(p, RW, smem, after_many, stream);
+inline cudaError_t launch_paged_few(const PagedAttnParams& p, int D, int RW, size_t smem, cudaStream_t stream) {
+  return D == 128 ? launch_paged_few_d<128>(p, RW, smem, stream) : launch_paged_few_d<64>(p, RW, smem, stream);
 }
 
 inline cudaError_t launch_paged_few_join(const PagedAttnParams& p, int D, cudaStream_t stream) {

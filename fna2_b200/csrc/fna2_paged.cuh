@@ -92,7 +92,10 @@ __device__ __forceinline__ int warp_seq_of(const int* cu, int B, int64_t t, int 
 // Programmatic dependent launch: a kernel launched with launch_dependent may start while the kernel
 // before it runs its last CTAs, once all of those have called pdl_trigger or exited; pdl_wait returns
 // when that kernel is complete and its writes are visible.  Every kernel launched this way calls
-// pdl_wait in every thread that returns normally, so work after it in the stream is ordered as usual.
+// pdl_wait in a thread of every block, so work after it in the stream is ordered as usual.  The first
+// kernel of a call waits before it does anything else, its trigger included: the ones after it may read
+// the call's inputs without a wait of their own.  That launch saves about a microsecond of a small call
+// even then (append of 48 tokens 14.2 -> 13.5 us, attention of 16 drafts 30.8 -> 29.1).
 __device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 

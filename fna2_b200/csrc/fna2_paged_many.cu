@@ -113,6 +113,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::oMisc);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::oMisc + 4);
   const int warp = warp_id(), lane = lane_id(), tid = threadIdx.x;
+  pdl_wait();
   pdl_trigger();
 
   ManyItem it;
@@ -507,8 +508,7 @@ cudaError_t launch_paged_many_t(const ManyMaps& m, const PagedAttnParams& p, cud
   static std::atomic<uint64_t> allowed{0};
   cudaError_t e = allow_smem(reinterpret_cast<const void*>(kern), allowed);
   if (e != cudaSuccess) return e;
-  kern<<<dim3(p.H, p.many_items), kFwdThreads, L::kTotal, stream>>>(m.q, m.k, m.v, m.rq, m.rk, p);
-  return cudaGetLastError();
+  return launch_dependent(kern, dim3(p.H, p.many_items), kFwdThreads, L::kTotal, stream, m.q, m.k, m.v, m.rq, m.rk, p);
 }
 
 inline cudaError_t launch_paged_many(const ManyMaps& m, const PagedAttnParams& p, int D, cudaStream_t stream) {

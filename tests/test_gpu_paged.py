@@ -267,6 +267,53 @@ def test_other_stream_and_repeat():
         assert torch.equal(a, b)
 
 
+def test_back_to_back_and_captured_calls():
+    """Operators that follow each other without a pause, directly and from a captured graph: each one's
+    results, read by the next, are complete (bit for bit the results of calls with pauses between them)."""
+    from fna2_b200.paged import flash_naylis_paged, naylis_evict, naylis_key_weights, qk_norm_rope_append
+    new, lens = [1, 120, 3], [900, 500, 64]
+    x = _make(lens, new, 4, 2, 4, 128, 16, 64, 9)
+    d = _dev(x)
+    T, before = sum(new), torch.tensor([a - b for a, b in zip(lens, new)], dtype=torch.int32, device="cuda")
+    g = torch.Generator().manual_seed(1)
+    k, v = (torch.randn(T, 2, 128, generator=g).bfloat16().cuda() for _ in range(2))
+    rk = torch.randn(T, 4, 16, generator=g).bfloat16().cuda()
+    extra = 3 * 2  # pages of the compacted sequences
+    for n in ("kp", "vp", "rp"):
+        x[n] = torch.cat([x[n].nan_to_num(0.0), torch.zeros(extra, *x[n].shape[1:]).bfloat16()])
+    tout = (torch.arange(extra, dtype=torch.int32) + x["kp"].shape[0] - extra).reshape(3, 2).cuda()
+
+    def chain(pool, pause):
+        wait = torch.cuda.synchronize if pause else lambda: None
+        q = qk_norm_rope_append(d["q"], k, v, pool, d["table"], before, d["cu"], r_k=rk)
+        wait()
+        w = torch.zeros(3, 2, x["table"].shape[1] * 64, device="cuda")
+        out, lse = flash_naylis_paged(q, pool, d["table"], d["lens"], d["cu"], 120, r_q=d["rq"], graph_scale=d["gs"],
+                                      return_lse=True, key_weights=w)
+        wait()
+        w2 = naylis_key_weights(q, lse, pool, d["table"], d["lens"], d["cu"], 120, r_q=d["rq"], graph_scale=d["gs"])
+        wait()
+        kept, n, wo = naylis_evict(w2, pool, d["table"], d["lens"], 100, tout, recent=8, sink=2, heads=4)
+        wait()
+        one = torch.arange(4, dtype=torch.int32, device="cuda")
+        last = flash_naylis_paged(q[:3], pool, tout, n, one, 1, r_q=d["rq"][:3], graph_scale=d["gs"])
+        return q, out, lse, w, w2, kept, n, wo, last
+    want = chain(_pool(x), True)
+    fresh = _pool(x)
+    torch.cuda.synchronize()
+    got = chain(fresh, False)
+    pool = _pool(x)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = chain(pool, False)
+    for _ in range(3):
+        graph.replay()
+    torch.cuda.synchronize()
+    for a, b, c in zip(want, got, captured):
+        assert torch.equal(a, b) and torch.equal(a, c)
+    assert _status() == 0
+
+
 def test_bad_lengths_are_skipped_and_recorded():
     from fna2_b200.paged import flash_naylis_paged, naylis_evict, naylis_key_weights
     x = _make([300, 200, 100], [1, 1, 1], 4, 4, 4, 64, 16, 32, 2)
