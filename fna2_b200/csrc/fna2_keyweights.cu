@@ -176,28 +176,45 @@ __device__ __forceinline__ void kw_write_ones(uint8_t* dst) {
   fence_proxy_async_smem();
 }
 
-// Sum over the QT columns of this thread's lane of 2^(sl2 S); MASK: of columns [lo, hi) only.
-// (Two copies: masks cost 5 instructions per column.)
-template <int QT, bool MASK>
-__device__ __forceinline__ float kw_sum(uint32_t t_addr, float2 sl2, int lo, int hi) {
+// Sum over columns [lo, hi) of this thread's lane of 2^(sl2 S), 16 at a time; `hi` is the warp's, `lo` the
+// thread's.  (Masks cost 5 instructions per column: `cut` says whether some thread of the tile has lo > 0,
+// and the chunk that hi ends in needs them; two loops, so that the common one stays unrolled.)
+template <int QT>
+__device__ __forceinline__ float kw_sum(uint32_t t_addr, float2 sl2, int lo, int hi, bool cut) {
   float2 a[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
   uint32_t r[2][16];
   tmem_ld16(t_addr, r[0]);
+  if (!cut && hi >= QT) {
 #pragma unroll
-  for (int c = 0; c < QT / 16; ++c) {
-    uint32_t* x = r[c & 1];
-    tmem_ld_wait16(x);
-    if (c + 1 < QT / 16) tmem_ld16(t_addr + 16 * (c + 1), r[(c + 1) & 1]);
+    for (int c = 0; c < QT / 16; ++c) {
+      uint32_t* x = r[c & 1];
+      tmem_ld_wait16(x);
+      if (c + 1 < QT / 16) tmem_ld16(t_addr + 16 * (c + 1), r[(c + 1) & 1]);
 #pragma unroll
-    for (int k = 0; k < 16; k += 2) {
-      const float2 y = __fmul2_rn(f32x2(x[k], x[k + 1]), sl2);
-      float2 e = make_float2(ex2(y.x), ex2(y.y));
-      if (MASK) {
-        const int col = 16 * c + k;
-        e.x = col >= lo && col < hi ? e.x : 0.f;
-        e.y = col + 1 >= lo && col + 1 < hi ? e.y : 0.f;
+      for (int k = 0; k < 16; k += 2) {
+        const float2 y = __fmul2_rn(f32x2(x[k], x[k + 1]), sl2);
+        a[k / 2 & 1] = __fadd2_rn(a[k / 2 & 1], make_float2(ex2(y.x), ex2(y.y)));
       }
-      a[k / 2 & 1] = __fadd2_rn(a[k / 2 & 1], e);
+    }
+  } else {
+#pragma unroll 1
+    for (int c0 = 0; c0 < QT && c0 < hi; c0 += 32) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int c = c0 + 16 * i;
+        uint32_t* x = r[i];
+        tmem_ld_wait16(x);
+        if (c + 16 < QT && c + 16 < hi) tmem_ld16(t_addr + c + 16, r[i ^ 1]);
+        if (c >= hi) continue;
+#pragma unroll
+        for (int k = 0; k < 16; k += 2) {
+          const float2 y = __fmul2_rn(f32x2(x[k], x[k + 1]), sl2);
+          float2 e = make_float2(ex2(y.x), ex2(y.y));
+          e.x = c + k >= lo && c + k < hi ? e.x : 0.f;
+          e.y = c + k + 1 >= lo && c + k + 1 < hi ? e.y : 0.f;
+          a[k / 2 & 1] = __fadd2_rn(a[k / 2 & 1], e);
+        }
+      }
     }
   }
   return (a[0].x + a[0].y) + (a[1].x + a[1].y);
@@ -418,8 +435,7 @@ __global__ void __launch_bounds__(kKwThreads, 1)
           // columns [first, nq - i0) belong to queries that see the key; the score of another sequence's
           // query is never read into a sum
           const int first = p.causal ? j - past - i0 : 0;
-          const bool whole = (!p.causal || tile0 + kBlockN - 1 <= past + i0) && i0 + QT <= nq;
-          w += whole ? kw_sum<QT, false>(at, sl2, 0, 0) : kw_sum<QT, true>(at, sl2, first, nq - i0);
+          w += kw_sum<QT>(at, sl2, first, nq - i0, p.causal && tile0 + kBlockN - 1 > past + i0);
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(&bars[kWbSEmpty + buf]);
@@ -763,10 +779,8 @@ __global__ void __launch_bounds__(kKwThreads, 1)
           tc_fence_after();
           // columns [first, nq) belong to queries that see the key; the score of another sequence's query
           // or of a head that the pair lacks is never read into a sum
-          const bool whole = (!p.causal || tile0 + kBlockN - 1 <= past) && nq == QT;
           if (2 * u + wi < heads)
-            w += whole ? kw_sum<QT, false>(t_lane + 128 * buf, sl2, 0, 0)
-                       : kw_sum<QT, true>(t_lane + 128 * buf, sl2, first, nq);
+            w += kw_sum<QT>(t_lane + 128 * buf, sl2, first, nq, p.causal && tile0 + kBlockN - 1 > past);
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(&bars[kVbSEmpty + buf]);
