@@ -33,13 +33,13 @@ struct RowPlace {
   int sp, ss, dp, ds;  // source page (-1: none) and slot, destination page and slot
 };
 
-// Copies kept rows [r0, r0 + ROWS) of (sequence b, KV head kh) with a block of THREADS threads.
+// Copies kept rows [r0, r1), at most ROWS of them, of (sequence b, KV head kh) with a block of THREADS threads.
 template <int THREADS, int ROWS>
-__device__ __forceinline__ void move_rows(const EvictParams& p, int b, int kh, int r0, RowPlace* s_at) {
-  const int* kept = p.kept + (static_cast<int64_t>(b) * p.kv.hkv + kh) * p.budget;
-  const int mask = (1 << p.kv.page_log2) - 1, tid = threadIdx.x;
-  if (tid < ROWS) {
-    const int r = r0 + tid, j = r < p.budget ? kept[r] : -1;
+__device__ __forceinline__ void move_rows(const EvictParams& p, int b, int kh, int r0, int r1, const int* kept,
+                                          RowPlace* s_at) {
+  const int mask = (1 << p.kv.page_log2) - 1, tid = threadIdx.x, rows = min(ROWS, r1 - r0);
+  if (tid < rows) {
+    const int r = r0 + tid, j = kept[r];
     RowPlace a{-1, j & mask, -1, r & mask};
     if (j >= 0) {
       a.sp = __ldg(p.kv.table + b * p.kv.table_sb + (j >> p.kv.page_log2));
@@ -58,14 +58,14 @@ __device__ __forceinline__ void move_rows(const EvictParams& p, int b, int kh, i
   const int sub = lane % lpr, is_v = sub >= lpr / 2, col = sub % (lpr / 2) * 8;
   const PagedRows kv = {is_v ? p.kv.v.ptr : p.kv.k.ptr, is_v ? p.kv.v.sp : p.kv.k.sp, is_v ? p.kv.v.st : p.kv.k.st,
                         is_v ? p.kv.v.sh : p.kv.k.sh};
-  for (int base = warp * rpw * U; base < ROWS; base += THREADS / 32 * rpw * U) {
+  for (int base = warp * rpw * U; base < rows; base += THREADS / 32 * rpw * U) {
     uint4 v[U];
     __nv_bfloat16* dst[U];
 #pragma unroll
     for (int i = 0; i < U; ++i) {
       const int r = base + i * rpw + lane / lpr;
       dst[i] = nullptr;
-      if (r < ROWS && s_at[r].sp >= 0) {
+      if (r < rows && s_at[r].sp >= 0) {
         const RowPlace a = s_at[r];
         v[i] = *reinterpret_cast<const uint4*>(kv.ptr + paged_off(kv, a.sp, a.ss, kh) + col);
         dst[i] = kv.ptr + paged_off(kv, a.dp, a.ds, kh) + col;
@@ -77,14 +77,14 @@ __device__ __forceinline__ void move_rows(const EvictParams& p, int b, int kh, i
   }
   // R_k of the KV head's query heads
   const int r8 = p.kv.rank / 8, pieces = max(0, min(p.G, p.kv.hg - kh * p.G)) * r8;
-  for (int base = tid; base < ROWS * pieces; base += THREADS * U) {
+  for (int base = tid; base < rows * pieces; base += THREADS * U) {
     uint4 v[U];
     __nv_bfloat16* dst[U];
 #pragma unroll
     for (int i = 0; i < U; ++i) {
       const int e = base + i * THREADS, r = e / pieces, c = e % pieces;
       dst[i] = nullptr;
-      if (e < ROWS * pieces && s_at[r].sp >= 0) {
+      if (e < rows * pieces && s_at[r].sp >= 0) {
         const RowPlace a = s_at[r];
         const int64_t at = (kh * p.G + c / r8) * p.kv.rk.sh + c % r8 * 8;
         v[i] = *reinterpret_cast<const uint4*>(p.kv.rk.ptr + paged_off(p.kv.rk, a.sp, a.ss, 0) + at);
@@ -97,6 +97,10 @@ __device__ __forceinline__ void move_rows(const EvictParams& p, int b, int kh, i
   }
 }
 
+// Kept rows up to which the select kernel moves them itself.  Of 4 sequences, 4 heads that takes as long on the
+// GPU as two kernels do (512 rows 8.4 us) and spares the host a launch (16.0 against 18.3 us per call); of 32
+// sequences 512 rows take 14.4 against 15.8 us, 1,024 rows 21.4 against 22.9.
+constexpr int kFusedBudget = 1024;
 constexpr int kSelThreads = 1024;
 constexpr int kSelBins = 2048;
 constexpr int kHistCopies = 2;  // lanes that count the same bin at once wait for each other: even and odd ones apart
@@ -107,14 +111,16 @@ __device__ __forceinline__ uint32_t ordered_bits(float x) {
   return x != x ? 0u : static_cast<uint32_t>(u ^ (u >> 31 | static_cast<int>(0x80000000u)));
 }
 
-// MOVE: the block also copies its rows (short sequences: one launch instead of two).  STAGED: the
+// MOVE: the block also copies rows (small budgets: one launch instead of two).  Then several blocks (z) find
+// the same keys, as long as there are SMs, and each copies its share of their rows.  STAGED: the
 // sequence's weights fit in shared memory and are read from there after the first pass (each pass over
 // 16,384 weights in global memory took 7 us, latency of dependent loads).
 template <bool MOVE, bool STAGED>
 __global__ void __launch_bounds__(kSelThreads) fna2_evict_select_kernel(const EvictParams p) {
   extern __shared__ float s_w[];
   __shared__ int hist[kHistCopies][kSelBins];
-  __shared__ RowPlace s_at[MOVE ? kSelThreads : 1];
+  __shared__ RowPlace s_at[MOVE ? kFusedBudget : 1];
+  __shared__ int s_kept[MOVE ? kFusedBudget : 1];
   __shared__ int s_warp[2][32];
   __shared__ int s_digit, s_above;
   const int kh = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -223,9 +229,13 @@ __global__ void __launch_bounds__(kSelThreads) fna2_evict_select_kernel(const Ev
   if (!all && !some) prefix = 0xffffffffu;  // above every weight
   int* kept = p.kept + (static_cast<int64_t>(b) * p.kv.hkv + kh) * p.budget;
   float* w_out = p.w_out + (static_cast<int64_t>(b) * p.kv.hkv + kh) * p.cap_out;
-  for (int j = tid; j < old_beg; j += kSelThreads) kept[j] = j, w_out[j] = STAGED ? s_w[j] : __ldg(w + j);
-  for (int j = old_end + tid; j < len; j += kSelThreads)
-    kept[keep - len + j] = j, w_out[keep - len + j] = STAGED ? s_w[j] : __ldg(w + j);
+  const bool writes = !MOVE || blockIdx.z == 0;
+  auto put = [&](int pos, int j, float x) {
+    if (MOVE) s_kept[pos] = j;
+    if (writes) kept[pos] = j, w_out[pos] = x;
+  };
+  for (int j = tid; j < old_beg; j += kSelThreads) put(j, j, STAGED ? s_w[j] : __ldg(w + j));
+  for (int j = old_end + tid; j < len; j += kSelThreads) put(keep - len + j, j, STAGED ? s_w[j] : __ldg(w + j));
   // Each warp owns a run of the keys: it counts the candidates that it takes, then writes from its offset on.
   const int run = (old_end + 4 * kSelThreads - 1) / (4 * kSelThreads) * 128;
   const int beg = min(old_end, warp * run), end = min(old_end, beg + run);
@@ -275,22 +285,22 @@ __global__ void __launch_bounds__(kSelThreads) fna2_evict_select_kernel(const Ev
     for (int i = 0; i < 4; ++i) {
       const bool take = mt >> i & 1, tie = me >> i & 1;
       if (take || (tie && e < want)) {
-        kept[a + min(e, want)] = j + i;
-        w_out[a + min(e, want)] = x[i];
+        put(a + min(e, want), j + i, x[i]);
       }
       a += take, e += tie;
     }
     const int total = __shfl_sync(0xffffffffu, incl, 31);
     takes_before += total & 0xffff, ties_before += total >> 16;
   }
-  for (int i = keep + tid; i < p.budget; i += kSelThreads) kept[i] = -1;
-  for (int i = keep + tid; i < p.cap_out; i += kSelThreads) w_out[i] = 0.f;
-  if (kh == 0 && tid == 0) p.lens_out[b] = keep;
+  if (writes) {
+    for (int i = keep + tid; i < p.budget; i += kSelThreads) kept[i] = -1;
+    for (int i = keep + tid; i < p.cap_out; i += kSelThreads) w_out[i] = 0.f;
+    if (kh == 0 && tid == 0) p.lens_out[b] = keep;
+  }
   if (MOVE) {
-    for (int r0 = 0; r0 < keep; r0 += kSelThreads) {
-      __syncthreads();  // kept is written; s_at has been read
-      move_rows<kSelThreads, kSelThreads>(p, b, kh, r0, s_at);
-    }
+    __syncthreads();  // s_kept is written
+    const int z = blockIdx.z, nz = gridDim.z;
+    move_rows<kSelThreads, kFusedBudget>(p, b, kh, keep * z / nz, keep * (z + 1) / nz, s_kept, s_at);
   }
 }
 
@@ -300,19 +310,17 @@ constexpr int kMoveRows = 32;
 __global__ void __launch_bounds__(kMoveThreads) fna2_evict_move_kernel(const EvictParams p) {
   __shared__ RowPlace s_at[kMoveRows];
   pdl_wait();
-  move_rows<kMoveThreads, kMoveRows>(p, blockIdx.z, blockIdx.y, blockIdx.x * kMoveRows, s_at);
+  const int b = blockIdx.z, kh = blockIdx.y, r0 = blockIdx.x * kMoveRows;
+  move_rows<kMoveThreads, kMoveRows>(p, b, kh, r0, p.budget, p.kept + (static_cast<int64_t>(b) * p.kv.hkv + kh) * p.budget,
+                                     s_at);
 }
 
-// A block of the select kernel moves about 60 GB/s; up to this many kept rows that costs less than a
-// second launch.
-constexpr int kFusedBudget = 512;
-
-// Weights whose ordered bits fit in shared memory beside the histogram.
-constexpr int kStagedKeys = 48 * 1024;
+// Weights that fit in shared memory beside the histograms and the kept rows' places.
+constexpr int kStagedKeys = 40 * 1024;
 
 template <bool MOVE>
 cudaError_t launch_evict_select(const EvictParams& p, cudaStream_t stream) {
-  const dim3 heads(p.kv.hkv, p.B);
+  const dim3 heads(p.kv.hkv, p.B, MOVE ? std::max(1, std::min(8, kSms / (p.kv.hkv * p.B))) : 1);
   if (p.max_k <= kStagedKeys) {
     auto kern = fna2_evict_select_kernel<MOVE, true>;
     static std::atomic<uint64_t> allowed{0};
