@@ -789,22 +789,29 @@ int many_splits(int64_t base, int64_t tiles, double row_bytes) {
 
 int paged_plan(const Fna2PagedKV* kv, const Fna2PagedAttnArgs* a, PagedAttnParams* p, PagedPlan* l) {
   const int D = kv->head_dim, max_rows = std::max(1, p->bd.max_q * p->G);
-  const bool all_few = max_rows <= kFewRows;
+  const int few_limit = std::min(kFewRows, kFewTokens * p->G);
+  const bool all_few = max_rows <= few_limit;
   l->few = all_few || p->bd.B > 1;
   l->many = !all_few;
   p->few_rows = all_few ? max_rows : l->few ? kFewRowsMixed : 0;
   const int few_max = std::min(max_rows, p->few_rows);
-  l->RW = !all_few || max_rows <= 16 ? 1 : max_rows <= 32 ? 2 : 4;
-  for (;; l->RW /= 2) {
-    p->ng_max = std::min({p->G, 16 * l->RW, p->kv.hg});
+  auto fits = [&](int RW, int stages, int bytes) {
+    l->RW = RW;
+    p->ng_max = std::min({p->G, 16 * RW, p->kv.hg});
     p->nh_max = std::min({p->G, 16, p->kv.hg});
     // ring depth: about 64 KB of tiles per CTA, at most 4 and at least 2 of them
-    const FewSmem one(D, l->RW, p->ng_max, p->nh_max, p->RP, 1, p->few_rows);
-    p->stages = std::max(2, std::min(4, 72 * 1024 / ((one.kv_stage + one.r_stage) * (4 / l->RW))));
-    l->smem = FewSmem(D, l->RW, p->ng_max, p->nh_max, p->RP, p->stages, p->few_rows).total;
-    if (l->smem <= kMaxDynamicSmem || l->RW == 1) break;
-  }
-  FNA2_CHECK(l->smem <= kMaxDynamicSmem, "heads per KV head and rank need too much shared memory");
+    const FewSmem one(D, RW, p->ng_max, p->nh_max, p->RP, 1, p->few_rows);
+    p->stages = std::max(2, std::min(stages, 72 * 1024 / ((one.kv_stage + one.r_stage) * (4 / RW))));
+    l->smem = FewSmem(D, RW, p->ng_max, p->nh_max, p->RP, p->stages, p->few_rows).total;
+    return l->smem <= bytes;
+  };
+  // As many row blocks as the rows fill, so that two CTAs fit on an SM; twice as many, with half the key
+  // groups and so half the rings, where only that lets two fit (16 rows, 4 graph heads, rank 16, D = 128, 8
+  // sequences of 4,000 keys: 38.7 us with one CTA per SM, 28.8 with two); else whatever fits.
+  const int fill = !all_few || max_rows <= 16 ? 1 : max_rows <= 32 ? 2 : 4;
+  bool found = fits(fill, 4, kHalfSmem);
+  for (int stages = 4; !found && fill <= 2 && stages >= 2; --stages) found = fits(2 * fill, stages, kHalfSmem);
+  for (int RW = fill; !found && !(found = fits(RW, 4, kMaxDynamicSmem)) && RW > 1;) RW /= 2;
   p->block_rows = 16 * l->RW;
   p->unit_keys = 64 / l->RW;
   p->row_blocks = std::max(1, (few_max + p->block_rows - 1) / p->block_rows);
@@ -830,7 +837,7 @@ int paged_plan(const Fna2PagedKV* kv, const Fna2PagedAttnArgs* a, PagedAttnParam
     p->many_items = static_cast<int>((pairs + longer) * ns);
     p->ns = static_cast<int>(ns);
   }
-  l->logits = p->kw && all_few;
+  l->logits = p->kw && all_few && max_rows <= kLogitRows;
   l->many_join = l->many && p->ns > 1;
   l->few_join = l->few && !p->whole && p->runs > 1;
   p->logit_sr = (static_cast<int64_t>(p->bd.max_k) + 15) / 16 * 16;

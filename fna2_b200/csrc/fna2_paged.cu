@@ -92,11 +92,23 @@ __device__ __forceinline__ int few_runs(const PagedAttnParams& p, int64_t U) {
 __device__ __forceinline__ int64_t few_first(int64_t U, int C, int c) { return U * c / C; }
 __device__ __forceinline__ int few_run_of(int64_t U, int C, int64_t u) { return static_cast<int>(((u + 1) * C - 1) / U); }
 
-// Query rows per KV head (new tokens x query heads of the group) up to which a sequence is streamed
-// by the mma.sync kernel; above it the tensor-core kernel's 128-row tiles are worth filling.
-constexpr int kFewRows = 64;
-// ... in a call that has longer ones: its few-row sequences mostly add one token, in one 16-row block.
+// New tokens, and query rows per KV head (new tokens x query heads of the group), up to which a sequence is
+// streamed by the mma.sync kernel.  Its time goes by KV heads and blocks of up to 64 rows; the tensor-core
+// kernel's by query heads and 128-row tiles, however few rows fill them.  8 sequences of 4,000 keys, 16 query
+// heads, D = 128, mma.sync against tensor-core kernel: 32 tokens of 4 KV heads (128 rows) 57 / 74 us, 48
+// tokens 75 / 67; of 2 KV heads, 16 tokens (128 rows) 56 / 72, 24 tokens 80 / 73; of 16 KV heads, 32 tokens
+// (32 rows) 53 / 73, 64 tokens 94 / 73.
+constexpr int kFewTokens = 32;
+constexpr int kFewRows = 128;
+// Rows up to which the mma.sync kernel keeps its logits for the key weights, rather than have them formed
+// again by the key weights' kernels: 16 sequences of 1,000 to 4,000 keys, 8 KV heads, D = 128, kept / formed
+// again: 4 rows 55 / 83 us, 16 rows 81 / 102 us, 32 rows 89 / 99 us, 64 rows 146 / 132 us.
+constexpr int kLogitRows = 32;
+// ... rows in a call that has longer sequences: its few-row ones mostly add one token, in one 16-row block
+// (26 sequences, chunks of up to 500 tokens next to single ones: 123 us; up to 32 rows 158, 64 rows 250).
 constexpr int kFewRowsMixed = 16;
+// Dynamic shared memory of which two CTAs fit on an SM (228 KB, 1 KB reserved per CTA).
+constexpr int kHalfSmem = 113 * 1024;
 
 constexpr int kFewThreads = 128;
 constexpr int kFewKeys = 16;  // keys per tile
@@ -621,7 +633,7 @@ __global__ void __launch_bounds__(kTailThreads) fna2_paged_few_join_kernel(const
 constexpr int kLogitKeys = 4 * kTailThreads;
 
 __global__ void __launch_bounds__(kTailThreads) fna2_paged_logit_weights_kernel(const PagedAttnParams p) {
-  __shared__ float s_x[kFewRows];
+  __shared__ float s_x[kLogitRows];
   pdl_wait();
   const int kh = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
   const PagedSeq sq = paged_seq(p.bd, b);

@@ -12,7 +12,6 @@ namespace fna2 {
 constexpr int kSms = 148;  // of a B200
 
 // Site codes recorded in g_device_error (read by fna2_device_status).
-constexpr int kStatusSmemBase = 199;      // the dynamic shared memory base was not 1024-byte aligned
 constexpr int kStatusBadSeqAppend = 631;  // append: bad length / offsets, or a page id outside the pool
 constexpr int kStatusBadSeqPaged = 641;   // attention, key weights: bad length or offsets
 constexpr int kStatusBadSeqEvict = 651;   // eviction: bad length, or a page id outside the pool
