@@ -6,27 +6,35 @@
 // On the tensor cores, the transposed scores
 //   S^T - LSE/scale = [K | R_k | R_k | 1] [Q | R~_q hi | R~_q lo | -LSE/scale]^T
 // put a key on every TMEM lane, so the thread that owns a key sums its weights over
-// the columns in a register: no reduction between threads (but one addition, below),
-// no atomics on the result, which does not depend on timing.  The LSE is one more
-// K slice, three bf16 terms that hold its 24 bits, so that a column costs the sum
-// warps one exp2, half a multiplication and half an addition (packed pairs).  A small
-// kernel first writes the R~_q hi / lo and LSE columns.  Persistent CTAs, one per SM,
-// draw items from a counter and work on units of 128 columns:
+// the columns in a register: no reduction within a warp, no atomics on the result, which
+// does not depend on timing.  The LSE is one more K slice, three bf16 terms that hold its
+// 24 bits, so that a column costs the sum warps one exp2, half a multiplication and half an
+// addition (packed pairs).  A small kernel first writes the R~_q hi / lo and LSE columns.
+// Persistent CTAs, one per SM, work on units of 128 columns:
 //   fna2_key_weights_kernel         key-stationary: an item is a pair of 128-key tiles
-//     of a (sequence, KV head), a unit 128 queries of one head; warpgroup i sums key
-//     tile i, every Q tile serves both.
+//     of a (sequence, KV head), drawn from a counter (items differ: early keys are seen
+//     by more queries), a unit 128 queries of one head; every Q tile serves both.
+//     Warpgroup i sums key tile i % 2 of every second unit.
 //   fna2_key_weights_window_kernel  query-stationary, when no sequence has more than
-//     64 queries: an item is a run of key tiles, the queries of up to four heads stay
-//     in shared memory while K and R_k stream (streaming Q past each key tile instead
-//     took 128 KB per tile from L2 where this takes 48, and ran at its rate); a unit
-//     is two heads side by side (one N = 128 product with K, then each head's R_k
-//     against its half), warpgroup i sums head i's half, and the two are added.
-// Warps 0-7: sums (thread t = key t = TMEM lane t); warp 8: draws items, TMA (K and R_k
-// page by page, as in fna2_paged_many.cu); warp 9: TMEM allocation, MMA issue; warp 10:
-// waits for warp 9 (a wait by the warp that issued MMAs returns only when its own MMAs
-// have drained; a named barrier does not).
-// Bound: exp2, 16 per clock and SM (2048 clk for the 2 x 128 x 128 of a key-stationary
-// unit), beside about 100 clk per MMA and the operands' way from L2.
+//     64 queries: a CTA takes an equal run of all key tiles, the queries of up to four
+//     heads stay in shared memory while K and R_k stream (streaming Q past each key tile
+//     instead took 128 KB per tile from L2 where this takes 48: 64 queries, 4 caches of up
+//     to 16,000 keys, 32 heads 82 against 37 us, 8 heads 38 / 26); a unit is two heads side
+//     by side (one N = 128 product with K, then each head's R_k against its half).
+//     Warpgroup i sums head i % 2 of every second unit.
+// Warps 0-15: sums (four warps per scheduler: with two, waits between units showed); 16:
+// TMA (K and R_k page by page, as in fna2_paged_many.cu); 17: TMEM allocation, MMA issue;
+// 18: waits for warp 17 (a wait by the warp that issued MMAs returns only when its own MMAs
+// have drained; a named barrier does not); 19: adds the warpgroups' sums of a key tile and
+// updates the weights (a load per key that the sum warps would wait for).
+// Bound: the products.  The 26 MMAs of a unit pair take 1,860 clk: at M = N = 128 reading
+// both operands takes the whole bandwidth of shared memory, 64 clk each.  With loads and
+// hand-offs 2,450 clk key-stationary (4,095 queries and keys, 16 heads, D = 128, rank 32:
+// 55.5 us, 780 TFLOP/s), 2,400 per key tile query-stationary, where a tile's 48 KB also need
+// 2,900 clk from a freed stage to a full one and two stages fit (64 queries, 4 caches of up to
+// 16,000 keys, 8 KV heads of 4, rank 16: 37 us, 3.5 TB/s).  exp2 (2,048 clk of the same) is
+// not what bounds it: a polynomial on the FMA pipe for a quarter of them halved the sums' time
+// and changed neither kernel's.  Nor did two issuing warps, or two loading ones.
 #include "fna2_paged.cuh"
 
 namespace fna2 {

@@ -359,7 +359,8 @@ const char* fna2_last_error(void);
  *   1xx-10xx  a bounded mbarrier wait gave up after its budget (4 s): the
  *             kernel raised its CTA's abort flag, skipped the rest of the
  *             tile and deallocated its tensor memory (hundreds digit = kernel
- *             role: 1-3 forward, 4-7 dK/dV, 8-10 dQ);
+ *             role: 1-3 forward, paged attention and key weights, 4-7 dK/dV,
+ *             8-10 dQ);
  *   199, 499  the dynamic shared memory base was not 1024-byte aligned;
  *   601       decode: a cache length < 0 or above the capacity (zeros written);
  *   621       forward, packed batch: a sequence with inconsistent cu_seqlens
