@@ -775,8 +775,8 @@ size_t kw_workspace_bytes(int64_t T, int H, int RP) { return up256(static_cast<s
 
 // Splits of the tensor-core kernel's keys: `base` CTAs without splits, `tiles` key tiles each.  One
 // CTA runs per SM; a tile counts 2, a CTA's start and end 6, and the join moves 8 D bytes per row and
-// split.  Takes the count with the least estimate (26 sequences, chunks of up to 500 tokens: 2 splits,
-// the best of 1, 2, 3, 4 and 8; a chunk of 2,048 tokens over 30,717 keys: within 2 % from 1 to 8).
+// split.  Takes the count with the least estimate (a chunk of 2,048 tokens over 30,717 keys: 1,377 to
+// 1,418 us so, 1,429 and more unsplit, 1,419 to 1,439 with 4 splits, in one process).
 int many_splits(int64_t base, int64_t tiles, double row_bytes) {
   int best = 1;
   double best_us = 1e30;

@@ -27,10 +27,10 @@
 // 18: waits for warp 17 (a wait by the warp that issued MMAs returns only when its own MMAs
 // have drained; a named barrier does not); 19: adds the warpgroups' sums of a key tile and
 // updates the weights (a load per key that the sum warps would wait for).
-// Bound: the products.  The 26 MMAs of a unit pair take 1,860 clk: at M = N = 128 reading
-// both operands takes the whole bandwidth of shared memory, 64 clk each.  With loads and
-// hand-offs 2,450 clk key-stationary (4,095 queries and keys, 16 heads, D = 128, rank 32:
-// 55.5 us, 780 TFLOP/s), 2,400 per key tile query-stationary, where a tile's 48 KB also need
+// Bound: the products and their hand-offs.  The 26 MMAs of a unit (two key tiles) take 1,860
+// clk, 1,660 of them at the tensor pipe's rate; with waits and hand-offs a unit takes 2,450
+// clk key-stationary (4,095 queries and keys, 16 heads, D = 128, rank 32:
+// 55.5 us, 780 TFLOP/s), 2,400 per key tile and four heads query-stationary, where a tile's 48 KB also need
 // 2,900 clk from a freed stage to a full one and two stages fit (64 queries, 4 caches of up to
 // 16,000 keys, 8 KV heads of 4, rank 16: 37 us, 3.5 TB/s).  exp2 (2,048 clk of the same) is
 // not what bounds it: a polynomial on the FMA pipe for a quarter of them halved the sums' time
