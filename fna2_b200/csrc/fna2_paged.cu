@@ -122,14 +122,15 @@ constexpr int kFewKeys = 16;  // keys per tile
 // of a block's rows, nh: heads that the 16 rows of one warp span.
 struct FewSmem {
   int a_stride, kv_stage, r_head, r_stage, o_kv, o_r, o_join, o_bar, total;
-  // (of the row block's rows only `rows`, its bound, are joined)
+  // (of the row blocks' rows only `rows`, their bound, have a place in A and are joined)
   __host__ __device__ FewSmem(int D, int RW, int ng, int nh, int RP, int stages, int rows) {
     a_stride = (D + 2 * nh * RP) * 2 + 16;
     kv_stage = 2 * kFewKeys * D * 2;
     r_head = kFewKeys * RP * 2;
     r_stage = ng * r_head;
     const int rings = 4 / RW * stages;
-    o_kv = (16 * RW * a_stride + 1023) / 1024 * 1024;
+    const int blocks = rows < 16 * RW ? (rows + 15) / 16 : RW;  // row blocks that can hold a row
+    o_kv = (16 * blocks * a_stride + 1023) / 1024 * 1024;
     o_r = o_kv + rings * kv_stage;
     o_join = o_r + (rings * r_stage + 1023) / 1024 * 1024;
     o_bar = o_join + 512 + 4 / RW * (rows < 16 * RW ? rows : 16 * RW) * D * 4;
@@ -348,8 +349,10 @@ __global__ void __launch_bounds__(kFewThreads, 2) fna2_paged_few_kernel(const Pa
   const int wr0 = r0 + rw * 16;
   const int wg_lo = wr0 / sq.n, wg_hi = min(min(rows - 1, wr0 + 15) / sq.n, p.kv.hg - kh * p.G - 1);
   const int wn = wr0 < rows ? max(0, wg_hi - wg_lo + 1) : 0;
-  uint8_t* sa = dsm + rw * 16 * L.a_stride;
-  {
+  // (a warp that can hold no row computes on the first one's, for nobody: skipping cost the others 2 %)
+  const bool holds = RW == 1 || rw * 16 < p.few_rows;
+  uint8_t* sa = dsm + (holds ? rw : 0) * 16 * L.a_stride;
+  if (holds) {
     constexpr int TPR = 2 * KW;  // threads per row
     const int part = kg * 32 + lane, row = part / TPR, sub = part % TPR, r = wr0 + row;
     const bool real = r < rows;

@@ -106,6 +106,8 @@ CASES = [
     ([500, 130], [16, 9], 4, 4, 4, 64, 32, 128),
     ([130, 300, 5, 1], [130, 100, 5, 1], 4, 2, 3, 128, 32, 64),
     ([1000, 2, 700], [300, 1, 513], 2, 2, 2, 64, 16, 16),
+    ([600, 77, 1500], [1, 1, 1], 16, 2, 16, 128, 32, 64),  # wide rows of few tokens
+    ([600, 77, 1500], [1, 2, 2], 16, 2, 13, 128, 24, 64),
     ([3, 10], [7, 12], 4, 2, 4, 64, 16, 16),  # fewer cached keys than new tokens: the first rows see none
 ]
 
