@@ -799,11 +799,10 @@ int paged_plan(const Fna2PagedKV* kv, const Fna2PagedAttnArgs* a, PagedAttnParam
   auto fits = [&](int RW, int stages, int bytes) {
     l->RW = RW;
     p->ng_max = std::min({p->G, 16 * RW, p->kv.hg});
-    p->nh_max = std::min({p->G, 16, p->kv.hg});
     // ring depth: about 64 KB of tiles per CTA, at most 4 and at least 2 of them
-    const FewSmem one(D, RW, p->ng_max, p->nh_max, p->RP, 1, p->few_rows);
+    const FewSmem one(D, RW, p->ng_max, p->RP, 1, p->few_rows);
     p->stages = std::max(2, std::min(stages, 72 * 1024 / ((one.kv_stage + one.r_stage) * (4 / RW))));
-    l->smem = FewSmem(D, RW, p->ng_max, p->nh_max, p->RP, p->stages, p->few_rows).total;
+    l->smem = FewSmem(D, RW, p->ng_max, p->RP, p->stages, p->few_rows).total;
     return l->smem <= bytes;
   };
   // As many row blocks as the rows fill, so that two CTAs fit on an SM; twice as many, with half the key

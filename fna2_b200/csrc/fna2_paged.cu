@@ -75,7 +75,7 @@ struct PagedAttnParams {
   int whole;          // sequences are not cut (they are short): a unit is a sequence
   int runs;           // at most
   int row_blocks;     // row blocks per KV head; CTA = (run * HKV + KV head) * row_blocks + row block
-  int ng_max, nh_max, stages;
+  int ng_max, stages;
   // Sequences of more than few_rows query rows (new tokens x query heads of a KV head) go to
   // fna2_paged_many_kernel, the others to fna2_paged_few_kernel; a call launches those it may need.
   int few_rows;
@@ -119,12 +119,12 @@ constexpr int kFewKeys = 16;  // keys per tile
 
 // Shared-memory geometry (host and device agree on it): [A of the RW row blocks | K and V ring of
 // the key groups | R_k ring | m, l and accumulators of the key groups | scan]; ng: graph heads
-// of a block's rows, nh: heads that the 16 rows of one warp span.
+// of a block's rows.
 struct FewSmem {
   int a_stride, kv_stage, r_head, r_stage, o_kv, o_r, o_join, o_bar, total;
   // (of the row blocks' rows only `rows`, their bound, have a place in A and are joined)
-  __host__ __device__ FewSmem(int D, int RW, int ng, int nh, int RP, int stages, int rows) {
-    a_stride = (D + 2 * nh * RP) * 2 + 16;
+  __host__ __device__ FewSmem(int D, int RW, int ng, int RP, int stages, int rows) {
+    a_stride = (D + 2 * RP) * 2 + 16;
     kv_stage = 2 * kFewKeys * D * 2;
     r_head = kFewKeys * RP * 2;
     r_stage = ng * r_head;
@@ -155,6 +155,16 @@ __device__ __forceinline__ void few_cp16(uint32_t dst, const void* src, bool val
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
 }
 
+// d = a b + c
+__device__ __forceinline__ void mma_bf16_from(float (&d)[4], const float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
+                                              uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%10,%11,%12,%13};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
+}
+
 // Four columns of a finished row: O = acc / (l + 1e-6), LSE = m + log(l + 1e-6).
 template <int D>
 __device__ __forceinline__ void few_store(const PagedAttnParams& p, int64_t tok, int h, int d, float M, float Ls,
@@ -179,7 +189,7 @@ __global__ void __launch_bounds__(kFewThreads, 2) fna2_paged_few_kernel(const Pa
   const int kh = cta % lanes / p.row_blocks, r0 = cta % p.row_blocks * (16 * RW);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int rw = warp % RW, kg = warp / RW;
-  const FewSmem L(D, RW, p.ng_max, p.nh_max, p.RP, p.stages, p.few_rows);
+  const FewSmem L(D, RW, p.ng_max, p.RP, p.stages, p.few_rows);
   int64_t* s_scan = reinterpret_cast<int64_t*>(dsm + L.o_bar);  // [4] warps' sums, [4]: units before the first sequence
   int* s_first = reinterpret_cast<int*>(s_scan + 5);            // first sequence: b, q0, n, len
 
@@ -345,7 +355,7 @@ __global__ void __launch_bounds__(kFewThreads, 2) fna2_paged_few_kernel(const Pa
 
   int stage = 0;
   while (true) {
-  // A = [q | R~_q hi, lo of the warp's heads] of the row blocks' 16 rows each (rows past the end are zero)
+  // A = [q | R~_q hi, lo] of the row blocks' 16 rows each (rows past the end are zero)
   const int wr0 = r0 + rw * 16;
   const int wg_lo = wr0 / sq.n, wg_hi = min(min(rows - 1, wr0 + 15) / sq.n, p.kv.hg - kh * p.G - 1);
   const int wn = wr0 < rows ? max(0, wg_hi - wg_lo + 1) : 0;
@@ -363,18 +373,17 @@ __global__ void __launch_bounds__(kFewThreads, 2) fna2_paged_few_kernel(const Pa
     for (int k = 0; k < D / 8 / TPR; ++k)
       v[k] = real ? *reinterpret_cast<const uint4*>(p.q + tok * p.q_st + h * p.q_sh + (sub + k * TPR) * 8)
                   : make_uint4(0, 0, 0, 0);
-    // block-diagonal: a row holds its own head's R~_q
     const bool graph = real && h < p.kv.hg;
     const float f = graph ? __ldg(p.gs + h) * p.inv_scale : 0.f;
-    for (int x = sub; x < wn * 2 * rp8; x += TPR) {
-      const int gg = x / (2 * rp8), c = x % rp8;
-      uint32_t hi[4] = {0, 0, 0, 0}, lo[4] = {0, 0, 0, 0};
-      if (graph && hh == wg_lo + gg && c < r8)
-        split_bias(*reinterpret_cast<const uint4*>(p.rq + tok * p.rq_st + h * p.rq_sh + c * 8), f, hi, lo);
-      const bool is_lo = x % (2 * rp8) >= rp8;
-      *reinterpret_cast<uint4*>(sa + row * L.a_stride + (D + x * 8) * 2) =
-          is_lo ? make_uint4(lo[0], lo[1], lo[2], lo[3]) : make_uint4(hi[0], hi[1], hi[2], hi[3]);
-    }
+    if (wn > 0)
+      for (int c = sub; c < rp8; c += TPR) {
+        uint32_t hi[4] = {0, 0, 0, 0}, lo[4] = {0, 0, 0, 0};
+        if (graph && c < r8)
+          split_bias(*reinterpret_cast<const uint4*>(p.rq + tok * p.rq_st + h * p.rq_sh + c * 8), f, hi, lo);
+        uint8_t* dst = sa + row * L.a_stride + (D + c * 8) * 2;
+        *reinterpret_cast<uint4*>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        *reinterpret_cast<uint4*>(dst + p.RP * 2) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+      }
 #pragma unroll
     for (int k = 0; k < D / 8 / TPR; ++k) *reinterpret_cast<uint4*>(sa + row * L.a_stride + (sub + k * TPR) * 16) = v[k];
   }
@@ -382,6 +391,7 @@ __global__ void __launch_bounds__(kFewThreads, 2) fna2_paged_few_kernel(const Pa
 
   const int g = lane >> 2, t = lane & 3;
   const int ra = wr0 + g, rc = ra + 8;  // the two rows of this thread's fragments
+  const int head_a = ra / sq.n - wg_lo, head_c = rc / sq.n - wg_lo;
   // (rows past the end are zero rows that see every key: they are not written)
   auto row_limit = [&](int r) { return min(k_end, p.causal && r < rows ? max(0, past + r % sq.n + 1) : sq.len); };
   const int lim0 = row_limit(ra), lim1 = row_limit(rc);
@@ -426,18 +436,32 @@ __global__ void __launch_bounds__(kFewThreads, 2) fna2_paged_few_kernel(const Pa
       mma_bf16(s0, aq[ks], kb[0], kb[1]);
       mma_bf16(s1, aq[ks], kb[2], kb[3]);
     }
-    for (int c = 0; c < wn; ++c)
-      for (int ks = 0; ks < p.RP / 16; ++ks) {
-        uint32_t a[4], kb[4];
-        ldsm_x4(kb, rk_addr + c * L.r_head + ((k_sel + ks * 32) ^ r_sw));
-        const uint32_t aw = a_addr + (D + 2 * c * p.RP) * 2 + ks * 32;
-        ldsm_x4(a, aw);
-        mma_bf16(s0, a, kb[0], kb[1]);
-        mma_bf16(s1, a, kb[2], kb[3]);
-        ldsm_x4(a, aw + p.RP * 2);
-        mma_bf16(s0, a, kb[0], kb[1]);
-        mma_bf16(s1, a, kb[2], kb[3]);
+    // The bias: the 16 rows against one head's R_k at a time, of which that head's rows take the sum.  (Zeros
+    // in the other heads' columns of one wide A instead would carry an infinity or NaN of one head's R_k into
+    // the other heads' rows: 0 * NaN.)
+    for (int c = 0; c < wn; ++c) {
+      float t0[4], t1[4];
+      uint32_t a[4], kb[4];
+      ldsm_x4(kb, rk_addr + c * L.r_head + (k_sel ^ r_sw));
+      ldsm_x4(a, a_addr + D * 2);
+      mma_bf16_from(t0, s0, a, kb[0], kb[1]);
+      mma_bf16_from(t1, s1, a, kb[2], kb[3]);
+      ldsm_x4(a, a_addr + (D + p.RP) * 2);
+      mma_bf16(t0, a, kb[0], kb[1]);
+      mma_bf16(t1, a, kb[2], kb[3]);
+      if (p.RP == 32) {
+        ldsm_x4(kb, rk_addr + c * L.r_head + ((k_sel + 32) ^ r_sw));
+        ldsm_x4(a, a_addr + D * 2 + 32);
+        mma_bf16(t0, a, kb[0], kb[1]);
+        mma_bf16(t1, a, kb[2], kb[3]);
+        ldsm_x4(a, a_addr + (D + 32) * 2 + 32);
+        mma_bf16(t0, a, kb[0], kb[1]);
+        mma_bf16(t1, a, kb[2], kb[3]);
       }
+      const bool ma = head_a == c, mc = head_c == c;
+      s0[0] = ma ? t0[0] : s0[0], s0[1] = ma ? t0[1] : s0[1], s1[0] = ma ? t1[0] : s1[0], s1[1] = ma ? t1[1] : s1[1];
+      s0[2] = mc ? t0[2] : s0[2], s0[3] = mc ? t0[3] : s0[3], s1[2] = mc ? t1[2] : s1[2], s1[3] = mc ? t1[3] : s1[3];
+    }
     // online softmax: row ra holds x[0..3], row rc x[4..7]; keys j0 + {2t, 2t+1, 8+2t, 9+2t}
     float x[8] = {s0[0], s0[1], s1[0], s1[1], s0[2], s0[3], s1[2], s1[3]};
     if (j0 + kFewKeys > lim_all) {
