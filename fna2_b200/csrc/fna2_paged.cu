@@ -165,7 +165,11 @@ __device__ __forceinline__ void mma_bf16_from(float (&d)[4], const float (&c)[4]
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
 }
 
-// Four columns of a finished row: O = acc / (l + 1e-6), LSE = m + log(l + 1e-6).
+// Factor of a part with maximum m in a row of maximum M (log2 domain).  A part that saw no key has m = -inf and
+// sum 0; one whose logits are all NaN has m = -inf and sum NaN, which stays.
+__device__ __forceinline__ float part_factor(float m, float M) { return m == M ? 1.f : ex2(m - M); }
+
+// Four columns of a finished row: O = acc / (l + 1e-6), LSE = m + log(l + 1e-6): 0 and -inf where no key was seen.
 template <int D>
 __device__ __forceinline__ void few_store(const PagedAttnParams& p, int64_t tok, int h, int d, float M, float Ls,
                                           const float4& O) {
@@ -173,7 +177,7 @@ __device__ __forceinline__ void few_store(const PagedAttnParams& p, int64_t tok,
   *reinterpret_cast<uint2*>(p.out + tok * p.o_st + h * p.o_sh + d) =
       make_uint2(pack_bf16(O.x * inv, O.y * inv), pack_bf16(O.z * inv, O.w * inv));
   if (d == 0) {
-    const float lse2 = M == -INFINITY ? M : M + log2f(Ls + kEps);
+    const float lse2 = M + log2f(Ls + kEps);
     if (p.lse) p.lse[h * p.lse_sh + tok] = lse2 * kLn2;
     if (p.lse2) p.lse2[tok * p.H + h] = lse2;
   }
@@ -564,14 +568,12 @@ __global__ void __launch_bounds__(kFewThreads, 2) fna2_paged_few_kernel(const Pa
     for (int w = 0; w < KW; ++w) M = fmaxf(M, cm[w * 16 * RW + row]);
     float Ls = 0.f;
     float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (M != -INFINITY) {
 #pragma unroll
-      for (int w = 0; w < KW; ++w) {
-        const float f = ex2(cm[w * 16 * RW + row] - M);
-        const float4 a = *reinterpret_cast<const float4*>(co + (w * kept + row) * D + d);
-        Ls += cl[w * 16 * RW + row] * f;
-        O.x += a.x * f, O.y += a.y * f, O.z += a.z * f, O.w += a.w * f;
-      }
+    for (int w = 0; w < KW; ++w) {
+      const float f = part_factor(cm[w * 16 * RW + row], M);
+      const float4 a = *reinterpret_cast<const float4*>(co + (w * kept + row) * D + d);
+      Ls += cl[w * 16 * RW + row] * f;
+      O.x += a.x * f, O.y += a.y * f, O.z += a.z * f, O.w += a.w * f;
     }
     if (cut) {
       *reinterpret_cast<float4*>(p.part_acc + static_cast<int64_t>(part + row) * D + d) = O;
@@ -612,14 +614,13 @@ __device__ __forceinline__ RowParts row_parts(const PagedAttnParams& p, int64_t 
   }
 #pragma unroll
   for (int s = 16; s > 0; s >>= 1) o.M = fmaxf(o.M, __shfl_xor_sync(0xffffffffu, o.M, s));
-  if (o.M == -INFINITY) return o;
   if (c1 - c0 < 32) {
-    o.f = ex2(v.x - o.M);
+    o.f = part_factor(v.x, o.M);
     o.Ls = v.y * o.f;
   } else {
     for (int c = c0 + lane; c <= c1; c += 32) {
       v = p.part_ml[index(c)];
-      o.Ls += v.y * ex2(v.x - o.M);
+      o.Ls += v.y * part_factor(v.x, o.M);
     }
   }
 #pragma unroll
@@ -644,18 +645,17 @@ __global__ void __launch_bounds__(kTailThreads) fna2_paged_few_join_kernel(const
   float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
   constexpr int LD = D / 4;  // lanes that hold columns
   const int d = lane % LD * 4;
-  if (o.M != -INFINITY)
-    for (int c = c0; c <= c1; c += 32) {
-      // lane i holds part c + i (for more than 32 parts: found again)
-      const RowParts q = c1 - c0 < 32 ? o : row_parts(p, U, C, s0, c, min(c1, c + 31), kh, r, lane);
-      const float scale = c1 - c0 < 32 ? 1.f : ex2(q.M - o.M);
-      for (int i = 0; i <= min(31, c1 - c); ++i) {
-        const int64_t w = __shfl_sync(0xffffffffu, q.w, i);
-        const float f = __shfl_sync(0xffffffffu, q.f, i) * scale;
-        const float4 a = *reinterpret_cast<const float4*>(p.part_acc + w * D + d);
-        O.x += a.x * f, O.y += a.y * f, O.z += a.z * f, O.w += a.w * f;
-      }
+  for (int c = c0; c <= c1; c += 32) {
+    // lane i holds part c + i (for more than 32 parts: found again)
+    const RowParts q = c1 - c0 < 32 ? o : row_parts(p, U, C, s0, c, min(c1, c + 31), kh, r, lane);
+    const float scale = c1 - c0 < 32 ? 1.f : part_factor(q.M, o.M);
+    for (int i = 0; i <= min(31, c1 - c); ++i) {
+      const int64_t w = __shfl_sync(0xffffffffu, q.w, i);
+      const float f = __shfl_sync(0xffffffffu, q.f, i) * scale;
+      const float4 a = *reinterpret_cast<const float4*>(p.part_acc + w * D + d);
+      O.x += a.x * f, O.y += a.y * f, O.z += a.z * f, O.w += a.w * f;
     }
+  }
   if (lane < LD) few_store<D>(p, sq.q0 + r % sq.n, kh * p.G + r / sq.n, d, o.M, o.Ls, O);
 }
 
@@ -718,21 +718,20 @@ __global__ void __launch_bounds__(128) fna2_paged_many_join_kernel(const PagedAt
   float O[D / 32];
 #pragma unroll
   for (int i = 0; i < D / 32; ++i) O[i] = 0.f;
-  if (M != -INFINITY)
-    for (int s = 0; s < ns; ++s) {
-      const float2 v = ml[s];
-      if (v.x == -INFINITY) continue;
-      const float f = exp2f(v.x - M);
-      Ls += v.y * f;
-      const float* a = p.ws_acc + (th * p.ns + s) * D + lane * (D / 32);
+  for (int s = 0; s < ns; ++s) {
+    const float2 v = ml[s];
+    if (v.x == -INFINITY && v.y == 0.f) continue;  // no key of this split was seen, its output is not written
+    const float f = part_factor(v.x, M);
+    Ls += v.y * f;
+    const float* a = p.ws_acc + (th * p.ns + s) * D + lane * (D / 32);
 #pragma unroll
-      for (int i = 0; i < D / 32; ++i) O[i] += a[i] * f;
-    }
+    for (int i = 0; i < D / 32; ++i) O[i] += a[i] * f;
+  }
   const float inv = 1.f / (Ls + kEps);
   __nv_bfloat16* o = p.out + tok * p.o_st + h * p.o_sh + lane * (D / 32);
 #pragma unroll
   for (int i = 0; i < D / 32; i += 2) *reinterpret_cast<uint32_t*>(o + i) = pack_bf16(O[i] * inv, O[i + 1] * inv);
-  if (lane == 0 && p.lse) p.lse[h * p.lse_sh + tok] = M == -INFINITY ? M : (M + log2f(Ls + kEps)) * kLn2;
+  if (lane == 0 && p.lse) p.lse[h * p.lse_sh + tok] = (M + log2f(Ls + kEps)) * kLn2;
 }
 
 // ---------------------------------------------------------------------------

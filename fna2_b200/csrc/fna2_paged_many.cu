@@ -467,9 +467,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
         const float inv = corr / (l_true + kEps);
         __nv_bfloat16* o0 = p.out + static_cast<int64_t>(sq.q0 + row0) * p.o_st + h * p.o_sh;
         store_o_rows<D>(smem + L::oK + warp * 32 * 64, tO, inv, o0, p.o_st, sq.n - row0);
-        if (row_ok && p.lse)
-          p.lse[h * p.lse_sh + sq.q0 + q_local] =
-              (m_true == -INFINITY) ? -INFINITY : (m_true + lg2(l_true + kEps)) * kLn2;
+        if (row_ok && p.lse) p.lse[h * p.lse_sh + sq.q0 + q_local] = (m_true + lg2(l_true + kEps)) * kLn2;
       } else {
         const int64_t w = (static_cast<int64_t>(sq.q0 + q_local) * p.H + h) * p.ns + it.split;
         if (row_ok) p.ws_ml[w] = make_float2(m_true, l_true);

@@ -38,3 +38,45 @@ def test_one_heads_r_k_stays_with_that_head(shape, value):
     _close_lse(l2[rest], lse[rest])
     if value != value:  # every query of that head has a NaN logit
         assert torch.isnan(out[:, h]).all() and torch.isnan(l2[h]).all()
+
+
+@pytest.mark.parametrize("splits", [1, 5])
+@pytest.mark.parametrize("new", [1, 3, 40, 300])
+def test_a_query_of_nan_gives_nan(new, splits):
+    """All logits of the row are NaN; the other rows are what they were."""
+    x = _make([900], [new], 4, 2, 4, 64, 16, 32, 17)
+    ref, lse, _ = PO.attention(x, True)
+    x["q"][new // 2, 1] = float("nan")
+    out, l2 = _attend(x, splits)
+    assert torch.isnan(out[new // 2, 1]).all() and torch.isnan(l2[1, new // 2])
+    keep = torch.ones(new, 4, dtype=torch.bool)
+    keep[new // 2, 1] = False
+    _close_out("the others", out.cpu()[keep], ref[keep])
+    _close_lse(l2.cpu().t()[keep], lse.t()[keep])
+
+
+@pytest.mark.parametrize("splits", [1, 9, 70])
+@pytest.mark.parametrize("new", [1, 6, 300])
+@pytest.mark.parametrize("keys", [(40, 41), (0, 512)])
+def test_keys_of_nan_reach_the_rows_that_see_them(new, splits, keys):
+    """One key, and all keys of a split: NaN logits are not taken for keys that are not there."""
+    x = _make([2048], [new], 2, 1, 2, 64, 16, 32, 19)
+    j = torch.arange(*keys)
+    x["kp"][x["table"][0].long()[j // 32], j % 32] = float("nan")
+    out, l2 = _attend(x, splits)
+    assert torch.isnan(out).all() and torch.isnan(l2).all()
+
+
+@pytest.mark.parametrize("splits", [1, 4])
+def test_keys_of_nan_are_not_seen_before_their_time(splits):
+    """New tokens whose own key is NaN leave the tokens before them as they were."""
+    for new in (5, 200):
+        x = _make([700], [new], 4, 2, 4, 128, 32, 64, 23)
+        ref, lse, _ = PO.attention(x, True)
+        j = torch.tensor([700 - new // 2 - 1])  # new token `at`'s own key
+        at = new - new // 2 - 1
+        x["kp"][x["table"][0].long()[j // 64], j % 64] = float("nan")
+        out, l2 = _attend(x, splits)
+        _close_out("before", out[:at], ref[:at])
+        _close_lse(l2[:, :at], lse[:, :at])
+        assert torch.isnan(out[at:]).all() and torch.isnan(l2[:, at:]).all()
