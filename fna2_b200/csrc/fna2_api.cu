@@ -792,10 +792,8 @@ int paged_plan(const Fna2PagedKV* kv, const Fna2PagedAttnArgs* a, PagedAttnParam
   const int D = kv->head_dim, max_rows = std::max(1, p->bd.max_q * p->G);
   const int few_limit = std::min(kFewRows, kFewTokens * p->G);
   const bool all_few = max_rows <= few_limit;
-  l->few = all_few || p->bd.B > 1;
-  l->many = !all_few;
+  l->few = all_few || (p->bd.B > 1 && p->G <= kFewRowsMixed);  // (a token has G rows)
   p->few_rows = all_few ? max_rows : l->few ? kFewRowsMixed : 0;
-  const int few_max = std::min(max_rows, p->few_rows);
   auto fits = [&](int RW, int stages, int bytes) {
     l->RW = RW;
     p->ng_max = std::min({p->G, 16 * RW, p->kv.hg});
@@ -807,11 +805,18 @@ int paged_plan(const Fna2PagedKV* kv, const Fna2PagedAttnArgs* a, PagedAttnParam
   };
   // As many row blocks as the rows fill, so that two CTAs fit on an SM; twice as many, with half the key
   // groups and so half the rings, where only that lets two fit (16 rows, 4 graph heads, rank 16, D = 128, 8
-  // sequences of 4,000 keys: 38.7 us with one CTA per SM, 28.8 with two); else whatever fits.
+  // sequences of 4,000 keys: 38.7 us with one CTA per SM, 28.8 with two); else whatever fits, the fewest first
+  // below and then above (R_k rings of 16 graph heads at rank 32 leave room for two key groups, not for four: 16
+  // heads of 2 KV heads, 8 sequences of 4,000 keys, one token 79 us, 163 on the tensor-core kernel).  Four row
+  // blocks, one key group and two stages always fit: 201 KB with 64 graph heads.
   const int fill = !all_few || max_rows <= 16 ? 1 : max_rows <= 32 ? 2 : 4;
   bool found = fits(fill, 4, kHalfSmem);
   for (int stages = 4; !found && fill <= 2 && stages >= 2; --stages) found = fits(2 * fill, stages, kHalfSmem);
-  for (int RW = fill; !found && !(found = fits(RW, 4, kMaxDynamicSmem)) && RW > 1;) RW /= 2;
+  for (int RW = fill; !found && RW >= 1; RW /= 2) found = fits(RW, 4, kMaxDynamicSmem);
+  for (int RW = 2 * fill; !found && RW <= 4; RW *= 2) found = fits(RW, 4, kMaxDynamicSmem);
+  FNA2_CHECK(found || !l->few, "no room for %d query rows with %d graph heads per KV head", p->few_rows, p->ng_max);
+  l->many = !all_few;
+  const int few_max = std::min(max_rows, p->few_rows);
   p->block_rows = 16 * l->RW;
   p->unit_keys = 64 / l->RW;
   p->row_blocks = std::max(1, (few_max + p->block_rows - 1) / p->block_rows);
