@@ -838,7 +838,8 @@ int paged_plan(const Fna2PagedKV* kv, const Fna2PagedAttnArgs* a, PagedAttnParam
                                         : many_splits(pairs * p->H, tiles, static_cast<double>(p->bd.T) * p->H * D * 8);
     p->chunk_many = static_cast<int>((tiles + s - 1) / s) * kBlockN;
     const int64_t ns = (max_k + p->chunk_many - 1) / p->chunk_many;
-    FNA2_CHECK((pairs + longer) * ns <= 65535, "too many query tiles and splits (%lld)", (long long)((pairs + longer) * ns));
+    FNA2_CHECK((pairs + longer) * ns * p->H < (1ll << 31), "too many query tiles, splits and heads (%lld)",
+               (long long)((pairs + longer) * ns * p->H));
     p->many_items = static_cast<int>((pairs + longer) * ns);
     p->ns = static_cast<int>(ns);
   }

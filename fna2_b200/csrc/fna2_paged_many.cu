@@ -120,9 +120,9 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
   pdl_trigger();
 
   ManyItem it;
-  if (!many_item(p, blockIdx.y, lane, &it)) return;
+  if (!many_item(p, blockIdx.x / p.H, lane, &it)) return;
   const PagedSeq sq = it.sq;
-  const int h = blockIdx.x, hk = h / p.G;
+  const int h = blockIdx.x % p.H, hk = h / p.G;
   const bool graph = h < p.kv.hg;
   const int q0 = it.pair * 2 * kBlockM, past = sq.len - sq.n;
   // key tiles [t0, t1) of this split; n_t: how many of them each query tile sees
@@ -509,7 +509,7 @@ cudaError_t launch_paged_many_t(const ManyMaps& m, const PagedAttnParams& p, cud
   static std::atomic<uint64_t> allowed{0};
   cudaError_t e = allow_smem(reinterpret_cast<const void*>(kern), allowed);
   if (e != cudaSuccess) return e;
-  return launch_dependent(kern, dim3(p.H, p.many_items), kFwdThreads, L::kTotal, stream, m.q, m.k, m.v, m.rq, m.rk, p);
+  return launch_dependent(kern, dim3(p.H * p.many_items), kFwdThreads, L::kTotal, stream, m.q, m.k, m.v, m.rq, m.rk, p);
 }
 
 inline cudaError_t launch_paged_many(const ManyMaps& m, const PagedAttnParams& p, int D, cudaStream_t stream) {

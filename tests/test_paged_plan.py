@@ -31,3 +31,12 @@ def test_every_group_size_has_a_kernel(D, rank):
             for batch in (1, 3):
                 _, error = _query(G, 1, D, rank, tokens, batch, 4096)
                 assert error == "", (G, tokens, batch, error)
+
+
+@pytest.mark.parametrize("total,G,kv_heads,batch,tokens,max_k", [
+    (26071, 16, 1, 16130, 31, 907776), (33172, 8, 1, 30805, 74, 137344), (1 << 21, 4, 2, 60000, 2000, 8192),
+    (1 << 25, 1, 1, 65535, 1 << 20, 4096)])
+def test_many_sequences_and_tokens_are_accepted(total, G, kv_heads, batch, tokens, max_k):
+    """Splits of long keys times tens of thousands of short sequences: the grid has room for them."""
+    _, error = _query(G, kv_heads, 128, 16, tokens, batch, max_k, total=total)
+    assert error == ""
