@@ -768,6 +768,16 @@ struct PagedPlan {
   size_t acc, ml, part_acc, part_ml, prefix, logit, lse2, lse, kw, total;
 };
 
+// Kept logits are padded to the longest sequence, so one long sequence among short ones would multiply their
+// place: 4.3 GB for 256 sequences decoding one token with 32 heads beside 131,072 keys.  Their limit is half of
+// the pool's K (what 32 rows of every slot take at D = 128), at least 64 MB and at most 2 GB; beyond it the key
+// weights' kernels form the logits again, which needs a few KB per token.
+constexpr double kLogitBytesMin = 64e6, kLogitBytesMax = 2e9;
+double logit_bytes_limit(const Fna2PagedKV* kv) {
+  const double k_bytes = 2.0 * kv->num_pages * kv->page_size * kv->kv_heads * kv->head_dim;
+  return std::max(kLogitBytesMin, std::min(kLogitBytesMax, k_bytes / 2));
+}
+
 size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 
 // Workspace of the key weights: the R~_q hi / lo and LSE columns, and the item counter.
@@ -843,10 +853,11 @@ int paged_plan(const Fna2PagedKV* kv, const Fna2PagedAttnArgs* a, PagedAttnParam
     p->many_items = static_cast<int>((pairs + longer) * ns);
     p->ns = static_cast<int>(ns);
   }
-  l->logits = p->kw && all_few && max_rows <= kLogitRows;
   l->many_join = l->many && p->ns > 1;
   l->few_join = l->few && !p->whole && p->runs > 1;
   p->logit_sr = (static_cast<int64_t>(p->bd.max_k) + 15) / 16 * 16;
+  const double logit_bytes = 4.0 * p->bd.B * p->kv.hkv * max_rows * p->logit_sr;
+  l->logits = p->kw && all_few && max_rows <= kLogitRows && logit_bytes <= logit_bytes_limit(kv);
   const size_t th = static_cast<size_t>(p->bd.T) * p->H;
   size_t at = 0;
   auto take = [&at](bool need, size_t bytes) {

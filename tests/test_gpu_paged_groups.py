@@ -30,3 +30,22 @@ def test_large_groups(group, kv_heads, graph, D, rank, kind):
     _close_lse(lse, rl)
     _close_w(w, rw)
     assert _status() == 0
+
+
+def test_weights_of_one_long_sequence_among_many():
+    """Key weights of single tokens where their logits would take more than the pool: formed again."""
+    from fna2_b200.paged import flash_naylis_paged
+    lens = [3] * 300 + [70000] + [1] * 99
+    x = _make(lens, [1] * 400, 8, 2, 8, 64, 8, 256, 40)
+    d = _dev(x)
+    w = torch.zeros(400, 2, x["table"].shape[1] * 256, device="cuda")
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    out, lse = flash_naylis_paged(d["q"], _pool(x), d["table"], d["lens"], d["cu"], 1, r_q=d["rq"], graph_scale=d["gs"],
+                                  return_lse=True, key_weights=w, max_seqlen_k=70000)
+    assert torch.cuda.max_memory_allocated() - before < 400e6  # the logits alone: 400 * 8 * 70,000 * 4 bytes = 900 MB
+    ro, rl, rw = PO.attention(x, True)
+    _close_out("out", out, ro)
+    _close_lse(lse, rl)
+    _close_w(w, rw)

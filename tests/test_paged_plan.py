@@ -40,3 +40,22 @@ def test_many_sequences_and_tokens_are_accepted(total, G, kv_heads, batch, token
     """Splits of long keys times tens of thousands of short sequences: the grid has room for them."""
     _, error = _query(G, kv_heads, 128, 16, tokens, batch, max_k, total=total)
     assert error == ""
+
+
+@pytest.mark.parametrize("batch,tokens,group", [(256, 1, 4), (64, 8, 4), (64, 8, 1), (64, 1, 32), (2000, 1, 4)])
+@pytest.mark.parametrize("pages", [1 << 12, 1 << 14])
+def test_workspace_of_key_weights_is_bounded(batch, tokens, group, pages):
+    """Bounds of 131,072 keys, which one sequence of a batch may reach: never more than half of the pool's K
+    (64 MB at least) and 2 GB, beside what a call without weights takes."""
+    plain, _ = _query(group, 8, 128, 16, tokens, batch, 131072, num_pages=pages)
+    n, error = _query(group, 8, 128, 16, tokens, batch, 131072, weights=True, num_pages=pages)
+    k_bytes = pages * 64 * 8 * 128 * 2
+    tokens_bytes = batch * tokens * 8 * group * (4 + 2 * (2 * 16 + 16)) + 4096  # LSE, R~_q and LSE columns
+    assert error == "" and n - plain <= max(64e6, min(2e9, k_bytes / 2)) + tokens_bytes
+
+
+def test_workspace_keeps_the_logits_of_ordinary_calls():
+    """A pool filled by equal sequences: what their logits take is within the limit."""
+    plain, _ = _query(4, 8, 128, 16, 1, 64, 4096, num_pages=64 * 64)
+    n, _ = _query(4, 8, 128, 16, 1, 64, 4096, weights=True, num_pages=64 * 64)
+    assert n - plain >= 64 * 32 * 4096 * 4
