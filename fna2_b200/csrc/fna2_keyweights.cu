@@ -286,9 +286,10 @@ __global__ void __launch_bounds__(kKwThreads, 1)
     };
     auto page_of = [&](const KwItem& it) {
       const int key = it.k0 + lane * bk;
-      return it.n_units >= 0 && lane * bk < 2 * kBlockN && key < it.len
-                 ? __ldg(p.kv.table + it.b * p.kv.table_sb + (key >> lg))
-                 : -1;
+      if (it.n_units < 0 || lane * bk >= 2 * kBlockN || key >= it.len) return -1;
+      const int page = __ldg(p.kv.table + it.b * p.kv.table_sb + (key >> lg));
+      check_page(p.kv, page);
+      return page;
     };
     KwItem it = kw_item(p, blockIdx.x, 2 * kBlockN, lane), next = it;
     int page = page_of(it), next_page = -1;
@@ -651,6 +652,7 @@ __global__ void __launch_bounds__(kKwThreads, 1)
           const int s = gt & 1, key = it.k0 + t * kBlockN + row;
           const bool mine = row < kBlockN && key < it.len;
           const int page = mine ? __ldg(p.kv.table + it.b * p.kv.table_sb + (key >> lg)) : 0;
+          if (mine) check_page(p.kv, page);
           const bool room = gt < 2 || mbar_wait(&bars[kVbEmpty + s], ((gt >> 1) - 1) & 1, abort_flag, 126);
           if (!(ok = __all_sync(0xffffffffu, room))) return;
           const int boxes = __popc(__ballot_sync(0xffffffffu, mine));

@@ -327,6 +327,7 @@ __global__ void __launch_bounds__(kFewThreads, 2) fna2_paged_few_kernel(const Pa
           ks += STEP * p.kv.k.st, vs += STEP * p.kv.v.st;
         }
       } else {
+        if (nv == 0 && lane == 0) check_page(p.kv, page);
         for (int k = 0; k < NI; ++k) {
           const uint32_t d = (dk ^ ((k * STEP & 7) * 16)) + k * STEP * 128;
           const bool valid = row0 + k * STEP < nv;

@@ -13,7 +13,7 @@ constexpr int kSms = 148;  // of a B200
 
 // Site codes recorded in g_device_error (read by fna2_device_status).
 constexpr int kStatusBadSeqAppend = 631;  // append: bad length / offsets, or a page id outside the pool
-constexpr int kStatusBadSeqPaged = 641;   // attention, key weights: bad length or offsets
+constexpr int kStatusBadSeqPaged = 641;   // attention, key weights: bad length or offsets, or a page id outside the pool
 constexpr int kStatusBadSeqEvict = 651;   // eviction: bad length, or a page id outside the pool
 
 struct PagedRows {  // one tensor of the pool: element (page, slot, head, column), column stride 1
@@ -33,6 +33,12 @@ struct PagedPool {
 // First element of key j's row of head `head` (page id already looked up).
 __device__ __forceinline__ int64_t paged_off(const PagedRows& r, int page_id, int slot, int head) {
   return page_id * r.sp + slot * r.st + head * r.sh;
+}
+
+// Attention and key weights: a page id that a key needs, outside the pool, is recorded; its keys read as zeros
+// (bounds checks here, out-of-range tensor-map coordinates there).
+__device__ __forceinline__ void check_page(const PagedPool& kv, int page) {
+  if (page < 0 || page >= kv.pages) atomicCAS(&g_device_error, 0, kStatusBadSeqPaged);
 }
 
 struct PagedSeq {

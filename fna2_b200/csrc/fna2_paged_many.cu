@@ -210,6 +210,7 @@ __global__ void __launch_bounds__(kFwdThreads, 1)
       const int s = j & 1, key = (t0 + j) * kBlockN + lane * bk;
       const bool mine = lane * bk < kBlockN && key < sq.len;
       const int page = mine ? __ldg(table + (key >> lg)) : 0;
+      if (mine) check_page(p.kv, page);
       const bool free = j < 2 || mbar_wait(&bars[kMbKEmpty + s], ((j >> 1) - 1) & 1, abort_flag, 111);
       if (!__all_sync(0xffffffffu, free)) return false;
       const int boxes = __popc(__ballot_sync(0xffffffffu, mine));

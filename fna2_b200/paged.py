@@ -18,7 +18,8 @@ len = cache_seqlens[b] counts the new tokens: the rows equal the last n rows of
 flash_naylis_attn over the whole sequence.  Sequence lengths and page tables are
 int32 on the device and are never read on the host; a sequence whose lengths
 break the bounds of a call is skipped and a status recorded (fna2_device_status:
-631 append, 641 attention and key weights, 651 eviction).
+631 append, 641 attention and key weights, 651 eviction).  So is a page id outside
+the pool: append and eviction do not write its rows, the others read them as zeros.
 
 NaylisPagedCache keeps the pool, the tables and the lengths, and runs the four.
 """

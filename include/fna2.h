@@ -257,9 +257,11 @@ int fna2_decode(const Fna2DecodeArgs* args, void* workspace, size_t workspace_by
  * page_table[b * table_stride + j / page_size].  Entries past a sequence's
  * length are not read, and what a page holds past it is never used.
  * page_table, cache_seqlens and cu_seqlens are int32 on the device and are not
- * read on the host.  A sequence whose device-side values break the bounds given
+ * read on the host.  A sequence whose lengths or offsets break the bounds given
  * in the arguments is skipped before any access and a status is recorded
  * (fna2_device_status: 631 append, 641 attention and key weights, 651 eviction).
+ * So is a page id outside the pool that a key in use has: append and eviction
+ * do not write its rows, attention and key weights read them as zeros.
  * --------------------------------------------------------------------------- */
 typedef struct Fna2PagedKV {
   int32_t num_pages, page_size, kv_heads, graph_heads, head_dim, rank;
@@ -370,7 +372,8 @@ const char* fna2_last_error(void);
  *   631       append: a sequence with inconsistent cache_seqlens / cu_seqlens or
  *             a page id outside the pool (its tokens are not written);
  *   641       paged attention, key weights: a sequence whose cu_seqlens or
- *             cache_seqlens break the call's bounds (its rows are not written);
+ *             cache_seqlens break the call's bounds (its rows are not written),
+ *             or a page id outside the pool (its keys read as zeros);
  *   651       eviction: a length outside [0, max_seqlen_k], or a page id outside
  *             the pool (the row is not copied);
  *   622       backward pre-pass, packed batch: the same check; the sequence

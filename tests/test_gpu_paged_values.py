@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from oracle import paged_oracle as PO
-from test_gpu_paged import _close_lse, _close_out, _dev, _make, _pool
+from test_gpu_paged import _close_lse, _close_out, _close_w, _dev, _make, _pool, _status
 
 pytestmark = pytest.mark.gpu
 
@@ -80,3 +80,28 @@ def test_keys_of_nan_are_not_seen_before_their_time(splits):
         _close_out("before", out[:at], ref[:at])
         _close_lse(l2[:, :at], lse[:, :at])
         assert torch.isnan(out[at:]).all() and torch.isnan(l2[:, at:]).all()
+
+
+@pytest.mark.parametrize("new", [[1, 1, 1], [8, 8, 8], [150, 70, 150]])
+@pytest.mark.parametrize("bad", [-1, "past the pool", 1 << 30])
+@pytest.mark.parametrize("page", [16, 128])
+def test_page_ids_outside_the_pool_are_recorded(new, bad, page):
+    """An entry within a sequence's length: recorded, its keys read as zeros, other sequences untouched."""
+    from fna2_b200.paged import flash_naylis_paged, naylis_key_weights
+    x = _make([500, 400, 300], new, 4, 2, 4, 64, 16, page, 29)
+    at = 256 // page
+    x["kp"][x["table"][1, at].long()] = 0.0
+    x["vp"][x["table"][1, at].long()] = 0.0
+    x["rp"][x["table"][1, at].long()] = 0.0
+    ref, lse, w = PO.attention(x, True)
+    d, pool = _dev(x), _pool(x)
+    d["table"][1, at] = pool.num_pages if bad == "past the pool" else bad
+    assert _status() == 0
+    kw = dict(r_q=d["rq"], graph_scale=d["gs"])
+    out, l2 = flash_naylis_paged(d["q"], pool, d["table"], d["lens"], d["cu"], max(new), return_lse=True, **kw)
+    assert _status() == 641
+    _close_out("out", out, ref)
+    _close_lse(l2, lse)
+    got = naylis_key_weights(d["q"], l2, pool, d["table"], d["lens"], d["cu"], max(new), **kw)
+    assert _status() == 641
+    _close_w(got, w)
