@@ -48,15 +48,20 @@ def _want(ok: bool, msg: str) -> None:
         raise ValueError(msg)
 
 
-def _rows(t: torch.Tensor, name: str, tokens: int, heads: int, cols: int, dtype: torch.dtype):
+# Every tensor of a call lies on the pool's device (`gpu`: its index): a kernel takes pointers as they are.
+def _elsewhere(t: torch.Tensor, name: str, gpu: int) -> ValueError:
+    return ValueError(f"{name} must be a CUDA tensor on the pool's device cuda:{gpu} (got {t.device})")
+
+
+def _rows(t: torch.Tensor, name: str, tokens: int, heads: int, cols: int, dtype: torch.dtype, gpu: int):
     """Checks a [tokens, heads, cols] tensor; returns it with its pointer and token and head
     strides.  Rows that are not 16-byte aligned or columns without unit stride are copied once."""
     if t.dtype is not dtype:
         raise TypeError(f"{name} must be {dtype} (got {t.dtype})")
     if t.shape != (tokens, heads, cols):
         raise ValueError(f"{name} must be [{tokens}, {heads}, {cols}] (got {tuple(t.shape)})")
-    if not t.is_cuda:
-        raise ValueError(f"{name} must be a CUDA tensor")
+    if t.get_device() != gpu:
+        raise _elsewhere(t, name, gpu)
     s0, s1, s2 = t.stride()
     p = t.data_ptr()
     if s2 != 1 or p & 15 or ((s0 | s1) * (2 if dtype is torch.bfloat16 else 4)) & 15:
@@ -65,15 +70,19 @@ def _rows(t: torch.Tensor, name: str, tokens: int, heads: int, cols: int, dtype:
     return t, p, s0, s1
 
 
-def _int32(t: torch.Tensor, name: str, n: int) -> torch.Tensor:
-    if t.dtype is not torch.int32 or not t.is_cuda or t.numel() != n:
+def _int32(t: torch.Tensor, name: str, n: int, gpu: int) -> torch.Tensor:
+    if t.dtype is not torch.int32 or t.numel() != n:
         raise ValueError(f"{name} must be a CUDA int32 tensor of {n} entries")
+    if t.get_device() != gpu:
+        raise _elsewhere(t, name, gpu)
     return t if t.is_contiguous() else t.contiguous()
 
 
-def _table(t: torch.Tensor, name: str = "page_table") -> torch.Tensor:
-    if t.dtype is not torch.int32 or not t.is_cuda or t.dim() != 2:
+def _table(t: torch.Tensor, gpu: int, name: str = "page_table") -> torch.Tensor:
+    if t.dtype is not torch.int32 or t.dim() != 2:
         raise ValueError(f"{name} must be a CUDA int32 tensor [batch, pages]")
+    if t.get_device() != gpu:
+        raise _elsewhere(t, name, gpu)
     return t if t.stride(1) == 1 and t.stride(0) >= t.shape[1] else t.contiguous()
 
 
@@ -82,8 +91,12 @@ def _empty(like: torch.Tensor) -> torch.Tensor:
                                                                            device=like.device)
 
 
-def _stream(device: torch.device) -> int:
-    return torch._C._cuda_getCurrentRawStream(device.index)  # current_stream(device).cuda_stream, without the object
+def _launch(gpu: int, call, *args) -> int:
+    """call(*args, the GPU's current stream) with that GPU current, where the kernels go."""
+    if torch._C._cuda_getDevice() == gpu:
+        return call(*args, torch._C._cuda_getCurrentRawStream(gpu))  # current_stream().cuda_stream, without the object
+    with torch.cuda.device(gpu):
+        return call(*args, torch._C._cuda_getCurrentRawStream(gpu))
 
 
 class PagedKV:
@@ -99,6 +112,8 @@ class PagedKV:
             if t.dtype != torch.bfloat16:
                 raise TypeError(f"{name} must be bfloat16 (got {t.dtype})")
             _want(t.is_cuda, f"{name} must be a CUDA tensor")
+            if t.get_device() != k_pages.get_device():
+                raise _elsewhere(t, name, k_pages.get_device())
             _want(t.dim() == 4, f"{name} must be [pages, page_size, heads, columns] (got {tuple(t.shape)})")
             _want(t.stride(3) == 1, f"{name} must have unit stride in its last dim")
             _want(t.shape[:2] == k_pages.shape[:2], f"{name} must have the pages and page size of k_pages")
@@ -108,7 +123,7 @@ class PagedKV:
         self.graph_heads, self.rank = (0, 16) if rk_pages is None else rk_pages.shape[2:]
         if self.graph_heads == 0:
             rk_pages = None
-        self.device = k_pages.device
+        self.device, self.gpu = k_pages.device, k_pages.get_device()
         c = _lib.Fna2PagedKV(self.num_pages, self.page_size, self.kv_heads, self.graph_heads, self.head_dim, self.rank)
         c.k, c.v = k_pages.data_ptr(), v_pages.data_ptr()
         c.k_page_stride, c.k_token_stride, c.k_head_stride = k_pages.stride()[:3]
@@ -136,26 +151,29 @@ def qk_norm_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, pool:
     if dt not in _DT:
         raise TypeError(f"q must be fp32 or bf16 (got {dt})")
     _want(q.dim() == 3, f"q must be [T, H, D] (got {tuple(q.shape)})")
-    T, H, D = q.shape
-    q, q_p, q_0, q_1 = _rows(q, "q", T, H, pool.head_dim, dt)
-    k, k_p, k_0, k_1 = _rows(k, "k", T, pool.kv_heads, D, dt)
-    v, v_p, v_0, v_1 = _rows(v, "v", T, pool.kv_heads, D, dt)
+    (T, H, D), gpu = q.shape, pool.gpu
+    q, q_p, q_0, q_1 = _rows(q, "q", T, H, pool.head_dim, dt, gpu)
+    k, k_p, k_0, k_1 = _rows(k, "k", T, pool.kv_heads, D, dt, gpu)
+    v, v_p, v_0, v_1 = _rows(v, "v", T, pool.kv_heads, D, dt, gpu)
     _want((r_k is not None) == (pool.graph_heads > 0), "r_k goes with a pool that has rk_pages")
     r_p = r_0 = r_1 = 0
     if r_k is not None:
-        r_k, r_p, r_0, r_1 = _rows(r_k, "r_k", T, pool.graph_heads, pool.rank, dt)
-    table = _table(page_table)
+        r_k, r_p, r_0, r_1 = _rows(r_k, "r_k", T, pool.graph_heads, pool.rank, dt, gpu)
+    table = _table(page_table, gpu)
     B, max_pages = table.shape
-    lens, cu = _int32(cache_seqlens, "cache_seqlens", B), _int32(cu_seqlens, "cu_seqlens", B + 1)
+    lens, cu = _int32(cache_seqlens, "cache_seqlens", B, gpu), _int32(cu_seqlens, "cu_seqlens", B + 1, gpu)
     if positions is not None:
-        positions = _int32(positions, "positions", B)
+        positions = _int32(positions, "positions", B, gpu)
     _want((q_norm is None) == (k_norm is None), "give both norms or neither")
     wq_p = wk_p = f_p = 0
     eps, w_dt, rope_dt = 0.0, 0, _DT[dt]
     if q_norm is not None:
         wq, wk, eps = q_norm.weight, k_norm.weight, float(q_norm.eps)
-        _want(wq.dtype in _DT and wk.dtype == wq.dtype and wq.numel() == D and wk.numel() == D and wq.is_cuda and
-              wk.is_cuda, "norm weights: CUDA fp32 or bf16 [head_dim], same dtype")
+        _want(wq.dtype in _DT and wk.dtype == wq.dtype and wq.numel() == D and wk.numel() == D,
+              "norm weights: CUDA fp32 or bf16 [head_dim], same dtype")
+        for w, name in ((wq, "q_norm.weight"), (wk, "k_norm.weight")):
+            if w.get_device() != gpu:
+                raise _elsewhere(w, name, gpu)
         _want(eps == float(k_norm.eps), "the two norms must share eps")
         wq, wk = wq.contiguous(), wk.contiguous()
         wq_p, wk_p, w_dt, rope_dt = wq.data_ptr(), wk.data_ptr(), _DT[wq.dtype], _DT[torch.promote_types(dt, wq.dtype)]
@@ -169,35 +187,39 @@ def qk_norm_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, pool:
     a = _APPEND_ARGS.pack(B, H, max_pages, _DT[dt], w_dt, rope_dt, T, q_p, q_0, q_1, k_p, k_0, k_1, v_p, v_0, v_1, r_p,
                           r_0, r_1, out.data_ptr(), H * D, D, table.data_ptr(), table.stride(0), lens.data_ptr(),
                           cu.data_ptr(), 0 if positions is None else positions.data_ptr(), wq_p, wk_p, eps, f_p)
-    rc = _lib.load().fna2_paged_append(pool._ref, a, _stream(pool.device))
+    rc = _launch(gpu, _lib.load().fna2_paged_append, pool._ref, a)
     if rc:
         _lib.check(rc, "fna2_paged_append")
     return out
 
 
-def _weights_ok(w: torch.Tensor, B: int, heads: int, keys: int) -> None:
-    if w.dtype is not torch.float32 or not w.is_cuda or w.dim() != 3 or w.shape[0] != B or w.shape[1] != heads or \
+def _weights_ok(w: torch.Tensor, B: int, heads: int, keys: int, gpu: int) -> None:
+    if w.dtype is not torch.float32 or w.dim() != 3 or w.shape[0] != B or w.shape[1] != heads or \
             w.shape[2] < keys or w.stride(2) != 1:
         raise ValueError(f"key_weights must be CUDA fp32 [{B}, {heads}, >= {keys}] with unit stride in its last dim")
+    if w.get_device() != gpu:
+        raise _elsewhere(w, "key_weights", gpu)
 
 
 def _attention(name, q, pool, page_table, cache_seqlens, cu_seqlens_q, max_seqlen_q, r_q, graph_scale, softmax_scale,
                is_causal, key_weights, max_seqlen_k, num_splits, out, lse, clear=0):
     """Packs the arguments of fna2_paged_attn or fna2_key_weights and calls it."""
-    T, H, D = q.shape
-    q, q_p, q_0, q_1 = _rows(q, "q", T, H, pool.head_dim, torch.bfloat16)
-    table = _table(page_table)
+    (T, H, D), gpu = q.shape, pool.gpu
+    q, q_p, q_0, q_1 = _rows(q, "q", T, H, pool.head_dim, torch.bfloat16, gpu)
+    table = _table(page_table, gpu)
     B, max_pages = table.shape
-    lens, cu = _int32(cache_seqlens, "cache_seqlens", B), _int32(cu_seqlens_q, "cu_seqlens_q", B + 1)
+    lens, cu = _int32(cache_seqlens, "cache_seqlens", B, gpu), _int32(cu_seqlens_q, "cu_seqlens_q", B + 1, gpu)
     max_k = max_pages * pool.page_size
     if max_seqlen_k is not None and max_seqlen_k < max_k:
         max_k = int(max_seqlen_k)
     r_p = r_0 = r_1 = gs_p = 0
     if pool.graph_heads:
         _want(r_q is not None and graph_scale is not None, "graph heads need r_q and graph_scale")
-        r_q, r_p, r_0, r_1 = _rows(r_q, "r_q", T, pool.graph_heads, pool.rank, torch.bfloat16)
+        r_q, r_p, r_0, r_1 = _rows(r_q, "r_q", T, pool.graph_heads, pool.rank, torch.bfloat16, gpu)
         gs = graph_scale
-        _want(gs.numel() == pool.graph_heads and gs.is_cuda, "graph_scale must be a CUDA tensor [H_G]")
+        _want(gs.numel() == pool.graph_heads, "graph_scale must be a CUDA tensor [H_G]")
+        if gs.get_device() != gpu:
+            raise _elsewhere(gs, "graph_scale", gpu)
         if gs.dtype is not torch.float32 or not gs.is_contiguous():
             gs = gs.detach().float().contiguous()
         gs_p = gs.data_ptr()
@@ -205,7 +227,7 @@ def _attention(name, q, pool, page_table, cache_seqlens, cu_seqlens_q, max_seqle
         _want(r_q is None, "r_q goes with a pool that has rk_pages")
     w_p = w_0 = w_1 = 0
     if key_weights is not None:
-        _weights_ok(key_weights, B, pool.kv_heads, max_k)
+        _weights_ok(key_weights, B, pool.kv_heads, max_k, gpu)
         w_p, (w_0, w_1, _) = key_weights.data_ptr(), key_weights.stride()
     l_p, l_0 = (0, 0) if lse is None else (lse.data_ptr(), lse.stride(0))
     a = _ATTN_ARGS.pack(B, H, T, int(max_seqlen_q), max_k, max_pages, 1 if is_causal else 0, num_splits,
@@ -219,7 +241,7 @@ def _attention(name, q, pool, page_table, cache_seqlens, cu_seqlens_q, max_seqle
     if n:
         ws = torch.empty(n, dtype=torch.uint8, device=pool.device)
         ws_p = ws.data_ptr()
-    rc = call(pool._ref, a, ws_p, n, _stream(pool.device))
+    rc = _launch(gpu, call, pool._ref, a, ws_p, n)
     if rc:
         _lib.check(rc, name)
 
@@ -259,8 +281,10 @@ def naylis_key_weights(q: torch.Tensor, lse: torch.Tensor, pool: PagedKV, page_t
     same keys.  The queries may be the last tokens of each sequence only (they vote for the
     rest).  Adds to key_weights, or to zeros [B, H_KV, pages * page_size] when None; returns it."""
     _want(q.dim() == 3, f"q must be [T, H, D] (got {tuple(q.shape)})")
-    if lse.dtype is not torch.float32 or not lse.is_cuda or lse.shape != (q.shape[1], q.shape[0]):
+    if lse.dtype is not torch.float32 or lse.shape != (q.shape[1], q.shape[0]):
         raise ValueError(f"lse must be CUDA fp32 [{q.shape[1]}, {q.shape[0]}] (got {lse.dtype} {tuple(lse.shape)})")
+    if lse.get_device() != pool.gpu:
+        raise _elsewhere(lse, "lse", pool.gpu)
     if lse.stride(1) != 1:
         lse = lse.contiguous()
     clear = 0
@@ -283,24 +307,24 @@ def naylis_evict(key_weights: torch.Tensor, pool: PagedKV, page_table: torch.Ten
     free.  heads: query heads (R_k moves with the KV head of its query head).
     Returns kept [B, H_KV, budget] int32 (-1 past the count), the new lengths [B] int32, and the
     kept keys' weights [B, H_KV, pages_out * page_size] (0 past the count)."""
-    table, table_out = _table(page_table), _table(page_table_out, "page_table_out")
+    dev, gpu = pool.device, pool.gpu
+    table, table_out = _table(page_table, gpu), _table(page_table_out, gpu, "page_table_out")
     B, max_pages = table.shape
     pages_out = table_out.shape[1]
     _want(table_out.shape[0] == B, "page_table_out must have a row for every sequence")
-    lens = _int32(cache_seqlens, "cache_seqlens", B)
+    lens = _int32(cache_seqlens, "cache_seqlens", B, gpu)
     max_k = max_pages * pool.page_size
     if max_seqlen_k is not None and max_seqlen_k < max_k:
         max_k = int(max_seqlen_k)
-    _weights_ok(key_weights, B, pool.kv_heads, max_k)
+    _weights_ok(key_weights, B, pool.kv_heads, max_k, gpu)
     w_0, w_1, _ = key_weights.stride()
-    dev = pool.device
     kept = torch.empty((B, pool.kv_heads, max(budget, 0)), dtype=torch.int32, device=dev)
     lens_out = torch.empty_like(lens)
     w_out = torch.empty((B, pool.kv_heads, pages_out * pool.page_size), dtype=torch.float32, device=dev)
     a = _EVICT_ARGS.pack(B, heads, max_k, max_pages, pages_out, budget, sink, recent, table.data_ptr(), table.stride(0),
                          table_out.data_ptr(), table_out.stride(0), lens.data_ptr(), key_weights.data_ptr(), w_0, w_1,
                          kept.data_ptr(), lens_out.data_ptr(), w_out.data_ptr())
-    rc = _lib.load().fna2_evict(pool._ref, a, _stream(dev))
+    rc = _launch(gpu, _lib.load().fna2_evict, pool._ref, a)
     if rc:
         _lib.check(rc, "fna2_evict")
     return kept, lens_out, w_out
