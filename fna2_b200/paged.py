@@ -433,10 +433,14 @@ class NaylisPagedCache:
         fresh = self._take(per * len(over))
         rows = [fresh[i * per:(i + 1) * per] for i in range(len(over))]
         dev = self.pool.device
-        idx = torch.tensor(over, device=dev)
-        table_out = torch.tensor(rows, dtype=torch.int32, device=dev)
-        _, lens, w = naylis_evict(self.key_weights[idx], self.pool, self.page_table[idx], self.seqlens[idx], budget,
-                                  table_out, self.heads, recent, sink, max(self.lengths))
+        try:
+            idx = torch.tensor(over, device=dev)
+            table_out = torch.tensor(rows, dtype=torch.int32, device=dev)
+            _, lens, w = naylis_evict(self.key_weights[idx], self.pool, self.page_table[idx], self.seqlens[idx], budget,
+                                      table_out, self.heads, recent, sink, max(self.lengths))
+        except Exception:
+            self._free += fresh[::-1]
+            raise
         self.page_table[idx] = -1
         self.page_table[idx, :per] = table_out
         self.seqlens[idx] = lens
