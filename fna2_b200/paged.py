@@ -376,13 +376,13 @@ class NaylisPagedCache:
         taken, self._free = self._free[len(self._free) - n:], self._free[:len(self._free) - n]
         return taken[::-1]
 
-    def _grow(self, new: Sequence[int]) -> None:
-        """Pages for new[b] more tokens of each slot."""
-        need = [-(-(n + m) // self.page_size) - len(p) for n, m, p in zip(self.lengths, new, self._pages)]
+    def _grow(self, new: Sequence[int]) -> List[int]:
+        """Pages for new[b] more tokens of each slot; returns how many each slot got."""
+        need = [max(0, -(-(n + m) // self.page_size) - len(p)) for n, m, p in zip(self.lengths, new, self._pages)]
         for b, (n, m) in enumerate(zip(self.lengths, new)):
             _want(m >= 0 and -(-(n + m) // self.page_size) <= self.max_pages,
                   f"slot {b}: {n} + {m} tokens do not fit its {self.max_pages} pages")
-        taken = self._take(sum(max(0, x) for x in need))
+        taken = self._take(sum(need))
         at = 0
         for b, x in enumerate(need):
             if x > 0:
@@ -390,6 +390,14 @@ class NaylisPagedCache:
                 self._pages[b] += taken[at:at + x]
                 self.page_table[b, first:first + x] = torch.tensor(taken[at:at + x], dtype=torch.int32)
                 at += x
+        return need
+
+    def _shrink(self, got: Sequence[int]) -> None:
+        """Takes back what _grow gave."""
+        for b in reversed(range(self.batch)):
+            if got[b]:
+                self._free += self._pages[b][:-got[b] - 1:-1]
+                del self._pages[b][-got[b]:]
 
     def append(self, q, k, v, new: Sequence[int], r_k=None, q_norm=None, k_norm=None, rope=None) -> torch.Tensor:
         """new[b] new tokens of every slot b (0 for none), packed in slot order: q, k through the
@@ -397,17 +405,22 @@ class NaylisPagedCache:
         q for attend()."""
         new = [int(n) for n in new]
         _want(len(new) == self.batch and sum(new) == q.shape[0], "new must give the tokens of every slot")
-        self._grow(new)
-        ones = all(n == 1 for n in new)
-        if ones:
-            self._cu = self._one_each
-        else:
-            cu = [0]
-            for n in new:
-                cu.append(cu[-1] + n)
-            self._cu = torch.tensor(cu, dtype=torch.int32).to(self.pool.device, non_blocking=True)
-        out = qk_norm_rope_append(q, k, v, self.pool, self.page_table, self.seqlens, self._cu, r_k, self.positions,
-                                  q_norm, k_norm, rope)
+        got = self._grow(new)
+        try:
+            ones = all(n == 1 for n in new)
+            if ones:
+                cu = self._one_each
+            else:
+                starts = [0]
+                for n in new:
+                    starts.append(starts[-1] + n)
+                cu = torch.tensor(starts, dtype=torch.int32).to(self.pool.device, non_blocking=True)
+            out = qk_norm_rope_append(q, k, v, self.pool, self.page_table, self.seqlens, cu, r_k, self.positions,
+                                      q_norm, k_norm, rope)
+        except Exception:
+            self._shrink(got)
+            raise
+        self._cu = cu
         added = 1 if ones else self._cu[1:] - self._cu[:-1]
         self.seqlens += added
         self.positions += added

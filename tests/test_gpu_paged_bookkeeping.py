@@ -35,3 +35,17 @@ def test_a_refused_evict_changes_nothing(budget, recent, sink):
             cache.evict(budget, recent, sink)
     assert _same(_state(cache), before)
     assert cache.evict(48, 8, 2) == [0, 2] and cache.lengths == [48, 20, 48]
+
+
+def test_a_refused_append_changes_nothing():
+    cache = _cache()
+    q0, rq0 = _fill(cache, [30, 20, 5])
+    gs = torch.randn(4, device="cuda")
+    first = cache.attend(q0, rq0, gs, weigh=False)
+    before = _state(cache)
+    q, k, v, _, rk = _tokens(90, 4)
+    for bad in (dict(r_k=None), dict(k=k.float()), dict(v=v[:, :1]), dict(q_norm=torch.nn.Identity())):
+        with pytest.raises((RuntimeError, ValueError, TypeError, AttributeError)):
+            cache.append(**{**dict(q=q, k=k, v=v, new=[70, 0, 20], r_k=rk), **bad})
+    assert _same(_state(cache), before)
+    assert torch.equal(cache.attend(q0, rq0, gs, weigh=False), first)  # still the tokens of the last append
