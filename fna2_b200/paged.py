@@ -362,7 +362,8 @@ class NaylisPagedCache:
         self.lengths: List[int] = [0] * batch
         self._pages: List[List[int]] = [[] for _ in range(batch)]
         self._free = list(range(num_pages))[::-1]
-        self._new: List[int] = [0] * batch
+        self._new: List[int] = [0] * batch  # tokens of the last append
+        self._evicted: List[int] = []       # slots that have lost some of them since
         self._cu = torch.zeros(batch + 1, dtype=torch.int32, device=dev)
         self._one_each = torch.arange(batch + 1, dtype=torch.int32, device=dev)
 
@@ -420,7 +421,7 @@ class NaylisPagedCache:
         except Exception:
             self._shrink(got)
             raise
-        self._cu = cu
+        self._cu, self._evicted = cu, []
         added = 1 if ones else self._cu[1:] - self._cu[:-1]
         self.seqlens += added
         self.positions += added
@@ -430,7 +431,11 @@ class NaylisPagedCache:
 
     def attend(self, q, r_q=None, graph_scale=None, softmax_scale=None, weigh: bool = True, return_lse: bool = False):
         """Attention of the tokens of the last append over their slots' keys (flash_naylis_paged);
-        weigh: add the attention weights to key_weights."""
+        weigh: add the attention weights to key_weights.  Slots that were released since have no
+        keys: 0 and -inf.  An evict that took some of these tokens' own keys away comes after it."""
+        _want(q.dim() == 3 and q.shape[0] == sum(self._new), "attend takes the tokens of the last append")
+        if self._evicted:
+            raise RuntimeError(f"slots {self._evicted}: tokens of the last append were evicted, attend comes before evict")
         return flash_naylis_paged(q, self.pool, self.page_table, self.seqlens, self._cu, max(self._new), r_q,
                                   graph_scale, softmax_scale, True, self.key_weights if weigh else None, return_lse,
                                   max(self.lengths))
@@ -463,12 +468,14 @@ class NaylisPagedCache:
             self._free += self._pages[b]
             self._pages[b] = list(row)
             self.lengths[b] = budget
+        self._evicted += [b for b in over if recent < self._new[b]]
         return over
 
     def release(self, slot: int) -> None:
         """Empty a slot; its pages go back to the pool."""
         self._free += self._pages[slot]
-        self._pages[slot], self.lengths[slot], self._new[slot] = [], 0, 0
+        self._pages[slot], self.lengths[slot] = [], 0
+        self._evicted = [b for b in self._evicted if b != slot]
         self.page_table[slot] = -1
         self.seqlens[slot] = 0
         self.positions[slot] = 0

@@ -49,3 +49,63 @@ def test_a_refused_append_changes_nothing():
             cache.append(**{**dict(q=q, k=k, v=v, new=[70, 0, 20], r_k=rk), **bad})
     assert _same(_state(cache), before)
     assert torch.equal(cache.attend(q0, rq0, gs, weigh=False), first)  # still the tokens of the last append
+
+
+def test_attend_takes_the_tokens_of_the_last_append():
+    cache = _cache()
+    gs = torch.randn(4, device="cuda")
+    q, _, _, rq, _ = _tokens(6, 5)
+    with pytest.raises(ValueError, match="last append"):
+        cache.attend(q, rq, gs)
+    qa, rqa = _fill(cache, [30, 20, 5])
+    with pytest.raises(ValueError, match="last append"):
+        cache.attend(q, rq, gs)
+    assert torch.isfinite(cache.attend(qa, rqa, gs)).all()
+
+
+@pytest.mark.parametrize("gone", [0, 2])
+def test_attend_after_a_release(gone):
+    """The released slot's tokens see no key, the others what they saw."""
+    from fna2_b200 import _lib
+    cache = _cache()
+    gs = torch.randn(4, device="cuda")
+    new = [90, 3, 20]
+    q, rq = _fill(cache, new)
+    want, wl = cache.attend(q, rq, gs, weigh=False, return_lse=True)
+    cache.release(gone)
+    out, lse = cache.attend(q, rq, gs, weigh=False, return_lse=True)
+    torch.cuda.synchronize()
+    assert _lib.load().fna2_device_status(1) == 0
+    for b, (o, w, l, m) in enumerate(zip(out.split(new), want.split(new), lse.split(new, 1), wl.split(new, 1))):
+        if b == gone:
+            assert (o == 0).all() and torch.isneginf(l).all()
+        else:
+            assert (o.float() - w.float()).abs().max() <= 2.0 ** -7 * w.float().abs().max()
+            assert torch.allclose(l, m, atol=30 * 2.0 ** -16 + 2e-5)
+
+
+def test_attend_after_an_evict():
+    """As long as the eviction kept the last tokens' own keys; not when it took some."""
+    for recent, ok in ((3, True), (2, False)):
+        cache = _cache()
+        gs = torch.randn(4, device="cuda")
+        q, rq = _fill(cache, [100, 20, 65])
+        cache.attend(q, rq, gs)
+        q, k, v, rq, rk = _tokens(9, 8)
+        q = cache.append(q, k, v, [3, 3, 3], rk)
+        cache.attend(q, rq, gs)
+        cut = cache.evict(48, recent, 2)
+        assert cut == [0, 2]
+        if ok:
+            x = dict(kp=cache.pool.k_pages.cpu(), vp=cache.pool.v_pages.cpu(), rp=cache.pool.rk_pages.cpu(),
+                     table=cache.page_table.cpu(), lens=cache.lengths, cu=torch.tensor([0, 3, 6, 9]), q=q.cpu(),
+                     rq=rq.cpu(), gs=gs.cpu())
+            _close_out("after evict", cache.attend(q, rq, gs), PO.attention(x, True)[0])
+            continue
+        with pytest.raises(RuntimeError, match="before evict"):
+            cache.attend(q, rq, gs)
+        cache.release(0)
+        with pytest.raises(RuntimeError, match="before evict"):
+            cache.attend(q, rq, gs)
+        q, k, v, rq, rk = _tokens(3, 9)
+        assert torch.isfinite(cache.attend(cache.append(q, k, v, [1, 1, 1], rk), rq, gs)).all()
