@@ -334,8 +334,8 @@ class NaylisPagedCache:
     """The paged cache of one layer: a pool, and per batch slot its pages, length, next rotary
     position and key weights.
 
-    Lengths are kept on the host (they follow from the calls) and on the device, so no call
-    waits for the device.  A slot's pages are taken from a free list as it grows; evict moves
+    Lengths are kept on the host (they follow from the calls) and on the device, and what the
+    host decides goes there from pinned memory, so no call waits for the device.  A slot's pages are taken from a free list as it grows; evict moves
     what it keeps to fresh pages and returns the old ones.  All work is ordered by the current
     stream; pages that are returned are reused by later calls on the same stream.
 
@@ -371,6 +371,10 @@ class NaylisPagedCache:
     def free_pages(self) -> int:
         return len(self._free)
 
+    def _send(self, values: Sequence[int], dtype=torch.int64) -> torch.Tensor:
+        """Integers to the device, in stream order and without a wait (pinned memory is kept until it is copied)."""
+        return torch.tensor(values, dtype=dtype, pin_memory=True).to(self.pool.device, non_blocking=True)
+
     def _take(self, n: int) -> List[int]:
         if n > len(self._free):
             raise RuntimeError(f"the pool has {len(self._free)} free pages, {n} are needed")
@@ -384,13 +388,15 @@ class NaylisPagedCache:
             _want(m >= 0 and -(-(n + m) // self.page_size) <= self.max_pages,
                   f"slot {b}: {n} + {m} tokens do not fit its {self.max_pages} pages")
         taken = self._take(sum(need))
-        at = 0
+        at, places = 0, []
         for b, x in enumerate(need):
-            if x > 0:
-                first = len(self._pages[b])
-                self._pages[b] += taken[at:at + x]
-                self.page_table[b, first:first + x] = torch.tensor(taken[at:at + x], dtype=torch.int32)
-                at += x
+            first = b * self.max_pages + len(self._pages[b])
+            places += range(first, first + x)
+            self._pages[b] += taken[at:at + x]
+            at += x
+        if taken:  # one copy and one launch, however many slots take pages
+            entries = self._send(places + taken)
+            self.page_table.view(-1).index_copy_(0, entries[:at], entries[at:].int())
         return need
 
     def _shrink(self, got: Sequence[int]) -> None:
@@ -415,7 +421,7 @@ class NaylisPagedCache:
                 starts = [0]
                 for n in new:
                     starts.append(starts[-1] + n)
-                cu = torch.tensor(starts, dtype=torch.int32).to(self.pool.device, non_blocking=True)
+                cu = self._send(starts, torch.int32)
             out = qk_norm_rope_append(q, k, v, self.pool, self.page_table, self.seqlens, cu, r_k, self.positions,
                                       q_norm, k_norm, rope)
         except Exception:
@@ -450,20 +456,19 @@ class NaylisPagedCache:
         per = -(-budget // self.page_size)
         fresh = self._take(per * len(over))
         rows = [fresh[i * per:(i + 1) * per] for i in range(len(over))]
-        dev = self.pool.device
         try:
-            idx = torch.tensor(over, device=dev)
-            table_out = torch.tensor(rows, dtype=torch.int32, device=dev)
+            sent = self._send(over + fresh)
+            idx, table_out = sent[:len(over)], sent[len(over):].view(len(over), per).int()
             _, lens, w = naylis_evict(self.key_weights[idx], self.pool, self.page_table[idx], self.seqlens[idx], budget,
                                       table_out, self.heads, recent, sink, max(self.lengths))
         except Exception:
             self._free += fresh[::-1]
             raise
-        self.page_table[idx] = -1
-        self.page_table[idx, :per] = table_out
-        self.seqlens[idx] = lens
-        self.key_weights[idx] = 0.0
-        self.key_weights[idx, :, :w.shape[2]] = w
+        self.page_table.index_fill_(0, idx, -1)
+        self.page_table[:, :per].index_copy_(0, idx, table_out)
+        self.seqlens.index_copy_(0, idx, lens)
+        self.key_weights.index_fill_(0, idx, 0.0)
+        self.key_weights[:, :, :w.shape[2]].index_copy_(0, idx, w)
         for b, row in zip(over, rows):
             self._free += self._pages[b]
             self._pages[b] = list(row)
@@ -476,8 +481,8 @@ class NaylisPagedCache:
         self._free += self._pages[slot]
         self._pages[slot], self.lengths[slot] = [], 0
         self._evicted = [b for b in self._evicted if b != slot]
-        self.page_table[slot] = -1
-        self.seqlens[slot] = 0
-        self.positions[slot] = 0
+        self.page_table[slot].fill_(-1)  # (assigning a number copies it from the host)
+        self.seqlens[slot].zero_()
+        self.positions[slot].zero_()
         if self.key_weights is not None:
-            self.key_weights[slot] = 0.0
+            self.key_weights[slot].zero_()

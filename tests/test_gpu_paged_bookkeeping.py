@@ -109,3 +109,40 @@ def test_attend_after_an_evict():
             cache.attend(q, rq, gs)
         q, k, v, rq, rk = _tokens(3, 9)
         assert torch.isfinite(cache.attend(cache.append(q, k, v, [1, 1, 1], rk), rq, gs)).all()
+
+
+def test_no_call_waits_for_the_device():
+    """Appends that take pages (all slots one token, or different numbers), attention, eviction and release
+    return while the device is still busy with what came before."""
+    cache = _cache(num_pages=60)
+    gs = torch.randn(4, device="cuda")
+    steps = [[100, 31, 64], [1, 1, 1], [12, 0, 16], [1, 1, 1]]
+    data = [_tokens(sum(new), 20 + i) for i, new in enumerate(steps)]
+
+    def serve(c):
+        outs = []
+        for new, (q, k, v, rq, rk) in zip(steps, data):
+            q = c.append(q, k, v, new, rk)
+            outs.append(c.attend(q, rq, gs))
+        c.evict(48, 16, 2)
+        c.release(1)
+        q, k, v, rq, rk = data[1]
+        outs.append(c.attend(c.append(q, k, v, [1, 1, 1], rk), rq, gs))
+        return outs
+    want = serve(_cache(num_pages=60))  # (and the library, its kernels and the allocators' blocks are there)
+    torch.cuda.synchronize()
+    mode = torch.cuda.get_sync_debug_mode()
+    done = torch.cuda.Event()
+    torch.cuda.set_sync_debug_mode("error")
+    try:
+        torch.cuda._sleep(2 ** 30)  # about half a second
+        done.record()
+        got = serve(cache)
+        busy = not done.query()
+    finally:
+        torch.cuda.set_sync_debug_mode(mode)
+    torch.cuda.synchronize()
+    assert busy
+    for a, b in zip(want, got):
+        assert torch.equal(a, b)
+    assert cache.page_table[1].tolist()[:1] != [-1] and cache.seqlens.tolist() == cache.lengths
