@@ -682,8 +682,9 @@ bool strides_ok(std::initializer_list<int64_t> v, int64_t vec = 8) {
   return true;
 }
 
-// Checks of the pool and the page table, shared by every paged entry point.
-int paged_pool(const Fna2PagedKV* kv, int heads, const int32_t* table, int64_t table_stride, int max_pages,
+// Checks of the pool and the page table, shared by every paged entry point.  (Tensors without an element may be
+// NULL: those of an empty batch, the table of sequences that own no page.)
+int paged_pool(const Fna2PagedKV* kv, int heads, int batch, const int32_t* table, int64_t table_stride, int max_pages,
                PagedPool* d) {
   FNA2_CHECK(kv != nullptr, "null pool");
   FNA2_CHECK(kv->head_dim == 64 || kv->head_dim == 128, "head_dim must be 64 or 128 (got %d)", kv->head_dim);
@@ -702,7 +703,8 @@ int paged_pool(const Fna2PagedKV* kv, int heads, const int32_t* table, int64_t t
                          kv->v_token_stride, kv->v_head_stride}) &&
                  (kv->graph_heads == 0 || strides_ok({kv->rk_page_stride, kv->rk_token_stride, kv->rk_head_stride})),
              "pool strides must be non-negative multiples of 8 elements");
-  FNA2_CHECK(table != nullptr && max_pages >= 0 && table_stride >= max_pages, "bad page table");
+  FNA2_CHECK((table != nullptr || batch == 0 || max_pages == 0) && max_pages >= 0 && table_stride >= max_pages,
+             "bad page table");
   FNA2_CHECK(static_cast<int64_t>(max_pages) * kv->page_size < (1ll << 31), "a sequence's pages hold 2^31 keys or more");
   using bf = __nv_bfloat16;
   d->pages = kv->num_pages;
@@ -724,13 +726,13 @@ int paged_pool(const Fna2PagedKV* kv, int heads, const int32_t* table, int64_t t
 template <class P>
 int paged_queries(const Fna2PagedKV* kv, const Fna2PagedAttnArgs* a, P* p) {
   FNA2_CHECK(a != nullptr, "null arguments");
-  if (int rc = paged_pool(kv, a->heads, a->page_table, a->table_stride, a->max_pages, &p->kv)) return rc;
+  if (int rc = paged_pool(kv, a->heads, a->batch, a->page_table, a->table_stride, a->max_pages, &p->kv)) return rc;
   FNA2_CHECK(a->batch >= 0 && a->batch <= 65535 && a->total_q >= 0, "bad sizes (batch 0 to 65535)");
   FNA2_CHECK(a->max_seqlen_q >= 0 && a->max_seqlen_k >= 0, "negative length bound");
   FNA2_CHECK(a->max_seqlen_k <= static_cast<int64_t>(a->max_pages) * kv->page_size,
              "max_seqlen_k (%d) is above what a page table row holds", a->max_seqlen_k);
   FNA2_CHECK(a->softmax_scale > 0.f, "softmax_scale must be positive");
-  FNA2_CHECK(a->cache_seqlens && a->cu_seqlens_q, "null sequence tensor");
+  FNA2_CHECK((a->cache_seqlens || a->batch == 0) && a->cu_seqlens_q, "null sequence tensor");
   FNA2_CHECK(a->q != nullptr || a->total_q == 0, "null tensor pointer: q");
   FNA2_CHECK(aligned16(a->q) && strides_ok({a->q_token_stride, a->q_head_stride}),
              "q must be 16-byte aligned with strides of multiples of 8 elements");
@@ -930,7 +932,7 @@ extern "C" int fna2_paged_append(const Fna2PagedKV* kv, const Fna2AppendArgs* a,
   g_last_error.clear();
   FNA2_CHECK(a != nullptr, "null arguments");
   AppendParams p{};
-  if (int rc = paged_pool(kv, a->heads, a->page_table, a->table_stride, a->max_pages, &p.kv)) return rc;
+  if (int rc = paged_pool(kv, a->heads, a->batch, a->page_table, a->table_stride, a->max_pages, &p.kv)) return rc;
   FNA2_CHECK(a->batch >= 0 && a->total_tokens >= 0 && a->total_tokens < (1ll << 31), "bad sizes");
   FNA2_CHECK(a->in_dtype == FNA2_DTYPE_F32 || a->in_dtype == FNA2_DTYPE_BF16, "bad in_dtype %d", a->in_dtype);
   FNA2_CHECK(a->weight_dtype == FNA2_DTYPE_F32 || a->weight_dtype == FNA2_DTYPE_BF16, "bad weight_dtype %d",
@@ -939,7 +941,7 @@ extern "C" int fna2_paged_append(const Fna2PagedKV* kv, const Fna2AppendArgs* a,
   FNA2_CHECK((a->q_weight == nullptr) == (a->k_weight == nullptr), "set both RMSNorm weights or neither");
   FNA2_CHECK(aligned16(a->q_weight) && aligned16(a->k_weight), "RMSNorm weights must be 16-byte aligned");
   FNA2_CHECK(a->eps >= 0.f, "eps must be >= 0");
-  FNA2_CHECK(a->cache_seqlens && a->cu_seqlens, "null sequence tensor");
+  FNA2_CHECK((a->cache_seqlens || a->batch == 0) && a->cu_seqlens, "null sequence tensor");
   if (a->batch == 0 || a->total_tokens == 0) return FNA2_OK;
   const int eb = a->in_dtype == FNA2_DTYPE_BF16 ? 2 : 4;
   if (int rc = check_rows(a->q, a->heads, eb, kv->head_dim, "q")) return rc;
@@ -1035,7 +1037,9 @@ extern "C" int fna2_key_weights(const Fna2PagedKV* kv, const Fna2PagedAttnArgs* 
   g_last_error.clear();
   KeyWeightsParams p{};
   if (int rc = paged_queries(kv, a, &p)) return rc;
-  FNA2_CHECK(a->key_weights != nullptr && (a->lse != nullptr || a->total_q == 0), "key weights need lse and key_weights");
+  FNA2_CHECK((a->key_weights != nullptr || p.bd.B == 0 || (p.bd.max_k == 0 && a->kw_clear == 0)) &&
+                 (a->lse != nullptr || a->total_q == 0),
+             "key weights need lse and key_weights");
   FNA2_CHECK(a->kw_clear >= 0 && (a->kw_clear == 0 || a->kw_clear >= p.bd.max_k), "kw_clear (%lld) is below max_seqlen_k",
              static_cast<long long>(a->kw_clear));
   FNA2_CHECK(a->kw_clear == 0 || (((a->kw_clear | a->kw_batch_stride | a->kw_head_stride) & 3) == 0 && aligned16(a->key_weights)),
@@ -1061,20 +1065,21 @@ extern "C" int fna2_evict(const Fna2PagedKV* kv, const Fna2EvictArgs* a, void* s
   g_last_error.clear();
   FNA2_CHECK(a != nullptr, "null arguments");
   EvictParams p{};
-  if (int rc = paged_pool(kv, a->heads, a->page_table, a->table_stride, a->max_pages, &p.kv)) return rc;
+  if (int rc = paged_pool(kv, a->heads, a->batch, a->page_table, a->table_stride, a->max_pages, &p.kv)) return rc;
   FNA2_CHECK(a->batch >= 0 && a->batch <= 65535, "bad batch");
   FNA2_CHECK(a->max_seqlen_k >= 0 && a->max_seqlen_k <= static_cast<int64_t>(a->max_pages) * kv->page_size,
              "max_seqlen_k (%d) is above what a page table row holds", a->max_seqlen_k);
-  FNA2_CHECK(a->page_table_out != nullptr && a->max_pages_out >= 0 && a->table_out_stride >= a->max_pages_out,
+  FNA2_CHECK((a->page_table_out != nullptr || a->batch == 0) && a->max_pages_out >= 0 && a->table_out_stride >= a->max_pages_out,
              "bad output page table");
   FNA2_CHECK(a->budget >= 1 && a->sink >= 0 && a->recent >= 0 && static_cast<int64_t>(a->sink) + a->recent <= a->budget,
              "budget (%d) must be >= 1 and hold sink (%d) + recent (%d)", a->budget, a->sink, a->recent);
   FNA2_CHECK(a->budget <= static_cast<int64_t>(a->max_pages_out) * kv->page_size &&
                  static_cast<int64_t>(a->max_pages_out) * kv->page_size < (1ll << 31),
              "the output page table holds fewer than budget (%d) keys", a->budget);
-  FNA2_CHECK(a->cache_seqlens && a->key_weights && a->kept && a->seqlens_out && a->weights_out, "null tensor pointer");
   FNA2_CHECK(a->kw_batch_stride >= 0 && a->kw_head_stride >= 0, "negative key_weights stride");
   if (a->batch == 0) return FNA2_OK;
+  FNA2_CHECK(a->cache_seqlens && (a->key_weights || a->max_seqlen_k == 0) && a->kept && a->seqlens_out && a->weights_out,
+             "null tensor pointer");
   p.lens = a->cache_seqlens;
   p.B = a->batch;
   p.G = a->heads / kv->kv_heads;
