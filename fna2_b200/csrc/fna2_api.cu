@@ -772,9 +772,9 @@ struct PagedPlan {
 
 // Kept logits are padded to the longest sequence, so one long sequence among short ones would multiply their
 // place: 4.3 GB for 256 sequences decoding one token with 32 heads beside 131,072 keys.  Their limit is half of
-// the pool's K (what 32 rows of every slot take at D = 128), at least 64 MB and at most 2 GB; beyond it the key
+// the pool's K (what 32 rows of every slot take at D = 128), at least 256 MB and at most 2 GB; beyond it the key
 // weights' kernels form the logits again, which needs a few KB per token.
-constexpr double kLogitBytesMin = 64e6, kLogitBytesMax = 2e9;
+constexpr double kLogitBytesMin = 256e6, kLogitBytesMax = 2e9;
 double logit_bytes_limit(const Fna2PagedKV* kv) {
   const double k_bytes = 2.0 * kv->num_pages * kv->page_size * kv->kv_heads * kv->head_dim;
   return std::max(kLogitBytesMin, std::min(kLogitBytesMax, k_bytes / 2));
