@@ -787,8 +787,8 @@ size_t kw_workspace_bytes(int64_t T, int H, int RP) { return up256(static_cast<s
 
 // Splits of the tensor-core kernel's keys: `base` CTAs without splits, `tiles` key tiles each.  One
 // CTA runs per SM; a tile counts 2, a CTA's start and end 6, and the join moves 8 D bytes per row and
-// split.  Takes the count with the least estimate (a chunk of 2,048 tokens over 30,717 keys: 1,377 to
-// 1,418 us so, 1,429 and more unsplit, 1,419 to 1,439 with 4 splits, in one process).
+// split.  Takes the count with the least estimate (a chunk of 2,048 tokens over 30,717 keys, the one shape that
+// the constants were fitted to: 1,377 to 1,418 us so, 1,429 and more unsplit, 1,419 to 1,439 with 4 splits).
 int many_splits(int64_t base, int64_t tiles, double row_bytes) {
   int best = 1;
   double best_us = 1e30;
@@ -817,7 +817,8 @@ int paged_plan(const Fna2PagedKV* kv, const Fna2PagedAttnArgs* a, PagedAttnParam
   };
   // As many row blocks as the rows fill, so that two CTAs fit on an SM; twice as many, with half the key
   // groups and so half the rings, where only that lets two fit (16 rows, 4 graph heads, rank 16, D = 128, 8
-  // sequences of 4,000 keys: 38.7 us with one CTA per SM, 28.8 with two); else whatever fits, the fewest first
+  // sequences of 4,000 keys: 38.7 us with one CTA per SM, 34.0 with two; of 100 to 4,000 keys 35.9 and 26.4);
+  // else whatever fits, the fewest first
   // below and then above (R_k rings of 16 graph heads at rank 32 leave room for two key groups, not for four: 16
   // heads of 2 KV heads, 8 sequences of 4,000 keys, one token 79 us, 163 on the tensor-core kernel).  Four row
   // blocks, one key group and two stages always fit: 201 KB with 64 graph heads.

@@ -13,7 +13,10 @@
 // of two bf16 numbers, hi = bf16(f r_q) and lo = bf16(f r_q - hi) (2^-17
 // relative): the LSE and the attention weights are fp32 results, and one bf16
 // rounding of the bias would show in them (2^-9 of the bias).  P is rounded to
-// bf16 for P V (the output is bf16); the row sums use the unrounded P.
+// bf16 for P V, as in the prefill kernels; the row sums use the unrounded P.  The
+// bf16 output then lies 2.3e-3 (2-norm) from the 64-bit one, of which 1.7e-3 is its own
+// rounding; the rest of P as a second bf16 operand would leave only that, for 2 to 7 %
+// of the time (131,071 keys: 332 -> 354 us).
 //
 // A unit is 64/RW keys of a sequence.  The units of all sequences, in order, are
 // cut into equal runs, whatever the lengths, and each run is taken by one CTA for
@@ -33,10 +36,11 @@
 // issuing warp about 110 clk, 580 of the 1800 clk of a tile; a general address per
 // copy: 820 instructions a tile.)
 // Bound: HBM; each cached key is read once per row block.  One token of one sequence of
-// 131,071 keys, 32 separate heads, D = 128, rank 16: 326 us with the join, 7.0 TB/s; of 64
-// sequences of up to 4,096 keys, 8 KV heads of 4: 118 us, 5.8 TB/s, the join and the key
-// weights 13 more.  Short sequences are bound by latency (the scan, a page lookup, the first
-// tiles, the join: 16 sequences of up to 2,048 keys, 4 KV heads: 29 us, of which HBM 7).
+// 131,071 keys, 32 separate heads, D = 128, rank 16: 332 us with the join, 6.9 TB/s; of 64
+// sequences of up to 4,096 keys, 8 KV heads of 4: 117 us, 5.8 TB/s, the join and the key
+// weights 16 more.  Short sequences are bound by latency (the scan, a page lookup, the first
+// tiles) and by the join's second grid (16 sequences of up to 2,048 keys, 4 KV heads: 27 us,
+// of which HBM 7).
 #include "fna2_paged.cuh"
 
 namespace fna2 {
@@ -98,18 +102,19 @@ __device__ __forceinline__ int few_run_of(int64_t U, int C, int64_t u) { return 
 
 // New tokens, and query rows per KV head (new tokens x query heads of the group), up to which a sequence is
 // streamed by the mma.sync kernel.  Its time goes by KV heads and blocks of up to 64 rows; the tensor-core
-// kernel's by query heads and 128-row tiles, however few rows fill them.  8 sequences of 4,000 keys, 16 query
-// heads, D = 128, mma.sync against tensor-core kernel: 32 tokens of 4 KV heads (128 rows) 57 / 74 us, 48
-// tokens 75 / 67; of 2 KV heads, 16 tokens (128 rows) 56 / 72, 24 tokens 80 / 73; of 16 KV heads, 32 tokens
-// (32 rows) 53 / 73, 64 tokens 94 / 73.
+// kernel's by query heads and 128-row tiles, however few rows fill them.  8 sequences of 100 to 4,000 keys, 16
+// query heads with bias of rank 16, D = 128, mma.sync against tensor-core kernel: 32 tokens of 4 KV heads (128
+// rows) 54 / 71 us, 48 tokens 70 / 64; of 16 KV heads, 32 tokens (32 rows) 53 / 74, 48 tokens 83 / 65.  With 2
+// KV heads the limit is low: 16 tokens (128 rows) 35 / 68, 24 tokens 47 / 70, 32 tokens 54 / 71.
 constexpr int kFewTokens = 32;
 constexpr int kFewRows = 128;
 // Rows up to which the mma.sync kernel keeps its logits for the key weights, rather than have them formed
 // again by the key weights' kernels: 16 sequences of 1,000 to 4,000 keys, 8 KV heads, D = 128, kept / formed
-// again: 4 rows 55 / 83 us, 16 rows 81 / 102 us, 32 rows 89 / 99 us, 64 rows 146 / 132 us.
+// again: 4 rows 53 / 82 us, 16 rows 75 / 97 us, 32 rows 88 / 99 us, 64 rows 138 / 129 us.
 constexpr int kLogitRows = 32;
 // ... rows in a call that has longer sequences: its few-row ones mostly add one token, in one 16-row block
-// (26 sequences, chunks of up to 500 tokens next to single ones: 123 us; up to 32 rows 158, 64 rows 250).
+// (26 sequences, chunks of up to 500 tokens next to single ones: 123 us; up to 32 rows 158, 64 rows 250.  Measured
+// with one query head per KV head; groups of more than 16 leave the kernel nothing in such a call).
 constexpr int kFewRowsMixed = 16;
 // Dynamic shared memory of which two CTAs fit on an SM (228 KB, 1 KB reserved per CTA).
 constexpr int kHalfSmem = 113 * 1024;

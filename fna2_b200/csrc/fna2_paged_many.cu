@@ -16,9 +16,11 @@
 //     warps zero them before P V (P is 0 there, but 0 * NaN is not);
 //   - a sequence's keys may be split over CTAs (`chunk` keys each) when there are
 //     too few query tiles to fill the GPU; fna2_paged_many_join_kernel joins them.
-// Bound: the softmax warps and the tensor pipe take turns as in fna2_fwd_kernel, and the power
-// limit: 2,048 tokens over 32,765 keys, 32 heads, D = 128, rank 32: 1,320 us from a cool
-// start, 1,450 (830 TFLOP/s) sustained.
+// Bound: the hand-offs of the two query tiles' chains (product, TMEM load, exp2, TMEM store, product).
+// 2,048 tokens over 30,717 keys, 32 heads, D = 128, rank 32: 1,440 us in a loop (830 TFLOP/s; SM clock
+// 1,680 to 1,760 MHz under the power cap).  A key tile against both query tiles takes 5,200 to 5,600 clk,
+// of which 2,560 are products and 2,048 exp2; with 148 equal CTAs the tensor pipe is active 52 % of the
+// cycles, the exp2 pipe 42 %.
 #include "fna2_paged.cuh"
 
 namespace fna2 {

@@ -22,6 +22,12 @@ break the bounds of a call is skipped and a status recorded (fna2_device_status:
 the pool: append and eviction do not write its rows, the others read them as zeros.
 
 NaylisPagedCache keeps the pool, the tables and the lengths, and runs the four.
+
+These are calls for inference: results carry no gradient, whether or not the inputs
+require one (as in flash_naylis_decode), and pools and key weights are written in place
+without autograd or torch.compile knowing of it (call them outside compiled regions).
+Every tensor of a call lies on the pool's device; the work goes to that device's
+current stream.
 """
 from __future__ import annotations
 

@@ -298,7 +298,8 @@ int fna2_paged_append(const Fna2PagedKV* kv, const Fna2AppendArgs* args, void* s
  * own keys, already appended, are the last of them): the last query rows of the
  * prefill op.  New token i of n sees key j iff j < cache_seqlens[b] and, when
  * causal, j <= cache_seqlens[b] - n + i.  A row that sees no key gets out 0 and
- * lse -inf.  out is bf16, lse (optional) fp32 [H][lse_head_stride].  With
+ * lse -inf, one with a NaN logit NaN.  (An infinity or NaN in the V row of a key
+ * reaches rows that do not see the key too, as in the prefill op: 0 * NaN.)  out is bf16, lse (optional) fp32 [H][lse_head_stride].  With
  * key_weights, the attention weight that each key received,
  * sum over the new tokens and the query heads of the KV head of
  * exp(S - LSE), is added to key_weights[b][kv_head][key]. */
