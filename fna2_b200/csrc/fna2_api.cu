@@ -996,6 +996,7 @@ extern "C" int fna2_paged_attn(const Fna2PagedKV* kv, const Fna2PagedAttnArgs* a
       return fail(FNA2_ERR_WORKSPACE, "paged attention workspace: need %zu bytes, got %zu", l.total, workspace_bytes);
     FNA2_CHECK((reinterpret_cast<uintptr_t>(workspace) & 255u) == 0, "workspace must be 256-byte aligned");
   }
+  FNA2_CHECK(a->out != a->q, "out must not be q: other CTAs read q after the first rows are written");
   p.out = static_cast<__nv_bfloat16*>(a->out), p.o_st = a->out_token_stride, p.o_sh = a->out_head_stride;
   p.lse = a->lse, p.lse_sh = a->lse_head_stride;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
@@ -1081,6 +1082,8 @@ extern "C" int fna2_evict(const Fna2PagedKV* kv, const Fna2EvictArgs* a, void* s
   if (a->batch == 0) return FNA2_OK;
   FNA2_CHECK(a->cache_seqlens && (a->key_weights || a->max_seqlen_k == 0) && a->kept && a->seqlens_out && a->weights_out,
              "null tensor pointer");
+  FNA2_CHECK(a->seqlens_out != a->cache_seqlens && a->weights_out != a->key_weights,
+             "seqlens_out and weights_out must not be cache_seqlens and key_weights: other CTAs read those later");
   p.lens = a->cache_seqlens;
   p.B = a->batch;
   p.G = a->heads / kv->kv_heads;

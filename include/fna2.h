@@ -299,7 +299,8 @@ int fna2_paged_append(const Fna2PagedKV* kv, const Fna2AppendArgs* args, void* s
  * prefill op.  New token i of n sees key j iff j < cache_seqlens[b] and, when
  * causal, j <= cache_seqlens[b] - n + i.  A row that sees no key gets out 0 and
  * lse -inf, one with a NaN logit NaN.  (An infinity or NaN in the V row of a key
- * reaches rows that do not see the key too, as in the prefill op: 0 * NaN.)  out is bf16, lse (optional) fp32 [H][lse_head_stride].  With
+ * reaches rows that do not see the key too, as in the prefill op: 0 * NaN.)
+ * out is bf16 and must not be q, lse (optional) fp32 [H][lse_head_stride].  With
  * key_weights, the attention weight that each key received,
  * sum over the new tokens and the query heads of the KV head of
  * exp(S - LSE), is added to key_weights[b][kv_head][key]. */
@@ -336,7 +337,8 @@ int fna2_key_weights(const Fna2PagedKV* kv, const Fna2PagedAttnArgs* args, void*
  * `sink`, the last `recent`, and of the others those of the largest key weight
  * (ties to the lowest index, NaN below every number).  Their rows of K, V and of
  * the KV head's query heads' R_k are copied in order to slots [0, kept) of the
- * pages in page_table_out, which must not be pages of page_table's sequences.
+ * pages in page_table_out, which must not be pages of page_table's sequences;
+ * no output may be an input.
  * kept [batch][kv_heads][budget] gets the indices (-1 past the count), seqlens_out
  * [batch] the counts, weights_out [batch][kv_heads][max_pages_out * page_size]
  * the kept keys' weights (0 past the count). */
